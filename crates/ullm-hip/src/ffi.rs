@@ -118,6 +118,56 @@ unsafe extern "C" {
         n_kv_head: c_int, head_dim: c_int, y: *mut f32, stream: *mut c_void) -> c_int;
     pub fn ullm_hip_matmul(w: *const c_void, w_dtype: c_int, x: *const f32, y: *mut f32,
         in_dim: c_int, out_dim: c_int, n_cols: c_int, stream: *mut c_void) -> c_int;
+    /// Drafted trees: append, attention, the accepted rows, the next block table.
+    pub fn ullm_hip_qkv_append_tree(q_in: *const f32, k_in: *const f32, v_in: *const f32,
+        q_bias: *const f32, k_bias: *const f32, v_bias: *const f32, q_norm: *const f32,
+        k_norm: *const f32, eps: f32, rope_cs: *const f32, rope_n_pos: c_int, rope_neox: c_int,
+        rotary_dim: c_int, batch: c_int, max_nodes: c_int, seq_lens: *const i32,
+        n_nodes: *const i32, positions: *const i32, n_head: c_int, n_kv_head: c_int,
+        head_dim: c_int, q_out: *mut c_void, q_dtype: c_int, k_cache: *mut c_void,
+        v_cache: *mut c_void, kv_dtype: c_int, kv_stride: i64, seq_stride: i64, n_ctx: c_int,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_qkv_append_tree_paged(q_in: *const f32, k_in: *const f32, v_in: *const f32,
+        q_bias: *const f32, k_bias: *const f32, v_bias: *const f32, q_norm: *const f32,
+        k_norm: *const f32, eps: f32, rope_cs: *const f32, rope_n_pos: c_int, rope_neox: c_int,
+        rotary_dim: c_int, batch: c_int, max_nodes: c_int, seq_lens: *const i32,
+        n_nodes: *const i32, positions: *const i32, n_head: c_int, n_kv_head: c_int,
+        head_dim: c_int, q_out: *mut c_void, q_dtype: c_int, k_pages: *mut c_void,
+        v_pages: *mut c_void, kv_dtype: c_int, kv_stride: i64, page_size: c_int,
+        n_pages: c_int, block_table: *const i32, table_stride: c_int,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_attn_tree(q: *const c_void, k_cache: *const c_void, v_cache: *const c_void,
+        dtype: c_int, kv_stride: i64, seq_stride: i64, mask: *const i64, seq_lens: *const i32,
+        n_nodes: *const i32, positions: *const i32, max_nodes: c_int, max_len: c_int,
+        window: c_int, batch: c_int, n_head: c_int, n_kv_head: c_int, head_dim: c_int,
+        scale: f32, out: *mut c_void, out_dtype: c_int, workspace: *mut c_void,
+        workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_attn_tree_paged(q: *const c_void, k_pages: *const c_void,
+        v_pages: *const c_void, dtype: c_int, kv_stride: i64, page_size: c_int, n_pages: c_int,
+        block_table: *const i32, table_stride: c_int, mask: *const i64, seq_lens: *const i32,
+        n_nodes: *const i32, positions: *const i32, max_nodes: c_int, max_len: c_int,
+        window: c_int, batch: c_int, n_head: c_int, n_kv_head: c_int, head_dim: c_int,
+        scale: f32, out: *mut c_void, out_dtype: c_int, workspace: *mut c_void,
+        workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_tree_workspace_bytes(dtype: c_int, batch: c_int, max_nodes: c_int,
+        max_len: c_int, window: c_int, n_head: c_int, n_kv_head: c_int,
+        head_dim: c_int) -> usize;
+    pub fn ullm_hip_kv_accept(k_cache: *mut c_void, v_cache: *mut c_void, dtype: c_int,
+        kv_stride: i64, seq_stride: i64, n_ctx: c_int, kv_dim: c_int, n_layer: c_int,
+        layer_stride: i64, path: *const i32, path_stride: c_int, n_accept: *const i32,
+        seq_lens: *const i32, lens_out: *mut i32, batch: c_int, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_kv_accept_paged(k_pages: *mut c_void, v_pages: *mut c_void, dtype: c_int,
+        kv_stride: i64, page_size: c_int, n_pages: c_int, kv_dim: c_int, n_layer: c_int,
+        layer_stride: i64, block_table: *const i32, table_stride: c_int, path: *const i32,
+        path_stride: c_int, n_accept: *const i32, seq_lens: *const i32, lens_out: *mut i32,
+        batch: c_int, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_kv_pages_update(k_pages: *mut c_void, v_pages: *mut c_void, dtype: c_int,
+        kv_stride: i64, page_size: c_int, n_pages: c_int, n_layer: c_int, layer_stride: i64,
+        block_table: *const i32, table_stride: c_int, seq_lens: *const i32, n_seq: c_int,
+        parent: *const i32, capacity: *const i32, held: *const u8, table_out: *mut i32,
+        out_stride: c_int, lens_out: *mut i32, n_out: c_int, info: *mut i32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_kv_pages_workspace_bytes(n_out: c_int, n_pages: c_int) -> usize;
 }
 
 /// Status -> ullm_core::Error, as forward.rs:369-380 reports unsupported dtypes.

@@ -352,6 +352,152 @@ int ullm_hip_attn_prefill_paged_ws(const void *q, const void *k_pages, const voi
                                    int head_dim, float scale, float *out, void *workspace,
                                    size_t workspace_bytes, void *stream);
 
+/* ---- decoding several drafted tokens of a sequence at once ----
+ * No counterpart in the reference, which decodes one token at a time
+ * (crates/ullm-model/src/lib.rs:807-969).  A draft is a tree of up to max_nodes
+ * tokens (nodes) that go on from a sequence of seq_lens[b] positions; node i is
+ * stored at position slot seq_lens[b] + i and stands at position positions[b][i]
+ * (the length plus its depth).  A step is ullm_hip_kv_pages_update (room for the
+ * nodes), per layer ullm_hip_qkv_append_tree(_paged) and
+ * ullm_hip_attn_tree(_paged), then ullm_hip_kv_accept(_paged) over all layers.
+ * Common arguments, all DEVICE:
+ * seq_lens:  int32[batch], positions of the sequence before the draft (>= 0)
+ * n_nodes:   int32[batch], nodes of each tree (clamped to 0..max_nodes), or
+ *            NULL: max_nodes each
+ * positions: int32[batch][max_nodes], or NULL: seq_lens[b] + i (a chain) */
+
+/* The append of drafted trees: ullm_hip_qkv_append on batch*max_nodes rows, row
+ * b*max_nodes + i being node i of sequence b.  q and k are rotated to
+ * positions[b][i]; the K/V rows go to slot seq_lens[b] + i.  Rows from
+ * n_nodes[b] on, and rows whose position is outside [0, rope_n_pos), give zeros
+ * in q_out and nothing in the cache; a slot outside the cache (n_ctx rows per
+ * sequence), the table or the pool drops the K/V row.
+ * seq_stride: elements from sequence to sequence (ignored when batch == 1).
+ * Every tensor and row stride 16-byte aligned (norms, rope_cs and the int32
+ * arrays: by their elements). */
+int ullm_hip_qkv_append_tree(const float *q_in, const float *k_in, const float *v_in,
+                             const float *q_bias, const float *k_bias, const float *v_bias,
+                             const float *q_norm, const float *k_norm, float eps,
+                             const float *rope_cs, int rope_n_pos, int rope_neox, int rotary_dim,
+                             int batch, int max_nodes, const int32_t *seq_lens,
+                             const int32_t *n_nodes, const int32_t *positions, int n_head,
+                             int n_kv_head, int head_dim, void *q_out, int q_dtype, void *k_cache,
+                             void *v_cache, int kv_dtype, int64_t kv_stride, int64_t seq_stride,
+                             int n_ctx, void *stream);
+/* page_size: a power of two; the layout of ullm_hip_attn_decode_paged. */
+int ullm_hip_qkv_append_tree_paged(const float *q_in, const float *k_in, const float *v_in,
+                                   const float *q_bias, const float *k_bias, const float *v_bias,
+                                   const float *q_norm, const float *k_norm, float eps,
+                                   const float *rope_cs, int rope_n_pos, int rope_neox,
+                                   int rotary_dim, int batch, int max_nodes,
+                                   const int32_t *seq_lens, const int32_t *n_nodes,
+                                   const int32_t *positions, int n_head, int n_kv_head,
+                                   int head_dim, void *q_out, int q_dtype, void *k_pages,
+                                   void *v_pages, int kv_dtype, int64_t kv_stride, int page_size,
+                                   int n_pages, const int32_t *block_table, int table_stride,
+                                   void *stream);
+
+/* Attention of drafted trees over the cache that holds their sequences and
+ * their own K/V rows:
+ *   out[b,i,h,:] = softmax_t(scale * q[b,i,h,:].K[t,j,:]) . V[t,j,:]
+ * over the keys t that node i sees: those of the sequence (t < seq_lens[b]; with
+ * a window > 0 those with t > positions[b][i] - window) and of the nodes' keys
+ * seq_lens[b] + c those whose bit c its mask has (with a window those with
+ * positions[b][c] > positions[b][i] - window).  What a key that a node does not
+ * see holds, NaN and infinities included, does not reach the node.  A node that
+ * sees no key, and rows from n_nodes[b] on, give zeros.
+ * q, out: [batch][max_nodes][n_head][head_dim]; q in the cache's dtype (f32, f16
+ *         or bf16), out in the cache's dtype or f32 (out_dtype).  The softmax
+ *         weights enter P.V in the cache's dtype where out has it, and in twice
+ *         its bits for an f32 out of a 16-bit cache; an f32 cache runs on f32
+ *         products throughout
+ * mask:   int64[batch][max_nodes][ceil(max_nodes/64)], bit c % 64 of word c / 64
+ *         (its own bit too: a node sees itself only by it), or NULL: node i sees
+ *         the nodes up to i.  positions must be given where window > 0 and mask
+ *         is
+ * max_len: host-side upper bound of seq_lens[b] + n_nodes[b]; keys from it on are
+ *         not attended.  Keys 0..max_len-1 of a contiguous cache must be
+ *         readable
+ * workspace: DEVICE memory of ullm_hip_tree_workspace_bytes, 256-byte aligned,
+ *         needs no initialisation, one call at a time; a workspace for max_len,
+ *         batch and max_nodes serves every call with smaller ones
+ * max_nodes <= 1024; head_dim 64, 128 or 256; n_head % n_kv_head == 0; tensors
+ * and row strides 16-byte aligned. */
+int ullm_hip_attn_tree(const void *q, const void *k_cache, const void *v_cache, int dtype,
+                       int64_t kv_stride, int64_t seq_stride, const int64_t *mask,
+                       const int32_t *seq_lens, const int32_t *n_nodes, const int32_t *positions,
+                       int max_nodes, int max_len, int window, int batch, int n_head,
+                       int n_kv_head, int head_dim, float scale, void *out, int out_dtype,
+                       void *workspace, size_t workspace_bytes, void *stream);
+/* Over pages, as ullm_hip_attn_decode_paged lays them out: page_size a power of
+ * two >= 32, pages outside [0, n_pages) read as zeros, table_stride * page_size
+ * >= max_len. */
+int ullm_hip_attn_tree_paged(const void *q, const void *k_pages, const void *v_pages, int dtype,
+                             int64_t kv_stride, int page_size, int n_pages,
+                             const int32_t *block_table, int table_stride, const int64_t *mask,
+                             const int32_t *seq_lens, const int32_t *n_nodes,
+                             const int32_t *positions, int max_nodes, int max_len, int window,
+                             int batch, int n_head, int n_kv_head, int head_dim, float scale,
+                             void *out, int out_dtype, void *workspace, size_t workspace_bytes,
+                             void *stream);
+size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int max_len, int window,
+                                     int n_head, int n_kv_head, int head_dim);
+
+/* Compaction of the accepted path: row seq_lens[b] + j of K and V takes what row
+ * seq_lens[b] + path[b][j] held before the call, for j < n_accept[b] (clamped to
+ * 0..path_stride), in each of n_layer layers layer_stride elements apart, in
+ * place.  path: int32[batch][path_stride], any order, a node also twice; entries
+ * below 0 and rows outside the cache (n_ctx rows per sequence, the table, the
+ * pool) are left as they are.  kv_dim elements of each row are moved.
+ * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; not seq_lens itself.
+ * path_stride <= 1024; pools, rows and strides 16-byte aligned.  Sequences must
+ * not share the pages of their drafts (ullm_hip_kv_pages_update sees to it). */
+int ullm_hip_kv_accept(void *k_cache, void *v_cache, int dtype, int64_t kv_stride,
+                       int64_t seq_stride, int n_ctx, int kv_dim, int n_layer,
+                       int64_t layer_stride, const int32_t *path, int path_stride,
+                       const int32_t *n_accept, const int32_t *seq_lens, int32_t *lens_out,
+                       int batch, void *stream);
+int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
+                             int page_size, int n_pages, int kv_dim, int n_layer,
+                             int64_t layer_stride, const int32_t *block_table, int table_stride,
+                             const int32_t *path, int path_stride, const int32_t *n_accept,
+                             const int32_t *seq_lens, int32_t *lens_out, int batch, void *stream);
+
+/* The block table of the next step of a paged cache: sequences that go on, grow,
+ * are cut back, fork, end and begin, in one call.  All pages that a sequence of
+ * the old table holds and no sequence of the new one keeps are free after it.
+ * Sequence s of the new table goes on from sequence parent[s] of the old one (a
+ * number outside [0, n_seq): from nothing), keeps the first
+ *   kept = min(seq_lens[parent[s]], capacity[s])
+ * positions and has pages for capacity[s] (>= 0, cut to its table row):
+ *  - pages that kept positions fill are shared by all that keep them;
+ *  - a page that they fill in part stays with the first sequence (lowest s) that
+ *    keeps it so, unless it is a whole page of another's or held; every other
+ *    such sequence gets a page of its own, into which those positions are copied
+ *    in every layer;
+ *  - the others are taken, lowest number first, sequence by sequence, from the
+ *    pages that no sequence keeps and that are not held;
+ *  - entries past capacity[s], and where no page is left, are -1.
+ * table_out: int32[n_out][out_stride]; not block_table itself
+ * lens_out:  int32[n_out], kept (less the positions that should have been copied
+ *            where no page was left); may be seq_lens itself
+ * held:      uint8[n_pages], pages to leave alone where not 0 (a stored prefix),
+ *            or NULL
+ * info:      int32[3]: pages copied, pages taken, pages missing
+ * The pools hold n_layer layers, layer_stride elements apart (0: only the table
+ * is made and nothing is copied).  page_size: a power of two; n_pages <= 2^20;
+ * n_out <= 65535 (0: nothing is written); pools and strides 16-byte aligned.
+ * workspace: DEVICE memory of ullm_hip_kv_pages_workspace_bytes, 256-byte
+ * aligned, needs no initialisation, one call at a time. */
+int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
+                             int page_size, int n_pages, int n_layer, int64_t layer_stride,
+                             const int32_t *block_table, int table_stride, const int32_t *seq_lens,
+                             int n_seq, const int32_t *parent, const int32_t *capacity,
+                             const uint8_t *held, int32_t *table_out, int out_stride,
+                             int32_t *lens_out, int n_out, int32_t *info, void *workspace,
+                             size_t workspace_bytes, void *stream);
+size_t ullm_hip_kv_pages_workspace_bytes(int n_out, int n_pages);
+
 /* Measurement calibration (no counterpart in the reference): reads `bytes`
  * bytes of DEVICE memory at `src` (16-byte aligned) once, with 16-byte loads
  * split over `workgroups` 256-thread workgroups, and writes at most one word

@@ -10,9 +10,17 @@ from .attention import (  # noqa: F401
     GpuAttention,
     attn_decode,
     attn_prefill,
+    attn_tree,
+    attn_tree_paged,
     decode_workspace_bytes,
+    kv_accept,
+    kv_accept_paged,
+    kv_pages_update,
     qkv_append,
+    qkv_append_tree,
+    qkv_append_tree_paged,
     rope_table,
+    tree_masks,
 )
 
 __version__ = "0.1.0"

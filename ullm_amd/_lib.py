@@ -80,6 +80,41 @@ SIGNATURES = {
         [_vp, _vp, _vp, _i, _i64, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _vp, _sz,
          _vp],
     ),
+    "ullm_hip_qkv_append_tree": (
+        _i,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i,
+         _vp, _i, _vp, _vp, _i, _i64, _i64, _i, _vp],
+    ),
+    "ullm_hip_qkv_append_tree_paged": (
+        _i,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i,
+         _vp, _i, _vp, _vp, _i, _i64, _i, _i, _vp, _i, _vp],
+    ),
+    "ullm_hip_attn_tree": (
+        _i,
+        [_vp, _vp, _vp, _i, _i64, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _i,
+         _vp, _sz, _vp],
+    ),
+    "ullm_hip_attn_tree_paged": (
+        _i,
+        [_vp, _vp, _vp, _i, _i64, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f,
+         _vp, _i, _vp, _sz, _vp],
+    ),
+    "ullm_hip_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "ullm_hip_kv_accept": (
+        _i,
+        [_vp, _vp, _i, _i64, _i64, _i, _i, _i, _i64, _vp, _i, _vp, _vp, _vp, _i, _vp],
+    ),
+    "ullm_hip_kv_accept_paged": (
+        _i,
+        [_vp, _vp, _i, _i64, _i, _i, _i, _i, _i64, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp],
+    ),
+    "ullm_hip_kv_pages_update": (
+        _i,
+        [_vp, _vp, _i, _i64, _i, _i, _i, _i64, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp,
+         _vp, _sz, _vp],
+    ),
+    "ullm_hip_kv_pages_workspace_bytes": (_sz, [_i, _i]),
 }
 
 

@@ -14,6 +14,7 @@ import math
 from dataclasses import dataclass
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -161,6 +162,124 @@ def qkv_append(q, k, v, k_cache, v_cache, rope_cs, *, start_pos, n_head, n_kv_he
                      kv_stride, stream)
 
 
+def tree_masks(parents):
+    """(mask, depth) of drafted trees, for attn_tree: parents is a whole-number
+    array or tensor [..., nodes], the node that each node goes on from (below 0:
+    from the sequence itself), always an earlier one.  mask: int64 [..., nodes,
+    ceil(nodes/64)], bit c of row i (bit c % 64 of word c // 64) set for node i
+    and the nodes that it goes on from; depth: int32 [..., nodes], to be added to
+    the sequence's length for the nodes' positions.  Both on the host: a draft
+    of fixed shape makes them once."""
+    p = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+    n = p.shape[-1]
+    flat = p.reshape(math.prod(p.shape[:-1]), n).astype(np.int64)
+    if (flat >= np.arange(n)).any():
+        raise L.UllmHipError(L.E_INVALID, "a node must go on from an earlier one")
+    mask = np.zeros((*flat.shape, -(-n // 64)), np.uint64)
+    depth = np.zeros(flat.shape, np.int32)
+    trees = np.arange(len(flat))
+    for i in range(n):
+        up = flat[:, i]
+        mask[:, i] = np.where((up >= 0)[:, None], mask[trees, up], 0)
+        depth[:, i] = np.where(up >= 0, depth[trees, up] + 1, 0)
+        mask[:, i, i // 64] |= np.uint64(1 << (i % 64))
+    return (torch.from_numpy(mask.view(np.int64).reshape(*p.shape, -(-n // 64))),
+            torch.from_numpy(depth.reshape(p.shape)))
+
+
+def attn_tree(q, k_cache, v_cache, mask, seq_lens, max_len, n_kv_head, *, n_nodes=None,
+              positions=None, window=0, scale=None, kv_stride=None, seq_stride=0, out=None,
+              out_dtype=None, workspace=None, stream=None):
+    """Attention of a tree of drafted tokens over the cache that holds its
+    sequence and, from row seq_lens[b] on, the tokens themselves
+    (ullm_hip_attn_tree has the rules).
+
+    q: [B, nodes, n_head, D] in the cache's dtype.  k_cache/v_cache: layer base
+    with `kv_stride` elements per position (default n_kv_head*D) and
+    `seq_stride` between sequences.  mask: int64 [B, nodes, ceil(nodes/64)] (see
+    tree_masks), or None: each node sees the nodes up to itself.  seq_lens:
+    int32 [B], positions before the draft; n_nodes: int32 [B], nodes of each
+    sequence (default: all); positions: int32 [B, nodes] (default: seq_lens + i).
+    max_len: at least seq_lens + n_nodes of every sequence.  Returns [B, nodes,
+    n_head, D] in q's dtype, or `out_dtype` f32.
+    """
+    return _F.attn_tree(q, k_cache, v_cache, None, mask, seq_lens, max_len, n_kv_head, n_nodes,
+                        positions, window, scale, kv_stride, seq_stride, out, out_dtype, workspace,
+                        stream)
+
+
+def attn_tree_paged(q, k_pages, v_pages, block_table, mask, seq_lens, max_len, n_kv_head, *,
+                    n_nodes=None, positions=None, window=0, scale=None, out=None, out_dtype=None,
+                    workspace=None, stream=None):
+    """attn_tree over a paged cache: k_pages/v_pages [n_pages, page_size,
+    kv_stride], block_table int32 [B, table_stride] (see attn_decode_paged)."""
+    return _F.attn_tree(q, k_pages, v_pages, block_table, mask, seq_lens, max_len, n_kv_head,
+                        n_nodes, positions, window, scale, None, 0, out, out_dtype, workspace,
+                        stream)
+
+
+def qkv_append_tree(q, k, v, k_cache, v_cache, rope_cs, seq_lens, positions=None, *, n_head,
+                    n_kv_head, head_dim, n_nodes=None, rotary_dim=None, neox=True, q_norm=None,
+                    k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None, q_out=None,
+                    q_dtype=None, kv_stride=None, seq_stride=0, n_ctx=None, stream=None):
+    """qkv_append of drafted tokens: q [B, nodes, n_head*D], k/v [B, nodes,
+    n_kv_head*D] f32.  Node i of sequence b is rotated to positions[b, i]
+    (default seq_lens[b] + i), its K/V rows land at position seq_lens[b] + i of
+    a cache of n_ctx (default: the caches' second-last dimension) positions per
+    sequence.  Returns q_out [B, nodes, n_head*D] (q_dtype); rows past
+    n_nodes[b] are zeros and are not stored."""
+    return _F.append_tree(q, k, v, k_cache, v_cache, None, seq_lens, n_nodes, positions, rope_cs,
+                          n_head, n_kv_head, head_dim, rotary_dim, neox, q_norm, k_norm, eps, q_bias,
+                          k_bias, v_bias, q_out, q_dtype, kv_stride, seq_stride, n_ctx, stream)
+
+
+def qkv_append_tree_paged(q, k, v, k_pages, v_pages, rope_cs, seq_lens, positions, block_table, *,
+                          n_head, n_kv_head, head_dim, n_nodes=None, rotary_dim=None, neox=True,
+                          q_norm=None, k_norm=None, eps=1e-6, q_bias=None, k_bias=None,
+                          v_bias=None, q_out=None, q_dtype=None, stream=None):
+    """qkv_append_tree into a paged cache (block_table int32 [B, table_stride])."""
+    return _F.append_tree(q, k, v, k_pages, v_pages, block_table, seq_lens, n_nodes, positions,
+                          rope_cs, n_head, n_kv_head, head_dim, rotary_dim, neox, q_norm, k_norm, eps,
+                          q_bias, k_bias, v_bias, q_out, q_dtype, None, 0, None, stream)
+
+
+def kv_accept(k_cache, v_cache, path, n_accept, seq_lens, *, lens_out=None, stream=None):
+    """Move the accepted nodes' rows together, in place: row seq_lens[b] + j takes
+    what row seq_lens[b] + path[b, j] held, j < n_accept[b], in every layer.
+
+    k_cache/v_cache: [n_layer, B, n_ctx, kv_dim], [B, n_ctx, kv_dim], or for one
+    sequence [n_layer, n_ctx, kv_dim] or [n_ctx, kv_dim].  path: int32 [B, nodes];
+    n_accept, seq_lens: int32 [B].  Returns the new lengths, int32 [B]."""
+    return _F.accept(k_cache, v_cache, None, path, n_accept, seq_lens, lens_out, stream)
+
+
+def kv_accept_paged(k_pages, v_pages, block_table, path, n_accept, seq_lens, *, lens_out=None,
+                    stream=None):
+    """kv_accept over a paged cache: pools [n_pages, page_size, kv_dim] or
+    [n_layer, n_pages, page_size, kv_dim], block_table int32 [B, table_stride]."""
+    return _F.accept(k_pages, v_pages, block_table, path, n_accept, seq_lens, lens_out, stream)
+
+
+def kv_pages_update(k_pages, v_pages, block_table, seq_lens, parent, capacity, *, held=None,
+                    table_stride=None, table_out=None, lens_out=None, info=None, workspace=None,
+                    stream=None):
+    """The block table of the next step: sequence s of it goes on from sequence
+    parent[s] of block_table (below 0: from nothing), keeps min(seq_lens[parent],
+    capacity[s]) positions and has pages for capacity[s].  Whole pages are
+    shared, a part-filled page that two sequences would go on writing is copied
+    (in every layer of the pools), what nobody keeps is free, and what is missing
+    is taken from the free pages, lowest first (ullm_hip_kv_pages_update has the
+    rules).  Growing, forking, cutting back, ending and beginning are all this
+    call.
+
+    Pools as for kv_accept_paged; block_table int32 [B, table_stride], seq_lens
+    int32 [B]; parent, capacity: int32 [n]; held: bool [n_pages], pages to leave
+    alone.  Returns (table [n, table_stride], lengths [n], info int32 [3]: pages
+    copied, taken, missing)."""
+    return _F.pages_update(k_pages, v_pages, block_table, seq_lens, parent, capacity, held,
+                           table_stride, table_out, lens_out, info, workspace, stream)
+
+
 _proj_ws = {}
 
 
@@ -300,6 +419,8 @@ class GpuAttention:
         # the device slice holding pos + 1 (no per-token copy or fill, nothing
         # for a captured graph to replay but kernels).
         self._lens = torch.arange(1, p.n_ctx + 1, dtype=torch.int32, device=self.device)
+        # the same for drafts: entry pos holds pos, the length before the draft
+        self._old_lens = torch.arange(p.n_ctx + 1, dtype=torch.int32, device=self.device)
 
     def supports_batched_prefill(self) -> bool:
         """Prefill runs on MFMA for every cache dtype and head_dim (an f32
@@ -386,6 +507,36 @@ class GpuAttention:
         return attn_prefill(qr, self.key_cache[layer], self.val_cache[layer], p.n_head,
                             p.n_kv_head, p.head_dim, start_pos=start_pos,
                             window=self._window(layer), scale=self.scale)
+
+    def forward_tree(self, layer: int, q, k, v, pos: int, mask, positions, q_norm=None, k_norm=None,
+                     q_bias=None, k_bias=None, v_bias=None):
+        """Attend a draft of T tokens that go on from the first `pos` positions:
+        q [T, n_head*D], k/v [T, kv_dim] f32; mask int64 [T, ceil(T/64)] and
+        positions int32 [T] on the GPU (tree_masks; positions = pos + depth), or
+        None for a chain.  The tokens' rows are stored at pos.. in their order;
+        `accept` keeps those of the accepted path.  Returns [T, n_head*D] f32."""
+        p = self.p
+        T = q.shape[0]
+        if pos < 0 or pos + T > p.n_ctx:
+            raise L.UllmHipError(L.E_INVALID, "draft exceeds the context")
+        kc, vc, lens = self.key_cache[layer], self.val_cache[layer], self._old_lens[pos:pos + 1]
+        at = None if positions is None else positions.view(1, T)
+        qr = qkv_append_tree(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), kc, vc, self.rope_cs, lens, at,
+                             n_head=p.n_head, n_kv_head=p.n_kv_head, head_dim=p.head_dim,
+                             rotary_dim=self.rotary_dim, neox=p.rope_neox, q_norm=q_norm, k_norm=k_norm,
+                             eps=p.eps, q_bias=q_bias, k_bias=k_bias, v_bias=v_bias, q_dtype=p.kv_dtype)
+        out = attn_tree(qr.view(1, T, p.n_head, p.head_dim), kc, vc,
+                        None if mask is None else mask.unsqueeze(0), lens, pos + T, p.n_kv_head,
+                        positions=at, window=self._window(layer), scale=self.scale,
+                        out_dtype=torch.float32)
+        return out.view(T, -1)
+
+    def accept(self, path, n_accept, pos: int):
+        """Keep the accepted nodes of the draft at `pos` in every layer: path int32
+        [T] (node numbers, in order) and n_accept int32 [1] on the GPU.  Returns
+        the new length, int32 [1] on the GPU."""
+        return kv_accept(self.key_cache, self.val_cache, path.view(1, -1), n_accept,
+                         self._old_lens[pos:pos + 1])
 
     # ---- attention blocks from the normed hidden state ----
 

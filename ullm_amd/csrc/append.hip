@@ -56,6 +56,19 @@ struct PageMap {
     int stride, shift, n_pages, rope_n_pos;
 };
 
+// Rows of a batch of drafted trees: row r is node i = r % nodes of sequence
+// b = r / nodes.  It is rotated to position pos[r] (null: len[b] + i) and its
+// K/V rows go to slot len[b] + i of the sequence, in the contiguous cache
+// (tab == nullptr, n_ctx slots, seq_stride elements from sequence to sequence)
+// or its pages.  Rows from n[b] (null: nodes) on, and rows whose position is
+// outside [0, rope_n_pos), store a q of zeros and nothing in the cache; a slot
+// outside the cache, the table or the pool drops the K/V rows.
+struct TreeMap {
+    const int32_t *len, *n, *pos, *tab;
+    int nodes, stride, shift, n_pages, rope_n_pos, n_ctx;
+    int64_t seq_stride;
+};
+
 // Head epilogue of qkv_append_kernel in its split-half lane layout: a head
 // vector of D elements is held by L = D/4 lanes, lane m of the head holding
 // elements {2m, 2m+1} (x[0], x[1]) and {D/2+2m, D/2+2m+1} (x[2], x[3]), so a
@@ -157,14 +170,14 @@ struct SplitEpi {
 // of a batch issued before any is used.
 // SUM: rows are the sum of several partials (the loads cost registers that the
 // plain kernel's occupancy needs: 2048 rows of 32/8 heads x 128 15.8 us without, 18.2 with).
-template <int D, int QDT, int KVDT, bool SUM>
+template <int D, int QDT, int KVDT, bool SUM, class MAP>
 __global__ __launch_bounds__(kAppendWaves * 64) void qkv_append_kernel(
     const float *__restrict__ q_in, const float *__restrict__ k_in, const float *__restrict__ v_in,
     const float *__restrict__ q_bias, const float *__restrict__ k_bias,
     const float *__restrict__ v_bias, const float *__restrict__ q_norm,
     const float *__restrict__ k_norm, float eps, const float *__restrict__ cs, int neox,
     int rotary_dim, int rows, int start_pos, int n_head, int n_kv_head, void *q_out,
-    void *k_cache, void *v_cache, int64_t kv_stride, PageMap pm, int gpw, AppendSrc as) {
+    void *k_cache, void *v_cache, int64_t kv_stride, MAP pm, int gpw, AppendSrc as) {
     using Epi = SplitEpi<D>;
     constexpr int L = Epi::L, HPW = Epi::HPW;
     __shared__ float buf[kAppendWaves][HPW * D];
@@ -174,24 +187,55 @@ __global__ __launch_bounds__(kAppendWaves * 64) void qkv_append_kernel(
     const int gq = (n_head + HPW - 1) / HPW, gk = (n_kv_head + HPW - 1) / HPW;
     const int groups = gq + 2 * gk;
     const int64_t q_dim = (int64_t)n_head * D;
-    int pos = start_pos + row;
-    int64_t crow = pos;
-    if (pm.pos) {  // wave-uniform
-        pos = __builtin_amdgcn_readfirstlane(pm.pos[row]);
-        const int pg = pos >> pm.shift;
-        const bool in = pos >= 0 && pos < pm.rope_n_pos && pg < pm.stride;
-        const int phys = in ? __builtin_amdgcn_readfirstlane(pm.tab[(int64_t)row * pm.stride + pg]) : -1;
-        if (phys < 0 || phys >= pm.n_pages) return;
-        crow = ((int64_t)phys << pm.shift) + (pos & ((1 << pm.shift) - 1));
+    // This workgroup's groups: [gbeg, gend) of the row (gpw per workgroup
+    // along blockIdx.y; all of them when gridDim.y == 1).
+    const int gbeg = (int)blockIdx.y * gpw, gend = min(groups, gbeg + gpw);
+    int pos;
+    int64_t crow = 0;    // element of the row's K/V in the cache
+    bool store = true;   // the row has a place there
+    if constexpr (__is_same(MAP, TreeMap)) {
+        const int b = row / pm.nodes, i = row - b * pm.nodes;
+        const int len = __builtin_amdgcn_readfirstlane(pm.len[b]);
+        const int n = pm.n ? __builtin_amdgcn_readfirstlane(pm.n[b]) : pm.nodes;
+        const int64_t slot = (int64_t)len + i;
+        const int64_t at = pm.pos ? __builtin_amdgcn_readfirstlane(pm.pos[row]) : slot;
+        if (i >= n || at < 0 || at >= pm.rope_n_pos) {
+            // elements of the q groups among this workgroup's
+            const int64_t e1 = min((int64_t)min(gend, gq) * HPW * D, q_dim);
+            const float zero[2] = {0.f, 0.f};
+            for (int64_t e = (int64_t)gbeg * HPW * D + 2 * (int)threadIdx.x; e < e1; e += 2 * kAppendWaves * 64)
+                store_e<QDT, 2>(q_out, row * q_dim + e, zero);
+            return;
+        }
+        pos = (int)at;
+        if (pm.tab) {
+            const int64_t pg = slot >> pm.shift;
+            const int phys = slot >= 0 && pg < pm.stride
+                                 ? __builtin_amdgcn_readfirstlane(pm.tab[(int64_t)b * pm.stride + pg]) : -1;
+            store = phys >= 0 && phys < pm.n_pages;
+            crow = (((int64_t)phys << pm.shift) + (slot & ((1 << pm.shift) - 1))) * kv_stride;
+        } else {
+            store = slot >= 0 && slot < pm.n_ctx;
+            crow = b * pm.seq_stride + slot * kv_stride;
+        }
+    } else {
+        pos = start_pos + row;
+        int64_t slot = pos;
+        if (pm.pos) {  // wave-uniform
+            pos = __builtin_amdgcn_readfirstlane(pm.pos[row]);
+            const int pg = pos >> pm.shift;
+            const bool in = pos >= 0 && pos < pm.rope_n_pos && pg < pm.stride;
+            const int phys = in ? __builtin_amdgcn_readfirstlane(pm.tab[(int64_t)row * pm.stride + pg]) : -1;
+            if (phys < 0 || phys >= pm.n_pages) return;
+            slot = ((int64_t)phys << pm.shift) + (pos & ((1 << pm.shift) - 1));
+        }
+        crow = slot * kv_stride;
     }
     const Epi epi(cs, pos, rotary_dim, neox, q_norm, k_norm, eps);
     const int c0 = 2 * epi.m, c1 = D / 2 + 2 * epi.m;  // element offsets of x[0..1], x[2..3]
     const unsigned loff = (unsigned)(hl * D + c0);      // of x[0..1] from the group's first head
     const bool has_bias = q_bias || k_bias || v_bias;
 
-    // This workgroup's groups: [gbeg, gend) of the row (gpw per workgroup
-    // along blockIdx.y; all of them when gridDim.y == 1).
-    const int gbeg = (int)blockIdx.y * gpw, gend = min(groups, gbeg + gpw);
     for (int g0 = gbeg + wave; g0 < gend; g0 += kAppendWaves * kBatch) {
         float x[kBatch][4], bv[kBatch][4];
         int kind[kBatch], head[kBatch];
@@ -262,9 +306,9 @@ __global__ __launch_bounds__(kAppendWaves * 64) void qkv_append_kernel(
                 void *dst = (char *)q_out + (row * q_dim + (int64_t)h0 * D) * (QDT == ULLM_DT_F32 ? 4 : 2);
                 store_e<QDT, 2>(dst, loff, lo);
                 store_e<QDT, 2>(dst, loff + D / 2, hi);
-            } else {
+            } else if (store) {
                 void *dst = (char *)(kind[b] == 1 ? k_cache : v_cache) +
-                            (crow * kv_stride + (int64_t)h0 * D) * (KVDT == ULLM_DT_F32 ? 4 : 2);
+                            (crow + (int64_t)h0 * D) * (KVDT == ULLM_DT_F32 ? 4 : 2);
                 store_e<KVDT, 2>(dst, loff, lo);
                 store_e<KVDT, 2>(dst, loff + D / 2, hi);
             }
@@ -441,31 +485,32 @@ __global__ __launch_bounds__(proj_waves(NSP) * 64) void qkv_proj_kernel(
                              k_cache, v_cache, kv_stride);
 }
 
-template <int D, int QDT>
+template <int D, int QDT, class MAP>
 static void launch_kv(int kvdt, dim3 g, dim3 b, hipStream_t st, const float *qi, const float *ki,
                       const float *vi, const float *qb, const float *kb, const float *vb,
                       const float *qn, const float *kn, float eps, const float *cs, int neox,
                       int rd, int rows, int sp, int nh, int nkv, void *qo, void *kc, void *vc,
-                      int64_t kvs, PageMap pm, int gpw, AppendSrc as) {
+                      int64_t kvs, MAP pm, int gpw, AppendSrc as) {
     auto go = [&](auto kern) {
         launch_kernel(kern, g, b, 0, st, qi, ki, vi, qb, kb, vb, qn, kn, eps, cs, neox, rd, rows, sp, nh, nkv, qo, kc, vc, kvs, pm, gpw, as);
     };
     auto pick = [&](auto kvc) {
         constexpr int KVDT = decltype(kvc)::value;
-        if (as.ns > 1) go(qkv_append_kernel<D, QDT, KVDT, true>);
-        else go(qkv_append_kernel<D, QDT, KVDT, false>);
+        if constexpr (__is_same(MAP, PageMap))
+            if (as.ns > 1) return go(qkv_append_kernel<D, QDT, KVDT, true, MAP>);
+        go(qkv_append_kernel<D, QDT, KVDT, false, MAP>);
     };
     if (kvdt == ULLM_DT_F32) pick(Int<ULLM_DT_F32>{});
     else if (kvdt == ULLM_DT_F16) pick(Int<ULLM_DT_F16>{});
     else pick(Int<ULLM_DT_BF16>{});
 }
 
-template <int D>
+template <int D, class MAP>
 static void launch_q(int qdt, int kvdt, dim3 g, dim3 b, hipStream_t st, const float *qi,
                      const float *ki, const float *vi, const float *qb, const float *kb,
                      const float *vb, const float *qn, const float *kn, float eps,
                      const float *cs, int neox, int rd, int rows, int sp, int nh, int nkv,
-                     void *qo, void *kc, void *vc, int64_t kvs, PageMap pm, int gpw, AppendSrc as) {
+                     void *qo, void *kc, void *vc, int64_t kvs, MAP pm, int gpw, AppendSrc as) {
     if (qdt == ULLM_DT_F32) launch_kv<D, ULLM_DT_F32>(kvdt, g, b, st, qi, ki, vi, qb, kb, vb, qn, kn, eps, cs, neox, rd, rows, sp, nh, nkv, qo, kc, vc, kvs, pm, gpw, as);
     else if (qdt == ULLM_DT_F16) launch_kv<D, ULLM_DT_F16>(kvdt, g, b, st, qi, ki, vi, qb, kb, vb, qn, kn, eps, cs, neox, rd, rows, sp, nh, nkv, qo, kc, vc, kvs, pm, gpw, as);
     else launch_kv<D, ULLM_DT_BF16>(kvdt, g, b, st, qi, ki, vi, qb, kb, vb, qn, kn, eps, cs, neox, rd, rows, sp, nh, nkv, qo, kc, vc, kvs, pm, gpw, as);
@@ -603,6 +648,85 @@ extern "C" int ullm_hip_qkv_append_paged(const float *q_in, const float *k_in, c
         default: launch_q<256>(q_dtype, kv_dtype, grid, block, st, q_in, k_in, v_in, q_bias, k_bias, v_bias, q_norm, k_norm, eps, rope_cs, rope_neox, rotary_dim, rows, 0, n_head, n_kv_head, q_out, k_pages, v_pages, kv_stride, pm, gpw, as); break;
     }
     return check_hip(hipGetLastError(), "qkv_append_paged launch");
+}
+
+// The drafted trees' append, contiguous (tab == nullptr) and paged.
+static int append_tree(const char *fn, const float *q_in, const float *k_in, const float *v_in,
+                       const float *q_bias, const float *k_bias, const float *v_bias, const float *q_norm,
+                       const float *k_norm, float eps, const float *rope_cs, int rope_neox, int rotary_dim,
+                       int batch, TreeMap tm, int n_head, int n_kv_head, int head_dim, void *q_out, int q_dtype,
+                       void *k_cache, void *v_cache, int kv_dtype, int64_t kv_stride, void *stream) {
+    if (!dtype_ok(q_dtype) || !dtype_ok(kv_dtype))
+        return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: dtype q=%d kv=%d", fn, q_dtype, kv_dtype);
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: head_dim %d not in {64,128,256}", fn, head_dim);
+    if (batch < 0 || tm.nodes < 0 || (int64_t)batch * tm.nodes > 0x7fffffff / 4)
+        return set_error(ULLM_HIP_E_INVALID, "%s: bad batch/max_nodes", fn);
+    if (n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || (int64_t)n_head * head_dim > 0x7fffffff)
+        return set_error(ULLM_HIP_E_INVALID, "%s: bad heads", fn);
+    if (rotary_dim < 2 || rotary_dim > head_dim || (rotary_dim & 1))
+        return set_error(ULLM_HIP_E_INVALID, "%s: rotary_dim %d", fn, rotary_dim);
+    if (kv_stride < (int64_t)n_kv_head * head_dim) return set_error(ULLM_HIP_E_INVALID, "%s: kv_stride too small", fn);
+    if (tm.rope_n_pos < 1) return set_error(ULLM_HIP_E_INVALID, "%s: rope_n_pos < 1", fn);
+    if (batch == 0 || tm.nodes == 0) return ULLM_HIP_OK;
+    if (!q_in || !k_in || !v_in || !rope_cs || !q_out || !k_cache || !v_cache || !tm.len)
+        return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
+    if (q_out == (void *)q_in && q_dtype != ULLM_DT_F32)
+        return set_error(ULLM_HIP_E_INVALID, "%s: in-place q needs q_dtype f32", fn);
+    if (((uintptr_t)q_in | (uintptr_t)k_in | (uintptr_t)v_in | (uintptr_t)q_bias | (uintptr_t)k_bias |
+         (uintptr_t)v_bias | (uintptr_t)q_out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15 ||
+        kv_stride * dtype_bytes(kv_dtype) % 16 || tm.seq_stride * dtype_bytes(kv_dtype) % 16)
+        return set_error(ULLM_HIP_E_INVALID, "%s: tensors and row strides must be 16-byte aligned", fn);
+    const int rows = batch * tm.nodes;
+    const AppendSrc as{(int64_t)n_head * head_dim, (int64_t)n_kv_head * head_dim, 1, 0};
+    int gpw;
+    const dim3 grid = append_grid(rows, n_head, n_kv_head, head_dim, gpw), block(kAppendWaves * 64);
+    if (grid.y > 65535) return set_error(ULLM_HIP_E_INVALID, "%s: too many heads", fn);
+    auto go = [&](auto dc) {
+        launch_q<decltype(dc)::value>(q_dtype, kv_dtype, grid, block, (hipStream_t)stream, q_in, k_in, v_in, q_bias,
+                                      k_bias, v_bias, q_norm, k_norm, eps, rope_cs, rope_neox, rotary_dim, rows, 0,
+                                      n_head, n_kv_head, q_out, k_cache, v_cache, kv_stride, tm, gpw, as);
+    };
+    if (head_dim == 64) go(Int<64>{});
+    else if (head_dim == 128) go(Int<128>{});
+    else go(Int<256>{});
+    return check_hip(hipGetLastError(), "qkv_append_tree launch");
+}
+
+extern "C" int ullm_hip_qkv_append_tree(const float *q_in, const float *k_in, const float *v_in, const float *q_bias,
+                                        const float *k_bias, const float *v_bias, const float *q_norm,
+                                        const float *k_norm, float eps, const float *rope_cs, int rope_n_pos,
+                                        int rope_neox, int rotary_dim, int batch, int max_nodes,
+                                        const int32_t *seq_lens, const int32_t *n_nodes, const int32_t *positions,
+                                        int n_head, int n_kv_head, int head_dim, void *q_out, int q_dtype,
+                                        void *k_cache, void *v_cache, int kv_dtype, int64_t kv_stride,
+                                        int64_t seq_stride, int n_ctx, void *stream) {
+    if (n_ctx < 0 || seq_stride < 0) return set_error(ULLM_HIP_E_INVALID, "qkv_append_tree: bad n_ctx/seq_stride");
+    const TreeMap tm{seq_lens, n_nodes, positions, nullptr, max_nodes, 0, 0, 0, rope_n_pos, n_ctx,
+                     batch > 1 ? seq_stride : 0};
+    return append_tree("qkv_append_tree", q_in, k_in, v_in, q_bias, k_bias, v_bias, q_norm, k_norm, eps, rope_cs,
+                       rope_neox, rotary_dim, batch, tm, n_head, n_kv_head, head_dim, q_out, q_dtype, k_cache, v_cache,
+                       kv_dtype, kv_stride, stream);
+}
+
+extern "C" int ullm_hip_qkv_append_tree_paged(
+    const float *q_in, const float *k_in, const float *v_in, const float *q_bias, const float *k_bias,
+    const float *v_bias, const float *q_norm, const float *k_norm, float eps, const float *rope_cs, int rope_n_pos,
+    int rope_neox, int rotary_dim, int batch, int max_nodes, const int32_t *seq_lens, const int32_t *n_nodes,
+    const int32_t *positions, int n_head, int n_kv_head, int head_dim, void *q_out, int q_dtype, void *k_pages,
+    void *v_pages, int kv_dtype, int64_t kv_stride, int page_size, int n_pages, const int32_t *block_table,
+    int table_stride, void *stream) {
+    if (page_size < 1 || (page_size & (page_size - 1)))
+        return set_error(ULLM_HIP_E_INVALID, "qkv_append_tree_paged: page_size %d must be a power of two", page_size);
+    if (n_pages < 1 || table_stride < 1)
+        return set_error(ULLM_HIP_E_INVALID, "qkv_append_tree_paged: n_pages/table_stride < 1");
+    if (batch > 0 && max_nodes > 0 && !block_table)
+        return set_error(ULLM_HIP_E_INVALID, "qkv_append_tree_paged: null tensor pointer");
+    const TreeMap tm{seq_lens, n_nodes, positions, block_table, max_nodes, table_stride, __builtin_ctz(page_size),
+                     n_pages, rope_n_pos, 0, 0};
+    return append_tree("qkv_append_tree_paged", q_in, k_in, v_in, q_bias, k_bias, v_bias, q_norm, k_norm, eps, rope_cs,
+                       rope_neox, rotary_dim, batch, tm, n_head, n_kv_head, head_dim, q_out, q_dtype, k_pages, v_pages,
+                       kv_dtype, kv_stride, stream);
 }
 
 namespace ullm {

@@ -13,6 +13,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <climits>
 #include <cmath>
@@ -485,6 +486,263 @@ at::Tensor token(const Args &a) {
     return out;
 }
 
+// ---- drafted trees and the pages of a cache ----
+// Every tensor of a call on one GPU, which is made the current one for it.
+c10::Device one_gpu(std::initializer_list<const at::Tensor *> ts) {
+    need_cuda(ts);
+    std::optional<c10::Device> d;
+    for (const at::Tensor *t : ts) {
+        if (!t) continue;
+        if (d && *d != t->device()) invalid("tensors must live on one GPU");
+        d = t->device();
+    }
+    return *d;
+}
+const int32_t *i32s(const at::Tensor *t, at::IntArrayRef shape, const char *msg) {
+    if (!t) return nullptr;
+    if (t->scalar_type() != at::kInt || t->sizes() != shape || !t->is_contiguous()) invalid(msg);
+    return (const int32_t *)t->data_ptr();
+}
+const float *f32s(const at::Tensor *t, int64_t n, const char *msg) {
+    if (!t) return nullptr;
+    if (!f32_rows(*t) || t->numel() != n) invalid(msg);
+    return (const float *)t->data_ptr();
+}
+// Elements of t's memory from its first one on.
+int64_t elements_from(const at::Tensor &t) {
+    return (int64_t)t.storage().nbytes() / (int64_t)t.element_size() - t.storage_offset();
+}
+int small(int64_t v, const char *msg) {
+    if (v != (int)v) invalid(msg);
+    return (int)v;
+}
+void out_check(const at::Tensor &t, at::IntArrayRef shape, const char *msg) {
+    if (t.sizes() != shape || !t.is_contiguous()) invalid(msg);
+}
+
+at::Tensor attn_tree(const Args &a) {
+    // q k v table mask lens max_len n_kv n_nodes positions window scale kv_stride seq_stride out out_dtype ws stream
+    const at::Tensor &q = a.t(0), &k = a.t(1), &v = a.t(2), &lens = a.t(5);
+    const at::Tensor *tab = a.ot(3), *mask = a.ot(4), *nn = a.ot(8), *pos = a.ot(9), *given = a.ot(14), *gws = a.ot(16);
+    if (q.dim() != 4) raise(PyExc_ValueError, "q must be [B, nodes, n_head, head_dim]");
+    const c10::DeviceGuard on(one_gpu({&q, &k, &v, &lens, tab, mask, nn, pos, given, gws}));
+    const int B = small(q.size(0), "q: batch"), T = small(q.size(1), "q: nodes"), H = small(q.size(2), "q: n_head"),
+              D = small(q.size(3), "q: head_dim"), max_len = a.i32(6), hk = a.i32(7), win = a.window(10);
+    if (!q.is_contiguous()) invalid("q must be contiguous [B, nodes, n_head, head_dim]");
+    if (q.scalar_type() != k.scalar_type() || q.scalar_type() != v.scalar_type()) invalid("q and cache dtypes differ");
+    const int32_t *len_p = i32s(&lens, {B}, "seq_lens must be contiguous int32 [B]"),
+                  *nn_p = i32s(nn, {B}, "n_nodes must be contiguous int32 [B]"),
+                  *pos_p = i32s(pos, {B, T}, "positions must be contiguous int32 [B, nodes]");
+    if (mask && (mask->scalar_type() != at::kLong || mask->sizes() != at::IntArrayRef({B, T, (T + 63) / 64}) ||
+                 !mask->is_contiguous()))
+        invalid("mask must be contiguous int64 [B, nodes, ceil(nodes/64)]");
+    const float scale = a.none(11) ? (float)(1.0 / std::sqrt((double)D)) : (float)a.f(11);
+    int64_t kvs, ss = a.i64(13);
+    if (tab) {
+        if (k.dim() != 3 || k.sizes() != v.sizes() || !k.is_contiguous() || !v.is_contiguous())
+            invalid("k_pages/v_pages must be contiguous [n_pages, page_size, kv_stride]");
+        if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(0) != B || !tab->is_contiguous())
+            invalid("block_table must be contiguous int32 [B, table_stride]");
+        kvs = k.size(2);
+    } else {
+        kvs = a.none(12) ? (int64_t)hk * D : a.i64(12);
+        const int64_t last = B && max_len > 0 ? (B - 1) * ss + (max_len - 1) * kvs + (int64_t)hk * D : 0;
+        if (kvs < 0 || ss < 0 || last > elements_from(k) || last > elements_from(v))
+            invalid("the caches end before max_len positions of every sequence");
+    }
+    const Stream st(a, 17);
+    const at::ScalarType od = given ? given->scalar_type() : a.none(15) ? q.scalar_type() : dtype_arg(a, 15);
+    if (given) out_check(*given, q.sizes(), "out must be contiguous [B, nodes, n_head, head_dim]");
+    const at::Tensor out = out_or(given, q.sizes(), q, od);
+    const int dtype = dt(q), odt = dt(out);
+    at::Tensor ws;
+    if (gws) ws = *gws;
+    else if (const size_t need = ullm_hip_tree_workspace_bytes(dtype, B, T, max_len, win, H, hk, D))
+        ws = st.scratch(q, need);
+    void *const ws_p = ws.defined() ? ws.data_ptr() : nullptr;
+    const size_t ws_n = ws.defined() ? ws.nbytes() : 0;
+    call([&] {
+        return tab ? ullm_hip_attn_tree_paged(q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, kvs, (int)k.size(1),
+                                              (int)k.size(0), (const int32_t *)tab->data_ptr(), (int)tab->size(1),
+                                              (const int64_t *)ptr(mask), len_p, nn_p, pos_p, T, max_len, win, B, H, hk,
+                                              D, scale, out.data_ptr(), odt, ws_p, ws_n, st.s)
+                   : ullm_hip_attn_tree(q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, kvs, ss,
+                                        (const int64_t *)ptr(mask), len_p, nn_p, pos_p, T, max_len, win, B, H, hk, D,
+                                        scale, out.data_ptr(), odt, ws_p, ws_n, st.s);
+    });
+    return out;
+}
+
+at::Tensor append_tree(const Args &a) {
+    // q k v k_cache v_cache table lens n_nodes positions <Prep> q_out q_dtype kv_stride seq_stride n_ctx stream
+    const at::Tensor &q = a.t(0), &k = a.t(1), &v = a.t(2), &kc = a.t(3), &vc = a.t(4), &lens = a.t(6);
+    const at::Tensor *tab = a.ot(5), *nn = a.ot(7), *pos = a.ot(8);
+    const Prep p(a, 9);
+    constexpr int R = 9 + Prep::N;
+    const at::Tensor *given = a.ot(R);
+    const c10::DeviceGuard on(
+        one_gpu({&q, &k, &v, &kc, &vc, tab, &lens, nn, pos, &p.cs, p.qn, p.kn, p.qb, p.kb, p.vb, given}));
+    if (q.dim() != 3) raise(PyExc_ValueError, "q must be [B, nodes, n_head*head_dim]");
+    const int B = small(q.size(0), "q: batch"), T = small(q.size(1), "q: nodes");
+    const int64_t qd = (int64_t)p.H * p.D, kvd = (int64_t)p.hk * p.D;
+    f32s(&q, (int64_t)B * T * qd, "q must be contiguous f32 [B, nodes, n_head*head_dim]");
+    f32s(&k, (int64_t)B * T * kvd, "k must be contiguous f32 [B, nodes, n_kv_head*head_dim]");
+    f32s(&v, (int64_t)B * T * kvd, "v must be contiguous f32 [B, nodes, n_kv_head*head_dim]");
+    f32s(p.qb, qd, "q_bias must be f32 [n_head*head_dim]");
+    f32s(p.kb, kvd, "k_bias must be f32 [n_kv_head*head_dim]");
+    f32s(p.vb, kvd, "v_bias must be f32 [n_kv_head*head_dim]");
+    f32s(p.qn, p.D, "q_norm must be f32 [head_dim]");
+    f32s(p.kn, p.D, "k_norm must be f32 [head_dim]");
+    const int64_t n_pos = p.cs.dim() ? p.cs.size(0) : 0;
+    f32s(&p.cs, n_pos * p.rd, "rope_cs must be f32 [n_pos, rotary_dim/2, 2]");
+    const int32_t *len_p = i32s(&lens, {B}, "seq_lens must be contiguous int32 [B]"),
+                  *nn_p = i32s(nn, {B}, "n_nodes must be contiguous int32 [B]"),
+                  *pos_p = i32s(pos, {B, T}, "positions must be contiguous int32 [B, nodes]");
+    if (kc.scalar_type() != vc.scalar_type()) invalid("k and v cache dtypes differ");
+    int64_t kvs, ss = a.i64(R + 3), n_ctx = 0;
+    if (tab) {
+        if (kc.dim() != 3 || kc.sizes() != vc.sizes() || !kc.is_contiguous() || !vc.is_contiguous())
+            invalid("k_pages/v_pages must be contiguous [n_pages, page_size, kv_stride]");
+        if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(0) != B || !tab->is_contiguous())
+            invalid("block_table must be contiguous int32 [B, table_stride]");
+        kvs = kc.size(2);
+    } else {
+        kvs = a.none(R + 2) ? kvd : a.i64(R + 2);
+        if (kc.dim() < 2 && a.none(R + 4)) invalid("caches must be [..., n_ctx, kv_dim], or n_ctx given");
+        n_ctx = a.none(R + 4) ? kc.size(-2) : a.i64(R + 4);
+        const int64_t last = B && n_ctx > 0 ? (B - 1) * ss + (n_ctx - 1) * kvs + kvd : 0;
+        if (kvs < 0 || ss < 0 || last > elements_from(kc) || last > elements_from(vc))
+            invalid("the caches end before n_ctx positions of every sequence");
+    }
+    const Stream st(a, R + 5);
+    if (given) out_check(*given, {B, T, qd}, "q_out must be contiguous [B, nodes, n_head*head_dim]");
+    const at::Tensor qo = out_or(given, {B, T, qd}, q, dtype_arg(a, R + 1));
+    const int qdt = dt(qo), kd = dt(kc), ctx = small(n_ctx, "n_ctx"), np = small(n_pos, "rope_cs");
+    call([&] {
+        return tab ? ullm_hip_qkv_append_tree_paged(
+                         fptr(&q), fptr(&k), fptr(&v), fptr(p.qb), fptr(p.kb), fptr(p.vb), fptr(p.qn), fptr(p.kn),
+                         p.eps, fptr(&p.cs), np, p.neox, p.rd, B, T, len_p, nn_p, pos_p, p.H, p.hk, p.D, qo.data_ptr(),
+                         qdt, kc.data_ptr(), vc.data_ptr(), kd, kvs, (int)kc.size(1), (int)kc.size(0),
+                         (const int32_t *)tab->data_ptr(), (int)tab->size(1), st.s)
+                   : ullm_hip_qkv_append_tree(
+                         fptr(&q), fptr(&k), fptr(&v), fptr(p.qb), fptr(p.kb), fptr(p.vb), fptr(p.qn), fptr(p.kn),
+                         p.eps, fptr(&p.cs), np, p.neox, p.rd, B, T, len_p, nn_p, pos_p, p.H, p.hk, p.D, qo.data_ptr(),
+                         qdt, kc.data_ptr(), vc.data_ptr(), kd, kvs, ss, ctx, st.s);
+    });
+    return qo;
+}
+
+// The pools of one or all layers: [n_pages, page_size, kv_dim] or with a first
+// dimension of layers, rows at any stride.
+struct Pools {
+    const at::Tensor &k, &v;
+    int layers = 1, pages, page;
+    int64_t layer_stride = 0, kvs, kvd;
+    Pools(const at::Tensor &k_, const at::Tensor &v_) : k(k_), v(v_) {
+        const int64_t d = k.dim();
+        if ((d != 3 && d != 4) || k.sizes() != v.sizes() || k.strides() != v.strides() ||
+            k.scalar_type() != v.scalar_type() || k.stride(-1) != 1 || k.stride(-3) != k.size(-2) * k.stride(-2))
+            invalid("k_pages/v_pages must be [n_pages, page_size, kv_dim] or [n_layer, n_pages, page_size, kv_dim], "
+                    "alike, with pages of whole rows");
+        pages = small(k.size(-3), "n_pages"), page = small(k.size(-2), "page_size");
+        kvs = k.stride(-2), kvd = k.size(-1);
+        if (d == 4) {
+            layers = small(k.size(0), "n_layer"), layer_stride = k.stride(0);
+            if (layers > 1 && layer_stride == 0) invalid("layers must not share memory");
+        }
+    }
+};
+
+at::Tensor accept(const Args &a) {
+    // k v table path n_accept lens lens_out stream
+    const at::Tensor &k = a.t(0), &v = a.t(1), &path = a.t(3), &count = a.t(4), &lens = a.t(5);
+    const at::Tensor *tab = a.ot(2), *given = a.ot(6);
+    const c10::DeviceGuard on(one_gpu({&k, &v, tab, &path, &count, &lens, given}));
+    if (path.dim() != 2) raise(PyExc_ValueError, "path must be [B, nodes]");
+    const int B = small(path.size(0), "path: batch"), A = small(path.size(1), "path: nodes");
+    const int32_t *path_p = i32s(&path, {B, A}, "path must be contiguous int32 [B, nodes]"),
+                  *count_p = i32s(&count, {B}, "n_accept must be contiguous int32 [B]"),
+                  *len_p = i32s(&lens, {B}, "seq_lens must be contiguous int32 [B]");
+    if (given) i32s(given, {B}, "lens_out must be contiguous int32 [B]");
+    const Stream st(a, 7);
+    const at::Tensor out = out_or(given, {B}, lens, at::kInt);
+    const int kd = dt(k);
+    if (tab) {
+        const Pools p(k, v);
+        if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(0) != B || !tab->is_contiguous())
+            invalid("block_table must be contiguous int32 [B, table_stride]");
+        const int kvd = small(p.kvd, "kv_dim");
+        call([&] {
+            return ullm_hip_kv_accept_paged(k.data_ptr(), v.data_ptr(), kd, p.kvs, p.page, p.pages, kvd, p.layers,
+                                            p.layer_stride, (const int32_t *)tab->data_ptr(), (int)tab->size(1), path_p,
+                                            A, count_p, len_p, (int32_t *)out.data_ptr(), B, st.s);
+        });
+        return out;
+    }
+    // [n_ctx, kv_dim], [B, n_ctx, kv_dim] (one sequence: [n_layer, n_ctx, kv_dim]),
+    // [n_layer, B, n_ctx, kv_dim]
+    const int64_t d = k.dim();
+    const bool fits = d == 2 ? B == 1 : d == 3 ? B == 1 || k.size(0) == B : d == 4 && k.size(1) == B;
+    if (!fits || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type() ||
+        k.stride(-1) != 1)
+        invalid("caches must be [n_ctx, kv_dim], [B, n_ctx, kv_dim], [n_layer, n_ctx, kv_dim] of one sequence or "
+                "[n_layer, B, n_ctx, kv_dim], alike");
+    const bool layered = d == 4 || (d == 3 && B == 1);
+    const int layers = layered ? small(k.size(0), "n_layer") : 1;
+    const int64_t ls = layered ? k.stride(0) : 0, ss = d == 4 ? k.stride(1) : d == 3 && !layered ? k.stride(0) : 0;
+    if ((layers > 1 && !ls) || (B > 1 && !ss)) invalid("layers and sequences must not share memory");
+    const int n_ctx = small(k.size(-2), "n_ctx"), kvd = small(k.size(-1), "kv_dim");
+    call([&] {
+        return ullm_hip_kv_accept(k.data_ptr(), v.data_ptr(), kd, k.stride(-2), ss, n_ctx, kvd, layers, ls, path_p, A,
+                                  count_p, len_p, (int32_t *)out.data_ptr(), B, st.s);
+    });
+    return out;
+}
+
+PyObject *pages_update(const Args &a) {
+    // k_pages v_pages table lens parent capacity held table_stride table_out lens_out info ws stream
+    const at::Tensor &k = a.t(0), &v = a.t(1), &tab = a.t(2), &lens = a.t(3), &parent = a.t(4), &cap = a.t(5);
+    const at::Tensor *held = a.ot(6), *gt = a.ot(8), *gl = a.ot(9), *gi = a.ot(10), *gws = a.ot(11);
+    const c10::DeviceGuard on(one_gpu({&k, &v, &tab, &lens, &parent, &cap, held, gt, gl, gi, gws}));
+    const Pools p(k, v);
+    if (tab.scalar_type() != at::kInt || tab.dim() != 2 || !tab.is_contiguous())
+        invalid("block_table must be contiguous int32 [B, table_stride]");
+    const int S = small(tab.size(0), "block_table"), N = small(parent.numel(), "parent");
+    const int32_t *len_p = i32s(&lens, {S}, "seq_lens must be contiguous int32 [B]"),
+                  *par_p = i32s(&parent, {N}, "parent must be contiguous int32 [n]"),
+                  *cap_p = i32s(&cap, {N}, "capacity must be contiguous int32 [n], as parent");
+    if (held && ((held->scalar_type() != at::kBool && held->scalar_type() != at::kByte) || held->numel() != p.pages ||
+                 !held->is_contiguous()))
+        invalid("held must be bool or uint8 [n_pages]");
+    const int cols = a.none(7) ? (int)(gt && gt->dim() == 2 ? gt->size(1) : tab.size(1)) : a.i32(7);
+    if (cols < 1) invalid("table_stride < 1");
+    if (gt) i32s(gt, {N, cols}, "table_out must be contiguous int32 [n, table_stride]");
+    if (gl) i32s(gl, {N}, "lens_out must be contiguous int32 [n]");
+    if (gi) i32s(gi, {3}, "info must be contiguous int32 [3]");
+    const Stream st(a, 12);
+    const at::Tensor to = out_or(gt, {N, cols}, tab, at::kInt), lo = out_or(gl, {N}, tab, at::kInt);
+    const at::Tensor info = gi ? *gi : N ? at::empty({3}, tab.options()) : at::zeros({3}, tab.options());
+    at::Tensor ws;
+    if (gws) ws = *gws;
+    else if (const size_t need = ullm_hip_kv_pages_workspace_bytes(N, p.pages)) ws = st.scratch(tab, need);
+    void *const ws_p = ws.defined() ? ws.data_ptr() : nullptr;
+    const size_t ws_n = ws.defined() ? ws.nbytes() : 0;
+    const int kd = dt(k);
+    call([&] {
+        return ullm_hip_kv_pages_update(k.data_ptr(), v.data_ptr(), kd, p.kvs, p.page, p.pages, p.layers,
+                                        p.layer_stride, (const int32_t *)tab.data_ptr(), (int)tab.size(1), len_p, S,
+                                        par_p, cap_p, held ? (const uint8_t *)held->data_ptr() : nullptr,
+                                        (int32_t *)to.data_ptr(), cols, (int32_t *)lo.data_ptr(), N,
+                                        (int32_t *)info.data_ptr(), ws_p, ws_n, st.s);
+    });
+    PyObject *r = PyTuple_New(3);
+    if (!r) throw PyRaised{};
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(to));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lo));
+    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(info));
+    return r;
+}
+
 // ---- Python entry ----
 template <class F>
 PyObject *guard(F &&f) {
@@ -512,6 +770,10 @@ PyObject *proj_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 8 + Prep::N + 5) return PyErr_Format(PyExc_TypeError, "%zd arguments given", n), nullptr;
     return guard([&] { return proj(Args{args}); });
 }
+PyObject *pages_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments expected, %zd given", n), nullptr;
+    return guard([&] { return pages_update(Args{args}); });
+}
 PyObject *set_error(PyObject *, PyObject *cls) {
     Py_INCREF(cls);
     Py_XSETREF(g_error, cls);
@@ -529,6 +791,10 @@ PyMethodDef methods[] = {
     {"prefill", FAST((entry<prefill, 13>)), METH_FASTCALL, nullptr},
     {"prefill_paged", FAST((entry<prefill_paged, 12>)), METH_FASTCALL, nullptr},
     {"token", FAST((entry<token, 9 + Prep::N + 5>)), METH_FASTCALL, nullptr},
+    {"attn_tree", FAST((entry<attn_tree, 18>)), METH_FASTCALL, nullptr},
+    {"append_tree", FAST((entry<append_tree, 9 + Prep::N + 6>)), METH_FASTCALL, nullptr},
+    {"accept", FAST((entry<accept, 8>)), METH_FASTCALL, nullptr},
+    {"pages_update", FAST(pages_entry), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,343 @@
+// Rows and pages of a KV cache moved, shared, copied and given back:
+// ullm_hip_kv_accept(_paged) and ullm_hip_kv_pages_update.
+#include <climits>
+#include "common.hpp"
+
+namespace ullm {
+
+// ---- the accepted rows of a drafted tree ----
+// Row len + j of sequence b takes what row len + path[b][j] held, j < count[b],
+// for K and V of every layer.  A workgroup owns a slice of 16*C bytes of one
+// sequence's rows, reads all of its source rows into registers, and stores
+// after a barrier: any path is right, also one that is not increasing or names
+// a row twice.  No other workgroup touches the slice.
+struct AcceptArgs {
+    char *k, *v;
+    int64_t rb, seq_b, layer_b;  // bytes of a row, from sequence to sequence, from layer to layer
+    const int32_t *tab;          // null: contiguous, n_ctx rows
+    int tab_stride, shift, n_pages, n_ctx;
+    const int32_t *path, *count, *len;
+    int path_stride, cols;  // 16-byte columns of a row that are moved
+    int32_t *len_out;
+};
+constexpr int kAcceptT = 256, kAcceptU = 8;
+constexpr int kAcceptMax = 1024;  // nodes of a path
+
+// Byte offset of position t of sequence b, < 0 where the cache has none.
+__device__ __forceinline__ int64_t accept_row(const AcceptArgs &a, int b, int64_t t) {
+    if (t < 0) return -1;
+    if (!a.tab) return t < a.n_ctx ? b * a.seq_b + t * a.rb : -1;
+    const int64_t pg = t >> a.shift;
+    const int phys = pg < a.tab_stride ? a.tab[(int64_t)b * a.tab_stride + pg] : -1;
+    if (phys < 0 || phys >= a.n_pages) return -1;
+    return (((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1))) * a.rb;
+}
+
+// log_c: the slice is 2^log_c columns, of which kAcceptT >> log_c rows are
+// handled at a time by each of the kAcceptU loads of a thread.
+__global__ __launch_bounds__(kAcceptT) void kv_accept_kernel(AcceptArgs a, int log_c) {
+    const int tid = threadIdx.x, b = blockIdx.y;
+    const int len = a.len[b], n = min(max(a.count[b], 0), a.path_stride);
+    if (a.len_out && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) a.len_out[b] = len + n;
+    const int col = ((int)blockIdx.x << log_c) + (tid & ((1 << log_c) - 1));
+    const int r0 = tid >> log_c, step = kAcceptT >> log_c;
+    char *base = ((blockIdx.z & 1) ? a.v : a.k) + (blockIdx.z >> 1) * a.layer_b + (int64_t)col * 16;
+    u32x4 x[kAcceptU];
+    int64_t to[kAcceptU];
+#pragma unroll
+    for (int u = 0; u < kAcceptU; u++) {
+        const int j = r0 + u * step;
+        to[u] = -1;
+        if (j < n && col < a.cols) {
+            const int node = a.path[(int64_t)b * a.path_stride + j];
+            const int64_t from = node < 0 || node == j ? -1 : accept_row(a, b, (int64_t)len + node);
+            if (from >= 0) {
+                to[u] = accept_row(a, b, (int64_t)len + j);
+                x[u] = *(const u32x4 *)(base + from);
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kAcceptU; u++)
+        if (to[u] >= 0) *(u32x4 *)(base + to[u]) = x[u];
+}
+
+static bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + nb && y < x + na;
+}
+
+static int kv_accept(const char *fn, AcceptArgs a, int dtype, int64_t kv_stride, int64_t seq_stride, int kv_dim,
+                     int n_layer, int64_t layer_stride, int batch, void *stream) {
+    if (!dtype_ok(dtype)) return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: dtype %d", fn, dtype);
+    if (batch < 0 || batch > 65535 || a.path_stride < 0 || a.path_stride > kAcceptMax)
+        return set_error(ULLM_HIP_E_INVALID, "%s: batch %d not in 0..65535 or path of %d not in 0..%d", fn, batch,
+                         a.path_stride, kAcceptMax);
+    if (n_layer < 1 || n_layer > 32767 || kv_dim < 1 || kv_stride < kv_dim || seq_stride < 0 || layer_stride < 0)
+        return set_error(ULLM_HIP_E_INVALID, "%s: bad n_layer/kv_dim/strides", fn);
+    if (batch == 0) return ULLM_HIP_OK;
+    const int eb = dtype_bytes(dtype);
+    if (!a.k || !a.v || !a.count || !a.len || (!a.path && a.path_stride))
+        return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
+    if (((uintptr_t)a.k | (uintptr_t)a.v) & 15 || (int64_t)kv_dim * eb % 16 || kv_stride * eb % 16 ||
+        seq_stride * eb % 16 || layer_stride * eb % 16)
+        return set_error(ULLM_HIP_E_INVALID, "%s: caches, rows and strides must be 16-byte aligned", fn);
+    if (overlap(a.len_out, 4 * (size_t)batch, a.len, 4 * (size_t)batch) ||
+        overlap(a.len_out, 4 * (size_t)batch, a.count, 4 * (size_t)batch))
+        return set_error(ULLM_HIP_E_INVALID, "%s: lens_out overlaps seq_lens or n_accept", fn);
+    a.rb = kv_stride * eb, a.seq_b = batch > 1 ? seq_stride * eb : 0, a.layer_b = layer_stride * eb;
+    a.cols = (int)((int64_t)kv_dim * eb / 16);
+    int log_c = 8;
+    while (log_c > 0 && (1 << (log_c - 1)) >= a.cols) log_c--;
+    while (((int64_t)a.path_stride << log_c) > kAcceptT * kAcceptU) log_c--;
+    const dim3 grid((a.cols + (1 << log_c) - 1) >> log_c, batch, 2 * n_layer);
+    launch_kernel(kv_accept_kernel, grid, dim3(kAcceptT), 0, (hipStream_t)stream, a, log_c);
+    return check_hip(hipGetLastError(), "kv_accept launch");
+}
+
+// ---- the block table of the next step ----
+// Sequence s of the new table goes on from sequence parent[s] of the old one
+// (none: starts empty), keeps min(its length, capacity[s]) positions and has
+// pages for capacity[s].  Pages that kept positions fill are shared; a page
+// that they fill in part is the first such sequence's own, if it is no one's
+// whole page and not held, and copied for every other.  New pages are those
+// that nothing keeps, lowest number first.
+struct PagesArgs {
+    char *k, *v;
+    int64_t rb, layer_b;
+    const int32_t *tab, *len, *parent, *cap;
+    const uint8_t *held;
+    int32_t *tab_out, *len_out, *info;
+    int stride, n_seq, out_stride, n_out, n_pages, shift;
+    // workspace
+    int32_t *owner, *free_list, *total;  // [n_pages], [n_pages], [2]: pages free, pages asked for
+    struct PagesSeq *seq;
+};
+// What becomes of one sequence: old row, whole kept pages, kept positions of
+// the next one, pages needed, the first of its new ones, and the part-filled
+// page (-1: none) with whether it is kept as it is.
+struct PagesSeq {
+    int32_t p, full, part, need, first, last, keeps, pad;
+};
+constexpr int kPagesT = 1024;
+constexpr int kPagesMax = 1 << 20;  // pages of a pool: a bit each in LDS
+
+// Exclusive sum of v over the workgroup, and the total.
+__device__ __forceinline__ int block_scan(int v, int *tmp, int &total) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) tmp[w] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kPagesT / 64; i++) {
+        if (i < w) before += tmp[i];
+        total += tmp[i];
+    }
+    return before + x - v;
+}
+
+__global__ __launch_bounds__(kPagesT) void pages_plan_kernel(PagesArgs a) {
+    extern __shared__ uint32_t bits[];  // pages that stay: held or kept
+    __shared__ int tmp[kPagesT / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int words = (a.n_pages + 31) / 32;
+    for (int w = tid; w < words; w += kPagesT) {
+        uint32_t x = 0;
+        if (a.held)
+            for (int i = 0; i < 32 && w * 32 + i < a.n_pages; i++) x |= a.held[w * 32 + i] ? 1u << i : 0u;
+        bits[w] = x;
+    }
+    __syncthreads();
+    const int64_t room = (int64_t)a.out_stride << a.shift, had = (int64_t)a.stride << a.shift;
+    // whole pages
+    for (int s = wave; s < a.n_out; s += kPagesT / 64) {
+        const int p = a.parent[s], cap = (int)min((int64_t)max(a.cap[s], 0), room);
+        const int kept = p >= 0 && p < a.n_seq ? (int)min(min((int64_t)max(a.len[p], 0), had), (int64_t)cap) : 0;
+        const int full = kept >> a.shift, part = kept & ((1 << a.shift) - 1);
+        const int32_t *row = a.tab + (int64_t)p * a.stride;
+        for (int j = lane; j < full; j += 64) {
+            const int pg = row[j];
+            if (pg >= 0 && pg < a.n_pages) atomicOr(&bits[pg >> 5], 1u << (pg & 31));
+        }
+        if (lane == 0) {
+            int last = part ? row[full] : -1;
+            if (last < 0 || last >= a.n_pages) last = -1;
+            if (last >= 0) __hip_atomic_store(a.owner + last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            a.seq[s] = PagesSeq{p, full, part, (int)((cap + (1ll << a.shift) - 1) >> a.shift), 0, last, 0, 0};
+        }
+    }
+    __syncthreads();
+    for (int s = tid; s < a.n_out; s += kPagesT)
+        if (a.seq[s].last >= 0) atomicMin(a.owner + a.seq[s].last, s);
+    __syncthreads();
+    // who keeps its part-filled page, and the new pages of each
+    int copies = 0, asked = 0;
+    for (int s0 = 0; s0 < a.n_out; s0 += kPagesT) {
+        const int s = s0 + tid;
+        int take = 0;
+        if (s < a.n_out) {
+            const PagesSeq q = a.seq[s];
+            const bool mine = q.last >= 0 && !(bits[q.last >> 5] >> (q.last & 31) & 1) &&
+                              __hip_atomic_load(a.owner + q.last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == s;
+            a.seq[s].keeps = mine;
+            take = q.need - q.full - mine;
+        }
+        int total;
+        const int first = block_scan(take, tmp, total);
+        if (s < a.n_out) a.seq[s].first = asked + first;
+        asked += total;
+    }
+    __syncthreads();
+    for (int s = tid; s < a.n_out; s += kPagesT) {
+        const int last = a.seq[s].last;
+        if (last >= 0) atomicOr(&bits[last >> 5], 1u << (last & 31));
+    }
+    __syncthreads();
+    // the free pages in order, as many as are asked for
+    const int per = (words + kPagesT - 1) / kPagesT, w0 = tid * per, w1 = min(w0 + per, words);
+    int mine = 0, n_free;
+    for (int w = w0; w < w1; w++) {
+        const uint32_t there = w * 32 + 32 <= a.n_pages ? ~0u : (1u << (a.n_pages & 31)) - 1;
+        mine += __popc(~bits[w] & there);
+    }
+    int rank = block_scan(mine, tmp, n_free);
+    for (int w = w0; w < w1 && rank < asked; w++) {
+        const uint32_t there = w * 32 + 32 <= a.n_pages ? ~0u : (1u << (a.n_pages & 31)) - 1;
+        for (uint32_t f = ~bits[w] & there; f && rank < asked; f &= f - 1)
+            a.free_list[rank++] = w * 32 + __builtin_ctz(f);
+    }
+    // the new lengths: a part-filled page that should have been copied and could not is lost
+    for (int s = tid; s < a.n_out; s += kPagesT) {
+        const PagesSeq q = a.seq[s];
+        const bool copy = q.last >= 0 && !q.keeps, lost = copy && q.first >= n_free;
+        copies += copy && !lost;
+        a.len_out[s] = (q.full << a.shift) + (lost ? 0 : q.part);
+    }
+    int n_copies;
+    block_scan(copies, tmp, n_copies);
+    if (tid == 0) {
+        a.total[0] = n_free;
+        a.info[0] = n_copies;
+        a.info[1] = min(asked, n_free);
+        a.info[2] = max(asked - n_free, 0);
+    }
+}
+
+// Rows of the new table (blockIdx.z == 0), and the copies of part-filled pages
+// in K and V of every layer.
+__global__ __launch_bounds__(256) void pages_apply_kernel(PagesArgs a) {
+    const int s = blockIdx.y, tid = threadIdx.x, n_free = a.total[0];
+    const PagesSeq q = a.seq[s];
+    if (blockIdx.z == 0) {
+        for (int j = blockIdx.x * 256 + tid; j < a.out_stride; j += gridDim.x * 256) {
+            int pg = -1;
+            if (j < q.full) {
+                pg = a.tab[(int64_t)q.p * a.stride + j];
+                if (pg < 0 || pg >= a.n_pages) pg = -1;
+            } else if (j == q.full && q.keeps) {
+                pg = q.last;
+            } else if (j < q.need) {
+                const int nth = q.first + j - q.full - q.keeps;
+                if (nth < n_free) pg = a.free_list[nth];
+            }
+            a.tab_out[(int64_t)s * a.out_stride + j] = pg;
+        }
+        return;
+    }
+    if (q.last < 0 || q.keeps || q.first >= n_free) return;
+    const int z = blockIdx.z - 1;
+    char *base = ((z & 1) ? a.v : a.k) + (z >> 1) * a.layer_b;
+    const char *src = base + ((int64_t)q.last << a.shift) * a.rb;
+    char *dst = base + ((int64_t)a.free_list[q.first] << a.shift) * a.rb;
+    const int64_t n16 = q.part * a.rb / 16;
+    for (int64_t i = blockIdx.x * 256 + tid; i < n16; i += gridDim.x * 256)
+        *(u32x4 *)(dst + i * 16) = *(const u32x4 *)(src + i * 16);
+}
+
+static size_t pages_ws(int n_out, int n_pages) {
+    return 256 + (size_t)n_out * sizeof(PagesSeq) + 8 * (size_t)n_pages;
+}
+
+}  // namespace ullm
+
+using namespace ullm;
+
+extern "C" int ullm_hip_kv_accept(void *k_cache, void *v_cache, int dtype, int64_t kv_stride, int64_t seq_stride,
+                                  int n_ctx, int kv_dim, int n_layer, int64_t layer_stride, const int32_t *path,
+                                  int path_stride, const int32_t *n_accept, const int32_t *seq_lens,
+                                  int32_t *lens_out, int batch, void *stream) {
+    if (n_ctx < 0) return set_error(ULLM_HIP_E_INVALID, "kv_accept: n_ctx < 0");
+    const AcceptArgs a{(char *)k_cache, (char *)v_cache, 0, 0, 0, nullptr, 0, 0, 0, n_ctx,
+                       path, n_accept, seq_lens, path_stride, 0, lens_out};
+    return kv_accept("kv_accept", a, dtype, kv_stride, seq_stride, kv_dim, n_layer, layer_stride, batch, stream);
+}
+
+extern "C" int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype, int64_t kv_stride, int page_size,
+                                        int n_pages, int kv_dim, int n_layer, int64_t layer_stride,
+                                        const int32_t *block_table, int table_stride, const int32_t *path,
+                                        int path_stride, const int32_t *n_accept, const int32_t *seq_lens,
+                                        int32_t *lens_out, int batch, void *stream) {
+    if (page_size < 1 || (page_size & (page_size - 1)))
+        return set_error(ULLM_HIP_E_INVALID, "kv_accept_paged: page_size %d must be a power of two", page_size);
+    if (n_pages < 1 || table_stride < 1 || (batch > 0 && !block_table))
+        return set_error(ULLM_HIP_E_INVALID, "kv_accept_paged: bad n_pages/block_table");
+    const AcceptArgs a{(char *)k_pages, (char *)v_pages, 0, 0, 0, block_table, table_stride, __builtin_ctz(page_size),
+                       n_pages, 0, path, n_accept, seq_lens, path_stride, 0, lens_out};
+    return kv_accept("kv_accept_paged", a, dtype, kv_stride, 0, kv_dim, n_layer, layer_stride, batch, stream);
+}
+
+extern "C" size_t ullm_hip_kv_pages_workspace_bytes(int n_out, int n_pages) {
+    return n_out < 1 || n_pages < 1 ? 0 : pages_ws(n_out, n_pages);
+}
+
+extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride, int page_size,
+                                        int n_pages, int n_layer, int64_t layer_stride, const int32_t *block_table,
+                                        int table_stride, const int32_t *seq_lens, int n_seq, const int32_t *parent,
+                                        const int32_t *capacity, const uint8_t *held, int32_t *table_out,
+                                        int out_stride, int32_t *lens_out, int n_out, int32_t *info, void *workspace,
+                                        size_t workspace_bytes, void *stream) {
+    const char *fn = "kv_pages_update";
+    if (!dtype_ok(dtype)) return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: dtype %d", fn, dtype);
+    if (page_size < 1 || (page_size & (page_size - 1)))
+        return set_error(ULLM_HIP_E_INVALID, "%s: page_size %d must be a power of two", fn, page_size);
+    if (n_pages < 1 || n_pages > kPagesMax)
+        return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: n_pages %d not in 1..%d", fn, n_pages, kPagesMax);
+    if (n_seq < 0 || n_out < 0 || n_out > 65535 || table_stride < 1 || out_stride < 1 || n_layer < 0 ||
+        n_layer > 32767 || kv_stride < 1 || layer_stride < 0)
+        return set_error(ULLM_HIP_E_INVALID, "%s: bad sizes", fn);
+    if ((int64_t)page_size * table_stride > INT_MAX || (int64_t)page_size * out_stride > INT_MAX)
+        return set_error(ULLM_HIP_E_INVALID, "%s: a table of 2^31 positions or more", fn);
+    if (n_out == 0) return ULLM_HIP_OK;
+    if ((n_layer && (!k_pages || !v_pages)) || (n_seq && (!block_table || !seq_lens)) || !parent || !capacity ||
+        !table_out || !lens_out || !info)
+        return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
+    const int eb = dtype_bytes(dtype);
+    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || kv_stride * eb % 16 || layer_stride * eb % 16)
+        return set_error(ULLM_HIP_E_INVALID, "%s: pools and strides must be 16-byte aligned", fn);
+    const size_t nt = 4 * (size_t)n_out * out_stride, ot = 4 * (size_t)n_seq * table_stride;
+    if (overlap(table_out, nt, block_table, ot) || overlap(lens_out, 4 * (size_t)n_out, block_table, ot))
+        return set_error(ULLM_HIP_E_INVALID, "%s: the new table or lengths overlap the old table", fn);
+    const size_t need = pages_ws(n_out, n_pages);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255)
+        return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, need);
+    char *ws = (char *)workspace;
+    PagesArgs a{(char *)k_pages, (char *)v_pages, kv_stride * eb, layer_stride * eb, block_table, seq_lens, parent,
+                capacity, held, table_out, lens_out, info, table_stride, n_seq, out_stride, n_out, n_pages,
+                __builtin_ctz(page_size), nullptr, nullptr, (int32_t *)ws, (PagesSeq *)(ws + 256)};
+    a.owner = (int32_t *)(ws + 256 + (size_t)n_out * sizeof(PagesSeq));
+    a.free_list = a.owner + n_pages;
+    hipStream_t st = (hipStream_t)stream;
+    launch_kernel(pages_plan_kernel, dim3(1), dim3(kPagesT), (size_t)(n_pages + 31) / 32 * 4, st, a);
+    if (int rc = check_hip(hipGetLastError(), "kv_pages_update launch")) return rc;
+    launch_kernel(pages_apply_kernel, dim3(8, n_out, 1 + 2 * n_layer), dim3(256), 0, st, a);
+    return check_hip(hipGetLastError(), "kv_pages_update launch");
+}
