@@ -600,6 +600,7 @@ def test_serving_loop(dev):
     (dict(n=lambda x: x.float()), L.E_INVALID), (dict(pos=lambda x: x[:, :2]), L.E_INVALID),
     (dict(out=lambda x: x.double()), L.E_UNSUPPORTED), (dict(out=lambda x: x[:, :2]), L.E_INVALID),
     (dict(out=lambda x: x.bfloat16()), L.E_UNSUPPORTED), (dict(pos=lambda x: None), L.E_INVALID),
+    (dict(ws=lambda x: x[:8]), L.E_WORKSPACE), (dict(ws=lambda x: x[1:]), L.E_WORKSPACE),
 ])
 def test_refusals(dev, change, code):
     a = dict(q=torch.zeros(1, 5, 4, 64, device=dev, dtype=torch.float16), k=torch.zeros(1, 4096, 128, device=dev, dtype=torch.float16),
