@@ -120,7 +120,7 @@ struct PagesArgs {
 struct PagesSeq {
     int32_t p, full, part, need, first, last, keeps, pad;
 };
-constexpr int kPagesT = 1024;
+constexpr int kPagesT = 1024, kPagesU = 8;
 constexpr int kPagesMax = 1 << 20;  // pages of a pool: a bit each in LDS
 
 // Exclusive sum of v over the workgroup, and the total.
@@ -150,34 +150,42 @@ __global__ __launch_bounds__(kPagesT) void pages_plan_kernel(PagesArgs a) {
     __shared__ int tmp[kPagesT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int words = (a.n_pages + 31) / 32;
-    for (int w = tid; w < words; w += kPagesT) {
-        uint32_t x = 0;
-        if (a.held)
-            for (int i = 0; i < 32 && w * 32 + i < a.n_pages; i++) x |= a.held[w * 32 + i] ? 1u << i : 0u;
-        bits[w] = x;
+    if (a.held) {  // 64 pages a load of a wave
+        for (int c = wave; c * 64 < a.n_pages; c += kPagesT / 64) {
+            const int pg = c * 64 + lane;
+            const uint64_t m = __ballot(pg < a.n_pages && a.held[pg]);
+            if (lane < 2 && 2 * c + lane < words) bits[2 * c + lane] = (uint32_t)(m >> (32 * lane));
+        }
+    } else {
+        for (int w = tid; w < words; w += kPagesT) bits[w] = 0;
     }
     __syncthreads();
     const int64_t room = (int64_t)a.out_stride << a.shift, had = (int64_t)a.stride << a.shift;
-    // whole pages
-    for (int s = wave; s < a.n_out; s += kPagesT / 64) {
+    for (int s = tid; s < a.n_out; s += kPagesT) {
         const int p = a.parent[s], cap = (int)min((int64_t)max(a.cap[s], 0), room);
         const int kept = p >= 0 && p < a.n_seq ? (int)min(min((int64_t)max(a.len[p], 0), had), (int64_t)cap) : 0;
         const int full = kept >> a.shift, part = kept & ((1 << a.shift) - 1);
-        const int32_t *row = a.tab + (int64_t)p * a.stride;
-        for (int j = lane; j < full; j += 64) {
-            const int pg = row[j];
-            if (pg >= 0 && pg < a.n_pages) atomicOr(&bits[pg >> 5], 1u << (pg & 31));
-        }
-        if (lane == 0) {
-            int last = part ? row[full] : -1;
-            if (last < 0 || last >= a.n_pages) last = -1;
-            if (last >= 0) __hip_atomic_store(a.owner + last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            a.seq[s] = PagesSeq{p, full, part, (int)((cap + (1ll << a.shift) - 1) >> a.shift), 0, last, 0, 0};
-        }
+        int last = part ? a.tab[(int64_t)p * a.stride + full] : -1;
+        if (last < 0 || last >= a.n_pages) last = -1;
+        if (last >= 0) __hip_atomic_store(a.owner + last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        a.seq[s] = PagesSeq{p, full, part, (int)((cap + (1ll << a.shift) - 1) >> a.shift), 0, last, 0, 0};
     }
     __syncthreads();
     for (int s = tid; s < a.n_out; s += kPagesT)
         if (a.seq[s].last >= 0) atomicMin(a.owner + a.seq[s].last, s);
+    // whole pages: a wave takes a sequence, kPagesU loads of 64 entries in flight
+    for (int s = wave; s < a.n_out; s += kPagesT / 64) {
+        const PagesSeq q = a.seq[s];
+        const int32_t *row = a.tab + (int64_t)q.p * a.stride;
+        for (int j0 = 0; j0 < q.full; j0 += 64 * kPagesU) {
+            int pg[kPagesU];
+#pragma unroll
+            for (int u = 0; u < kPagesU; u++) pg[u] = j0 + u * 64 + lane < q.full ? row[j0 + u * 64 + lane] : -1;
+#pragma unroll
+            for (int u = 0; u < kPagesU; u++)
+                if (pg[u] >= 0 && pg[u] < a.n_pages) atomicOr(&bits[pg[u] >> 5], 1u << (pg[u] & 31));
+        }
+    }
     __syncthreads();
     // who keeps its part-filled page, and the new pages of each
     int copies = 0, asked = 0;

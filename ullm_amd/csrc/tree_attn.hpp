@@ -1,0 +1,813 @@
+#pragma once
+// Attention of a batch of drafted trees over the cache that holds their
+// sequences (ullm_hip_attn_tree, ullm_hip_attn_tree_paged).
+//
+// Node i of sequence b, at position p_i, sees keys t < len_b (the sequence's
+// own; with a window W those with t > p_i - W) and of the keys len_b + j the
+// nodes j whose bit its mask has (p_j > p_i - W):
+//   out[b,i,h] = sum_t softmax_t(scale * q[b,i,h] . K[t]) V[t]
+// over those, and zeros where there is none or i >= n_b.
+//
+// One pass over the keys with a running maximum and sum.  The rows of a kv head
+// are its nodes times the G query heads that share it, row r = node r / G, head
+// r % G; all of them see the same keys but for the mask, so K and V are read
+// once for as many rows as a workgroup holds.
+//  * S^T[16 keys x 16 rows] = K . Q^T and O^T[16 d x 16 rows] += V^T . P^T run
+//    on 16x16 matrix instructions.  A lane's column is one row in both, so a
+//    row's maximum, sum and rescale live in the four lanes that own its output,
+//    and P^T is the S^T accumulator exponentiated: P never moves between lanes.
+//    16-bit caches: 16x16x32, K by 16-byte LDS reads, V^T by the transposing
+//    LDS read.  f32: 16x16x4 products of f32, K and V by 16-byte reads, the four
+//    elements of a read being four k-steps (K) or four d tiles (V).
+//  * K and V tiles come by LDS DMA into a ring, one 32-key block a page lookup.
+//  * A workgroup is WR x WK waves of 16*NR rows: the WR waves of a key group
+//    share its tiles, the WK key groups take tiles in turn and are added up
+//    through LDS at the end.
+//  * The keys of a sequence are cut into parts, one workgroup each, so that the
+//    workgroups of all sequences are alike whatever their lengths; the lengths
+//    are on the device, so every workgroup works the cut out for itself
+//    (find_part).  tree_merge_kernel adds the parts up.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <type_traits>
+#include "common.hpp"
+#include "mfma_util.hpp"
+#include "wave.hpp"
+
+namespace ullm {
+
+// The keys of a call: row t of sequence b is b*seq_b + t*rb bytes into the
+// cache, or slot t % P of page tab[b*tab_stride + t / P] (P = 2^shift).
+struct TreeKv {
+    const char *k, *v;
+    int64_t rb, seq_b;
+    const int32_t *tab;
+    int tab_stride, shift, n_pages;
+};
+struct TreeArgs {
+    const void *q;
+    const uint32_t *mask;  // words of 32 nodes; null: node i sees the nodes up to i
+    const int32_t *len, *n, *pos;
+    int nodes, words, max_len, window, n_head, kv_mul;
+    float qs;   // |scale| * log2(e)
+    int neg;    // scale < 0: q enters with its sign turned
+    void *out;
+};
+// The cut of a call: slots of work along the keys (slots == batch: sequences
+// are not cut), row tiles of a kv head, blocks that a part has at least, and
+// the scratch for (m, l) and O of each slot, kv head, row tile and row.
+struct TreePlan {
+    int batch, slots, row_tiles, n_kv, least;
+    float *o;
+    float2 *ml;
+    int2 *seq;  // first slot and parts of each sequence
+};
+
+// One sequence: keys [lo, end) in blocks of 32 from block lo / 32 on.
+struct TreeSeq {
+    int n, len, end, lo, blocks;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
+    TreeSeq s;
+    s.n = a.n ? min(max(a.n[b], 0), a.nodes) : a.nodes;
+    s.len = min(max(a.len[b], 0), a.max_len);
+    s.end = min(s.len + s.n, a.max_len);
+    s.lo = a.window > 0 ? max(s.len - a.window + 1, 0) : 0;
+    s.blocks = s.n > 0 && s.end > s.lo ? (s.end + 31) / 32 - s.lo / 32 : 0;
+    return s;
+}
+
+__device__ __forceinline__ int wave_isum(int x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// Which sequence and part of it slot `slot` is: parts are of at most `per`
+// blocks, the least for which all sequences' parts fit the slots (to within a
+// sixteenth).  Every wave finds the same; at most 256 sequences are cut.
+struct TreePart {
+    int b, part, parts, slot0;
+};
+__device__ __forceinline__ TreePart find_part(const TreeArgs &a, const TreePlan &pl, int slot) {
+    const int lane = threadIdx.x & 63;
+    int nb[4], total = 0;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const int b = c * 64 + lane;
+        nb[c] = b < pl.batch ? tree_seq(a, b).blocks : 0;
+        total += nb[c];
+    }
+    total = wave_isum(total);
+    int per = max((total + pl.slots - 1) / pl.slots, pl.least), parts[4];
+    for (;;) {
+        int sum = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            parts[c] = 0;
+            if (c * 64 < pl.batch) parts[c] = c * 64 + lane < pl.batch ? max((nb[c] + per - 1) / per, 1) : 0;
+            sum += parts[c];
+        }
+        if (wave_isum(sum) <= pl.slots) break;
+        per += per / 16 + 1;  // ends: with per >= every nb there are `batch` parts
+    }
+    TreePart r{-1, 0, 0, 0};
+    int before = 0;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        if (c * 64 >= pl.batch) break;
+        int x = parts[c];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        const uint64_t at = __ballot(slot >= before + x - parts[c] && slot < before + x);
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            r.b = c * 64 + l;
+            r.parts = __shfl(parts[c], l);
+            r.slot0 = before + __shfl(x, l) - r.parts;
+            r.part = slot - r.slot0;
+        }
+        before += __shfl(x, 63);
+    }
+    return r;
+}
+
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A K tile's 16-byte chunk c of row r sits in slot c ^ tree_kswz(r), a V tile's
+// in c ^ tree_vswz(r) (prefill16.hip has the rates): conflict-free for the K
+// reads (16 rows, one chunk) and the transposing V reads (4 rows, two chunks).
+// f32 V tiles are read a contiguous row at a time and stay plain.
+template <class T, int D>
+__device__ __forceinline__ int tree_kswz(int r) {
+    return D * T::bytes >= 256 ? r & 15 : r & 7;
+}
+template <class T, int D>
+__device__ __forceinline__ int tree_vswz(int r) {
+    if constexpr (__is_same(T, F32)) return 0;
+    return D * T::bytes >= 256 ? ((r & 7) << 1) | ((r >> 3) & 1) : r & 7;
+}
+
+// Whether a 16-byte piece holds an infinity or a NaN.
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(const u32x4 &x) {
+    constexpr uint32_t m = __is_same(T, F32) ? 0x7fffffffu : 0x7fff7fffu;
+    constexpr uint32_t one = __is_same(T, F32) ? 0x00800000u : __is_same(T, F16) ? 0x04000400u : 0x00800080u;
+    constexpr uint32_t top = __is_same(T, F32) ? 0x80000000u : 0x80008000u;
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r |= (x[i] & m) + one;
+    return r & top;
+}
+
+template <int WK, int STAGE>
+constexpr int tree_stages() {
+    constexpr int n = 160 * 1024 / (WK * STAGE);
+    return n > 4 ? 4 : n;
+}
+
+template <class T, int D, int NR, int WR, int WK, int PB>
+__global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
+    constexpr bool F = __is_same(T, F32);
+    constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
+    constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
+    constexpr int TILE = KB * RB, STAGE = 2 * TILE, NST = tree_stages<WK, STAGE>();
+    constexpr int NI = TILE / 1024 / WR;  // DMA instructions of a wave for K, and for V
+    constexpr int NS = F ? D / 16 : D / 32;  // 16-byte reads of a K row by a lane
+    constexpr int NDT = D / 16;              // 16-wide d tiles of O^T
+    constexpr int ROWS = 16 * NR * WR, NT = 64 * WR * WK;
+    static_assert(NST >= 2 && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
+    constexpr int SMO = ROWS * (D + 4) * 4, SM = WK > 1 ? WK * (SMO + ROWS * 8) : 0;
+    constexpr int LDS = WK * NST * STAGE > SM ? WK * NST * STAGE : SM;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) char lds[LDS];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    const int n16 = lane & 15, kg = lane >> 4;
+    const int wr = wave % WR, wk = wave / WR;
+    // Work items (slot, kv head, row tile), the row tiles of one K/V range next
+    // to each other on one XCD (workgroups are dealt to the 8 XCDs in turn).
+    const int units = pl.n_kv * pl.row_tiles;
+    const int item = (int)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int slot = item / units, unit = item - slot * units;
+    if (slot >= pl.slots) return;
+    const int kvh = unit / pl.row_tiles, rt = unit - kvh * pl.row_tiles;
+    TreePart pt{slot, 0, 1, slot};
+    if (pl.slots > pl.batch) pt = find_part(a, pl, slot);
+    const int b = uni(pt.b), part = uni(pt.part), parts = uni(pt.parts);
+    if (b < 0) return;
+    if (pl.slots > pl.batch && part == 0 && unit == 0 && tid == 0) pl.seq[b] = int2{pt.slot0, parts};
+    const TreeSeq sq = tree_seq(a, b);
+    const int n = uni(sq.n), len = uni(sq.len), end = uni(sq.end);
+    const int G = a.kv_mul, rows = n * G, row0 = rt * ROWS;
+    const int64_t node_ld = (int64_t)a.n_head * D;  // elements of one node's heads
+    const int64_t out0 = (int64_t)b * a.nodes * node_ld + (int64_t)kvh * G * D;
+    auto out_at = [&](int r) { return out0 + r / G * node_ld + (int64_t)(r % G) * D; };
+    constexpr int ODT = PB == 1 && !F ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
+    auto store4 = [&](int64_t at, const f32x4 &o) {
+        if constexpr (ODT == ULLM_DT_F32) *(f32x4 *)((float *)a.out + at) = o;
+        else *(u32x2 *)((uint16_t *)a.out + at) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
+    };
+    if (part == 0) {  // rows of nodes that are not there
+        const int r0 = max(rows, row0), r1 = min(a.nodes * G, row0 + ROWS);
+        for (int i = tid; i < (r1 - r0) * (D / 4); i += NT) store4(out_at(r0 + i / (D / 4)) + i % (D / 4) * 4, f32x4{});
+    }
+    if (row0 >= rows) return;
+
+    // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
+    constexpr int BPT = KB / 32;
+    const int first = uni(sq.lo) / 32, size = ((sq.blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
+    const int blk0 = first + part * size, blk1 = min(blk0 + size, first + uni(sq.blocks));
+    const int tiles = max(blk1 - blk0 + BPT - 1, 0) / BPT;
+    const int steps = (tiles + WK - 1) / WK;
+
+    // ---- K/V DMA: instruction i of this wave writes RPI rows of the tile from
+    // row (wr*NI + i)*RPI on, lane -> (row, slot) ----
+    const int rb = (int)kv.rb;
+    const int drow = lane / SLOTS, dslot = lane % SLOTS;
+    constexpr int SUB = KB / WR < 32 ? 1 : KB / WR / 32;  // (a wave's rows lie in one block)
+    static_assert(SUB == 1, "rows of a wave in one block");
+    const int wblk = wr * (KB / WR) / 32;         // that block of the tile
+    const int wrow = wr * (KB / WR) - wblk * 32;  // and its first row there
+    int kofs[NI], vofs[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int r = wrow + i * RPI + drow;  // in the block; the swizzles go by r % 16
+        kofs[i] = r * rb + ((dslot ^ tree_kswz<T, D>(r)) * 16);
+        vofs[i] = r * rb + ((dslot ^ tree_vswz<T, D>(r)) * 16);
+    }
+    char *const ring = lds + wk * NST * STAGE;
+    // Pages of 128 page numbers from pg0 on, in two registers.
+    int pg0 = INT_MIN, pgv[2] = {0, 0};
+    auto issue = [&](int j) {  // step j's tile into stage j % NST
+        const int key0 = (blk0 + (j * WK + wk) * BPT + wblk) * 32;
+        const int valid = j * WK + wk < tiles ? min(end - key0, 32) : 0;
+        int64_t at;
+        bool ok = valid > 0;
+        if (kv.tab) {
+            const int pi = key0 >> kv.shift;
+            if (ok && (pi < pg0 || pi >= pg0 + 128)) {
+                pg0 = pi;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int p = pi + c * 64 + lane;
+                    pgv[c] = p < kv.tab_stride ? kv.tab[(int64_t)b * kv.tab_stride + p] : -1;
+                }
+            }
+            const int o = ok ? pi - pg0 : 0;
+            const int phys = __builtin_amdgcn_readlane(o < 64 ? pgv[0] : pgv[1], o & 63);
+            ok = ok && phys >= 0 && phys < kv.n_pages;
+            at = (((int64_t)phys << kv.shift) + (key0 & ((1 << kv.shift) - 1))) * kv.rb;
+        } else {
+            at = b * kv.seq_b + (int64_t)key0 * kv.rb;
+        }
+        at = ok ? at + (int64_t)kvh * RB : 0;
+        const int range = ok ? (valid - 1) * rb + RB : 0;  // rows from `end` on read as zeros
+        const auto kr = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(kv.k + at), 0, range, kRsrcWord3);
+        const auto vr = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(kv.v + at), 0, range, kRsrcWord3);
+        char *st = ring + j % NST * STAGE + wr * NI * 1024;
+#pragma unroll
+        for (int i = 0; i < NI; i++) dma16_cached(kr, st + i * 1024, kofs[i], 0);
+#pragma unroll
+        for (int i = 0; i < NI; i++) dma16_cached(vr, st + TILE + i * 1024, vofs[i], 0);
+    };
+
+    // ---- this wave's rows: Q^T operands, node, position ----
+    u32x4 q[NR][NS];
+    int node[NR], pos[NR];
+#pragma unroll
+    for (int x = 0; x < NR; x++) {
+        const int r = row0 + (wr * NR + x) * 16 + n16;
+        const bool ok = r < rows;
+        node[x] = ok ? r / G : -1;
+        pos[x] = 0;
+        if (a.window > 0 && ok)
+            pos[x] = a.pos ? max(a.pos[(int64_t)b * a.nodes + node[x]], len) : len + node[x];
+        const char *qp = (const char *)a.q + (ok ? out_at(r) : out0) * EB + kg * 16;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            q[x][s] = ok ? *(const u32x4 *)(qp + s * 64) : u32x4{};
+            if (a.neg) q[x][s] ^= F ? 0x80000000u : 0x80008000u;
+        }
+    }
+
+    f32x4 oacc[NR][NDT];
+    float m_run[NR], l_part[NR];
+#pragma unroll
+    for (int x = 0; x < NR; x++) {
+        m_run[x] = -INFINITY, l_part[x] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NDT; i++) oacc[x][i] = f32x4{};
+    }
+    // Per-lane operand addresses within a tile.
+    constexpr int NKA = RB >= 256 ? 4 : 2;  // chunks 16.. of a row sit 256 bytes on
+    uint32_t ka[NKA];
+#pragma unroll
+    for (int s = 0; s < NKA; s++) ka[s] = n16 * RB + (((4 * s + kg) ^ tree_kswz<T, D>(n16)) * 16);
+    constexpr int NVA = F ? 1 : RB >= 256 ? 8 : 4;
+    uint32_t va[NVA];
+    if constexpr (F) {
+        va[0] = TILE + kg * 4 * RB + n16 * 16;
+    } else {
+        const int r = kg * 4 + (n16 >> 2);
+#pragma unroll
+        for (int d = 0; d < NVA; d++)
+            va[d] = TILE + r * RB + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<T, D>(r)) * 16) + 8 * (n16 & 1);
+    }
+    // Column of element i of O tile t.
+    auto col = [&](int t, int i) { return F ? (t >> 2) * 64 + 16 * kg + 4 * i + (t & 3) : t * 16 + kg * 4 + i; };
+
+    // Which keys of block key0 row x sees, bit c being key key0 + c.
+    auto sees = [&](int x, int key0) -> uint32_t {
+        if (node[x] < 0) return 0;
+        const int own = len - key0;  // keys of the sequence in the block
+        uint32_t s = own >= 32 ? ~0u : own > 0 ? (1u << own) - 1 : 0u;
+        const int j0 = -own, i = node[x];  // node of the block's first key, if there
+        if (own < 32) {
+            uint32_t t;
+            if (!a.mask) {
+                const int c = i - j0;  // bits 0..c
+                t = c >= 31 ? ~0u : c >= 0 ? (2u << c) - 1 : 0u;
+            } else {
+                const uint32_t *w = a.mask + ((int64_t)b * a.nodes + i) * a.words;
+                if (j0 < 0) {
+                    t = w[0] << -j0;
+                } else {
+                    const uint32_t w0 = w[j0 >> 5], w1 = (j0 >> 5) + 1 < a.words ? w[(j0 >> 5) + 1] : 0;
+                    t = (uint32_t)((((uint64_t)w1 << 32) | w0) >> (j0 & 31));
+                }
+            }
+            s |= t & ~(own > 0 ? (1u << own) - 1 : 0u);
+            const int left = end - key0;  // keys that are there
+            if (left < 32) s &= left > 0 ? (1u << left) - 1 : 0u;
+        }
+        if (a.window > 0) {
+            const int64_t lo = (int64_t)pos[x] - a.window + 1 - key0;  // first key position, from the block's
+            if (own > 0 && lo > 0) {
+                const uint32_t mine = own >= 32 ? ~0u : (1u << own) - 1;
+                s &= ~(mine & (lo >= 32 ? ~0u : (1u << lo) - 1));
+            }
+            if (own < 32)
+                for (int c = max(own, 0); c < 32 && key0 + c < end; c++) {
+                    const int p = a.pos ? max(a.pos[(int64_t)b * a.nodes + c + j0], len) : key0 + c;
+                    if ((int64_t)p <= (int64_t)pos[x] - a.window) s &= ~(1u << c);
+                }
+        }
+        return s;
+    };
+    // Blocks from `clear0` up to `clear1` hold keys that every row sees.
+    int clear0 = 0;
+    if (a.window > 0) {
+        int most = INT_MIN;
+#pragma unroll
+        for (int x = 0; x < NR; x++) most = max(most, node[x] < 0 ? INT_MIN : pos[x]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
+        clear0 = uni(most) == INT_MIN ? 0 : max(uni(most) - a.window + 1, 0);
+    }
+    const int clear1 = len;
+
+    constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
+    auto block = [&](uint32_t sb, int key0) {
+        // ---- S^T: two tiles of 16 keys ----
+        f32x4 sacc[NR][2];
+#pragma unroll
+        for (int x = 0; x < NR; x++) sacc[x][0] = sacc[x][1] = f32x4{};
+        uint32_t kaddr[NKA];
+#pragma unroll
+        for (int s = 0; s < NKA; s++) kaddr[s] = sb + ka[s];
+        constexpr int CH = NS < 4 ? NS : 4, NB = 2 * NS / CH;  // reads of a batch, batches
+        u32x4 kb[2][CH];
+        auto rdk = [&](auto bc, u32x4 (&r)[CH]) {
+            static_for<0, CH>([&](auto ic) {
+                constexpr int idx = decltype(bc)::value * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
+                constexpr int c = NKA == 4 ? s & 3 : s & 1, off = NKA == 4 ? (s >> 2) * 256 : 0;
+                r[decltype(ic)::value] = lds_read_b128_at<off + t * 16 * RB>(kaddr[c]);
+            });
+        };
+        rdk(Int<0>{}, kb[0]);
+        static_for<0, NB>([&](auto bc) {
+            constexpr int B = decltype(bc)::value;
+            if constexpr (B + 1 < NB) {
+                rdk(Int<B + 1>{}, kb[(B + 1) & 1]);
+                lds_wait_n<CH>();
+            } else {
+                lds_wait_n<0>();
+            }
+            static_for<0, CH>([&](auto ic) {
+                constexpr int idx = B * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
+                u32x4 &k = kb[B & 1][decltype(ic)::value];
+                tie(k);
+#pragma unroll
+                for (int x = 0; x < NR; x++) {
+                    if constexpr (F) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            sacc[x][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[x][s][e]),
+                                                                              sacc[x][t], 0, 0, 0);
+                    } else {
+                        sacc[x][t] = mfma16<T>(k, q[x][s], sacc[x][t]);
+                    }
+                }
+            });
+        });
+        // ---- masks, running maximum, weights: lane = row n16, keys t*16 + kg*4 + i ----
+        const bool whole = key0 >= clear0 && key0 + 32 <= clear1;  // wave-uniform
+        u32x4 ph[NR], plo[NR];
+        float p[NR][8];
+#pragma unroll
+        for (int x = 0; x < NR; x++) {
+            float sv[8];
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sv[t * 4 + i] = sacc[x][t][i];
+            if (!whole) {
+                const uint32_t s = sees(x, key0) >> (kg * 4);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (!(s >> (t * 16 + i) & 1)) sv[t * 4 + i] = -INFINITY;
+            }
+            float mt = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+            mt = rows_max(mt) * a.qs;
+            if (__any(mt > m_run[x] + kLazy)) {
+                const float mn = fmaxf(m_run[x], mt), mu = mn == -INFINITY ? 0.f : mn;
+                const float corr = __builtin_amdgcn_exp2f(m_run[x] - mu);
+                l_part[x] *= corr;
+#pragma unroll
+                for (int i = 0; i < NDT; i++) oacc[x][i] *= corr;
+                m_run[x] = mn;
+            }
+            const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                p[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], a.qs, -mu));
+                l_part[x] += p[x][i];
+            }
+            if constexpr (!F) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (PB == 2) {
+                        const u32x2 hl = split2<T>(p[x][2 * i], p[x][2 * i + 1]);
+                        ph[x][i] = hl[0], plo[x][i] = hl[1];
+                    } else {
+                        ph[x][i] = pack2<T>(p[x][2 * i], p[x][2 * i + 1]);
+                    }
+                }
+            }
+        }
+        // ---- infinities and NaN in the V of keys that some row does not see: 0 times
+        // them is not 0, so such a block is added up by hand, for who sees them ----
+        if (!whole) {
+            uint32_t bad = 0;
+#pragma unroll 4
+            for (int i = 0; i < 32 * RB / 1024; i++) {
+                u32x4 v = lds_read_b128(sb + TILE + i * 1024 + lane * 16);
+                lds_wait_any();
+                tie(v);
+                bad |= not_finite<T>(v);
+            }
+            if (__any(bad != 0)) {
+#pragma unroll 1
+                for (int c = 0; c < 32; c++) {
+                    const int e = (c >> 4) * 4 + (c & 3), from = n16 + 16 * ((c >> 2) & 3);
+                    float w[NR];
+#pragma unroll
+                    for (int x = 0; x < NR; x++) {
+                        float y = p[x][0];
+#pragma unroll
+                        for (int i = 1; i < 8; i++) y = e == i ? p[x][i] : y;
+                        w[x] = __shfl(y, from);
+                    }
+                    const uint32_t vr = sb + TILE + c * RB;
+#pragma unroll
+                    for (int t = 0; t < NDT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int d = col(t, i), off = ((d * EB / 16) ^ tree_vswz<T, D>(c)) * 16 + d * EB % 16;
+                            uint32_t r = lds_read_b32(vr + (off & ~3));
+                            lds_wait_any();
+                            asm volatile("" : "+v"(r));
+                            float v;
+                            if constexpr (F) v = __uint_as_float(r);
+                            else if constexpr (__is_same(T, F16)) v = off & 2 ? f16_hi(r) : f16_lo(r);
+                            else v = off & 2 ? bf16_hi(r) : bf16_lo(r);
+#pragma unroll
+                            for (int x = 0; x < NR; x++) oacc[x][t][i] += w[x] != 0.f ? w[x] * v : 0.f;
+                        }
+                }
+                return;
+            }
+        }
+        // ---- O^T += V^T . P^T ----
+        if constexpr (F) {
+            constexpr int G64 = D / 64;
+            u32x4 vb[2][G64];
+            auto rdv = [&](auto kc, u32x4 (&r)[G64]) {  // k-step kc: keys t*16 + kg*4 + i
+                constexpr int k = decltype(kc)::value, t = k >> 2, i = k & 3;
+                static_for<0, G64>([&](auto gc) {
+                    r[decltype(gc)::value] = lds_read_b128_at<(t * 16 + i) * RB + decltype(gc)::value * 256>(sb + va[0]);
+                });
+            };
+            rdv(Int<0>{}, vb[0]);
+            static_for<0, 8>([&](auto kc) {
+                constexpr int k = decltype(kc)::value;
+                if constexpr (k < 7) {
+                    rdv(Int<k + 1>{}, vb[(k + 1) & 1]);
+                    lds_wait_n<G64>();
+                } else {
+                    lds_wait_n<0>();
+                }
+#pragma unroll
+                for (int g = 0; g < G64; g++) {
+                    tie(vb[k & 1][g]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int x = 0; x < NR; x++)
+                            oacc[x][g * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vb[k & 1][g][e]), p[x][k],
+                                                                                      oacc[x][g * 4 + e], 0, 0, 0);
+                }
+            });
+        } else {
+            uint32_t vaddr[NVA];
+#pragma unroll
+            for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
+            constexpr int CV = 4, NBV = NDT / CV;  // d tiles of a batch, batches
+            u32x2 vlo[2][CV], vhi[2][CV];
+            auto rdv = [&](auto bc) {
+                static_for<0, CV>([&](auto ic) {
+                    constexpr int B = decltype(bc)::value, i = decltype(ic)::value, d = B * CV + i;
+                    constexpr int off = d / NVA * 256;
+                    vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr[d % NVA]);
+                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RB>(vaddr[d % NVA]);
+                });
+            };
+            rdv(Int<0>{});
+            static_for<0, NBV>([&](auto bc) {
+                constexpr int B = decltype(bc)::value;
+                if constexpr (B + 1 < NBV) {
+                    rdv(Int<B + 1>{});
+                    lds_wait_n<2 * CV>();
+                } else {
+                    lds_wait_n<0>();
+                }
+#pragma unroll
+                for (int i = 0; i < CV; i++) {
+                    tie(vlo[B & 1][i]);
+                    tie(vhi[B & 1][i]);
+                    const u32x4 v = {vlo[B & 1][i][0], vlo[B & 1][i][1], vhi[B & 1][i][0], vhi[B & 1][i][1]};
+#pragma unroll
+                    for (int x = 0; x < NR; x++) {
+                        oacc[x][B * CV + i] = mfma16<T>(v, ph[x], oacc[x][B * CV + i]);
+                        if constexpr (PB == 2) oacc[x][B * CV + i] = mfma16<T>(v, plo[x], oacc[x][B * CV + i]);
+                    }
+                }
+            });
+        }
+    };
+    auto tile = [&](int j) {
+        const int t = j * WK + wk;
+        if (t >= tiles) return;
+        const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
+#pragma unroll
+        for (int s = 0; s < BPT; s++)
+            if (BPT == 1 || blk0 + t * BPT + s < blk1) block(sb + s * 32 * RB, (blk0 + t * BPT + s) * 32);
+    };
+
+    // ---- the pipeline: one key group's wave refills a stage as soon as it has
+    // read it; waves that share tiles refill behind the barrier that says that
+    // all have ----
+    if constexpr (WR == 1) {
+#pragma unroll
+        for (int j = 0; j < NST; j++)
+            if (j < steps) issue(j);
+        for (int j = 0; j < steps; j++) {
+            if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
+            else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+            lds_order();
+            tile(j);
+            lds_wait_any();
+            if (j + NST < steps) issue(j + NST);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NST - 1; j++)
+            if (j < steps) issue(j);
+        for (int j = 0; j < steps; j++) {
+            if (j + NST - 1 <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 2) * 2 * NI, 63)));
+            else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+            lds_wait_any();
+            wg_barrier();
+            if (j + NST - 1 < steps) issue(j + NST - 1);
+            tile(j);
+        }
+    }
+
+    // ---- results ----
+    const int64_t wrow0 = ((int64_t)slot * units + unit) * ROWS;  // of the scratch
+    auto emit = [&](int r, int d, const f32x4 &o, float m, float l) {  // r: row of the workgroup
+        if (row0 + r >= rows) return;
+        if (parts == 1) {
+            f32x4 y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = l == 0.f ? 0.f : o[i] / l;  // (a NaN score: NaN)
+            store4(out_at(row0 + r) + d, y);
+        } else {
+            *(f32x4 *)(pl.o + (wrow0 + r) * D + d) = o;
+            if (d == 0) pl.ml[wrow0 + r] = float2{m, l};
+        }
+    };
+#pragma unroll
+    for (int x = 0; x < NR; x++) l_part[x] = rows_sum(l_part[x]);
+    // Four consecutive columns from O tiles' registers: tile t (16-bit), or
+    // element c % 4 of four tiles (f32).
+    auto quad = [&](int x, int c) {
+        if constexpr (F) return f32x4{oacc[x][c & ~3][c & 3], oacc[x][(c & ~3) + 1][c & 3], oacc[x][(c & ~3) + 2][c & 3],
+                                      oacc[x][(c & ~3) + 3][c & 3]};
+        else return oacc[x][c];
+    };
+    auto qcol = [&](int c) { return F ? (c >> 2) * 64 + 16 * kg + 4 * (c & 3) : c * 16 + kg * 4; };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int x = 0; x < NR; x++)
+#pragma unroll
+            for (int c = 0; c < NDT; c++) emit((wr * NR + x) * 16 + n16, qcol(c), quad(x, c), m_run[x], l_part[x]);
+    } else {
+        __syncthreads();  // all tiles read
+        float *so = (float *)lds, *sml = (float *)(lds + WK * SMO);
+#pragma unroll
+        for (int x = 0; x < NR; x++) {
+            const int r = (wr * NR + x) * 16 + n16;
+#pragma unroll
+            for (int c = 0; c < NDT; c++) *(f32x4 *)(so + ((int64_t)wk * ROWS + r) * (D + 4) + qcol(c)) = quad(x, c);
+            if (kg == 0) *(float2 *)(sml + (wk * ROWS + r) * 2) = float2{m_run[x], l_part[x]};
+        }
+        __syncthreads();
+        for (int i = tid; i < ROWS * (D / 4); i += NT) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; w++) m = fmaxf(m, sml[(w * ROWS + r) * 2]);
+            const float mu = m == -INFINITY ? 0.f : m;
+            f32x4 o = {};
+#pragma unroll
+            for (int w = 0; w < WK; w++) {
+                const float c = __builtin_amdgcn_exp2f(sml[(w * ROWS + r) * 2] - mu);
+                l += sml[(w * ROWS + r) * 2 + 1] * c;
+                o += *(const f32x4 *)(so + ((int64_t)w * ROWS + r) * (D + 4) + d) * c;
+            }
+            emit(r, d, o, m, l);
+        }
+    }
+}
+
+// Adds up the parts of each row of the sequences that were cut.  A row is D/4
+// columns of four by 2^log_g groups of threads, each of which adds up every
+// 2^log_g-th part, four parts' loads in flight; the groups meet in LDS.  Bound by
+// the latency of those loads: 33 parts of 312 rows x 128 take 18.9 us with one
+// group and one part at a time.
+template <int D, int ODT>
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, TreePlan pl, int ROWS, int log_g) {
+    constexpr int C4 = D / 4, U = 4;
+    __shared__ f32x4 so[256];
+    __shared__ float2 sml[256];
+    const int tid = threadIdx.x, ng = 1 << log_g, c = tid % C4, g = tid / C4 & (ng - 1);
+    const int64_t row = (int64_t)blockIdx.x * (256 / C4 >> log_g) + (tid / C4 >> log_g);  // (node, head) of
+    const int b = blockIdx.y;                                                           // this sequence
+    const int2 sq = pl.seq[b];
+    if (sq.y < 2) return;  // uniform
+    const int i = (int)(row / a.n_head), h = (int)(row % a.n_head);
+    const int n = a.n ? min(max(a.n[b], 0), a.nodes) : a.nodes;
+    const bool there = i < n;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {};
+    if (there) {
+        const int G = a.kv_mul, kvh = h / G, r = i * G + h % G, rt = r / ROWS;
+        const int units = pl.n_kv * pl.row_tiles;
+        const int64_t at0 = ((int64_t)sq.x * units + kvh * pl.row_tiles + rt) * ROWS + r % ROWS, step = (int64_t)units * ROWS;
+        for (int p0 = g; p0 < sq.y; p0 += U * ng) {
+            float2 ml[U];
+            f32x4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int p = p0 + u * ng;
+                const int64_t at = at0 + min(p, sq.y - 1) * step;
+                ml[u] = pl.ml[at];
+                x[u] = *(const f32x4 *)(pl.o + at * D + c * 4);
+                if (p >= sq.y) ml[u] = float2{-INFINITY, 0.f}, x[u] = f32x4{};
+            }
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < U; u++) mn = fmaxf(mn, ml[u].x);
+            const float mu = mn == -INFINITY ? 0.f : mn, c0 = __builtin_amdgcn_exp2f(m - mu);
+            l *= c0;
+            o *= c0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float cu = __builtin_amdgcn_exp2f(ml[u].x - mu);
+                l += ml[u].y * cu;
+                o += x[u] * cu;
+            }
+            m = mn;
+        }
+    }
+    if (log_g) {
+        so[tid] = o;
+        sml[tid] = float2{m, l};
+        __syncthreads();
+        if (g) return;
+        float mn = m;
+        for (int k = 1; k < ng; k++) mn = fmaxf(mn, sml[tid + k * C4].x);
+        const float mu = mn == -INFINITY ? 0.f : mn, c0 = __builtin_amdgcn_exp2f(m - mu);
+        l *= c0;
+        o *= c0;
+        for (int k = 1; k < ng; k++) {
+            const float2 ml = sml[tid + k * C4];
+            const float cu = __builtin_amdgcn_exp2f(ml.x - mu);
+            l += ml.y * cu;
+            o += so[tid + k * C4] * cu;
+        }
+    }
+    if (!there) return;
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : o[e] / l;
+    const int64_t at = ((int64_t)b * a.nodes * a.n_head + row) * D + c * 4;
+    if constexpr (ODT == ULLM_DT_F32) *(f32x4 *)((float *)a.out + at) = y;
+    else if constexpr (ODT == ULLM_DT_F16) *(u32x2 *)((uint16_t *)a.out + at) = u32x2{pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3])};
+    else *(u32x2 *)((uint16_t *)a.out + at) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+}
+
+// Waves of a workgroup (WR x WK) and 16-row tiles of a wave for `rows` rows of a
+// kv head.
+struct TreeShape {
+    int nr, wr, wk;
+    int rows() const { return 16 * nr * wr; }
+};
+inline TreeShape tree_shape(int dtype, int D, int rows) {
+    const int rb = D * dtype_bytes(dtype);        // bytes of a key
+    const int most = D == 256 ? 1 : 2;            // row tiles of a wave: the registers hold no more
+    const int wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;  // key groups with two stages each in LDS
+    if (rows <= 16) return {1, 1, wk};
+    if (rows <= 16 * most) return {most, 1, wk};
+    int wr = 2;
+    while (wr < 8 && 16 * most * wr < rows) wr *= 2;
+    return {most, wr, std::min(wk, 8 / wr)};
+}
+template <class T, int D, int NR, int WR, int WK, int PB>
+static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
+    const int64_t items = (int64_t)p.slots * p.n_kv * p.row_tiles;
+    launch_kernel(tree_kernel<T, D, NR, WR, WK, PB>, dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WR * WK), 0, st, a, kv, p);
+    if (p.slots > p.batch) {
+        constexpr int ODT = PB == 1 && !__is_same(T, F32) ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
+        constexpr int RPB = 256 / (D / 4);  // rows of a workgroup with one group each
+        const int64_t rows = (int64_t)a.nodes * a.n_head;
+        int log_g = 0;  // groups for four of a sequence's parts each (8 sequences of 4 parts, 16384 rows x 128: 8.8
+                        // us with one group, 22.7 with eight; one sequence of 33, 312 rows: 18.9 and 5.0)
+        while ((RPB >> log_g) > 1 && (4 << log_g) < p.slots / p.batch) log_g++;
+        const int per = RPB >> log_g;
+        launch_kernel(tree_merge_kernel<D, ODT>, dim3((unsigned)((rows + per - 1) / per), p.batch), dim3(256), 0, st, a, p,
+                      16 * NR * WR, log_g);
+    }
+}
+template <class T, int D, int PB>
+static void launch_shape(const TreeShape &s, const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
+    constexpr int rb = D * T::bytes, most = D == 256 ? 1 : 2, wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;
+    if (s.wr == 8) launch_tree<T, D, most, 8, 1, PB>(a, kv, p, st);
+    else if (s.wr == 4) launch_tree<T, D, most, 4, std::min(wk, 2), PB>(a, kv, p, st);
+    else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
+    else if (s.nr == 2) {
+        if constexpr (most == 2) launch_tree<T, D, 2, 1, wk, PB>(a, kv, p, st);
+    } else {
+        launch_tree<T, D, 1, 1, wk, PB>(a, kv, p, st);
+    }
+}
+
+// One call's launches (a cache type each: tree_attn_f32.hip, .._f16.hip, .._bf16.hip).
+struct TreeCall {
+    TreeShape shape;
+    TreeArgs a;
+    TreeKv kv;
+    TreePlan plan;
+    int head_dim;
+    bool f32_out;
+    hipStream_t st;
+};
+template <class T, int PB>
+static void launch_dims(const TreeCall &c) {
+    if (c.head_dim == 64) launch_shape<T, 64, PB>(c.shape, c.a, c.kv, c.plan, c.st);
+    else if (c.head_dim == 128) launch_shape<T, 128, PB>(c.shape, c.a, c.kv, c.plan, c.st);
+    else launch_shape<T, 256, PB>(c.shape, c.a, c.kv, c.plan, c.st);
+}
+void launch_tree_f32(const TreeCall &c);
+void launch_tree_f16(const TreeCall &c);
+void launch_tree_bf16(const TreeCall &c);
+
+}  // namespace ullm

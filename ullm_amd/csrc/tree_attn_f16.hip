@@ -1,0 +1,6 @@
+// attn_tree over f16 caches (tree_attn.hpp).
+#include "tree_attn.hpp"
+
+namespace ullm {
+void launch_tree_f16(const TreeCall &c) { c.f32_out ? launch_dims<F16, 2>(c) : launch_dims<F16, 1>(c); }
+}  // namespace ullm
