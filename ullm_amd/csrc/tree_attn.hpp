@@ -152,18 +152,18 @@ __device__ __forceinline__ int tree_vswz(int r) {
     return D * T::bytes >= 256 ? ((r & 7) << 1) | ((r >> 3) & 1) : r & 7;
 }
 
-// Whether a 16-byte piece holds an infinity or a NaN.
+// Words of one f32 or two 16-bit values: the top bit of each that is an infinity
+// or NaN; a value's top bit spread over it.
 template <class T>
-__device__ __forceinline__ uint32_t not_finite(const u32x4 &x) {
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
     constexpr uint32_t m = __is_same(T, F32) ? 0x7fffffffu : 0x7fff7fffu;
     constexpr uint32_t one = __is_same(T, F32) ? 0x00800000u : __is_same(T, F16) ? 0x04000400u : 0x00800080u;
-    constexpr uint32_t top = __is_same(T, F32) ? 0x80000000u : 0x80008000u;
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) r |= (x[i] & m) + one;
-    return r & top;
+    return ((w & m) + one) & ~m;
 }
-
+template <class T>
+__device__ __forceinline__ uint32_t spread(uint32_t top) {
+    return top | (top - (top >> (__is_same(T, F32) ? 31 : 15)));
+}
 template <int WK, int STAGE>
 constexpr int tree_stages() {
     constexpr int n = 160 * 1024 / (WK * STAGE);
@@ -183,8 +183,9 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     static_assert(NST >= 2 && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
     constexpr int SMO = ROWS * (D + 4) * 4, SM = WK > 1 ? WK * (SMO + ROWS * 8) : 0;
     constexpr int LDS = WK * NST * STAGE > SM ? WK * NST * STAGE : SM;
-    static_assert(LDS <= 160 * 1024, "LDS");
+    static_assert(LDS + 16 <= 160 * 1024, "LDS");
     __shared__ __attribute__((aligned(1024))) char lds[LDS];
+    __shared__ int unfinite;  // a V tile had infinities or NaN taken out
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
     const int n16 = lane & 15, kg = lane >> 4;
@@ -218,6 +219,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     }
     if (row0 >= rows) return;
 
+    if (tid == 0) unfinite = 0;
+    __syncthreads();
     // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
     constexpr int BPT = KB / 32;
     const int first = uni(sq.lo) / 32, size = ((sq.blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     char *const ring = lds + wk * NST * STAGE;
     // Pages of 128 page numbers from pg0 on, in two registers.
     int pg0 = INT_MIN, pgv[2] = {0, 0};
-    auto issue = [&](int j) {  // step j's tile into stage j % NST
+    auto issue = [&](int j) __attribute__((always_inline)) {  // step j's tile into stage j % NST
         const int key0 = (blk0 + (j * WK + wk) * BPT + wblk) * 32;
         const int valid = j * WK + wk < tiles ? min(end - key0, 32) : 0;
         int64_t at;
@@ -318,12 +321,9 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int d = 0; d < NVA; d++)
             va[d] = TILE + r * RB + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<T, D>(r)) * 16) + 8 * (n16 & 1);
     }
-    // Column of element i of O tile t.
-    auto col = [&](int t, int i) { return F ? (t >> 2) * 64 + 16 * kg + 4 * i + (t & 3) : t * 16 + kg * 4 + i; };
-
     // Which keys of block key0 row x sees, bit c being key key0 + c.
-    auto sees = [&](int x, int key0) -> uint32_t {
-        if (node[x] < 0) return 0;
+    auto sees = [&](int x, int key0) __attribute__((always_inline)) -> uint32_t {
+        if (node[x] < 0 || key0 >= end) return 0;
         const int own = len - key0;  // keys of the sequence in the block
         uint32_t s = own >= 32 ? ~0u : own > 0 ? (1u << own) - 1 : 0u;
         const int j0 = -own, i = node[x];  // node of the block's first key, if there
@@ -359,44 +359,99 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         }
         return s;
     };
-    // Blocks from `clear0` up to `clear1` hold keys that every row sees.
+    // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0;
     if (a.window > 0) {
-        int most = INT_MIN;
+        int most = len;
+        for (int i = row0 / G + lane; i <= (min(row0 + ROWS, rows) - 1) / G; i += 64)
+            most = max(most, a.pos ? a.pos[(int64_t)b * a.nodes + i] : len + i);
 #pragma unroll
-        for (int x = 0; x < NR; x++) most = max(most, node[x] < 0 ? INT_MIN : pos[x]);
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor(most, o));
-        clear0 = uni(most) == INT_MIN ? 0 : max(uni(most) - a.window + 1, 0);
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+        clear0 = uni(most) - a.window + 1;
     }
     const int clear1 = len;
 
     constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
-    auto block = [&](uint32_t sb, int key0) {
-        // ---- S^T: two tiles of 16 keys ----
-        f32x4 sacc[NR][2];
+    constexpr int KT = KB / 16;   // 16-key tiles of S^T
+    auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
+    auto tile = [&](int j) __attribute__((always_inline)) {
+        const int tl = j * WK + wk;
+        if (tl >= tiles) return;
+        const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
+        const int key0 = (blk0 + tl * BPT) * 32;
+        const bool masked = !whole(key0);
+        // Infinities and NaN in V leave a tile that some row does not see all of:
+        // 0 times them would not be 0.  Who does see them gets them at the end.  (All
+        // waves that share the tile write the same.)
+        if (__builtin_expect(masked, 0)) {
+            uint32_t any = 0;
+#pragma unroll 1
+            for (int i = 0; i < TILE / 1024; i++) {
+                const uint32_t at = sb + TILE + i * 1024 + lane * 16;
+                u32x4 v = lds_read_b128(at);
+                lds_wait_any();
+                tie(v);
+                uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < NR; x++) sacc[x][0] = sacc[x][1] = f32x4{};
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t m = spread<T>(not_finite<T>(v[e]));
+                    v[e] &= ~m;
+                    bad |= m;
+                }
+                if (bad) lds_write_b128(at, v);
+                any |= bad;
+            }
+            if (any) unfinite = 1;
+        }
+        // ---- S^T ----
+        f32x4 sacc[NR][KT];
+#pragma unroll
+        for (int x = 0; x < NR; x++)
+#pragma unroll
+            for (int t = 0; t < KT; t++) sacc[x][t] = f32x4{};
         uint32_t kaddr[NKA];
 #pragma unroll
         for (int s = 0; s < NKA; s++) kaddr[s] = sb + ka[s];
-        constexpr int CH = NS < 4 ? NS : 4, NB = 2 * NS / CH;  // reads of a batch, batches
+        constexpr int CH = NS < 4 ? NS : 4, NB = KT * NS / CH;  // reads of a batch, batches
         u32x4 kb[2][CH];
-        auto rdk = [&](auto bc, u32x4 (&r)[CH]) {
+        auto rdk = [&](auto bc) {
             static_for<0, CH>([&](auto ic) {
                 constexpr int idx = decltype(bc)::value * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
                 constexpr int c = NKA == 4 ? s & 3 : s & 1, off = NKA == 4 ? (s >> 2) * 256 : 0;
-                r[decltype(ic)::value] = lds_read_b128_at<off + t * 16 * RB>(kaddr[c]);
+                kb[decltype(bc)::value & 1][decltype(ic)::value] = lds_read_b128_at<off + t * 16 * RB>(kaddr[c]);
             });
         };
-        rdk(Int<0>{}, kb[0]);
+        // V^T operands, batch by batch: CV d tiles of one 32-key block (16-bit), or
+        // one key of each group (f32); the first goes out ahead of the softmax.
+        constexpr int CV = F ? D / 64 : 4, NBV = F ? 4 * KT : BPT * NDT / CV;
+        uint32_t vaddr[NVA];
+#pragma unroll
+        for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
+        u32x4 vf[2][F ? CV : 1];
+        u32x2 vlo[2][F ? 1 : CV], vhi[2][F ? 1 : CV];
+        auto rdv = [&](auto bc) {
+            constexpr int B = decltype(bc)::value;
+            static_for<0, CV>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                if constexpr (F) {
+                    vf[B & 1][i] = lds_read_b128_at<((B >> 2) * 16 + (B & 3)) * RB + i * 256>(vaddr[0]);
+                } else {
+                    constexpr int d = B * CV % NDT + i, off = d / NVA * 256 + B * CV / NDT * 32 * RB;
+                    vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr[d % NVA]);
+                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RB>(vaddr[d % NVA]);
+                }
+            });
+        };
+        constexpr int VR = F ? CV : 2 * CV;  // reads of a batch
+        rdk(Int<0>{});
         static_for<0, NB>([&](auto bc) {
             constexpr int B = decltype(bc)::value;
             if constexpr (B + 1 < NB) {
-                rdk(Int<B + 1>{}, kb[(B + 1) & 1]);
+                rdk(Int<B + 1>{});
                 lds_wait_n<CH>();
             } else {
-                lds_wait_n<0>();
+                rdv(Int<0>{});
+                lds_wait_n<VR>();
             }
             static_for<0, CH>([&](auto ic) {
                 constexpr int idx = B * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
@@ -416,169 +471,98 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             });
         });
         // ---- masks, running maximum, weights: lane = row n16, keys t*16 + kg*4 + i ----
-        const bool whole = key0 >= clear0 && key0 + 32 <= clear1;  // wave-uniform
-        u32x4 ph[NR], plo[NR];
-        float p[NR][8];
+        if (__builtin_expect(masked, 0)) {
+#pragma unroll
+            for (int x = 0; x < NR; x++)
+#pragma unroll
+                for (int u = 0; u < BPT; u++) {
+                    const uint32_t s = sees(x, key0 + u * 32) >> (kg * 4);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (!(s >> (t * 16 + i) & 1)) sacc[x][2 * u + t][i] = -INFINITY;
+                }
+        }
+        float mt[NR];
+        bool up = false;
 #pragma unroll
         for (int x = 0; x < NR; x++) {
-            float sv[8];
+            float m = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int t = 0; t < KT; t++) m = fmaxf(m, fmaxf(fmaxf(sacc[x][t][0], sacc[x][t][1]), fmaxf(sacc[x][t][2], sacc[x][t][3])));
+            mt[x] = rows_max(m) * a.qs;
+            up |= mt[x] > m_run[x] + kLazy;
+        }
+        if (__any(up)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) sv[t * 4 + i] = sacc[x][t][i];
-            if (!whole) {
-                const uint32_t s = sees(x, key0) >> (kg * 4);
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!(s >> (t * 16 + i) & 1)) sv[t * 4 + i] = -INFINITY;
-            }
-            float mt = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-            mt = rows_max(mt) * a.qs;
-            if (__any(mt > m_run[x] + kLazy)) {
-                const float mn = fmaxf(m_run[x], mt), mu = mn == -INFINITY ? 0.f : mn;
+            for (int x = 0; x < NR; x++) {
+                const float mn = fmaxf(m_run[x], mt[x]), mu = mn == -INFINITY ? 0.f : mn;
                 const float corr = __builtin_amdgcn_exp2f(m_run[x] - mu);
                 l_part[x] *= corr;
 #pragma unroll
                 for (int i = 0; i < NDT; i++) oacc[x][i] *= corr;
                 m_run[x] = mn;
             }
+        }
+        u32x4 ph[NR][BPT], plo[NR][BPT];
+#pragma unroll
+        for (int x = 0; x < NR; x++) {
             const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], a.qs, -mu));
-                l_part[x] += p[x][i];
-            }
-            if constexpr (!F) {
+            for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if constexpr (PB == 2) {
-                        const u32x2 hl = split2<T>(p[x][2 * i], p[x][2 * i + 1]);
-                        ph[x][i] = hl[0], plo[x][i] = hl[1];
-                    } else {
-                        ph[x][i] = pack2<T>(p[x][2 * i], p[x][2 * i + 1]);
-                    }
+                    sacc[x][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[x][t][i], a.qs, -mu));
+                    l_part[x] += sacc[x][t][i];
                 }
-            }
-        }
-        // ---- infinities and NaN in the V of keys that some row does not see: 0 times
-        // them is not 0, so such a block is added up by hand, for who sees them ----
-        if (!whole) {
-            uint32_t bad = 0;
-#pragma unroll 4
-            for (int i = 0; i < 32 * RB / 1024; i++) {
-                u32x4 v = lds_read_b128(sb + TILE + i * 1024 + lane * 16);
-                lds_wait_any();
-                tie(v);
-                bad |= not_finite<T>(v);
-            }
-            if (__any(bad != 0)) {
-#pragma unroll 1
-                for (int c = 0; c < 32; c++) {
-                    const int e = (c >> 4) * 4 + (c & 3), from = n16 + 16 * ((c >> 2) & 3);
-                    float w[NR];
+            if constexpr (!F) {
 #pragma unroll
-                    for (int x = 0; x < NR; x++) {
-                        float y = p[x][0];
+                for (int u = 0; u < BPT; u++)
 #pragma unroll
-                        for (int i = 1; i < 8; i++) y = e == i ? p[x][i] : y;
-                        w[x] = __shfl(y, from);
-                    }
-                    const uint32_t vr = sb + TILE + c * RB;
-#pragma unroll
-                    for (int t = 0; t < NDT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int d = col(t, i), off = ((d * EB / 16) ^ tree_vswz<T, D>(c)) * 16 + d * EB % 16;
-                            uint32_t r = lds_read_b32(vr + (off & ~3));
-                            lds_wait_any();
-                            asm volatile("" : "+v"(r));
-                            float v;
-                            if constexpr (F) v = __uint_as_float(r);
-                            else if constexpr (__is_same(T, F16)) v = off & 2 ? f16_hi(r) : f16_lo(r);
-                            else v = off & 2 ? bf16_hi(r) : bf16_lo(r);
-#pragma unroll
-                            for (int x = 0; x < NR; x++) oacc[x][t][i] += w[x] != 0.f ? w[x] * v : 0.f;
+                    for (int i = 0; i < 4; i++) {
+                        const f32x4 &p = sacc[x][2 * u + (i >> 1)];
+                        if constexpr (PB == 2) {
+                            const u32x2 hl = split2<T>(p[2 * (i & 1)], p[2 * (i & 1) + 1]);
+                            ph[x][u][i] = hl[0], plo[x][u][i] = hl[1];
+                        } else {
+                            ph[x][u][i] = pack2<T>(p[2 * (i & 1)], p[2 * (i & 1) + 1]);
                         }
-                }
-                return;
+                    }
             }
         }
         // ---- O^T += V^T . P^T ----
-        if constexpr (F) {
-            constexpr int G64 = D / 64;
-            u32x4 vb[2][G64];
-            auto rdv = [&](auto kc, u32x4 (&r)[G64]) {  // k-step kc: keys t*16 + kg*4 + i
-                constexpr int k = decltype(kc)::value, t = k >> 2, i = k & 3;
-                static_for<0, G64>([&](auto gc) {
-                    r[decltype(gc)::value] = lds_read_b128_at<(t * 16 + i) * RB + decltype(gc)::value * 256>(sb + va[0]);
-                });
-            };
-            rdv(Int<0>{}, vb[0]);
-            static_for<0, 8>([&](auto kc) {
-                constexpr int k = decltype(kc)::value;
-                if constexpr (k < 7) {
-                    rdv(Int<k + 1>{}, vb[(k + 1) & 1]);
-                    lds_wait_n<G64>();
-                } else {
-                    lds_wait_n<0>();
-                }
+        static_for<0, NBV>([&](auto bc) {
+            constexpr int B = decltype(bc)::value;
+            if constexpr (B + 1 < NBV) {
+                rdv(Int<B + 1>{});
+                lds_wait_n<VR>();
+            } else {
+                lds_wait_n<0>();
+            }
 #pragma unroll
-                for (int g = 0; g < G64; g++) {
-                    tie(vb[k & 1][g]);
+            for (int i = 0; i < CV; i++) {
+                if constexpr (F) {
+                    tie(vf[B & 1][i]);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
 #pragma unroll
                         for (int x = 0; x < NR; x++)
-                            oacc[x][g * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vb[k & 1][g][e]), p[x][k],
-                                                                                      oacc[x][g * 4 + e], 0, 0, 0);
-                }
-            });
-        } else {
-            uint32_t vaddr[NVA];
-#pragma unroll
-            for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
-            constexpr int CV = 4, NBV = NDT / CV;  // d tiles of a batch, batches
-            u32x2 vlo[2][CV], vhi[2][CV];
-            auto rdv = [&](auto bc) {
-                static_for<0, CV>([&](auto ic) {
-                    constexpr int B = decltype(bc)::value, i = decltype(ic)::value, d = B * CV + i;
-                    constexpr int off = d / NVA * 256;
-                    vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr[d % NVA]);
-                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RB>(vaddr[d % NVA]);
-                });
-            };
-            rdv(Int<0>{});
-            static_for<0, NBV>([&](auto bc) {
-                constexpr int B = decltype(bc)::value;
-                if constexpr (B + 1 < NBV) {
-                    rdv(Int<B + 1>{});
-                    lds_wait_n<2 * CV>();
+                            oacc[x][i * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[B & 1][i][e]),
+                                                                                      sacc[x][B >> 2][B & 3], oacc[x][i * 4 + e], 0, 0, 0);
                 } else {
-                    lds_wait_n<0>();
-                }
-#pragma unroll
-                for (int i = 0; i < CV; i++) {
                     tie(vlo[B & 1][i]);
                     tie(vhi[B & 1][i]);
                     const u32x4 v = {vlo[B & 1][i][0], vlo[B & 1][i][1], vhi[B & 1][i][0], vhi[B & 1][i][1]};
+                    constexpr int u = B * CV / NDT, d0 = B * CV % NDT;
 #pragma unroll
                     for (int x = 0; x < NR; x++) {
-                        oacc[x][B * CV + i] = mfma16<T>(v, ph[x], oacc[x][B * CV + i]);
-                        if constexpr (PB == 2) oacc[x][B * CV + i] = mfma16<T>(v, plo[x], oacc[x][B * CV + i]);
+                        oacc[x][d0 + i] = mfma16<T>(v, ph[x][u], oacc[x][d0 + i]);
+                        if constexpr (PB == 2) oacc[x][d0 + i] = mfma16<T>(v, plo[x][u], oacc[x][d0 + i]);
                     }
                 }
-            });
-        }
-    };
-    auto tile = [&](int j) {
-        const int t = j * WK + wk;
-        if (t >= tiles) return;
-        const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
-#pragma unroll
-        for (int s = 0; s < BPT; s++)
-            if (BPT == 1 || blk0 + t * BPT + s < blk1) block(sb + s * 32 * RB, (blk0 + t * BPT + s) * 32);
+            }
+        });
     };
 
     // ---- the pipeline: one key group's wave refills a stage as soon as it has
@@ -610,20 +594,62 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         }
     }
 
+    // ---- infinities and NaN in V, to the rows that see their keys ----
+    __syncthreads();  // all tiles read, and the flag written
+    if (__builtin_expect(unfinite, 0)) {
+#pragma unroll 1
+        for (int k = 0; k < steps * BPT; k++) {
+            const int blk = blk0 + (k / BPT * WK + wk) * BPT + k % BPT, key0 = blk * 32;
+            if (blk >= blk1 || whole((blk0 + (k / BPT * WK + wk) * BPT) * 32)) continue;
+            uint32_t see[NR];
+#pragma unroll
+            for (int x = 0; x < NR; x++) see[x] = sees(x, key0);
+#pragma unroll 1
+            for (int c = 0; c < 32 && key0 + c < end; c++) {
+                int64_t at = b * kv.seq_b + (int64_t)(key0 + c) * kv.rb;
+                if (kv.tab) {
+                    const int pi = (key0 + c) >> kv.shift;
+                    const int phys = pi < kv.tab_stride ? kv.tab[(int64_t)b * kv.tab_stride + pi] : -1;
+                    if (phys < 0 || phys >= kv.n_pages) continue;
+                    at = (((int64_t)phys << kv.shift) + ((key0 + c) & ((1 << kv.shift) - 1))) * kv.rb;
+                }
+                const char *vp = kv.v + at + (int64_t)kvh * RB + (F ? 16 * kg * EB : kg * 4 * EB);
+#pragma unroll
+                for (int t = 0; t < NDT; t++) {
+                    float v[4];
+                    if constexpr (F) {
+                        const f32x4 r = *(const f32x4 *)(vp + ((t >> 2) * 64 + 4 * (t & 3)) * EB);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = r[e];
+                    } else {
+                        const u32x2 r = *(const u32x2 *)(vp + t * 16 * EB);
+                        unpack2<T>(r[0], v[0], v[1]);
+                        unpack2<T>(r[1], v[2], v[3]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool bad = not_finite<F32>(__float_as_uint(v[e]));
+#pragma unroll
+                        for (int x = 0; x < NR; x++) {
+                            f32x4 &o = F ? oacc[x][(t & ~3) + e] : oacc[x][t];
+                            if (bad && (see[x] >> c & 1)) o[F ? t & 3 : e] += v[e];
+                        }
+                    }
+                }
+            }
+        }
+    }
+
     // ---- results ----
     const int64_t wrow0 = ((int64_t)slot * units + unit) * ROWS;  // of the scratch
-    auto emit = [&](int r, int d, const f32x4 &o, float m, float l) {  // r: row of the workgroup
-        if (row0 + r >= rows) return;
-        if (parts == 1) {
-            f32x4 y;
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = l == 0.f ? 0.f : o[i] / l;  // (a NaN score: NaN)
-            store4(out_at(row0 + r) + d, y);
-        } else {
-            *(f32x4 *)(pl.o + (wrow0 + r) * D + d) = o;
-            if (d == 0) pl.ml[wrow0 + r] = float2{m, l};
-        }
+    // Element of the output (one part) or the scratch where row r of the workgroup
+    // begins, < 0 for a row that is not there.
+    auto row_at = [&](int r) -> int64_t { return row0 + r >= rows ? -1 : parts == 1 ? out_at(row0 + r) : (wrow0 + r) * D; };
+    auto emit = [&](int64_t at, const f32x4 &o, float inv) {
+        if (parts == 1) store4(at, o * inv);
+        else *(f32x4 *)(pl.o + at) = o;
     };
+    auto inverse = [&](float l) { return l == 0.f ? 0.f : 1.f / l; };  // (a NaN score: NaN)
 #pragma unroll
     for (int x = 0; x < NR; x++) l_part[x] = rows_sum(l_part[x]);
     // Four consecutive columns from O tiles' registers: tile t (16-bit), or
@@ -636,11 +662,16 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     auto qcol = [&](int c) { return F ? (c >> 2) * 64 + 16 * kg + 4 * (c & 3) : c * 16 + kg * 4; };
     if constexpr (WK == 1) {
 #pragma unroll
-        for (int x = 0; x < NR; x++)
+        for (int x = 0; x < NR; x++) {
+            const int r = (wr * NR + x) * 16 + n16;
+            const int64_t at = row_at(r);
+            if (at < 0) continue;
+            const float inv = inverse(l_part[x]);
 #pragma unroll
-            for (int c = 0; c < NDT; c++) emit((wr * NR + x) * 16 + n16, qcol(c), quad(x, c), m_run[x], l_part[x]);
+            for (int c = 0; c < NDT; c++) emit(at + qcol(c), quad(x, c), inv);
+            if (parts > 1 && kg == 0) pl.ml[wrow0 + r] = float2{m_run[x], l_part[x]};
+        }
     } else {
-        __syncthreads();  // all tiles read
         float *so = (float *)lds, *sml = (float *)(lds + WK * SMO);
 #pragma unroll
         for (int x = 0; x < NR; x++) {
@@ -652,6 +683,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         __syncthreads();
         for (int i = tid; i < ROWS * (D / 4); i += NT) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
+            const int64_t at = row_at(r);
+            if (at < 0) continue;
             float m = -INFINITY, l = 0.f;
 #pragma unroll
             for (int w = 0; w < WK; w++) m = fmaxf(m, sml[(w * ROWS + r) * 2]);
@@ -663,7 +696,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 l += sml[(w * ROWS + r) * 2 + 1] * c;
                 o += *(const f32x4 *)(so + ((int64_t)w * ROWS + r) * (D + 4) + d) * c;
             }
-            emit(r, d, o, m, l);
+            emit(at + d, o, inverse(l));
+            if (parts > 1 && d == 0) pl.ml[wrow0 + r] = float2{m, l};
         }
     }
 }
