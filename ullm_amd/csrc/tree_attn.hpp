@@ -164,6 +164,12 @@ template <class T>
 __device__ __forceinline__ uint32_t spread(uint32_t top) {
     return top | (top - (top >> (__is_same(T, F32) ? 31 : 15)));
 }
+// The largest, NaN if there is one: v_maximum3_f32.  (fmaxf, which passes NaN over,
+// first makes each operand quiet by an instruction of its own.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 template <int WK, int STAGE>
 constexpr int tree_stages() {
     constexpr int n = 160 * 1024 / (WK * STAGE);
@@ -279,6 +285,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int i = 0; i < NI; i++) dma16_cached(vr, st + TILE + i * 1024, vofs[i], 0);
     };
 
+    // The first tiles go out ahead of everything else.
+#pragma unroll
+    for (int j = 0; j < (WR == 1 ? NST : NST - 1); j++)
+        if (j < steps) issue(j);
+
     // ---- this wave's rows: Q^T operands, node, position ----
     u32x4 q[NR][NS];
     int node[NR], pos[NR];
@@ -376,7 +387,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
     auto tile = [&](int j) __attribute__((always_inline)) {
         const int tl = j * WK + wk;
-        if (tl >= tiles) return;
+        if (tl >= tiles || row0 + wr * NR * 16 >= rows) return;  // (a wave may have no rows)
         const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
         const int key0 = (blk0 + tl * BPT) * 32;
         const bool masked = !whole(key0);
@@ -490,8 +501,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int x = 0; x < NR; x++) {
             float m = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < KT; t++) m = fmaxf(m, fmaxf(fmaxf(sacc[x][t][0], sacc[x][t][1]), fmaxf(sacc[x][t][2], sacc[x][t][3])));
-            mt[x] = rows_max(m) * a.qs;
+            for (int t = 0; t < KT; t++) m = max3(max3(sacc[x][t][0], sacc[x][t][1], sacc[x][t][2]), sacc[x][t][3], m);
+            const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            m = __builtin_elementwise_maximum(__uint_as_float(r16[0]), __uint_as_float(r16[1]));
+            const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            // (NaN: not above it, and the row is NaN by its sum)
+            mt[x] = __builtin_elementwise_maximum(__uint_as_float(r32[0]), __uint_as_float(r32[1])) * a.qs;
             up |= mt[x] > m_run[x] + kLazy;
         }
         if (__any(up)) {
@@ -569,9 +584,6 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     // read it; waves that share tiles refill behind the barrier that says that
     // all have ----
     if constexpr (WR == 1) {
-#pragma unroll
-        for (int j = 0; j < NST; j++)
-            if (j < steps) issue(j);
         for (int j = 0; j < steps; j++) {
             if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -581,9 +593,6 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             if (j + NST < steps) issue(j + NST);
         }
     } else {
-#pragma unroll
-        for (int j = 0; j < NST - 1; j++)
-            if (j < steps) issue(j);
         for (int j = 0; j < steps; j++) {
             if (j + NST - 1 <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 2) * 2 * NI, 63)));
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
