@@ -47,6 +47,7 @@ static int attn_tree(const char *fn, TreeArgs a, TreeKv kv, int dtype, int64_t k
         return set_error(ULLM_HIP_E_INVALID, "%s: tensors and row strides must be 16-byte aligned", fn);
     a.words = 2 * ((a.nodes + 63) / 64);
     a.kv_mul = a.n_head / n_kv_head;
+    a.inv_g = a.kv_mul == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / a.kv_mul);
     a.neg = scale < 0.f;
     // (a scale of 0 by the least normal number: 0 times a masked score of -inf is none)
     a.qs = std::max(std::fabs(scale) * kLog2e, 1.17549435e-38f);
@@ -83,7 +84,7 @@ extern "C" int ullm_hip_attn_tree(const void *q, const void *k_cache, const void
                                   size_t workspace_bytes, void *stream) {
     if (seq_stride < 0) return set_error(ULLM_HIP_E_INVALID, "attn_tree: seq_stride < 0");
     const TreeArgs a{q, (const uint32_t *)mask, seq_lens, n_nodes, positions, max_nodes, 0, max_len, window, n_head, 1,
-                     0.f, 0, out};
+                     0, 0.f, 0, out};
     const TreeKv kv{(const char *)k_cache, (const char *)v_cache, 0,
                     batch > 1 && dtype_ok(dtype) ? seq_stride * dtype_bytes(dtype) : 0, nullptr, 0, 0, 0};
     return attn_tree("attn_tree", a, kv, dtype, kv_stride, batch, n_kv_head, head_dim, scale, out_dtype, workspace,
@@ -105,7 +106,7 @@ extern "C" int ullm_hip_attn_tree_paged(const void *q, const void *k_pages, cons
     if (batch > 0 && max_nodes > 0 && !block_table)
         return set_error(ULLM_HIP_E_INVALID, "attn_tree_paged: null tensor pointer");
     const TreeArgs a{q, (const uint32_t *)mask, seq_lens, n_nodes, positions, max_nodes, 0, max_len, window, n_head, 1,
-                     0.f, 0, out};
+                     0, 0.f, 0, out};
     const TreeKv kv{(const char *)k_pages, (const char *)v_pages, 0, 0, block_table, table_stride,
                     __builtin_ctz(page_size), n_pages};
     return attn_tree("attn_tree_paged", a, kv, dtype, kv_stride, batch, n_kv_head, head_dim, scale, out_dtype,

@@ -50,6 +50,7 @@ struct TreeArgs {
     const uint32_t *mask;  // words of 32 nodes; null: node i sees the nodes up to i
     const int32_t *len, *n, *pos;
     int nodes, words, max_len, window, n_head, kv_mul;
+    uint32_t inv_g;  // 2^32 / kv_mul, rounded down
     float qs;   // |scale| * log2(e)
     int neg;    // scale < 0: q enters with its sign turned
     void *out;
@@ -78,60 +79,75 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int b) {
     return s;
 }
 
-__device__ __forceinline__ int wave_isum(int x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+// Inclusive sums over the lanes (row shifts, then the row broadcasts).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xe, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xc, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
 }
+__device__ __forceinline__ int lane_of(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
 // Which sequence and part of it slot `slot` is: parts are of at most `per`
-// blocks, the least for which all sequences' parts fit the slots (to within a
-// sixteenth).  Every wave finds the same; at most 256 sequences are cut.
+// blocks, near the least for which all sequences' parts fit the slots.  Every
+// wave finds the same (any whole number of parts cuts a sequence rightly, so the
+// division need not be exact); at most 256 sequences are cut.  24 sequences take
+// 11000 cycles of a workgroup's start with cross-lane sums by LDS permutes and
+// steps of a sixteenth.
 struct TreePart {
     int b, part, parts, slot0;
+    TreeSeq sq;
 };
 __device__ __forceinline__ TreePart find_part(const TreeArgs &a, const TreePlan &pl, int slot) {
     const int lane = threadIdx.x & 63;
-    int nb[4], total = 0;
+    TreeSeq sq[4];
+    int total = 0;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        const int b = c * 64 + lane;
-        nb[c] = b < pl.batch ? tree_seq(a, b).blocks : 0;
-        total += nb[c];
+        sq[c] = TreeSeq{};
+        if (c * 64 < pl.batch) {  // uniform
+            if (c * 64 + lane < pl.batch) sq[c] = tree_seq(a, c * 64 + lane);
+            total += lane_of(wave_scan(sq[c].blocks), 63);
+        }
     }
-    total = wave_isum(total);
     int per = max((total + pl.slots - 1) / pl.slots, pl.least), parts[4];
     for (;;) {
+        const float inv = __builtin_amdgcn_rcpf((float)per);
         int sum = 0;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             parts[c] = 0;
-            if (c * 64 < pl.batch) parts[c] = c * 64 + lane < pl.batch ? max((nb[c] + per - 1) / per, 1) : 0;
-            sum += parts[c];
+            if (c * 64 < pl.batch) {
+                int n = (int)((float)sq[c].blocks * inv);
+                n += n * per < sq[c].blocks;
+                parts[c] = c * 64 + lane < pl.batch ? max(n, 1) : 0;
+                sum += lane_of(wave_scan(parts[c]), 63);
+            }
         }
-        if (wave_isum(sum) <= pl.slots) break;
-        per += per / 16 + 1;  // ends: with per >= every nb there are `batch` parts
+        if (sum <= pl.slots) break;
+        // ends: with per above every sequence's blocks there are `batch` parts
+        per = max(per + 1, (int)((float)per * (float)sum / (float)pl.slots));
     }
-    TreePart r{-1, 0, 0, 0};
+    TreePart r{-1, 0, 0, 0, {}};
     int before = 0;
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         if (c * 64 >= pl.batch) break;
-        int x = parts[c];
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(x, o);
-            if (lane >= o) x += y;
-        }
+        const int x = wave_scan(parts[c]);
         const uint64_t at = __ballot(slot >= before + x - parts[c] && slot < before + x);
         if (at) {
             const int l = __builtin_ctzll(at);
             r.b = c * 64 + l;
-            r.parts = __shfl(parts[c], l);
-            r.slot0 = before + __shfl(x, l) - r.parts;
+            r.parts = lane_of(parts[c], l);
+            r.slot0 = before + lane_of(x, l) - r.parts;
             r.part = slot - r.slot0;
+            r.sq = TreeSeq{lane_of(sq[c].n, l), lane_of(sq[c].len, l), lane_of(sq[c].end, l), lane_of(sq[c].lo, l),
+                           lane_of(sq[c].blocks, l)};
         }
-        before += __shfl(x, 63);
+        before += lane_of(x, 63);
     }
     return r;
 }
@@ -203,17 +219,25 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     const int slot = item / units, unit = item - slot * units;
     if (slot >= pl.slots) return;
     const int kvh = unit / pl.row_tiles, rt = unit - kvh * pl.row_tiles;
-    TreePart pt{slot, 0, 1, slot};
+    TreePart pt{slot, 0, 1, slot, {}};
     if (pl.slots > pl.batch) pt = find_part(a, pl, slot);
+    else pt.sq = tree_seq(a, slot);
     const int b = uni(pt.b), part = uni(pt.part), parts = uni(pt.parts);
     if (b < 0) return;
     if (pl.slots > pl.batch && part == 0 && unit == 0 && tid == 0) pl.seq[b] = int2{pt.slot0, parts};
-    const TreeSeq sq = tree_seq(a, b);
-    const int n = uni(sq.n), len = uni(sq.len), end = uni(sq.end);
+    const TreeSeq &sq = pt.sq;
+    const int n = uni(sq.n), len = uni(sq.len), end = uni(sq.end), blocks = uni(sq.blocks);
     const int G = a.kv_mul, rows = n * G, row0 = rt * ROWS;
+    auto node_of = [&](int r) {  // r / G
+        const int t = (int)__umulhi((uint32_t)r, a.inv_g);  // or one less
+        return t + (r - t * G >= G);
+    };
     const int64_t node_ld = (int64_t)a.n_head * D;  // elements of one node's heads
     const int64_t out0 = (int64_t)b * a.nodes * node_ld + (int64_t)kvh * G * D;
-    auto out_at = [&](int r) { return out0 + r / G * node_ld + (int64_t)(r % G) * D; };
+    auto out_at = [&](int r) {
+        const int t = node_of(r);
+        return out0 + t * node_ld + (int64_t)(r - t * G) * D;
+    };
     constexpr int ODT = PB == 1 && !F ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
     auto store4 = [&](int64_t at, const f32x4 &o) {
         if constexpr (ODT == ULLM_DT_F32) *(f32x4 *)((float *)a.out + at) = o;
@@ -225,12 +249,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     }
     if (row0 >= rows) return;
 
-    if (tid == 0) unfinite = 0;
-    __syncthreads();
+    // (waves that share tiles: the first barrier of the steps is behind it)
+    if (WR > 1 && tid == 0) unfinite = 0;
     // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
     constexpr int BPT = KB / 32;
-    const int first = uni(sq.lo) / 32, size = ((sq.blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
-    const int blk0 = first + part * size, blk1 = min(blk0 + size, first + uni(sq.blocks));
+    const int first = uni(sq.lo) / 32, size = ((blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
+    const int blk0 = first + part * size, blk1 = min(blk0 + size, first + blocks);
     const int tiles = max(blk1 - blk0 + BPT - 1, 0) / BPT;
     const int steps = (tiles + WK - 1) / WK;
 
@@ -297,7 +321,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     for (int x = 0; x < NR; x++) {
         const int r = row0 + (wr * NR + x) * 16 + n16;
         const bool ok = r < rows;
-        node[x] = ok ? r / G : -1;
+        node[x] = ok ? node_of(r) : -1;
         pos[x] = 0;
         if (a.window > 0 && ok)
             pos[x] = a.pos ? max(a.pos[(int64_t)b * a.nodes + node[x]], len) : len + node[x];
@@ -332,87 +356,114 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int d = 0; d < NVA; d++)
             va[d] = TILE + r * RB + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<T, D>(r)) * 16) + 8 * (n16 & 1);
     }
-    // Which keys of block key0 row x sees, bit c being key key0 + c.
-    auto sees = [&](int x, int key0) __attribute__((always_inline)) -> uint32_t {
-        if (node[x] < 0 || key0 >= end) return 0;
-        const int own = len - key0;  // keys of the sequence in the block
-        uint32_t s = own >= 32 ? ~0u : own > 0 ? (1u << own) - 1 : 0u;
-        const int j0 = -own, i = node[x];  // node of the block's first key, if there
-        if (own < 32) {
-            uint32_t t;
-            if (!a.mask) {
-                const int c = i - j0;  // bits 0..c
-                t = c >= 31 ? ~0u : c >= 0 ? (2u << c) - 1 : 0u;
-            } else {
-                const uint32_t *w = a.mask + ((int64_t)b * a.nodes + i) * a.words;
-                if (j0 < 0) {
-                    t = w[0] << -j0;
-                } else {
-                    const uint32_t w0 = w[j0 >> 5], w1 = (j0 >> 5) + 1 < a.words ? w[(j0 >> 5) + 1] : 0;
-                    t = (uint32_t)((((uint64_t)w1 << 32) | w0) >> (j0 & 31));
-                }
-            }
-            s |= t & ~(own > 0 ? (1u << own) - 1 : 0u);
-            const int left = end - key0;  // keys that are there
-            if (left < 32) s &= left > 0 ? (1u << left) - 1 : 0u;
-        }
-        if (a.window > 0) {
-            const int64_t lo = (int64_t)pos[x] - a.window + 1 - key0;  // first key position, from the block's
-            if (own > 0 && lo > 0) {
-                const uint32_t mine = own >= 32 ? ~0u : (1u << own) - 1;
-                s &= ~(mine & (lo >= 32 ? ~0u : (1u << lo) - 1));
-            }
-            if (own < 32)
-                for (int c = max(own, 0); c < 32 && key0 + c < end; c++) {
-                    const int p = a.pos ? max(a.pos[(int64_t)b * a.nodes + c + j0], len) : key0 + c;
-                    if ((int64_t)p <= (int64_t)pos[x] - a.window) s &= ~(1u << c);
-                }
-        }
-        return s;
-    };
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
-    int clear0 = 0;
+    int clear0 = 0, last = 0;
     if (a.window > 0) {
         int most = len;
-        for (int i = row0 / G + lane; i <= (min(row0 + ROWS, rows) - 1) / G; i += 64)
+        for (int i = node_of(row0) + lane; i <= node_of(min(row0 + ROWS, rows) - 1); i += 64)
             most = max(most, a.pos ? a.pos[(int64_t)b * a.nodes + i] : len + i);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
-        clear0 = uni(most) - a.window + 1;
+        last = uni(most);
+        clear0 = last - a.window + 1;
     }
     const int clear1 = len;
-
+    // Which keys of the tile of key0 row x sees, bit c of word u being key key0 +
+    // 32 u + c.  The mask's words of the tile are read ahead (`words`), so that
+    // they come while the tile is cleaned.
+    struct MaskWords {
+        uint32_t w[BPT + 1];
+    };
+    auto words = [&](int x, int key0) __attribute__((always_inline)) {
+        MaskWords m{};
+        if (!a.mask || node[x] < 0) return m;
+        const uint32_t *w = a.mask + ((int64_t)b * a.nodes + node[x]) * a.words;
+        const int w0 = max(key0 - len, 0) >> 5;
+#pragma unroll
+        for (int i = 0; i <= BPT; i++) m.w[i] = w0 + i < a.words ? w[w0 + i] : 0;
+        return m;
+    };
+    auto sees = [&](int x, int key0, const MaskWords &m, uint32_t (&see)[BPT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < BPT; u++) {
+            const int k0 = key0 + 32 * u, own = len - k0, j0 = -own;  // keys of the sequence in the block; its first node
+            const uint32_t mine = own >= 32 ? ~0u : own > 0 ? (1u << own) - 1 : 0u;
+            const int left = end - k0;  // keys that are there
+            const uint32_t there = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
+            uint32_t t = 0;
+            if (own < 32) {
+                if (!a.mask) {
+                    const int c = node[x] - j0;  // bits 0..c
+                    t = c >= 31 ? ~0u : c >= 0 ? (2u << c) - 1 : 0u;
+                } else if (j0 < 0) {
+                    t = m.w[0] << -j0;
+                } else {
+                    const bool next = (j0 >> 5) > max(key0 - len, 0) >> 5;  // uniform
+                    const uint32_t lo = next ? m.w[BPT - 1] : m.w[0], hi = next ? m.w[BPT] : m.w[1];
+                    t = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j0 & 31));
+                }
+            }
+            uint32_t s = (mine | (t & ~mine)) & there;
+            if (a.window > 0) {
+                const int64_t lo = (int64_t)pos[x] - a.window + 1 - k0;  // the window's first position, from the block's
+                if (lo > 0) s &= ~(mine & (lo >= 32 ? ~0u : (1u << lo) - 1));
+                if (own < 32 && last - a.window >= len) {  // the window may end among the nodes
+                    const int c = lane & 31, j = j0 + c;
+                    int p = k0 + c;
+                    if (a.pos && j >= 0 && j < n) p = max(a.pos[(int64_t)b * a.nodes + j], len);
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if ((int64_t)lane_of(p, i) <= (int64_t)pos[x] - a.window) s &= ~((1u << i) & ~mine);
+                }
+            }
+            see[u] = node[x] < 0 ? 0 : s;
+        }
+    };
     constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
     constexpr int KT = KB / 16;   // 16-key tiles of S^T
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
+    bool mine = false;  // this wave's own tiles had infinities or NaN taken out
     auto tile = [&](int j) __attribute__((always_inline)) {
         const int tl = j * WK + wk;
         if (tl >= tiles || row0 + wr * NR * 16 >= rows) return;  // (a wave may have no rows)
         const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
         const int key0 = (blk0 + tl * BPT) * 32;
         const bool masked = !whole(key0);
+        uint32_t see[NR][BPT];
         // Infinities and NaN in V leave a tile that some row does not see all of:
         // 0 times them would not be 0.  Who does see them gets them at the end.  (All
         // waves that share the tile write the same.)
         if (__builtin_expect(masked, 0)) {
-            uint32_t any = 0;
-#pragma unroll 1
-            for (int i = 0; i < TILE / 1024; i++) {
-                const uint32_t at = sb + TILE + i * 1024 + lane * 16;
-                u32x4 v = lds_read_b128(at);
-                lds_wait_any();
-                tie(v);
-                uint32_t bad = 0;
+            MaskWords mw[NR];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t m = spread<T>(not_finite<T>(v[e]));
-                    v[e] &= ~m;
-                    bad |= m;
+            for (int x = 0; x < NR; x++) mw[x] = words(x, key0);
+            uint32_t any = 0;
+            constexpr int U = TILE / 1024 < 8 ? TILE / 1024 : 8;  // pieces in flight
+#pragma unroll 1
+            for (int i = 0; i < TILE / 1024; i += U) {
+                const uint32_t at = sb + TILE + i * 1024 + lane * 16;
+                u32x4 v[U];
+                static_for<0, U>([&](auto uc) { v[decltype(uc)::value] = lds_read_b128_at<decltype(uc)::value * 1024>(at); });
+                lds_wait(v);
+#pragma unroll
+                for (int k = 0; k < U; k++) {
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) bad |= not_finite<T>(v[k][e]);
+                    any |= bad;
+                    if (bad) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[k][e] &= ~spread<T>(not_finite<T>(v[k][e]));
+                        lds_write_b128(at + k * 1024, v[k]);
+                    }
                 }
-                if (bad) lds_write_b128(at, v);
-                any |= bad;
             }
-            if (any) unfinite = 1;
+            if (__any(any != 0)) {
+                if constexpr (WR > 1) unfinite = 1;
+                else mine = true;
+            }
+#pragma unroll
+            for (int x = 0; x < NR; x++) sees(x, key0, mw[x], see[x]);
         }
         // ---- S^T ----
         f32x4 sacc[NR][KT];
@@ -487,7 +538,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             for (int x = 0; x < NR; x++)
 #pragma unroll
                 for (int u = 0; u < BPT; u++) {
-                    const uint32_t s = sees(x, key0 + u * 32) >> (kg * 4);
+                    const uint32_t s = see[x][u] >> (kg * 4);
 #pragma unroll
                     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -604,15 +655,19 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     }
 
     // ---- infinities and NaN in V, to the rows that see their keys ----
-    __syncthreads();  // all tiles read, and the flag written
-    if (__builtin_expect(unfinite, 0)) {
+    if constexpr (WR > 1 || WK > 1) __syncthreads();  // all tiles read, and the flag written
+    if (__builtin_expect(WR > 1 ? unfinite != 0 : mine, 0)) {
 #pragma unroll 1
         for (int k = 0; k < steps * BPT; k++) {
-            const int blk = blk0 + (k / BPT * WK + wk) * BPT + k % BPT, key0 = blk * 32;
-            if (blk >= blk1 || whole((blk0 + (k / BPT * WK + wk) * BPT) * 32)) continue;
+            const int t0 = blk0 + (k / BPT * WK + wk) * BPT, u = k % BPT, key0 = (t0 + u) * 32;  // tile, block of it
+            if (t0 + u >= blk1 || whole(t0 * 32)) continue;
             uint32_t see[NR];
 #pragma unroll
-            for (int x = 0; x < NR; x++) see[x] = sees(x, key0);
+            for (int x = 0; x < NR; x++) {
+                uint32_t s[BPT];
+                sees(x, t0 * 32, words(x, t0 * 32), s);
+                see[x] = u ? s[BPT - 1] : s[0];
+            }
 #pragma unroll 1
             for (int c = 0; c < 32 && key0 + c < end; c++) {
                 int64_t at = b * kv.seq_b + (int64_t)(key0 + c) * kv.rb;
