@@ -17,8 +17,12 @@
 //    row's maximum, sum and rescale live in the four lanes that own its output,
 //    and P^T is the S^T accumulator exponentiated: P never moves between lanes.
 //    16-bit caches: 16x16x32, K by 16-byte LDS reads, V^T by the transposing
-//    LDS read.  f32: 16x16x4 products of f32, K and V by 16-byte reads, the four
-//    elements of a read being four k-steps (K) or four d tiles (V).
+//    LDS read.  f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads,
+//    the four elements of a read being four k-steps (K) or four d tiles (V); they
+//    run at a sixteenth of the 16-bit rate, which the stream of K and V hides up
+//    to 64 rows.  f32, more rows (X3): every value as the sum of three bf16 (8 bits
+//    each, exact), six products of the 16-bit rate (those above 2^-24 of the
+//    whole), K and V tiles split once by the waves that fetched them.
 //  * K and V tiles come by LDS DMA into a ring, one 32-key block a page lookup.
 //  * A workgroup is WR x WK waves of 16*NR rows: the WR waves of a key group
 //    share its tiles, the WK key groups take tiles in turn and are added up
@@ -192,19 +196,38 @@ constexpr int tree_stages() {
     return n > 4 ? 4 : n;
 }
 
+// Two f32 as three words of bf16 pairs that add up to them: the leading 8 bits, the
+// next 8, the rest (an infinity: itself and zeros).
+__device__ __forceinline__ void split3(float x0, float x1, uint32_t (&w)[3]) {
+    constexpr uint32_t top = 0xffff0000u, pick = 0x07060302u;  // the upper halves of two words
+    const float h0 = __uint_as_float(__float_as_uint(x0) & top), h1 = __uint_as_float(__float_as_uint(x1) & top);
+    const float r0 = h0 == x0 ? 0.f : x0 - h0, r1 = h1 == x1 ? 0.f : x1 - h1;
+    const float m0 = __uint_as_float(__float_as_uint(r0) & top), m1 = __uint_as_float(__float_as_uint(r1) & top);
+    w[0] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), pick);
+    w[1] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), pick);
+    w[2] = __builtin_amdgcn_perm(__float_as_uint(r1 - m1), __float_as_uint(r0 - m0), pick);
+}
+
 template <class T, int D, int NR, int WR, int WK, int PB>
 __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr bool F = __is_same(T, F32);
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
     constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
-    constexpr int TILE = KB * RB, STAGE = 2 * TILE, NST = tree_stages<WK, STAGE>();
+    constexpr int TILE = KB * RB, STAGE = 2 * TILE;  // as fetched
+    constexpr bool X3 = F && WR >= 4 && D <= 128, FM = F && !X3;
+    using CT = typename std::conditional<X3, BF16, T>::type;  // operands
+    constexpr int NPL = X3 ? 3 : 1, NP = X3 ? 3 : PB;          // pieces of K, V and Q, and of P
+    constexpr int RBC = D * CT::bytes, CTILE = KB * RBC;       // a row and a tile of one piece
+    constexpr int CONV = 2 * NPL * CTILE;                      // K pieces, V pieces
+    constexpr int NST = X3 ? 1 : tree_stages<WK, STAGE>();
+    constexpr int GROUP = NST * STAGE + (X3 ? 2 * CONV : 0);   // LDS of a key group
     constexpr int NI = TILE / 1024 / WR;  // DMA instructions of a wave for K, and for V
-    constexpr int NS = F ? D / 16 : D / 32;  // 16-byte reads of a K row by a lane
-    constexpr int NDT = D / 16;              // 16-wide d tiles of O^T
+    constexpr int NS = FM ? D / 16 : D / 32;  // 16-byte reads of a K row by a lane
+    constexpr int NDT = D / 16;               // 16-wide d tiles of O^T
     constexpr int ROWS = 16 * NR * WR, NT = 64 * WR * WK;
-    static_assert(NST >= 2 && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
+    static_assert((X3 || NST >= 2) && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
     constexpr int SMO = ROWS * (D + 4) * 4, SM = WK > 1 ? WK * (SMO + ROWS * 8) : 0;
-    constexpr int LDS = WK * NST * STAGE > SM ? WK * NST * STAGE : SM;
+    constexpr int LDS = WK * GROUP > SM ? WK * GROUP : SM;
     static_assert(LDS + 16 <= 160 * 1024, "LDS");
     __shared__ __attribute__((aligned(1024))) char lds[LDS];
     __shared__ int unfinite;  // a V tile had infinities or NaN taken out
@@ -270,10 +293,10 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 #pragma unroll
     for (int i = 0; i < NI; i++) {
         const int r = wrow + i * RPI + drow;  // in the block; the swizzles go by r % 16
-        kofs[i] = r * rb + ((dslot ^ tree_kswz<T, D>(r)) * 16);
-        vofs[i] = r * rb + ((dslot ^ tree_vswz<T, D>(r)) * 16);
+        kofs[i] = r * rb + ((X3 ? dslot : dslot ^ tree_kswz<T, D>(r)) * 16);
+        vofs[i] = r * rb + ((X3 ? dslot : dslot ^ tree_vswz<T, D>(r)) * 16);
     }
-    char *const ring = lds + wk * NST * STAGE;
+    char *const ring = lds + wk * GROUP;
     // Pages of 128 page numbers from pg0 on, in two registers.
     int pg0 = INT_MIN, pgv[2] = {0, 0};
     auto issue = [&](int j) __attribute__((always_inline)) {  // step j's tile into stage j % NST
@@ -311,11 +334,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 
     // The first tiles go out ahead of everything else.
 #pragma unroll
-    for (int j = 0; j < (WR == 1 ? NST : NST - 1); j++)
+    for (int j = 0; j < (WR == 1 || X3 ? NST : NST - 1); j++)
         if (j < steps) issue(j);
 
     // ---- this wave's rows: Q^T operands, node, position ----
-    u32x4 q[NR][NS];
+    u32x4 q[NR][NPL][NS];
     int node[NR], pos[NR];
 #pragma unroll
     for (int x = 0; x < NR; x++) {
@@ -328,11 +351,31 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         const char *qp = (const char *)a.q + (ok ? out_at(r) : out0) * EB + kg * 16;
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            q[x][s] = ok ? *(const u32x4 *)(qp + s * 64) : u32x4{};
-            if (a.neg) q[x][s] ^= F ? 0x80000000u : 0x80008000u;
+            if constexpr (X3) {  // d = 32 s + 8 kg .. +7
+                const u32x4 *at = (const u32x4 *)(qp + s * 128 + kg * 16);
+                u32x4 f[2] = {ok ? at[0] : u32x4{}, ok ? at[1] : u32x4{}};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t w[3];
+                    split3(__uint_as_float(f[i >> 1][2 * (i & 1)]), __uint_as_float(f[i >> 1][2 * (i & 1) + 1]), w);
+#pragma unroll
+                    for (int k = 0; k < 3; k++) q[x][k][s][i] = w[k];
+                }
+            } else {
+                q[x][0][s] = ok ? *(const u32x4 *)(qp + s * 64) : u32x4{};
+            }
         }
     }
 
+    if (a.neg) {
+        asm volatile("");  // (a branch, not a select that would wait for q here)
+#pragma unroll
+        for (int x = 0; x < NR; x++)
+#pragma unroll
+            for (int k = 0; k < NPL; k++)
+#pragma unroll
+                for (int s = 0; s < NS; s++) q[x][k][s] ^= FM ? 0x80000000u : 0x80008000u;
+    }
     f32x4 oacc[NR][NDT];
     float m_run[NR], l_part[NR];
 #pragma unroll
@@ -342,19 +385,19 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int i = 0; i < NDT; i++) oacc[x][i] = f32x4{};
     }
     // Per-lane operand addresses within a tile.
-    constexpr int NKA = RB >= 256 ? 4 : 2;  // chunks 16.. of a row sit 256 bytes on
+    constexpr int NKA = RBC >= 256 ? 4 : 2;  // chunks 16.. of a row sit 256 bytes on
     uint32_t ka[NKA];
 #pragma unroll
-    for (int s = 0; s < NKA; s++) ka[s] = n16 * RB + (((4 * s + kg) ^ tree_kswz<T, D>(n16)) * 16);
-    constexpr int NVA = F ? 1 : RB >= 256 ? 8 : 4;
+    for (int s = 0; s < NKA; s++) ka[s] = n16 * RBC + (((4 * s + kg) ^ tree_kswz<CT, D>(n16)) * 16);
+    constexpr int NVA = FM ? 1 : RBC >= 256 ? 8 : 4;
     uint32_t va[NVA];
-    if constexpr (F) {
-        va[0] = TILE + kg * 4 * RB + n16 * 16;
+    if constexpr (FM) {
+        va[0] = CTILE + kg * 4 * RBC + n16 * 16;
     } else {
         const int r = kg * 4 + (n16 >> 2);
 #pragma unroll
         for (int d = 0; d < NVA; d++)
-            va[d] = TILE + r * RB + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<T, D>(r)) * 16) + 8 * (n16 & 1);
+            va[d] = NPL * CTILE + r * RBC + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<CT, D>(r)) * 16) + 8 * (n16 & 1);
     }
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0, last = 0;
@@ -426,7 +469,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     auto tile = [&](int j) __attribute__((always_inline)) {
         const int tl = j * WK + wk;
         if (tl >= tiles || row0 + wr * NR * 16 >= rows) return;  // (a wave may have no rows)
-        const uint32_t sb = lds_addr(ring) + j % NST * STAGE;
+        const uint32_t sb = lds_addr(ring) + (X3 ? NST * STAGE + (j & 1) * CONV : j % NST * STAGE);
         const int key0 = (blk0 + tl * BPT) * 32;
         const bool masked = !whole(key0);
         uint32_t see[NR][BPT];
@@ -437,6 +480,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             MaskWords mw[NR];
 #pragma unroll
             for (int x = 0; x < NR; x++) mw[x] = words(x, key0);
+            if constexpr (!X3) {
             uint32_t any = 0;
             constexpr int U = TILE / 1024 < 8 ? TILE / 1024 : 8;  // pieces in flight
 #pragma unroll 1
@@ -462,6 +506,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 if constexpr (WR > 1) unfinite = 1;
                 else mine = true;
             }
+            }
 #pragma unroll
             for (int x = 0; x < NR; x++) sees(x, key0, mw[x], see[x]);
         }
@@ -474,37 +519,40 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         uint32_t kaddr[NKA];
 #pragma unroll
         for (int s = 0; s < NKA; s++) kaddr[s] = sb + ka[s];
-        constexpr int CH = NS < 4 ? NS : 4, NB = KT * NS / CH;  // reads of a batch, batches
+        constexpr int KR = NS * NPL, CH = X3 ? 6 : NS < 4 ? NS : 4, NB = KT * KR / CH;  // reads of a key tile, of a batch
         u32x4 kb[2][CH];
         auto rdk = [&](auto bc) {
             static_for<0, CH>([&](auto ic) {
-                constexpr int idx = decltype(bc)::value * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
+                constexpr int idx = decltype(bc)::value * CH + decltype(ic)::value, t = idx / KR, s = idx % KR / NPL;
                 constexpr int c = NKA == 4 ? s & 3 : s & 1, off = NKA == 4 ? (s >> 2) * 256 : 0;
-                kb[decltype(bc)::value & 1][decltype(ic)::value] = lds_read_b128_at<off + t * 16 * RB>(kaddr[c]);
+                kb[decltype(bc)::value & 1][decltype(ic)::value] =
+                    lds_read_b128_at<off + t * 16 * RBC + idx % NPL * CTILE>(kaddr[c]);
             });
         };
-        // V^T operands, batch by batch: CV d tiles of one 32-key block (16-bit), or
-        // one key of each group (f32); the first goes out ahead of the softmax.
-        constexpr int CV = F ? D / 64 : 4, NBV = F ? 4 * KT : BPT * NDT / CV;
+        // V^T operands, batch by batch: CV d tiles of one 32-key block, or one key of
+        // each group (f32 products); the first goes out ahead of the softmax.
+        constexpr int CV = FM ? D / 64 : X3 ? 1 : 4, NBV = FM ? 4 * KT : BPT * NDT / CV;
         uint32_t vaddr[NVA];
 #pragma unroll
         for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
-        u32x4 vf[2][F ? CV : 1];
-        u32x2 vlo[2][F ? 1 : CV], vhi[2][F ? 1 : CV];
+        u32x4 vf[2][FM ? CV : 1];
+        u32x2 vlo[2][FM ? 1 : CV * NPL], vhi[2][FM ? 1 : CV * NPL];
         auto rdv = [&](auto bc) {
             constexpr int B = decltype(bc)::value;
-            static_for<0, CV>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
-                if constexpr (F) {
-                    vf[B & 1][i] = lds_read_b128_at<((B >> 2) * 16 + (B & 3)) * RB + i * 256>(vaddr[0]);
-                } else {
-                    constexpr int d = B * CV % NDT + i, off = d / NVA * 256 + B * CV / NDT * 32 * RB;
+            if constexpr (FM)
+                static_for<0, CV>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    vf[B & 1][i] = lds_read_b128_at<((B >> 2) * 16 + (B & 3)) * RBC + i * 256>(vaddr[0]);
+                });
+            else
+                static_for<0, CV * NPL>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value, d = B * CV % NDT + i / NPL;
+                    constexpr int off = d / NVA * 256 + B * CV / NDT * 32 * RBC + i % NPL * CTILE;
                     vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr[d % NVA]);
-                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RB>(vaddr[d % NVA]);
-                }
-            });
+                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RBC>(vaddr[d % NVA]);
+                });
         };
-        constexpr int VR = F ? CV : 2 * CV;  // reads of a batch
+        constexpr int VR = FM ? CV : 2 * CV * NPL;  // reads of a batch
         rdk(Int<0>{});
         static_for<0, NB>([&](auto bc) {
             constexpr int B = decltype(bc)::value;
@@ -516,18 +564,19 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 lds_wait_n<VR>();
             }
             static_for<0, CH>([&](auto ic) {
-                constexpr int idx = B * CH + decltype(ic)::value, t = idx / NS, s = idx % NS;
+                constexpr int idx = B * CH + decltype(ic)::value, t = idx / KR, s = idx % KR / NPL, pl = idx % NPL;
                 u32x4 &k = kb[B & 1][decltype(ic)::value];
                 tie(k);
 #pragma unroll
                 for (int x = 0; x < NR; x++) {
-                    if constexpr (F) {
+                    if constexpr (FM) {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            sacc[x][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[x][s][e]),
+                            sacc[x][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[x][0][s][e]),
                                                                               sacc[x][t], 0, 0, 0);
                     } else {
-                        sacc[x][t] = mfma16<T>(k, q[x][s], sacc[x][t]);
+#pragma unroll
+                        for (int k2 = 0; k2 + pl < NPL; k2++) sacc[x][t] = mfma16<CT>(k, q[x][k2][s], sacc[x][t]);
                     }
                 }
             });
@@ -571,7 +620,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 m_run[x] = mn;
             }
         }
-        u32x4 ph[NR][BPT], plo[NR][BPT];
+        u32x4 ph[NR][BPT][NP];
 #pragma unroll
         for (int x = 0; x < NR; x++) {
             const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
@@ -582,17 +631,23 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                     sacc[x][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[x][t][i], a.qs, -mu));
                     l_part[x] += sacc[x][t][i];
                 }
-            if constexpr (!F) {
+            if constexpr (!FM) {
 #pragma unroll
                 for (int u = 0; u < BPT; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const f32x4 &p = sacc[x][2 * u + (i >> 1)];
-                        if constexpr (PB == 2) {
-                            const u32x2 hl = split2<T>(p[2 * (i & 1)], p[2 * (i & 1) + 1]);
-                            ph[x][u][i] = hl[0], plo[x][u][i] = hl[1];
+                        const float p0 = p[2 * (i & 1)], p1 = p[2 * (i & 1) + 1];
+                        if constexpr (NP == 3) {
+                            uint32_t w[3];
+                            split3(p0, p1, w);
+#pragma unroll
+                            for (int k = 0; k < 3; k++) ph[x][u][k][i] = w[k];
+                        } else if constexpr (NP == 2) {
+                            const u32x2 hl = split2<CT>(p0, p1);
+                            ph[x][u][0][i] = hl[0], ph[x][u][1][i] = hl[1];
                         } else {
-                            ph[x][u][i] = pack2<T>(p[2 * (i & 1)], p[2 * (i & 1) + 1]);
+                            ph[x][u][0][i] = pack2<CT>(p0, p1);
                         }
                     }
             }
@@ -606,9 +661,9 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             } else {
                 lds_wait_n<0>();
             }
+            if constexpr (FM) {
 #pragma unroll
-            for (int i = 0; i < CV; i++) {
-                if constexpr (F) {
+                for (int i = 0; i < CV; i++) {
                     tie(vf[B & 1][i]);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
@@ -616,25 +671,76 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                         for (int x = 0; x < NR; x++)
                             oacc[x][i * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[B & 1][i][e]),
                                                                                       sacc[x][B >> 2][B & 3], oacc[x][i * 4 + e], 0, 0, 0);
-                } else {
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CV * NPL; i++) {
                     tie(vlo[B & 1][i]);
                     tie(vhi[B & 1][i]);
                     const u32x4 v = {vlo[B & 1][i][0], vlo[B & 1][i][1], vhi[B & 1][i][0], vhi[B & 1][i][1]};
                     constexpr int u = B * CV / NDT, d0 = B * CV % NDT;
 #pragma unroll
-                    for (int x = 0; x < NR; x++) {
-                        oacc[x][d0 + i] = mfma16<T>(v, ph[x][u], oacc[x][d0 + i]);
-                        if constexpr (PB == 2) oacc[x][d0 + i] = mfma16<T>(v, plo[x][u], oacc[x][d0 + i]);
-                    }
+                    for (int k = 0; k + i % NPL < NP; k++)
+#pragma unroll
+                        for (int x = 0; x < NR; x++) oacc[x][d0 + i / NPL] = mfma16<CT>(v, ph[x][u][k], oacc[x][d0 + i / NPL]);
                 }
             }
         });
+    };
+    // The pieces of the K and V that this wave fetched, from the f32 tile into pieces
+    // (X3); the next tile is fetched as soon as they are read.
+    auto convert = [&](int j) __attribute__((always_inline)) {
+        const uint32_t from = lds_addr(ring) + wr * NI * 1024 + lane * 16;
+        const uint32_t to = lds_addr(ring) + NST * STAGE + (j & 1) * CONV;
+        const bool masked = !whole((blk0 + (j * WK + wk) * BPT) * 32);
+        u32x4 x[2][NI];
+        static_for<0, NI>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            x[0][i] = lds_read_b128_at<i * 1024>(from);
+            x[1][i] = lds_read_b128_at<TILE + i * 1024>(from);
+        });
+        lds_wait_any();
+        if (j + 1 < steps) issue(j + 1);
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                u32x4 &v = x[z][i];
+                tie(v);
+                if (z == 1 && masked) {  // as above: out with V's infinities and NaN
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t bad = spread<T>(not_finite<T>(v[e]));
+                        v[e] &= ~bad;
+                        any |= bad;
+                    }
+                }
+                const int r = wblk * 32 + wrow + i * RPI + drow;  // of the tile
+                uint32_t w0[3], w1[3];
+                split3(__uint_as_float(v[0]), __uint_as_float(v[1]), w0);
+                split3(__uint_as_float(v[2]), __uint_as_float(v[3]), w1);
+                const int sw = z ? tree_vswz<CT, D>(r) : tree_kswz<CT, D>(r);
+                const uint32_t at = to + z * NPL * CTILE + r * RBC + (((dslot >> 1) ^ sw) * 16) + (dslot & 1) * 8;
+#pragma unroll
+                for (int k = 0; k < 3; k++) lds_write_b64(at + k * CTILE, u32x2{w0[k], w1[k]});
+            }
+        if (masked && __any(any != 0)) unfinite = 1;
     };
 
     // ---- the pipeline: one key group's wave refills a stage as soon as it has
     // read it; waves that share tiles refill behind the barrier that says that
     // all have ----
-    if constexpr (WR == 1) {
+    if constexpr (X3) {
+        for (int j = 0; j < steps; j++) {  // two buffers of pieces: one barrier a step
+            __builtin_amdgcn_s_waitcnt(vm_wait(0));
+            lds_order();
+            convert(j);
+            lds_wait_any();
+            wg_barrier();
+            tile(j);
+        }
+    } else if constexpr (WR == 1) {
         for (int j = 0; j < steps; j++) {
             if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -677,12 +783,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                     if (phys < 0 || phys >= kv.n_pages) continue;
                     at = (((int64_t)phys << kv.shift) + ((key0 + c) & ((1 << kv.shift) - 1))) * kv.rb;
                 }
-                const char *vp = kv.v + at + (int64_t)kvh * RB + (F ? 16 * kg * EB : kg * 4 * EB);
+                const char *vp = kv.v + at + (int64_t)kvh * RB + (FM ? 16 : 4) * kg * EB;
 #pragma unroll
                 for (int t = 0; t < NDT; t++) {
                     float v[4];
                     if constexpr (F) {
-                        const f32x4 r = *(const f32x4 *)(vp + ((t >> 2) * 64 + 4 * (t & 3)) * EB);
+                        const f32x4 r = *(const f32x4 *)(vp + (FM ? (t >> 2) * 64 + 4 * (t & 3) : t * 16) * EB);
 #pragma unroll
                         for (int e = 0; e < 4; e++) v[e] = r[e];
                     } else {
@@ -695,8 +801,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                         const bool bad = not_finite<F32>(__float_as_uint(v[e]));
 #pragma unroll
                         for (int x = 0; x < NR; x++) {
-                            f32x4 &o = F ? oacc[x][(t & ~3) + e] : oacc[x][t];
-                            if (bad && (see[x] >> c & 1)) o[F ? t & 3 : e] += v[e];
+                            f32x4 &o = FM ? oacc[x][(t & ~3) + e] : oacc[x][t];
+                            if (bad && (see[x] >> c & 1)) o[FM ? t & 3 : e] += v[e];
                         }
                     }
                 }
@@ -717,13 +823,13 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 #pragma unroll
     for (int x = 0; x < NR; x++) l_part[x] = rows_sum(l_part[x]);
     // Four consecutive columns from O tiles' registers: tile t (16-bit), or
-    // element c % 4 of four tiles (f32).
+    // element c % 4 of four tiles (f32 products).
     auto quad = [&](int x, int c) {
-        if constexpr (F) return f32x4{oacc[x][c & ~3][c & 3], oacc[x][(c & ~3) + 1][c & 3], oacc[x][(c & ~3) + 2][c & 3],
+        if constexpr (FM) return f32x4{oacc[x][c & ~3][c & 3], oacc[x][(c & ~3) + 1][c & 3], oacc[x][(c & ~3) + 2][c & 3],
                                       oacc[x][(c & ~3) + 3][c & 3]};
         else return oacc[x][c];
     };
-    auto qcol = [&](int c) { return F ? (c >> 2) * 64 + 16 * kg + 4 * (c & 3) : c * 16 + kg * 4; };
+    auto qcol = [&](int c) { return FM ? (c >> 2) * 64 + 16 * kg + 4 * (c & 3) : c * 16 + kg * 4; };
     if constexpr (WK == 1) {
 #pragma unroll
         for (int x = 0; x < NR; x++) {
@@ -854,6 +960,7 @@ inline TreeShape tree_shape(int dtype, int D, int rows) {
     const int most = D == 256 ? 1 : 2;            // row tiles of a wave: the registers hold no more
     const int wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;  // key groups with two stages each in LDS
     if (rows <= 16) return {1, 1, wk};
+    if (rb == 512 && most == 2 && rows > 64) return {1, 8, 1};  // f32 x 128 in pieces: three times the operands
     if (rows <= 16 * most) return {most, 1, wk};
     int wr = 2;
     while (wr < 8 && 16 * most * wr < rows) wr *= 2;
@@ -878,8 +985,11 @@ static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, 
 template <class T, int D, int PB>
 static void launch_shape(const TreeShape &s, const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
     constexpr int rb = D * T::bytes, most = D == 256 ? 1 : 2, wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;
-    if (s.wr == 8) launch_tree<T, D, most, 8, 1, PB>(a, kv, p, st);
-    else if (s.wr == 4) launch_tree<T, D, most, 4, std::min(wk, 2), PB>(a, kv, p, st);
+    constexpr bool x3_128 = __is_same(T, F32) && D == 128;
+    if (s.wr == 8) launch_tree<T, D, x3_128 ? 1 : most, 8, 1, PB>(a, kv, p, st);
+    else if (s.wr == 4) {
+        if constexpr (!x3_128) launch_tree<T, D, most, 4, std::min(wk, 2), PB>(a, kv, p, st);
+    }
     else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
     else if (s.nr == 2) {
         if constexpr (most == 2) launch_tree<T, D, 2, 1, wk, PB>(a, kv, p, st);
