@@ -1,6 +1,7 @@
 """The drafted trees' entry points on the CPU: bad arguments get their codes before
 any device work, sizes of the workspaces, and the masks."""
 import ctypes as C
+import re
 
 import numpy as np
 import pytest
@@ -137,6 +138,32 @@ def test_workspace_sizes():
     f = L.lib().ullm_hip_tree_workspace_bytes
     assert f(L.DT_F16, 1, 4, 100, 0, 8, 3, 128) == 0 and f(L.DT_F16, 1, 4, 100, 0, 8, 2, 96) == 0
     assert f(9, 1, 4, 100, 0, 8, 2, 128) == 0 and f(L.DT_F16, 0, 4, 100, 0, 8, 2, 128) == 0
+
+
+def _gpu_visible():
+    return torch.cuda.device_count() > 0
+
+
+@pytest.mark.parametrize("dt", [L.DT_F32, L.DT_F16, L.DT_BF16])
+@pytest.mark.parametrize("H,Hk,D", [(32, 8, 64), (12, 2, 128), (8, 4, 256), (32, 1, 128), (5, 5, 64)])
+def test_workspace_serves_every_smaller_call(dt, H, Hk, D):
+    """The header's promise, over shapes whose workgroups change with the sizes: what
+    a call needs is read from its refusal.  A call that needs none reaches a launch,
+    so this runs only where there is no GPU."""
+    if _gpu_visible():
+        pytest.skip("launches kernels on fake pointers when a GPU is visible; runs on CPU-only hosts")
+    for T in (1, 8, 17, 64, 130):
+        for win in (0, 100, 1024):
+            size = L.lib().ullm_hip_tree_workspace_bytes(dt, 8, T, 4096, win, H, Hk, D)
+            for B in (1, 3, 8):
+                for t in {1, T // 2 or 1, T}:
+                    for n in (1, 31, 40, 300, 1000, 4096):
+                        rc = call("attn_tree", ATTN, dtype=dt, odt=dt, kvs=Hk * D, ss=0, nodes=t, max_len=n, window=win,
+                                  batch=B, H=H, Hk=Hk, D=D, ws=None, wsn=0)
+                        if rc == L.E_WORKSPACE:
+                            assert int(re.search(rb"workspace of (\d+)", L.lib().ullm_hip_last_error()).group(1)) <= size
+                        else:
+                            assert rc in (L.OK, L.E_HIP)
 
 
 def test_tree_masks():

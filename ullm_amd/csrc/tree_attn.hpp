@@ -93,6 +93,16 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     return x;
 }
+__device__ __forceinline__ int wave_imax(int x) {
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor1, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor2, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppHalfMirror, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppMirror, 0xf, 0xf, false));
+    const auto r16 = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+    x = max((int)r16[0], (int)r16[1]);
+    const auto r32 = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+    return max((int)r32[0], (int)r32[1]);
+}
 __device__ __forceinline__ int lane_of(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
 // Which sequence and part of it slot `slot` is: parts are of at most `per`
@@ -106,6 +116,11 @@ struct TreePart {
     TreeSeq sq;
 };
 __device__ __forceinline__ TreePart find_part(const TreeArgs &a, const TreePlan &pl, int slot) {
+    if (pl.batch == 1) {
+        const TreeSeq q = tree_seq(a, 0);
+        const int per = max((q.blocks + pl.slots - 1) / pl.slots, pl.least), parts = max((q.blocks + per - 1) / per, 1);
+        return TreePart{slot < parts ? 0 : -1, slot, parts, 0, q};
+    }
     const int lane = threadIdx.x & 63;
     TreeSeq sq[4];
     int total = 0;
@@ -405,9 +420,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         int most = len;
         for (int i = node_of(row0) + lane; i <= node_of(min(row0 + ROWS, rows) - 1); i += 64)
             most = max(most, a.pos ? a.pos[(int64_t)b * a.nodes + i] : len + i);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
-        last = uni(most);
+        last = uni(wave_imax(most));
         clear0 = last - a.window + 1;
     }
     const int clear1 = len;
@@ -878,24 +891,27 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 // the latency of those loads: 33 parts of 312 rows x 128 take 18.9 us with one
 // group and one part at a time.
 template <int D, int ODT>
-__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, TreePlan pl, int ROWS, int log_g) {
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, TreePlan pl, int log_rows, int log_g) {
     constexpr int C4 = D / 4, U = 4;
     __shared__ f32x4 so[256];
     __shared__ float2 sml[256];
     const int tid = threadIdx.x, ng = 1 << log_g, c = tid % C4, g = tid / C4 & (ng - 1);
-    const int64_t row = (int64_t)blockIdx.x * (256 / C4 >> log_g) + (tid / C4 >> log_g);  // (node, head) of
-    const int b = blockIdx.y;                                                           // this sequence
+    const uint32_t row = blockIdx.x * (256 / C4 >> log_g) + (tid / C4 >> log_g);  // (node, head) of
+    const int b = blockIdx.y;                                                   // this sequence
     const int2 sq = pl.seq[b];
-    if (sq.y < 2) return;  // uniform
-    const int i = (int)(row / a.n_head), h = (int)(row % a.n_head);
+    const int i = (int)(row / (uint32_t)a.n_head), h = (int)(row - (uint32_t)i * a.n_head);
     const int n = a.n ? min(max(a.n[b], 0), a.nodes) : a.nodes;
+    if (sq.y < 2) return;  // uniform
     const bool there = i < n;
     float m = -INFINITY, l = 0.f;
     f32x4 o = {};
     if (there) {
-        const int G = a.kv_mul, kvh = h / G, r = i * G + h % G, rt = r / ROWS;
-        const int units = pl.n_kv * pl.row_tiles;
-        const int64_t at0 = ((int64_t)sq.x * units + kvh * pl.row_tiles + rt) * ROWS + r % ROWS, step = (int64_t)units * ROWS;
+        const int G = a.kv_mul;
+        int kvh = (int)__umulhi((uint32_t)h, a.inv_g);
+        kvh += h - kvh * G >= G;
+        const int r = i * G + h - kvh * G, rt = r >> log_rows, units = pl.n_kv * pl.row_tiles;
+        const int64_t step = (int64_t)units << log_rows;
+        const int64_t at0 = sq.x * step + ((int64_t)(kvh * pl.row_tiles + rt) << log_rows) + (r & ((1 << log_rows) - 1));
         for (int p0 = g; p0 < sq.y; p0 += U * ng) {
             float2 ml[U];
             f32x4 x[U];
@@ -955,6 +971,7 @@ struct TreeShape {
     int nr, wr, wk;
     int rows() const { return 16 * nr * wr; }
 };
+// The widest shape for so many rows, and the next narrower one.
 inline TreeShape tree_shape(int dtype, int D, int rows) {
     const int rb = D * dtype_bytes(dtype);        // bytes of a key
     const int most = D == 256 ? 1 : 2;            // row tiles of a wave: the registers hold no more
@@ -966,6 +983,11 @@ inline TreeShape tree_shape(int dtype, int D, int rows) {
     while (wr < 8 && 16 * most * wr < rows) wr *= 2;
     return {most, wr, std::min(wk, 8 / wr)};
 }
+inline TreeShape tree_narrower(int dtype, int D, const TreeShape &s) {
+    const int rows = s.rows() > 64 || D == 256 ? s.rows() / 2 : 32;
+    return tree_shape(dtype, D, std::max(rows, 16));
+}
+
 template <class T, int D, int NR, int WR, int WK, int PB>
 static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
     const int64_t items = (int64_t)p.slots * p.n_kv * p.row_tiles;
@@ -979,7 +1001,7 @@ static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, 
         while ((RPB >> log_g) > 1 && (4 << log_g) < p.slots / p.batch) log_g++;
         const int per = RPB >> log_g;
         launch_kernel(tree_merge_kernel<D, ODT>, dim3((unsigned)((rows + per - 1) / per), p.batch), dim3(256), 0, st, a, p,
-                      16 * NR * WR, log_g);
+                      __builtin_ctz(16 * NR * WR), log_g);
     }
 }
 template <class T, int D, int PB>
