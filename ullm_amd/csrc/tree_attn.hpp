@@ -357,7 +357,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     int node[NR], pos[NR];
 #pragma unroll
     for (int x = 0; x < NR; x++) {
-        const int r = row0 + (wr * NR + x) * 16 + n16;
+        const int r = row0 + (x * WR + wr) * 16 + n16;  // (row tiles are dealt to the waves in turn)
         const bool ok = r < rows;
         node[x] = ok ? node_of(r) : -1;
         pos[x] = 0;
@@ -479,20 +479,22 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     constexpr int KT = KB / 16;   // 16-key tiles of S^T
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
     bool mine = false;  // this wave's own tiles had infinities or NaN taken out
-    auto tile = [&](int j) __attribute__((always_inline)) {
+    // One tile for the first NX of the wave's row tiles.
+    auto tile_of = [&](auto nxc, int j) __attribute__((always_inline)) {
+        constexpr int NX = decltype(nxc)::value;
         const int tl = j * WK + wk;
-        if (tl >= tiles || row0 + wr * NR * 16 >= rows) return;  // (a wave may have no rows)
+        if (tl >= tiles) return;
         const uint32_t sb = lds_addr(ring) + (X3 ? NST * STAGE + (j & 1) * CONV : j % NST * STAGE);
         const int key0 = (blk0 + tl * BPT) * 32;
         const bool masked = !whole(key0);
-        uint32_t see[NR][BPT];
+        uint32_t see[NX][BPT];
         // Infinities and NaN in V leave a tile that some row does not see all of:
         // 0 times them would not be 0.  Who does see them gets them at the end.  (All
         // waves that share the tile write the same.)
         if (__builtin_expect(masked, 0)) {
-            MaskWords mw[NR];
+            MaskWords mw[NX];
 #pragma unroll
-            for (int x = 0; x < NR; x++) mw[x] = words(x, key0);
+            for (int x = 0; x < NX; x++) mw[x] = words(x, key0);
             if constexpr (!X3) {
             uint32_t any = 0;
             constexpr int U = TILE / 1024 < 8 ? TILE / 1024 : 8;  // pieces in flight
@@ -521,12 +523,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             }
             }
 #pragma unroll
-            for (int x = 0; x < NR; x++) sees(x, key0, mw[x], see[x]);
+            for (int x = 0; x < NX; x++) sees(x, key0, mw[x], see[x]);
         }
         // ---- S^T ----
-        f32x4 sacc[NR][KT];
+        f32x4 sacc[NX][KT];
 #pragma unroll
-        for (int x = 0; x < NR; x++)
+        for (int x = 0; x < NX; x++)
 #pragma unroll
             for (int t = 0; t < KT; t++) sacc[x][t] = f32x4{};
         uint32_t kaddr[NKA];
@@ -581,7 +583,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 u32x4 &k = kb[B & 1][decltype(ic)::value];
                 tie(k);
 #pragma unroll
-                for (int x = 0; x < NR; x++) {
+                for (int x = 0; x < NX; x++) {
                     if constexpr (FM) {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         // ---- masks, running maximum, weights: lane = row n16, keys t*16 + kg*4 + i ----
         if (__builtin_expect(masked, 0)) {
 #pragma unroll
-            for (int x = 0; x < NR; x++)
+            for (int x = 0; x < NX; x++)
 #pragma unroll
                 for (int u = 0; u < BPT; u++) {
                     const uint32_t s = see[x][u] >> (kg * 4);
@@ -608,10 +610,10 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                             if (!(s >> (t * 16 + i) & 1)) sacc[x][2 * u + t][i] = -INFINITY;
                 }
         }
-        float mt[NR];
+        float mt[NX];
         bool up = false;
 #pragma unroll
-        for (int x = 0; x < NR; x++) {
+        for (int x = 0; x < NX; x++) {
             float m = -INFINITY;
 #pragma unroll
             for (int t = 0; t < KT; t++) m = max3(max3(sacc[x][t][0], sacc[x][t][1], sacc[x][t][2]), sacc[x][t][3], m);
@@ -624,7 +626,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         }
         if (__any(up)) {
 #pragma unroll
-            for (int x = 0; x < NR; x++) {
+            for (int x = 0; x < NX; x++) {
                 const float mn = fmaxf(m_run[x], mt[x]), mu = mn == -INFINITY ? 0.f : mn;
                 const float corr = __builtin_amdgcn_exp2f(m_run[x] - mu);
                 l_part[x] *= corr;
@@ -633,9 +635,9 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 m_run[x] = mn;
             }
         }
-        u32x4 ph[NR][BPT][NP];
+        u32x4 ph[NX][BPT][NP];
 #pragma unroll
-        for (int x = 0; x < NR; x++) {
+        for (int x = 0; x < NX; x++) {
             const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
 #pragma unroll
             for (int t = 0; t < KT; t++)
@@ -681,7 +683,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 #pragma unroll
                     for (int e = 0; e < 4; e++)
 #pragma unroll
-                        for (int x = 0; x < NR; x++)
+                        for (int x = 0; x < NX; x++)
                             oacc[x][i * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vf[B & 1][i][e]),
                                                                                       sacc[x][B >> 2][B & 3], oacc[x][i * 4 + e], 0, 0, 0);
                 }
@@ -695,10 +697,15 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 #pragma unroll
                     for (int k = 0; k + i % NPL < NP; k++)
 #pragma unroll
-                        for (int x = 0; x < NR; x++) oacc[x][d0 + i / NPL] = mfma16<CT>(v, ph[x][u][k], oacc[x][d0 + i / NPL]);
+                        for (int x = 0; x < NX; x++) oacc[x][d0 + i / NPL] = mfma16<CT>(v, ph[x][u][k], oacc[x][d0 + i / NPL]);
                 }
             }
         });
+    };
+    auto tile = [&](int j) __attribute__((always_inline)) {
+        if (row0 + wr * 16 >= rows) return;  // uniform: a wave may have none, or fewer than NR
+        if (NR == 1 || row0 + (WR + wr) * 16 < rows) tile_of(Int<NR>{}, j);
+        else tile_of(Int<1>{}, j);
     };
     // The pieces of the K and V that this wave fetched, from the f32 tile into pieces
     // (X3); the next tile is fetched as soon as they are read.
@@ -846,7 +853,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     if constexpr (WK == 1) {
 #pragma unroll
         for (int x = 0; x < NR; x++) {
-            const int r = (wr * NR + x) * 16 + n16;
+            const int r = (x * WR + wr) * 16 + n16;
             const int64_t at = row_at(r);
             if (at < 0) continue;
             const float inv = inverse(l_part[x]);
@@ -858,7 +865,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         float *so = (float *)lds, *sml = (float *)(lds + WK * SMO);
 #pragma unroll
         for (int x = 0; x < NR; x++) {
-            const int r = (wr * NR + x) * 16 + n16;
+            const int r = (x * WR + wr) * 16 + n16;
 #pragma unroll
             for (int c = 0; c < NDT; c++) *(f32x4 *)(so + ((int64_t)wk * ROWS + r) * (D + 4) + qcol(c)) = quad(x, c);
             if (kg == 0) *(float2 *)(sml + (wk * ROWS + r) * 2) = float2{m_run[x], l_part[x]};
