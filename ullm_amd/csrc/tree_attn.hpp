@@ -228,13 +228,17 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     constexpr bool F = __is_same(T, F32);
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
     constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
-    constexpr int TILE = KB * RB, STAGE = 2 * TILE;  // as fetched
     constexpr bool X3 = F && WR >= 4 && D <= 128, FM = F && !X3;
+    // Where four tiles fit the ring, waves that share them take two a step: half the
+    // barriers (D = 128, 256 rows of bf16: 64 keys a step 240 us, 32 keys 305).
+    constexpr int FIT = tree_stages<WK, 2 * KB * RB>(), KS = !X3 && WR > 1 && FIT >= 4 ? 2 : 1;
+    constexpr int TILE = KS * KB * RB, STAGE = 2 * TILE;  // a step's tiles as fetched, K and K and V
     using CT = typename std::conditional<X3, BF16, T>::type;  // operands
     constexpr int NPL = X3 ? 3 : 1, NP = X3 ? 3 : PB;          // pieces of K, V and Q, and of P
     constexpr int RBC = D * CT::bytes, CTILE = KB * RBC;       // a row and a tile of one piece
     constexpr int CONV = 2 * NPL * CTILE;                      // K pieces, V pieces
-    constexpr int NST = X3 ? 1 : tree_stages<WK, STAGE>();
+    constexpr int VOFF = X3 ? NPL * CTILE : TILE;              // of V behind K
+    constexpr int NST = X3 ? 1 : FIT / KS;
     constexpr int GROUP = NST * STAGE + (X3 ? 2 * CONV : 0);   // LDS of a key group
     constexpr int NI = TILE / 1024 / WR;  // DMA instructions of a wave for K, and for V
     constexpr int NS = FM ? D / 16 : D / 32;  // 16-byte reads of a K row by a lane
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     // (waves that share tiles: the first barrier of the steps is behind it)
     if (WR > 1 && tid == 0) unfinite = 0;
     // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
-    constexpr int BPT = KB / 32;
+    constexpr int BPC = KB / 32, BPT = KS * BPC;  // blocks of a tile, of a step
     const int first = uni(sq.lo) / 32, size = ((blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
     const int blk0 = first + part * size, blk1 = min(blk0 + size, first + blocks);
     const int tiles = max(blk1 - blk0 + BPT - 1, 0) / BPT;
@@ -300,10 +304,10 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     // row (wr*NI + i)*RPI on, lane -> (row, slot) ----
     const int rb = (int)kv.rb;
     const int drow = lane / SLOTS, dslot = lane % SLOTS;
-    constexpr int SUB = KB / WR < 32 ? 1 : KB / WR / 32;  // (a wave's rows lie in one block)
-    static_assert(SUB == 1, "rows of a wave in one block");
-    const int wblk = wr * (KB / WR) / 32;         // that block of the tile
-    const int wrow = wr * (KB / WR) - wblk * 32;  // and its first row there
+    constexpr int WROWS = KS * KB / WR;  // rows that a wave fetches, in one block
+    static_assert(32 % WROWS == 0, "rows of a wave in one block");
+    const int wblk = wr * WROWS / 32;         // that block of the step
+    const int wrow = wr * WROWS - wblk * 32;  // and its first row there
     int kofs[NI], vofs[NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -407,12 +411,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     constexpr int NVA = FM ? 1 : RBC >= 256 ? 8 : 4;
     uint32_t va[NVA];
     if constexpr (FM) {
-        va[0] = CTILE + kg * 4 * RBC + n16 * 16;
+        va[0] = VOFF + kg * 4 * RBC + n16 * 16;
     } else {
         const int r = kg * 4 + (n16 >> 2);
 #pragma unroll
         for (int d = 0; d < NVA; d++)
-            va[d] = NPL * CTILE + r * RBC + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<CT, D>(r)) * 16) + 8 * (n16 & 1);
+            va[d] = VOFF + r * RBC + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<CT, D>(r)) * 16) + 8 * (n16 & 1);
     }
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0, last = 0;
@@ -428,7 +432,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     // 32 u + c.  The mask's words of the tile are read ahead (`words`), so that
     // they come while the tile is cleaned.
     struct MaskWords {
-        uint32_t w[BPT + 1];
+        uint32_t w[BPC + 1];
     };
     auto words = [&](int x, int key0) __attribute__((always_inline)) {
         MaskWords m{};
@@ -436,12 +440,12 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         const uint32_t *w = a.mask + ((int64_t)b * a.nodes + node[x]) * a.words;
         const int w0 = max(key0 - len, 0) >> 5;
 #pragma unroll
-        for (int i = 0; i <= BPT; i++) m.w[i] = w0 + i < a.words ? w[w0 + i] : 0;
+        for (int i = 0; i <= BPC; i++) m.w[i] = w0 + i < a.words ? w[w0 + i] : 0;
         return m;
     };
-    auto sees = [&](int x, int key0, const MaskWords &m, uint32_t (&see)[BPT]) __attribute__((always_inline)) {
+    auto sees = [&](int x, int key0, const MaskWords &m, uint32_t (&see)[BPC]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < BPT; u++) {
+        for (int u = 0; u < BPC; u++) {
             const int k0 = key0 + 32 * u, own = len - k0, j0 = -own;  // keys of the sequence in the block; its first node
             const uint32_t mine = own >= 32 ? ~0u : own > 0 ? (1u << own) - 1 : 0u;
             const int left = end - k0;  // keys that are there
@@ -455,7 +459,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                     t = m.w[0] << -j0;
                 } else {
                     const bool next = (j0 >> 5) > max(key0 - len, 0) >> 5;  // uniform
-                    const uint32_t lo = next ? m.w[BPT - 1] : m.w[0], hi = next ? m.w[BPT] : m.w[1];
+                    const uint32_t lo = next ? m.w[BPC - 1] : m.w[0], hi = next ? m.w[BPC] : m.w[1];
                     t = (uint32_t)((((uint64_t)hi << 32) | lo) >> (j0 & 31));
                 }
             }
@@ -479,15 +483,13 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     constexpr int KT = KB / 16;   // 16-key tiles of S^T
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
     bool mine = false;  // this wave's own tiles had infinities or NaN taken out
-    // One tile for the first NX of the wave's row tiles.
-    auto tile_of = [&](auto nxc, int j) __attribute__((always_inline)) {
+    // One tile, of block `blk` on, for the first NX of the wave's row tiles.  next: the
+    // step whose fetch goes out under this tile's products, if there is one.
+    auto tile_of = [&](auto nxc, uint32_t sb, int blk, int next) __attribute__((always_inline)) {
         constexpr int NX = decltype(nxc)::value;
-        const int tl = j * WK + wk;
-        if (tl >= tiles) return;
-        const uint32_t sb = lds_addr(ring) + (X3 ? NST * STAGE + (j & 1) * CONV : j % NST * STAGE);
-        const int key0 = (blk0 + tl * BPT) * 32;
+        const int key0 = blk * 32;
         const bool masked = !whole(key0);
-        uint32_t see[NX][BPT];
+        uint32_t see[NX][BPC];
         // Infinities and NaN in V leave a tile that some row does not see all of:
         // 0 times them would not be 0.  Who does see them gets them at the end.  (All
         // waves that share the tile write the same.)
@@ -497,10 +499,10 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             for (int x = 0; x < NX; x++) mw[x] = words(x, key0);
             if constexpr (!X3) {
             uint32_t any = 0;
-            constexpr int U = TILE / 1024 < 8 ? TILE / 1024 : 8;  // pieces in flight
+            constexpr int N = KB * RB / 1024, U = N < 8 ? N : 8;  // pieces, in flight
 #pragma unroll 1
-            for (int i = 0; i < TILE / 1024; i += U) {
-                const uint32_t at = sb + TILE + i * 1024 + lane * 16;
+            for (int i = 0; i < N; i += U) {
+                const uint32_t at = sb + VOFF + i * 1024 + lane * 16;
                 u32x4 v[U];
                 static_for<0, U>([&](auto uc) { v[decltype(uc)::value] = lds_read_b128_at<decltype(uc)::value * 1024>(at); });
                 lds_wait(v);
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         };
         // V^T operands, batch by batch: CV d tiles of one 32-key block, or one key of
         // each group (f32 products); the first goes out ahead of the softmax.
-        constexpr int CV = FM ? D / 64 : X3 ? 1 : 4, NBV = FM ? 4 * KT : BPT * NDT / CV;
+        constexpr int CV = FM ? D / 64 : X3 ? 1 : 4, NBV = FM ? 4 * KT : BPC * NDT / CV;
         uint32_t vaddr[NVA];
 #pragma unroll
         for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
@@ -596,12 +598,13 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 }
             });
         });
+        if (next < steps) issue(next);
         // ---- masks, running maximum, weights: lane = row n16, keys t*16 + kg*4 + i ----
         if (__builtin_expect(masked, 0)) {
 #pragma unroll
             for (int x = 0; x < NX; x++)
 #pragma unroll
-                for (int u = 0; u < BPT; u++) {
+                for (int u = 0; u < BPC; u++) {
                     const uint32_t s = see[x][u] >> (kg * 4);
 #pragma unroll
                     for (int t = 0; t < 2; t++)
@@ -635,7 +638,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 m_run[x] = mn;
             }
         }
-        u32x4 ph[NX][BPT][NP];
+        u32x4 ph[NX][BPC][NP];
 #pragma unroll
         for (int x = 0; x < NX; x++) {
             const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
@@ -648,7 +651,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
                 }
             if constexpr (!FM) {
 #pragma unroll
-                for (int u = 0; u < BPT; u++)
+                for (int u = 0; u < BPC; u++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const f32x4 &p = sacc[x][2 * u + (i >> 1)];
@@ -702,10 +705,20 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             }
         });
     };
-    auto tile = [&](int j) __attribute__((always_inline)) {
-        if (row0 + wr * 16 >= rows) return;  // uniform: a wave may have none, or fewer than NR
-        if (NR == 1 || row0 + (WR + wr) * 16 < rows) tile_of(Int<NR>{}, j);
-        else tile_of(Int<1>{}, j);
+    // Step j; next as above, INT_MAX: none.
+    auto step = [&](int j, int next) __attribute__((always_inline)) {
+        const int blk = blk0 + (j * WK + wk) * BPT;
+        if (row0 + wr * 16 >= rows || blk >= blk1) {  // uniform: a wave may have no rows, or fewer than NR tiles
+            if (next < steps) issue(next);
+            return;
+        }
+        const uint32_t sb = lds_addr(ring) + (X3 ? NST * STAGE + (j & 1) * CONV : j % NST * STAGE);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            if (s && blk + s * BPC >= blk1) break;
+            if (NR == 1 || row0 + (WR + wr) * 16 < rows) tile_of(Int<NR>{}, sb + s * KB * RB, blk + s * BPC, s ? INT_MAX : next);
+            else tile_of(Int<1>{}, sb + s * KB * RB, blk + s * BPC, s ? INT_MAX : next);
+        }
     };
     // The pieces of the K and V that this wave fetched, from the f32 tile into pieces
     // (X3); the next tile is fetched as soon as they are read.
@@ -758,14 +771,14 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             convert(j);
             lds_wait_any();
             wg_barrier();
-            tile(j);
+            step(j, INT_MAX);
         }
     } else if constexpr (WR == 1) {
         for (int j = 0; j < steps; j++) {
             if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
             lds_order();
-            tile(j);
+            step(j, INT_MAX);
             lds_wait_any();
             if (j + NST < steps) issue(j + NST);
         }
@@ -775,8 +788,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
             lds_wait_any();
             wg_barrier();
-            if (j + NST - 1 < steps) issue(j + NST - 1);
-            tile(j);
+            step(j, j + NST - 1);
         }
     }
 
@@ -785,14 +797,15 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     if (__builtin_expect(WR > 1 ? unfinite != 0 : mine, 0)) {
 #pragma unroll 1
         for (int k = 0; k < steps * BPT; k++) {
-            const int t0 = blk0 + (k / BPT * WK + wk) * BPT, u = k % BPT, key0 = (t0 + u) * 32;  // tile, block of it
+            const int t0 = blk0 + (k / BPT * WK + wk) * BPT + k % BPT / BPC * BPC, u = k % BPC;  // tile, block of it
+            const int key0 = (t0 + u) * 32;
             if (t0 + u >= blk1 || whole(t0 * 32)) continue;
             uint32_t see[NR];
 #pragma unroll
             for (int x = 0; x < NR; x++) {
-                uint32_t s[BPT];
+                uint32_t s[BPC];
                 sees(x, t0 * 32, words(x, t0 * 32), s);
-                see[x] = u ? s[BPT - 1] : s[0];
+                see[x] = u ? s[BPC - 1] : s[0];
             }
 #pragma unroll 1
             for (int c = 0; c < 32 && key0 + c < end; c++) {
