@@ -351,41 +351,57 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
         for (int i = 0; i < NI; i++) dma16_cached(vr, st + TILE + i * 1024, vofs[i], 0);
     };
 
-    // The first tiles go out ahead of everything else.
-#pragma unroll
-    for (int j = 0; j < (WR == 1 || X3 ? NST : NST - 1); j++)
-        if (j < steps) issue(j);
-
-    // ---- this wave's rows: Q^T operands, node, position ----
-    u32x4 q[NR][NPL][NS];
+    // ---- this wave's rows: Q^T operands, node, position.  Their loads go out ahead
+    // of the first tiles (loads return in order), and are waited for behind them. ----
+    u32x4 q[NR][NPL][NS], qf[NR][X3 ? 2 * NS : 1];
     int node[NR], pos[NR];
 #pragma unroll
     for (int x = 0; x < NR; x++) {
         const int r = row0 + (x * WR + wr) * 16 + n16;  // (row tiles are dealt to the waves in turn)
         const bool ok = r < rows;
         node[x] = ok ? node_of(r) : -1;
-        pos[x] = 0;
-        if (a.window > 0 && ok)
-            pos[x] = a.pos ? max(a.pos[(int64_t)b * a.nodes + node[x]], len) : len + node[x];
-        const char *qp = (const char *)a.q + (ok ? out_at(r) : out0) * EB + kg * 16;
+        const char *qp = (const char *)a.q + (ok ? out_at(r) : out0) * EB;
+#pragma unroll
+        for (int s = 0; s < (X3 ? 2 * NS : NS); s++) {
+            // X3: d = 32 s + 8 kg .. +7 of every two
+            const u32x4 v = *(const u32x4 *)(qp + (X3 ? (s >> 1) * 128 + kg * 32 + (s & 1) * 16 : s * 64 + kg * 16));
+            if constexpr (X3) qf[x][s] = v;
+            else q[x][0][s] = v;
+        }
+    }
+    // With a window: the rows' positions, and the last one among the workgroup's.
+    int most = len;
+    if (a.window > 0) {
+#pragma unroll
+        for (int x = 0; x < NR; x++)
+            pos[x] = node[x] < 0 ? 0 : a.pos ? a.pos[(int64_t)b * a.nodes + node[x]] : len + node[x];
+        const int i1 = node_of(min(row0 + ROWS, rows) - 1);
+        for (int i = node_of(row0) + lane; i <= i1; i += 64)
+            most = max(most, a.pos ? a.pos[(int64_t)b * a.nodes + i] : len + i);
+    }
+
+#pragma unroll
+    for (int j = 0; j < (WR == 1 || X3 ? NST : NST - 1); j++)
+        if (j < steps) issue(j);
+
+#pragma unroll
+    for (int x = 0; x < NR; x++) {
+        pos[x] = a.window > 0 ? max(pos[x], len) : 0;
+        const bool ok = node[x] >= 0;
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            if constexpr (X3) {  // d = 32 s + 8 kg .. +7
-                const u32x4 *at = (const u32x4 *)(qp + s * 128 + kg * 16);
-                u32x4 f[2] = {ok ? at[0] : u32x4{}, ok ? at[1] : u32x4{}};
+            if constexpr (X3) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
+                    const u32x4 &f = qf[x][2 * s + (i >> 1)];
                     uint32_t w[3];
-                    split3(__uint_as_float(f[i >> 1][2 * (i & 1)]), __uint_as_float(f[i >> 1][2 * (i & 1) + 1]), w);
+                    split3(__uint_as_float(f[2 * (i & 1)]), __uint_as_float(f[2 * (i & 1) + 1]), w);
 #pragma unroll
-                    for (int k = 0; k < 3; k++) q[x][k][s][i] = w[k];
+                    for (int k = 0; k < 3; k++) q[x][k][s][i] = ok ? w[k] : 0;
                 }
-            } else {
-                q[x][0][s] = ok ? *(const u32x4 *)(qp + s * 64) : u32x4{};
             }
         }
     }
-
     if (a.neg) {
         asm volatile("");  // (a branch, not a select that would wait for q here)
 #pragma unroll
@@ -421,9 +437,6 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0, last = 0;
     if (a.window > 0) {
-        int most = len;
-        for (int i = node_of(row0) + lane; i <= node_of(min(row0 + ROWS, rows) - 1); i += 64)
-            most = max(most, a.pos ? a.pos[(int64_t)b * a.nodes + i] : len + i);
         last = uni(wave_imax(most));
         clear0 = last - a.window + 1;
     }
@@ -884,23 +897,40 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
             if (kg == 0) *(float2 *)(sml + (wk * ROWS + r) * 2) = float2{m_run[x], l_part[x]};
         }
         __syncthreads();
-        for (int i = tid; i < ROWS * (D / 4); i += NT) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4;
-            const int64_t at = row_at(r);
-            if (at < 0) continue;
-            float m = -INFINITY, l = 0.f;
+        for (int r = tid; r < ROWS; r += NT) {  // the groups' weights in a row's sum
+            float m = -INFINITY, l = 0.f, c[WK];
 #pragma unroll
             for (int w = 0; w < WK; w++) m = fmaxf(m, sml[(w * ROWS + r) * 2]);
             const float mu = m == -INFINITY ? 0.f : m;
-            f32x4 o = {};
 #pragma unroll
             for (int w = 0; w < WK; w++) {
-                const float c = __builtin_amdgcn_exp2f(sml[(w * ROWS + r) * 2] - mu);
-                l += sml[(w * ROWS + r) * 2 + 1] * c;
-                o += *(const f32x4 *)(so + ((int64_t)w * ROWS + r) * (D + 4) + d) * c;
+                c[w] = __builtin_amdgcn_exp2f(sml[(w * ROWS + r) * 2] - mu);
+                l += sml[(w * ROWS + r) * 2 + 1] * c[w];
             }
-            emit(at + d, o, inverse(l));
-            if (parts > 1 && d == 0) pl.ml[wrow0 + r] = float2{m, l};
+            const float inv = parts == 1 ? inverse(l) : 1.f;
+#pragma unroll
+            for (int w = 0; w < WK; w++) sml[(w * ROWS + r) * 2] = c[w] * inv;
+            if (parts > 1 && row0 + r < rows) pl.ml[wrow0 + r] = float2{m, l};
+        }
+        __syncthreads();
+        constexpr int N = ROWS * (D / 4) / NT, U = N < 4 ? N : 4;  // quads of a thread, U at a time
+        static_assert(N % U == 0 && NT % (D / 4) == 0, "quads");
+        const int d = tid % (D / 4) * 4;
+        for (int i0 = 0; i0 < N; i0 += U) {
+            f32x4 o[U];
+            int64_t at[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int r = ((i0 + u) * NT + tid) / (D / 4);
+                at[u] = row_at(r);
+                o[u] = f32x4{};
+#pragma unroll
+                for (int w = 0; w < WK; w++)
+                    o[u] += *(const f32x4 *)(so + ((int64_t)w * ROWS + r) * (D + 4) + d) * sml[(w * ROWS + r) * 2];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (at[u] >= 0) emit(at[u] + d, o[u], 1.f);
         }
     }
 }
