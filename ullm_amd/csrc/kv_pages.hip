@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include "common.hpp"
+#include "wave.hpp"
 
 namespace ullm {
 
@@ -179,12 +180,7 @@ constexpr int kPagesMax = 1 << 20;  // pages of a pool: a bit each in LDS
 // Exclusive sum of v over the workgroup, and the total.
 __device__ __forceinline__ int block_scan(int v, int *tmp, int &total) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    const int x = wave_scan(v);
     __syncthreads();
     if (lane == 63) tmp[w] = x;
     __syncthreads();
@@ -198,42 +194,64 @@ __device__ __forceinline__ int block_scan(int v, int *tmp, int &total) {
     return before + x - v;
 }
 
+// One workgroup: marks the pages that stay in a bitmap in LDS, settles the
+// part-filled ones, and lists the free ones in order.  Bound by the latency of its
+// dependent loads (parent, length, table entry, page), which is why a thread keeps
+// the first sequence that is its own in registers and every loop has its loads in
+// flight together: 64 sequences of up to 16K in pages of 32 took 23.3 us with a
+// load at a time, 12.7 with 8 and the sequences kept in memory.
 __global__ __launch_bounds__(kPagesT) void pages_plan_kernel(PagesArgs a) {
     extern __shared__ uint32_t bits[];  // pages that stay: held or kept
     __shared__ int tmp[kPagesT / 64];
+    __shared__ int2 rows[kPagesT];  // old row and whole kept pages of the first sequences
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int words = (a.n_pages + 31) / 32;
-    if (a.held) {  // 64 pages a load of a wave
-        for (int c = wave; c * 64 < a.n_pages; c += kPagesT / 64) {
-            const int pg = c * 64 + lane;
-            const uint64_t m = __ballot(pg < a.n_pages && a.held[pg]);
-            if (lane < 2 && 2 * c + lane < words) bits[2 * c + lane] = (uint32_t)(m >> (32 * lane));
-        }
-    } else {
-        for (int w = tid; w < words; w += kPagesT) bits[w] = 0;
-    }
-    __syncthreads();
     const int64_t room = (int64_t)a.out_stride << a.shift, had = (int64_t)a.stride << a.shift;
-    for (int s = tid; s < a.n_out; s += kPagesT) {
+    auto first_look = [&](int s) {
         const int p = a.parent[s], cap = (int)min((int64_t)max(a.cap[s], 0), room);
         const int kept = p >= 0 && p < a.n_seq ? (int)min(min((int64_t)max(a.len[p], 0), had), (int64_t)cap) : 0;
         const int full = kept >> a.shift, part = kept & ((1 << a.shift) - 1);
         int last = part ? a.tab[(int64_t)p * a.stride + full] : -1;
         if (last < 0 || last >= a.n_pages) last = -1;
         if (last >= 0) __hip_atomic_store(a.owner + last, INT_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        a.seq[s] = PagesSeq{p, full, part, (int)((cap + (1ll << a.shift) - 1) >> a.shift), 0, last, 0, 0};
+        return PagesSeq{p, full, part, (int)((cap + (1ll << a.shift) - 1) >> a.shift), 0, last, 0, 0};
+    };
+    PagesSeq mine{};  // of sequence tid
+    if (tid < a.n_out) {
+        mine = first_look(tid);
+        rows[tid] = int2{mine.p, mine.full};
+    }
+    for (int s = tid + kPagesT; s < a.n_out; s += kPagesT) a.seq[s] = first_look(s);
+    if (a.held) {  // 64 pages a load of a wave
+        for (int c0 = wave; c0 * 64 < a.n_pages; c0 += kPagesU * (kPagesT / 64)) {
+            bool held[kPagesU];
+#pragma unroll
+            for (int u = 0; u < kPagesU; u++) {
+                const int pg = (c0 + u * (kPagesT / 64)) * 64 + lane;
+                held[u] = pg < a.n_pages && a.held[pg];
+            }
+#pragma unroll
+            for (int u = 0; u < kPagesU; u++) {
+                const int c = c0 + u * (kPagesT / 64);
+                const uint64_t m = __ballot(held[u]);
+                if (lane < 2 && 2 * c + lane < words) bits[2 * c + lane] = (uint32_t)(m >> (32 * lane));
+            }
+        }
+    } else {
+        for (int w = tid; w < words; w += kPagesT) bits[w] = 0;
     }
     __syncthreads();
-    for (int s = tid; s < a.n_out; s += kPagesT)
+    if (mine.last >= 0 && tid < a.n_out) atomicMin(a.owner + mine.last, tid);
+    for (int s = tid + kPagesT; s < a.n_out; s += kPagesT)
         if (a.seq[s].last >= 0) atomicMin(a.owner + a.seq[s].last, s);
     // whole pages: a wave takes a sequence, kPagesU loads of 64 entries in flight
     for (int s = wave; s < a.n_out; s += kPagesT / 64) {
-        const PagesSeq q = a.seq[s];
-        const int32_t *row = a.tab + (int64_t)q.p * a.stride;
-        for (int j0 = 0; j0 < q.full; j0 += 64 * kPagesU) {
+        int2 q = s < kPagesT ? rows[s] : int2{a.seq[s].p, a.seq[s].full};
+        const int32_t *row = a.tab + (int64_t)q.x * a.stride;
+        for (int j0 = 0; j0 < q.y; j0 += 64 * kPagesU) {
             int pg[kPagesU];
 #pragma unroll
-            for (int u = 0; u < kPagesU; u++) pg[u] = j0 + u * 64 + lane < q.full ? row[j0 + u * 64 + lane] : -1;
+            for (int u = 0; u < kPagesU; u++) pg[u] = j0 + u * 64 + lane < q.y ? row[j0 + u * 64 + lane] : -1;
 #pragma unroll
             for (int u = 0; u < kPagesU; u++)
                 if (pg[u] >= 0 && pg[u] < a.n_pages) atomicOr(&bits[pg[u] >> 5], 1u << (pg[u] & 31));
@@ -241,44 +259,48 @@ __global__ __launch_bounds__(kPagesT) void pages_plan_kernel(PagesArgs a) {
     }
     __syncthreads();
     // who keeps its part-filled page, and the new pages of each
-    int copies = 0, asked = 0;
+    auto keeps = [&](const PagesSeq &q, int s) {
+        return q.last >= 0 && !(bits[q.last >> 5] >> (q.last & 31) & 1) &&
+               __hip_atomic_load(a.owner + q.last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == s;
+    };
+    int asked = 0;
     for (int s0 = 0; s0 < a.n_out; s0 += kPagesT) {
         const int s = s0 + tid;
+        PagesSeq q = mine;
         int take = 0;
         if (s < a.n_out) {
-            const PagesSeq q = a.seq[s];
-            const bool mine = q.last >= 0 && !(bits[q.last >> 5] >> (q.last & 31) & 1) &&
-                              __hip_atomic_load(a.owner + q.last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == s;
-            a.seq[s].keeps = mine;
-            take = q.need - q.full - mine;
+            if (s0) q = a.seq[s];
+            q.keeps = keeps(q, s);
+            take = q.need - q.full - q.keeps;
         }
         int total;
-        const int first = block_scan(take, tmp, total);
-        if (s < a.n_out) a.seq[s].first = asked + first;
+        q.first = asked + block_scan(take, tmp, total);
+        if (s0 == 0) mine = q;
+        if (s < a.n_out) a.seq[s] = q;
         asked += total;
     }
-    __syncthreads();
-    for (int s = tid; s < a.n_out; s += kPagesT) {
+    // (every sum above is behind barriers: all have looked at the marks)
+    if (tid < a.n_out && mine.last >= 0) atomicOr(&bits[mine.last >> 5], 1u << (mine.last & 31));
+    for (int s = tid + kPagesT; s < a.n_out; s += kPagesT) {
         const int last = a.seq[s].last;
         if (last >= 0) atomicOr(&bits[last >> 5], 1u << (last & 31));
     }
     __syncthreads();
     // the free pages in order, as many as are asked for
     const int per = (words + kPagesT - 1) / kPagesT, w0 = tid * per, w1 = min(w0 + per, words);
-    int mine = 0, n_free;
-    for (int w = w0; w < w1; w++) {
+    auto free_of = [&](int w) {
         const uint32_t there = w * 32 + 32 <= a.n_pages ? ~0u : (1u << (a.n_pages & 31)) - 1;
-        mine += __popc(~bits[w] & there);
-    }
-    int rank = block_scan(mine, tmp, n_free);
-    for (int w = w0; w < w1 && rank < asked; w++) {
-        const uint32_t there = w * 32 + 32 <= a.n_pages ? ~0u : (1u << (a.n_pages & 31)) - 1;
-        for (uint32_t f = ~bits[w] & there; f && rank < asked; f &= f - 1)
-            a.free_list[rank++] = w * 32 + __builtin_ctz(f);
-    }
+        return ~bits[w] & there;
+    };
+    int count = 0, n_free;
+    for (int w = w0; w < w1; w++) count += __popc(free_of(w));
+    int rank = block_scan(count, tmp, n_free);
+    for (int w = w0; w < w1 && rank < asked; w++)
+        for (uint32_t f = free_of(w); f && rank < asked; f &= f - 1) a.free_list[rank++] = w * 32 + __builtin_ctz(f);
     // the new lengths: a part-filled page that should have been copied and could not is lost
+    int copies = 0;
     for (int s = tid; s < a.n_out; s += kPagesT) {
-        const PagesSeq q = a.seq[s];
+        const PagesSeq q = s == tid ? mine : a.seq[s];
         const bool copy = q.last >= 0 && !q.keeps, lost = copy && q.first >= n_free;
         copies += copy && !lost;
         a.len_out[s] = (q.full << a.shift) + (lost ? 0 : q.part);
