@@ -404,13 +404,15 @@ int ullm_hip_qkv_append_tree_paged(const float *q_in, const float *k_in, const f
  * a window > 0 those with t > positions[b][i] - window) and of the nodes' keys
  * seq_lens[b] + c those whose bit c its mask has (with a window those with
  * positions[b][c] > positions[b][i] - window).  What a key that a node does not
- * see holds, NaN and infinities included, does not reach the node.  A node that
- * sees no key, and rows from n_nodes[b] on, give zeros.
+ * see holds, NaN and infinities included, does not reach the node; an infinity in
+ * one that it sees may make it NaN.  A node that sees no key, and rows from
+ * n_nodes[b] on, give zeros.
  * q, out: [batch][max_nodes][n_head][head_dim]; q in the cache's dtype (f32, f16
  *         or bf16), out in the cache's dtype or f32 (out_dtype).  The softmax
  *         weights enter P.V in the cache's dtype where out has it, and in twice
  *         its bits for an f32 out of a 16-bit cache; an f32 cache runs on f32
- *         products throughout
+ *         products, or with many rows on exact bf16 pieces of its values whose
+ *         products are as good
  * mask:   int64[batch][max_nodes][ceil(max_nodes/64)], bit c % 64 of word c / 64
  *         (its own bit too: a node sees itself only by it), or NULL: node i sees
  *         the nodes up to i.  positions must be given where window > 0 and mask
@@ -421,8 +423,8 @@ int ullm_hip_qkv_append_tree_paged(const float *q_in, const float *k_in, const f
  * workspace: DEVICE memory of ullm_hip_tree_workspace_bytes, 256-byte aligned,
  *         needs no initialisation, one call at a time; a workspace for max_len,
  *         batch and max_nodes serves every call with smaller ones
- * max_nodes <= 1024; head_dim 64, 128 or 256; n_head % n_kv_head == 0; tensors
- * and row strides 16-byte aligned. */
+ * max_nodes <= 1024, max_nodes * n_head <= 2^23; head_dim 64, 128 or 256; n_head %
+ * n_kv_head == 0; tensors and row strides 16-byte aligned. */
 int ullm_hip_attn_tree(const void *q, const void *k_cache, const void *v_cache, int dtype,
                        int64_t kv_stride, int64_t seq_stride, const int64_t *mask,
                        const int32_t *seq_lens, const int32_t *n_nodes, const int32_t *positions,
@@ -448,7 +450,8 @@ size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int ma
  * 0..path_stride), in each of n_layer layers layer_stride elements apart, in
  * place.  path: int32[batch][path_stride], any order, a node also twice; entries
  * below 0 and rows outside the cache (n_ctx rows per sequence, the table, the
- * pool) are left as they are.  kv_dim elements of each row are moved.
+ * pool) are left as they are.  kv_dim elements of each row are moved; layers must
+ * not share rows, nor sequences of a contiguous cache (strides >= kv_dim).
  * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; not seq_lens itself.
  * path_stride <= 1024; pools, rows and strides 16-byte aligned.  Sequences must
  * not share the pages of their drafts (ullm_hip_kv_pages_update sees to it). */

@@ -34,7 +34,8 @@ BAD_ATTN = [
     (dict(kvs=255), L.E_INVALID), (dict(kvs=260), L.E_INVALID), (dict(kvs=1 << 40), L.E_INVALID),
     (dict(q=None), L.E_INVALID), (dict(k=None), L.E_INVALID), (dict(v=None), L.E_INVALID), (dict(lens=None), L.E_INVALID),
     (dict(out=None), L.E_INVALID), (dict(q=ODD), L.E_INVALID), (dict(k=ODD), L.E_INVALID), (dict(out=ODD), L.E_INVALID),
-    (dict(window=5, pos=None), L.E_INVALID),
+    (dict(window=5, pos=None), L.E_INVALID), (dict(nodes=1024, H=8200, Hk=2), L.E_INVALID),
+    (dict(batch=65535, H=512, Hk=256, kvs=256 * 128), L.E_INVALID),
 ]
 
 
@@ -98,7 +99,7 @@ ACCEPT = dict(k=FAKE, v=FAKE, dtype=L.DT_F16, kvs=256, ss=256 * 99, n_ctx=99, kv
     (dict(dtype=3), L.E_UNSUPPORTED), (dict(batch=-1), L.E_INVALID), (dict(batch=65536), L.E_INVALID), (dict(T=1025), L.E_INVALID),
     (dict(T=-1), L.E_INVALID), (dict(NL=0), L.E_INVALID), (dict(NL=40000), L.E_INVALID), (dict(kvd=0), L.E_INVALID),
     (dict(kvd=264), L.E_INVALID), (dict(kvd=4), L.E_INVALID), (dict(ss=-8), L.E_INVALID), (dict(ss=4), L.E_INVALID),
-    (dict(ls=4), L.E_INVALID), (dict(ls=-8), L.E_INVALID), (dict(n_ctx=-1), L.E_INVALID), (dict(k=None), L.E_INVALID),
+    (dict(ls=4), L.E_INVALID), (dict(ls=-8), L.E_INVALID), (dict(ls=0), L.E_INVALID), (dict(ss=0), L.E_INVALID), (dict(n_ctx=-1), L.E_INVALID), (dict(k=None), L.E_INVALID),
     (dict(path=None), L.E_INVALID), (dict(n=None), L.E_INVALID), (dict(lens=None), L.E_INVALID), (dict(k=ODD), L.E_INVALID),
     (dict(out=FAKE), L.E_INVALID), (dict(out=C.c_void_p(0x10004)), L.E_INVALID)])
 def test_accept_refuses(change, code):

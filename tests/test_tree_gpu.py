@@ -89,7 +89,7 @@ def ref(q, k, v, see, n, m, pos, window, scale, D):
             rows = vis[:, t]
             o[:m, h][rows] += p[rows, t, None] * vj[t]
             a[:m, h][rows] += p[rows, t, None] * vj[t].abs()
-        mag = (q[:m, h].abs() @ kj.nan_to_num(0, 0, 0).abs().t().contiguous() * scale).masked_fill(~vis, 0)
+        mag = (q[:m, h].abs() @ kj.nan_to_num(0, 0, 0).abs().t().contiguous() * abs(scale)).masked_fill(~vis, 0)
         e[:m, h, 0] = mag.amax(1)
     return o, a, e
 
@@ -174,6 +174,18 @@ CASES = [
     ("f16", "f16", 16, 2, 128, [1200], [300], 300, 64, 0, "tree", 0),
     ("f32", "f32", 4, 1, 128, [3000], [130], 130, 128, 0, "random", 0),
     ("f16", "f16", 3, 1, 64, [50], [1024], 1024, 32, 0, "tree", 0),
+    # enough keys and heads for workgroups of 65 rows and more, of each type and width
+    ("f32", "f32", 64, 32, 64, [1100], [60], 60, 64, 0, "tree", 0),
+    ("f32", "f32", 32, 16, 128, [1500, 700], [50, 41], 50, 32, 0, "random", 4),
+    ("f32", "f32", 64, 16, 64, [1300, 40], [64, 50], 64, 32, 21, "tree", 0),
+    ("f32", "f32", 32, 8, 256, [900, 300, 5], [30, 21, 30], 30, 64, 0, "tree", 0),
+    ("bf16", "f32", 64, 16, 128, [1500, 800], [64, 33], 64, 64, 0, "tree", 0),
+    ("f16", "f32", 32, 16, 256, [700, 801], [60, 59], 60, 0, 300, "tree", 8),
+    ("bf16", "bf16", 64, 16, 64, [1111, 2222], [50, 64], 64, 32, 0, "random", 0),
+    # more sequences than are looked at by a wave at once, of one workgroup each and cut
+    ("bf16", "bf16", 4, 2, 64, [(7 * i) % 201 for i in range(300)], [i % 4 for i in range(300)], 3, 32, 0, "tree", 0),
+    ("f16", "f16", 4, 1, 64, [6000 if i % 29 == 3 else 37 * i % 90 for i in range(130)], [5 - i % 3 for i in range(130)], 5, 32, 0, "tree", 0),
+    ("bf16", "bf16", 4, 2, 128, [5000 if i == 69 else 0 for i in range(70)], [1] * 70, 2, 64, 64, "chain", 0),
 ]
 
 
@@ -237,6 +249,45 @@ def test_unseen_keys_reach_no_node(dev, dt, D, page):
             assert out[b, 2].isnan().all()           # a NaN score
             assert out[b, 4, :H // Hk].isnan().all()  # a NaN value
             assert not torch.isfinite(out[b, 5]).all() and torch.isfinite(out[b, 5]).any()
+
+
+@pytest.mark.parametrize("dt,odt,D", [("f32", "f32", 64), ("f32", "f32", 128), ("f32", "f32", 256), ("bf16", "bf16", 128),
+                                      ("f16", "f32", 64), ("f16", "f16", 256), ("bf16", "f32", 256)])
+def test_unseen_keys_of_wide_trees(dev, dt, odt, D):
+    """The same with workgroups of 65 rows and more, whose waves share their tiles,
+    and with keys of a cut sequence: every node that does not see them is as if
+    they were zeros, every other is not finite."""
+    t, rng, H, Hk, T, n = DT[dt], np.random.default_rng(D + 1), 64, 32, 60, 1000
+    see, depth, _ = trees(rng, 1, T, "random")
+    see[0, :, 7] = see[0, :, 40] = False
+    see[0, 5, 7] = see[0, 33, 40] = True
+    pos = n + depth
+    caches, rows, _ = make(rng, dev, [n], [T], T, Hk, D, t, 0, 0, n + T)
+    q = torch.randn(1, T, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(3)).to(t)
+    args = (None, bits(see).to(dev), i32([n], dev), n + T, Hk, None, i32(pos, dev), 0)
+    for i in (7, 40):
+        for c in caches:
+            c[0, n + i] = 0
+    want = attend(q, caches, *args, out_dtype=DT[odt])
+    caches[0][0, n + 7], caches[1][0, n + 7] = NAN, math.inf
+    caches[1][0, n + 40, 1::2] = NAN
+    caches[1][0, n + 40, ::2] = -math.inf
+    out = attend(q, caches, *args, out_dtype=DT[odt])
+    others = [i for i in range(T) if i not in (5, 33)]
+    assert torch.equal(out[0, others], want[0, others])
+    assert not torch.isfinite(out[0, [5, 33]]).any()
+
+
+@pytest.mark.parametrize("dt,H,Hk,D,T", [("f32", 32, 16, 128, 50), ("f32", 4, 2, 64, 5), ("f16", 8, 2, 128, 20), ("bf16", 4, 4, 256, 40)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-3])
+def test_any_scale(dev, dt, H, Hk, D, T, scale):
+    t, n = DT[dt], 1200
+    g = torch.Generator(device=dev).manual_seed(8)
+    k, v = (torch.randn(1, n + T, Hk * D, device=dev, generator=g).to(t) for _ in "kv")
+    q = torch.randn(1, T, H, D, device=dev, generator=g).to(t)
+    out = A.attn_tree(q, k, v, None, i32([n], dev), n + T, Hk, scale=scale)
+    o, a, e = ref(q[0], k[0], v[0], np.tril(np.ones((T, T), bool)), n, T, np.arange(T) + n, 0, scale, D)
+    check(out[0], o, a, e, n + T, t, "scale")
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])

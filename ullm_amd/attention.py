@@ -529,7 +529,7 @@ class GpuAttention:
                         None if mask is None else mask.unsqueeze(0), lens, pos + T, p.n_kv_head,
                         positions=at, window=self._window(layer), scale=self.scale,
                         out_dtype=torch.float32)
-        return out.view(T, -1)
+        return out.view(T, p.n_head * p.head_dim)
 
     def accept(self, path, n_accept, pos: int):
         """Keep the accepted nodes of the draft at `pos` in every layer: path int32

@@ -46,6 +46,8 @@ static int attn_tree(const char *fn, TreeArgs a, TreeKv kv, int dtype, int64_t k
                          a.nodes);
     if (a.n_head < 1 || n_kv_head < 1 || a.n_head % n_kv_head || a.n_head > 65535)
         return set_error(ULLM_HIP_E_INVALID, "%s: bad heads", fn);
+    // (a grid has less than 2^32 threads)
+    if ((int64_t)a.nodes * a.n_head > 1 << 23) return set_error(ULLM_HIP_E_INVALID, "%s: too many rows", fn);
     if (a.max_len < 0 || a.window < 0) return set_error(ULLM_HIP_E_INVALID, "%s: bad max_len/window", fn);
     if (kv_stride < (int64_t)n_kv_head * head_dim || kv_stride > 0x7fffffff / 256)
         return set_error(ULLM_HIP_E_INVALID, "%s: kv_stride %lld", fn, (long long)kv_stride);
@@ -66,7 +68,7 @@ static int attn_tree(const char *fn, TreeArgs a, TreeKv kv, int dtype, int64_t k
     kv.rb = kv_stride * eb;
     TreeCut cut = tree_cut(dtype, batch, a.nodes, a.max_len, a.window, a.n_head, n_kv_head, head_dim);
     TreePlan &p = cut.plan;
-    if ((int64_t)p.slots * n_kv_head * p.row_tiles > 0x7fffffff / 2)
+    if ((int64_t)p.slots * n_kv_head * p.row_tiles > (1 << 23) - 8)
         return set_error(ULLM_HIP_E_INVALID, "%s: too many rows", fn);
     if (const size_t need = tree_bytes(cut.rows, batch, head_dim)) {
         if (!ws || ws_bytes < need || (uintptr_t)ws & 255)
@@ -126,7 +128,8 @@ extern "C" int ullm_hip_attn_tree_paged(const void *q, const void *k_pages, cons
 extern "C" size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int max_len, int window,
                                                 int n_head, int n_kv_head, int head_dim) {
     if (!dtype_ok(dtype) || (head_dim != 64 && head_dim != 128 && head_dim != 256) || batch < 1 || max_nodes < 1 ||
-        max_nodes > 1024 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || n_head > 65535 || max_len < 0)
+        max_nodes > 1024 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || n_head > 65535 || max_len < 0 ||
+        (int64_t)max_nodes * n_head > 1 << 23)
         return 0;
     // For every call with fewer sequences, nodes and positions too: at most 256
     // workgroups of at most the widest shape's rows, where there are keys to cut.

@@ -491,31 +491,31 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
 #pragma unroll
             for (int x = 0; x < NX; x++) mw[x] = words(x, key0);
             if constexpr (!X3) {
-            uint32_t any = 0;
-            constexpr int N = KB * RB / 1024, U = N < 8 ? N : 8;  // pieces, in flight
+                uint32_t any = 0;
+                constexpr int N = KB * RB / 1024, U = N < 8 ? N : 8;  // pieces, in flight
 #pragma unroll 1
-            for (int i = 0; i < N; i += U) {
-                const uint32_t at = sb + VOFF + i * 1024 + lane * 16;
-                u32x4 v[U];
-                static_for<0, U>([&](auto uc) { v[decltype(uc)::value] = lds_read_b128_at<decltype(uc)::value * 1024>(at); });
-                lds_wait(v);
+                for (int i = 0; i < N; i += U) {
+                    const uint32_t at = sb + VOFF + i * 1024 + lane * 16;
+                    u32x4 v[U];
+                    static_for<0, U>([&](auto uc) { v[decltype(uc)::value] = lds_read_b128_at<decltype(uc)::value * 1024>(at); });
+                    lds_wait(v);
 #pragma unroll
-                for (int k = 0; k < U; k++) {
-                    uint32_t bad = 0;
+                    for (int k = 0; k < U; k++) {
+                        uint32_t bad = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) bad |= not_finite<T>(v[k][e]);
-                    any |= bad;
-                    if (bad) {
+                        for (int e = 0; e < 4; e++) bad |= not_finite<T>(v[k][e]);
+                        any |= bad;
+                        if (bad) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) v[k][e] &= ~spread<T>(not_finite<T>(v[k][e]));
-                        lds_write_b128(at + k * 1024, v[k]);
+                            for (int e = 0; e < 4; e++) v[k][e] &= ~spread<T>(not_finite<T>(v[k][e]));
+                            lds_write_b128(at + k * 1024, v[k]);
+                        }
                     }
                 }
-            }
-            if (__any(any != 0)) {
-                if constexpr (WR > 1) unfinite = 1;
-                else mine = true;
-            }
+                if (__any(any != 0)) {
+                    if constexpr (WR > 1) unfinite = 1;
+                    else mine = true;
+                }
             }
 #pragma unroll
             for (int x = 0; x < NX; x++) sees(x, key0, mw[x], see[x]);
