@@ -5,11 +5,14 @@
 
 namespace ullm {
 
-// The cut of a call: as many slots as make one workgroup a CU, or one a sequence.
-// A workgroup holds as many rows as it can, so that K and V are read as few times
-// as can be, unless the keys are too few to give every CU a part of `least` blocks
-// (two tiles a key group): then fewer rows, and more workgroups (26 nodes x 6 heads
-// at 4K, 2 kv heads: 256 rows of a workgroup 14.3 us, 128 13.7, 64 12.2, 32 11.2).
+// The cut of a call: as many slots as make one workgroup a CU (two where they pair
+// up: 24 sequences of 1K and 35 rows, 8 kv heads, 21.2 us, by one a CU with all its
+// LDS 25.3), or one a sequence.  A workgroup holds as many rows as it can, so that K
+// and V are read as few times as can be, unless the keys are too few to give every
+// second CU a part of `least` blocks (two tiles a key group): then fewer rows, and
+// more workgroups (26 nodes x 6 heads at 4K, 2 kv heads: 256 rows of a workgroup 14.3
+// us, 128 12.1, 64 10.8, 32 11; 4 sequences of 66 rows x 256 with a window of 1K, 4 kv
+// heads: 128 rows 16.0, 64 17.6, 32 16.8).
 struct TreeCut {
     TreeShape shape;
     TreePlan plan;
@@ -25,8 +28,10 @@ static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window
         p.least = 2 * s.wk * (s.wr == 8 ? 2 : 1);
         const int64_t units = (int64_t)n_kv * p.row_tiles;
         const int64_t most = batch * ((keys / 32 + 2 + p.least - 1) / p.least);
-        if (s.wr > 1 && most * units < 256) continue;
-        p.slots = (int)std::max<int64_t>(batch, std::min<int64_t>(256 / units, most));
+        const bool pairs = tree_pairs(D * dtype_bytes(dtype), s.wr);
+        if (s.wr > 1 && most * units < (pairs ? 512 : 128)) continue;
+        p.slots = batch;
+        if (batch <= 256) p.slots = std::max(batch, (int)std::min<int64_t>((pairs ? 512 : 256) / units, most));
         return {s, p, p.slots > batch ? p.slots * units * s.rows() : 0};
     }
 }
@@ -131,9 +136,10 @@ extern "C" size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_no
         max_nodes > 1024 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || n_head > 65535 || max_len < 0 ||
         (int64_t)max_nodes * n_head > 1 << 23)
         return 0;
-    // For every call with fewer sequences, nodes and positions too: at most 256
-    // workgroups of at most the widest shape's rows, where there are keys to cut.
+    // For every call with fewer sequences, nodes and positions too: at most 256 cut
+    // sequences, and 256 workgroups of eight waves or 512 of fewer, of the widest
+    // shape's rows (of eight waves': or 512 of half), where there are keys to cut.
     const int64_t keys = window > 0 ? std::min<int64_t>(max_len, (int64_t)window + max_nodes) : max_len;
     const TreeShape s = tree_shape(dtype, head_dim, max_nodes * (n_head / n_kv_head));
-    return keys / 32 + 2 > 2 ? tree_bytes(256 * (int64_t)s.rows(), 255, head_dim) : 0;
+    return keys / 32 + 2 > 2 ? tree_bytes((s.wr == 8 ? 256 : 512) * (int64_t)s.rows(), 256, head_dim) : 0;
 }

@@ -185,9 +185,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
-template <int WK, int STAGE>
+// Two workgroups share a CU where the rings of both fit it (a workgroup of eight waves
+// has it to itself).
+constexpr bool tree_pairs(int rb, int wr) { return rb <= 512 && wr < 8; }
+constexpr int tree_waves(int rb, int wr, int wk) {  // of a SIMD
+    return std::max((tree_pairs(rb, wr) ? 2 : 1) * wr * wk / 4, 1);
+}
+template <int RB, int WR, int WK, int STAGE>
 constexpr int tree_stages() {
-    constexpr int n = 160 * 1024 / (WK * STAGE);
+    constexpr int n = (tree_pairs(RB, WR) ? 80 : 160) * 1024 / (WK * STAGE);
     return n > 4 ? 4 : n;
 }
 
@@ -204,14 +210,14 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t (&w)[3]) {
 }
 
 template <class T, int D, int NR, int WR, int WK, int PB>
-__global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
+__global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr bool F = __is_same(T, F32);
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
     constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
     constexpr bool X3 = F && WR >= 4 && D <= 128, FM = F && !X3;
     // Where four tiles fit the ring, waves that share them take two a step: half the
     // barriers (D = 128, 256 rows of bf16: 64 keys a step 240 us, 32 keys 305).
-    constexpr int FIT = tree_stages<WK, 2 * KB * RB>(), KS = !X3 && WR > 1 && FIT >= 4 ? 2 : 1;
+    constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && WR > 1 && FIT >= 4 ? 2 : 1;
     constexpr int TILE = KS * KB * RB, STAGE = 2 * TILE;  // a step's tiles as fetched, K and K and V
     using CT = typename std::conditional<X3, BF16, T>::type;  // operands
     constexpr int NPL = X3 ? 3 : 1, NP = X3 ? 3 : PB;          // pieces of K, V and Q, and of P
@@ -227,7 +233,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_kernel(TreeArgs a, TreeKv k
     static_assert((X3 || NST >= 2) && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
     constexpr int SMO = ROWS * (D + 4) * 4, SM = WK > 1 ? WK * (SMO + ROWS * 8) : 0;
     constexpr int LDS = WK * GROUP > SM ? WK * GROUP : SM;
-    static_assert(LDS + 16 <= 160 * 1024, "LDS");
+    static_assert(LDS + 16 <= (tree_pairs(RB, WR) ? 80 : 160) * 1024, "LDS");
     __shared__ __attribute__((aligned(1024))) char lds[LDS];
     __shared__ int unfinite;  // a V tile had infinities or NaN taken out
 
@@ -1005,13 +1011,13 @@ struct TreeShape {
 inline TreeShape tree_shape(int dtype, int D, int rows) {
     const int rb = D * dtype_bytes(dtype);        // bytes of a key
     const int most = D == 256 ? 1 : 2;            // row tiles of a wave: the registers hold no more
-    const int wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;  // key groups with two stages each in LDS
+    const int wk = rb <= 256 ? 2 : 1;             // key groups with two stages each in half a CU's LDS
     if (rows <= 16) return {1, 1, wk};
     if (rb == 512 && most == 2 && rows > 64) return {1, 8, 1};  // f32 x 128 in pieces: three times the operands
     if (rows <= 16 * most) return {most, 1, wk};
     int wr = 2;
     while (wr < 8 && 16 * most * wr < rows) wr *= 2;
-    return {most, wr, std::min(wk, 8 / wr)};
+    return {most, wr, wr <= 2 ? wk : 1};
 }
 inline TreeShape tree_narrower(int dtype, int D, const TreeShape &s) {
     const int rows = s.rows() > 64 || D == 256 ? s.rows() / 2 : 32;
@@ -1036,11 +1042,11 @@ static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, 
 }
 template <class T, int D, int PB>
 static void launch_shape(const TreeShape &s, const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
-    constexpr int rb = D * T::bytes, most = D == 256 ? 1 : 2, wk = rb <= 256 ? 4 : rb == 512 ? 2 : 1;
+    constexpr int rb = D * T::bytes, most = D == 256 ? 1 : 2, wk = rb <= 256 ? 2 : 1;
     constexpr bool x3_128 = __is_same(T, F32) && D == 128;
     if (s.wr == 8) launch_tree<T, D, x3_128 ? 1 : most, 8, 1, PB>(a, kv, p, st);
     else if (s.wr == 4) {
-        if constexpr (!x3_128) launch_tree<T, D, most, 4, std::min(wk, 2), PB>(a, kv, p, st);
+        if constexpr (!x3_128) launch_tree<T, D, most, 4, 1, PB>(a, kv, p, st);
     }
     else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
     else if (s.nr == 2) {
