@@ -31,6 +31,15 @@
 //    workgroups of all sequences are alike whatever their lengths; the lengths
 //    are on the device, so every workgroup works the cut out for itself
 //    (find_part).  tree_merge_kernel adds the parts up.
+// Measured (trace, this kernel without the merge): 8 sequences of 4K-32K, 64 nodes,
+// 32/4 heads of 128, bf16: 206 us, 143 GFLOP at 695 TFLOP/s (matrix instructions 31%
+// of the cycles, other vector instructions as many; the clock falls under it, 226 us
+// back to back; waves in two sets half a tile apart took 224); 24 sequences of 90-1500,
+// 7 nodes, 40/8 heads, bf16: 21.1 us, 84 MB at 4.0 TB/s, the chain of a workgroup's
+// start and end being 8 of them; f32, 2 sequences of 3K-8K, 48 nodes, 32/8 heads of 64:
+// 42.6 us, six products of 4.4 GFLOP at 620 TFLOP/s (with f32 products 75.6); one
+// sequence of 4K, 26 nodes, 12/2 heads of 128, f16: 11 us, of which the launch, the
+// first loads and the epilogue are 9.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -90,7 +99,7 @@ __device__ __forceinline__ int lane_of(int x, int l) { return __builtin_amdgcn_r
 // wave finds the same (any whole number of parts cuts a sequence rightly, so the
 // division need not be exact); at most 256 sequences are cut.  24 sequences take
 // 11000 cycles of a workgroup's start with cross-lane sums by LDS permutes and
-// steps of a sixteenth.
+// steps of a sixteenth, 3000 with row shifts and the estimate below.
 struct TreePart {
     int b, part, parts, slot0;
     TreeSeq sq;
@@ -405,21 +414,13 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
 #pragma unroll
         for (int i = 0; i < NDT; i++) oacc[x][i] = f32x4{};
     }
-    // Per-lane operand addresses within a tile.
-    constexpr int NKA = RBC >= 256 ? 4 : 2;  // chunks 16.. of a row sit 256 bytes on
-    uint32_t ka[NKA];
-#pragma unroll
-    for (int s = 0; s < NKA; s++) ka[s] = n16 * RBC + (((4 * s + kg) ^ tree_kswz<CT, D>(n16)) * 16);
-    constexpr int NVA = FM ? 1 : RBC >= 256 ? 8 : 4;
-    uint32_t va[NVA];
-    if constexpr (FM) {
-        va[0] = VOFF + kg * 4 * RBC + n16 * 16;
-    } else {
-        const int r = kg * 4 + (n16 >> 2);
-#pragma unroll
-        for (int d = 0; d < NVA; d++)
-            va[d] = VOFF + r * RBC + (((2 * d + ((n16 & 3) >> 1)) ^ tree_vswz<CT, D>(r)) * 16) + 8 * (n16 & 1);
-    }
+    // Per-lane operand addresses within a tile: of chunk 4s + kg of K, the others 64 s
+    // by exclusive or (a row of pieces is 128 bytes or more), chunks 16.. of a row 256
+    // bytes on; of d tile 0 of V^T, the others 32 d likewise.
+    constexpr int NKA = RBC >= 256 ? 4 : 2, NVA = RBC >= 256 ? 8 : 4;
+    const int ka = n16 * RBC + ((kg ^ tree_kswz<CT, D>(n16)) * 16), vrow = kg * 4 + (n16 >> 2);
+    const int va = FM ? VOFF + kg * 4 * RBC + n16 * 16
+                      : VOFF + vrow * RBC + ((((n16 & 3) >> 1) ^ tree_vswz<CT, D>(vrow)) * 16) + 8 * (n16 & 1);
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0, last = 0;
     if (a.window > 0) {
@@ -433,16 +434,16 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     struct MaskWords {
         uint32_t w[BPC + 1];
     };
-    auto words = [&](int x, int key0) __attribute__((always_inline)) {
+    auto words = [&](int node, int key0) __attribute__((always_inline)) {
         MaskWords m{};
-        if (!a.mask || node[x] < 0) return m;
-        const uint32_t *w = a.mask + ((int64_t)b * a.nodes + node[x]) * a.words;
+        if (!a.mask || node < 0) return m;
+        const uint32_t *w = a.mask + ((int64_t)b * a.nodes + node) * a.words;
         const int w0 = max(key0 - len, 0) >> 5;
 #pragma unroll
         for (int i = 0; i <= BPC; i++) m.w[i] = w0 + i < a.words ? w[w0 + i] : 0;
         return m;
     };
-    auto sees = [&](int x, int key0, const MaskWords &m, uint32_t (&see)[BPC]) __attribute__((always_inline)) {
+    auto sees = [&](int node, int pos, int lane, int key0, const MaskWords &m, uint32_t (&see)[BPC]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < BPC; u++) {
             const int k0 = key0 + 32 * u, own = len - k0, j0 = -own;  // keys of the sequence in the block; its first node
@@ -452,7 +453,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             uint32_t t = 0;
             if (own < 32) {
                 if (!a.mask) {
-                    const int c = node[x] - j0;  // bits 0..c
+                    const int c = node - j0;  // bits 0..c
                     t = c >= 31 ? ~0u : c >= 0 ? (2u << c) - 1 : 0u;
                 } else if (j0 < 0) {
                     t = m.w[0] << -j0;
@@ -464,18 +465,18 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             }
             uint32_t s = (mine | (t & ~mine)) & there;
             if (a.window > 0) {
-                const int64_t lo = (int64_t)pos[x] - a.window + 1 - k0;  // the window's first position, from the block's
+                const int64_t lo = (int64_t)pos - a.window + 1 - k0;  // the window's first position, from the block's
                 if (lo > 0) s &= ~(mine & (lo >= 32 ? ~0u : (1u << lo) - 1));
                 if (own < 32 && last - a.window >= len) {  // the window may end among the nodes
                     const int c = lane & 31, j = j0 + c;
                     int p = k0 + c;
                     if (a.pos && j >= 0 && j < n) p = max(a.pos[(int64_t)b * a.nodes + j], len);
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < 32; i++)
-                        if ((int64_t)lane_of(p, i) <= (int64_t)pos[x] - a.window) s &= ~((1u << i) & ~mine);
+                        if ((int64_t)lane_of(p, i) <= (int64_t)pos - a.window) s &= ~((1u << i) & ~mine);
                 }
             }
-            see[u] = node[x] < 0 ? 0 : s;
+            see[u] = node < 0 ? 0 : s;
         }
     };
     constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
@@ -493,15 +494,23 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
         // 0 times them would not be 0.  Who does see them gets them at the end.  (All
         // waves that share the tile write the same.)
         if (__builtin_expect(masked, 0)) {
+            // (copies that the compiler does not see through: what follows from them would
+            // take registers in the loop)
+            int nx[NX], px[NX], ln = lane;
+            asm volatile("" : "+v"(ln));
             MaskWords mw[NX];
 #pragma unroll
-            for (int x = 0; x < NX; x++) mw[x] = words(x, key0);
+            for (int x = 0; x < NX; x++) {
+                nx[x] = node[x], px[x] = pos[x];
+                asm volatile("" : "+v"(nx[x]), "+v"(px[x]));
+                mw[x] = words(nx[x], key0);
+            }
             if constexpr (!X3) {
                 uint32_t any = 0;
                 constexpr int N = KB * RB / 1024, U = N < 8 ? N : 8;  // pieces, in flight
 #pragma unroll 1
                 for (int i = 0; i < N; i += U) {
-                    const uint32_t at = sb + VOFF + i * 1024 + lane * 16;
+                    const uint32_t at = sb + VOFF + i * 1024 + ln * 16;
                     u32x4 v[U];
                     static_for<0, U>([&](auto uc) { v[decltype(uc)::value] = lds_read_b128_at<decltype(uc)::value * 1024>(at); });
                     lds_wait(v);
@@ -524,7 +533,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
                 }
             }
 #pragma unroll
-            for (int x = 0; x < NX; x++) sees(x, key0, mw[x], see[x]);
+            for (int x = 0; x < NX; x++) sees(nx[x], px[x], ln, key0, mw[x], see[x]);
         }
         // ---- S^T ----
         f32x4 sacc[NX][KT];
@@ -532,9 +541,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
         for (int x = 0; x < NX; x++)
 #pragma unroll
             for (int t = 0; t < KT; t++) sacc[x][t] = f32x4{};
-        uint32_t kaddr[NKA];
-#pragma unroll
-        for (int s = 0; s < NKA; s++) kaddr[s] = sb + ka[s];
+        const uint32_t kaddr = sb + ka;
         constexpr int KR = NS * NPL, CH = X3 ? 6 : NS < 4 ? NS : 4, NB = KT * KR / CH;  // reads of a key tile, of a batch
         u32x4 kb[2][CH];
         auto rdk = [&](auto bc) {
@@ -542,15 +549,13 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
                 constexpr int idx = decltype(bc)::value * CH + decltype(ic)::value, t = idx / KR, s = idx % KR / NPL;
                 constexpr int c = NKA == 4 ? s & 3 : s & 1, off = NKA == 4 ? (s >> 2) * 256 : 0;
                 kb[decltype(bc)::value & 1][decltype(ic)::value] =
-                    lds_read_b128_at<off + t * 16 * RBC + idx % NPL * CTILE>(kaddr[c]);
+                    lds_read_b128_at<off + t * 16 * RBC + idx % NPL * CTILE>(kaddr ^ 64 * c);
             });
         };
         // V^T operands, batch by batch: CV d tiles of one 32-key block, or one key of
         // each group (f32 products); the first goes out ahead of the softmax.
         constexpr int CV = FM ? D / 64 : X3 ? 1 : 4, NBV = FM ? 4 * KT : BPC * NDT / CV;
-        uint32_t vaddr[NVA];
-#pragma unroll
-        for (int d = 0; d < NVA; d++) vaddr[d] = sb + va[d];
+        const uint32_t vaddr = sb + va;
         u32x4 vf[2][FM ? CV : 1];
         u32x2 vlo[2][FM ? 1 : CV * NPL], vhi[2][FM ? 1 : CV * NPL];
         auto rdv = [&](auto bc) {
@@ -558,14 +563,14 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             if constexpr (FM)
                 static_for<0, CV>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
-                    vf[B & 1][i] = lds_read_b128_at<((B >> 2) * 16 + (B & 3)) * RBC + i * 256>(vaddr[0]);
+                    vf[B & 1][i] = lds_read_b128_at<((B >> 2) * 16 + (B & 3)) * RBC + i * 256>(vaddr);
                 });
             else
                 static_for<0, CV * NPL>([&](auto ic) {
                     constexpr int i = decltype(ic)::value, d = B * CV % NDT + i / NPL;
                     constexpr int off = d / NVA * 256 + B * CV / NDT * 32 * RBC + i % NPL * CTILE;
-                    vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr[d % NVA]);
-                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RBC>(vaddr[d % NVA]);
+                    vlo[B & 1][i] = lds_read_tr16_b64_at<off>(vaddr ^ 32 * (d % NVA));
+                    vhi[B & 1][i] = lds_read_tr16_b64_at<off + 16 * RBC>(vaddr ^ 32 * (d % NVA));
                 });
         };
         constexpr int VR = FM ? CV : 2 * CV * NPL;  // reads of a batch
@@ -803,7 +808,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
 #pragma unroll
             for (int x = 0; x < NR; x++) {
                 uint32_t s[BPC];
-                sees(x, t0 * 32, words(x, t0 * 32), s);
+                sees(node[x], pos[x], lane, t0 * 32, words(node[x], t0 * 32), s);
                 see[x] = u ? s[BPC - 1] : s[0];
             }
 #pragma unroll 1
