@@ -9,10 +9,11 @@ namespace ullm {
 // up: 24 sequences of 1K and 35 rows, 8 kv heads, 21.2 us, by one a CU with all its
 // LDS 25.3), or one a sequence.  A workgroup holds as many rows as it can, so that K
 // and V are read as few times as can be, unless the keys are too few to give every
-// second CU a part of `least` blocks (two tiles a key group): then fewer rows, and
-// more workgroups (26 nodes x 6 heads at 4K, 2 kv heads: 256 rows of a workgroup 14.3
-// us, 128 12.1, 64 10.8, 32 11; 4 sequences of 66 rows x 256 with a window of 1K, 4 kv
-// heads: 128 rows 16.0, 64 17.6, 32 16.8).
+// second CU a part of `least` blocks (three tiles a key group, below which the merge
+// grows by what the parts shrink): then fewer rows, and more workgroups (26 nodes x 6
+// heads at 4K, 2 kv heads, with the merge: 256 rows of a workgroup 18 us, 128 16.7, 64
+// 15.4, 32 14.8, in parts of two tiles 16.1 and of four 16.3; 4 sequences of 66 rows x
+// 256 with a window of 1K, 4 kv heads, without: 128 rows 16.0, 64 17.6, 32 16.8).
 struct TreeCut {
     TreeShape shape;
     TreePlan plan;
@@ -25,7 +26,7 @@ static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window
         TreePlan p{};
         p.batch = batch, p.n_kv = n_kv;
         p.row_tiles = (rows + s.rows() - 1) / s.rows();
-        p.least = 2 * s.wk * (s.wr == 8 ? 2 : 1);
+        p.least = s.wr == 8 ? 4 : 3 * s.wk;
         const int64_t units = (int64_t)n_kv * p.row_tiles;
         const int64_t most = batch * ((keys / 32 + 2 + p.least - 1) / p.least);
         const bool pairs = tree_pairs(D * dtype_bytes(dtype), s.wr);
