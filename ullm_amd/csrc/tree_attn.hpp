@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     constexpr bool F = __is_same(T, F32);
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
     constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
-    constexpr bool X3 = F && WR >= 4 && D <= 128, FM = F && !X3;
+    constexpr bool X3 = F && NR * WR > 4 && D <= 128, FM = F && !X3;
     // Where four tiles fit the ring, waves that share them take two a step: half the
     // barriers (D = 128, 256 rows of bf16: 64 keys a step 240 us, 32 keys 305).
     constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && WR > 1 && FIT >= 4 ? 2 : 1;
@@ -1012,21 +1012,21 @@ struct TreeShape {
     int nr, wr, wk;
     int rows() const { return 16 * nr * wr; }
 };
-// The widest shape for so many rows, and the next narrower one.
+// The widest shape for so many rows, and the next narrower one.  f32 products keep the
+// matrix units busy with one row tile of a wave, so up to 64 rows are dealt to more waves.
 inline TreeShape tree_shape(int dtype, int D, int rows) {
-    const int rb = D * dtype_bytes(dtype);        // bytes of a key
-    const int most = D == 256 ? 1 : 2;            // row tiles of a wave: the registers hold no more
-    const int wk = rb <= 256 ? 2 : 1;             // key groups with two stages each in half a CU's LDS
+    const int rb = D * dtype_bytes(dtype);  // bytes of a key
+    const int wk = rb <= 256 ? 2 : 1;       // key groups with two stages each in half a CU's LDS
+    // row tiles of a wave: the registers hold no more (f32 x 128 in pieces: three times the operands)
+    const int most = D == 256 || rb == 512 || (dtype == ULLM_DT_F32 && rows <= 64) ? 1 : 2;
     if (rows <= 16) return {1, 1, wk};
-    if (rb == 512 && most == 2 && rows > 64) return {1, 8, 1};  // f32 x 128 in pieces: three times the operands
     if (rows <= 16 * most) return {most, 1, wk};
     int wr = 2;
     while (wr < 8 && 16 * most * wr < rows) wr *= 2;
     return {most, wr, wr <= 2 ? wk : 1};
 }
 inline TreeShape tree_narrower(int dtype, int D, const TreeShape &s) {
-    const int rows = s.rows() > 64 || D == 256 ? s.rows() / 2 : 32;
-    return tree_shape(dtype, D, std::max(rows, 16));
+    return tree_shape(dtype, D, std::max(s.rows() / 2, 16));
 }
 
 template <class T, int D, int NR, int WR, int WK, int PB>
@@ -1047,13 +1047,16 @@ static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, 
 }
 template <class T, int D, int PB>
 static void launch_shape(const TreeShape &s, const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
-    constexpr int rb = D * T::bytes, most = D == 256 ? 1 : 2, wk = rb <= 256 ? 2 : 1;
-    constexpr bool x3_128 = __is_same(T, F32) && D == 128;
-    if (s.wr == 8) launch_tree<T, D, x3_128 ? 1 : most, 8, 1, PB>(a, kv, p, st);
+    constexpr bool F = __is_same(T, F32);
+    constexpr int rb = D * T::bytes, wide = D == 256 || rb == 512 ? 1 : 2, most = F ? 1 : wide, wk = rb <= 256 ? 2 : 1;
+    if (s.wr == 8) launch_tree<T, D, wide, 8, 1, PB>(a, kv, p, st);
     else if (s.wr == 4) {
-        if constexpr (!x3_128) launch_tree<T, D, most, 4, 1, PB>(a, kv, p, st);
-    }
-    else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
+        if (F && wide == 2 && s.nr == 2) {
+            if constexpr (F && wide == 2) launch_tree<T, D, 2, 4, 1, PB>(a, kv, p, st);
+        } else {
+            launch_tree<T, D, most, 4, 1, PB>(a, kv, p, st);
+        }
+    } else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
     else if (s.nr == 2) {
         if constexpr (most == 2) launch_tree<T, D, 2, 1, wk, PB>(a, kv, p, st);
     } else {
