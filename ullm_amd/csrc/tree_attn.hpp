@@ -197,6 +197,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Two workgroups share a CU where the rings of both fit it (a workgroup of eight waves
 // has it to itself).
 constexpr bool tree_pairs(int rb, int wr) { return rb <= 512 && wr < 8; }
+// Waves that share a tile's keys, 16 each: f32 products of few rows, whose rings leave
+// room for less than a wave a SIMD (8 sequences of 4K-8K, 14 rows x 256, 4 kv heads: 163
+// us with one wave a tile).
+constexpr int tree_halves(bool f32, int wr) { return f32 && wr <= 2 ? 2 : 1; }
 constexpr int tree_waves(int rb, int wr, int wk) {  // of a SIMD
     return std::max((tree_pairs(rb, wr) ? 2 : 1) * wr * wk / 4, 1);
 }
@@ -219,14 +223,17 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t (&w)[3]) {
 }
 
 template <class T, int D, int NR, int WR, int WK, int PB>
-__global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
+__global__ __launch_bounds__(64 * WR * WK * tree_halves(__is_same(T, F32), WR),
+                             tree_waves(D *T::bytes, WR, WK *tree_halves(__is_same(T, F32), WR)))
+void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr bool F = __is_same(T, F32);
+    constexpr int KH = tree_halves(F, WR), SH = WR * KH, GR = WK * KH;  // waves of a ring, groups of waves to add up
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
     constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile
     constexpr bool X3 = F && NR * WR > 4 && D <= 128, FM = F && !X3;
     // Where four tiles fit the ring, waves that share them take two a step: half the
     // barriers (D = 128, 256 rows of bf16: 64 keys a step 240 us, 32 keys 305).
-    constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && WR > 1 && FIT >= 4 ? 2 : 1;
+    constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && SH > 1 && FIT >= 4 ? 2 : 1;
     constexpr int TILE = KS * KB * RB, STAGE = 2 * TILE;  // a step's tiles as fetched, K and K and V
     using CT = typename std::conditional<X3, BF16, T>::type;  // operands
     constexpr int NPL = X3 ? 3 : 1, NP = X3 ? 3 : PB;          // pieces of K, V and Q, and of P
@@ -235,12 +242,12 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     constexpr int VOFF = X3 ? NPL * CTILE : TILE;              // of V behind K
     constexpr int NST = X3 ? 1 : FIT / KS;
     constexpr int GROUP = NST * STAGE + (X3 ? 2 * CONV : 0);   // LDS of a key group
-    constexpr int NI = TILE / 1024 / WR;  // DMA instructions of a wave for K, and for V
+    constexpr int NI = TILE / 1024 / SH;  // DMA instructions of a wave for K, and for V
     constexpr int NS = FM ? D / 16 : D / 32;  // 16-byte reads of a K row by a lane
     constexpr int NDT = D / 16;               // 16-wide d tiles of O^T
-    constexpr int ROWS = 16 * NR * WR, NT = 64 * WR * WK;
+    constexpr int ROWS = 16 * NR * WR, NT = 64 * SH * WK;
     static_assert((X3 || NST >= 2) && NI >= 1 && NI * RPI <= 32, "ring and DMA shape");
-    constexpr int SMO = ROWS * (D + 4) * 4, SM = WK > 1 ? WK * (SMO + ROWS * 8) : 0;
+    constexpr int SMO = ROWS * (D + 4) * 4, SM = GR > 1 ? GR * (SMO + ROWS * 8) : 0;
     constexpr int LDS = WK * GROUP > SM ? WK * GROUP : SM;
     static_assert(LDS + 16 <= (tree_pairs(RB, WR) ? 80 : 160) * 1024, "LDS");
     __shared__ __attribute__((aligned(1024))) char lds[LDS];
@@ -248,7 +255,8 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
     const int n16 = lane & 15, kg = lane >> 4;
-    const int wr = wave % WR, wk = wave / WR;
+    const int wr = wave % WR, wk = wave / SH, grp = wave / WR;  // grp: of the waves with all rows
+    const int wi = wave % SH, half = grp % KH;                 // of the ring; of a tile's keys
     // Work items (slot, kv head, row tile), the row tiles of one K/V range next
     // to each other on one XCD (workgroups are dealt to the 8 XCDs in turn).
     const int units = pl.n_kv * pl.row_tiles;
@@ -287,7 +295,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     if (row0 >= rows) return;
 
     // (waves that share tiles: the first barrier of the steps is behind it)
-    if (WR > 1 && tid == 0) unfinite = 0;
+    if (SH > 1 && tid == 0) unfinite = 0;
     // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
     constexpr int BPC = KB / 32, BPT = KS * BPC;  // blocks of a tile, of a step
     const int first = uni(sq.lo) / 32, size = ((blocks + parts - 1) / parts + BPT - 1) / BPT * BPT;
@@ -296,13 +304,13 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     const int steps = (tiles + WK - 1) / WK;
 
     // ---- K/V DMA: instruction i of this wave writes RPI rows of the tile from
-    // row (wr*NI + i)*RPI on, lane -> (row, slot) ----
+    // row (wi*NI + i)*RPI on, lane -> (row, slot) ----
     const int rb = (int)kv.rb;
     const int drow = lane / SLOTS, dslot = lane % SLOTS;
-    constexpr int WROWS = KS * KB / WR;  // rows that a wave fetches, in one block
+    constexpr int WROWS = KS * KB / SH;  // rows that a wave fetches, in one block
     static_assert(32 % WROWS == 0, "rows of a wave in one block");
-    const int wblk = wr * WROWS / 32;         // that block of the step
-    const int wrow = wr * WROWS - wblk * 32;  // and its first row there
+    const int wblk = wi * WROWS / 32;         // that block of the step
+    const int wrow = wi * WROWS - wblk * 32;  // and its first row there
     int kofs[NI], vofs[NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) {
@@ -339,7 +347,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
         const int range = ok ? (valid - 1) * rb + RB : 0;  // rows from `end` on read as zeros
         const auto kr = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(kv.k + at), 0, range, kRsrcWord3);
         const auto vr = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(kv.v + at), 0, range, kRsrcWord3);
-        char *st = ring + j % NST * STAGE + wr * NI * 1024;
+        char *st = ring + j % NST * STAGE + wi * NI * 1024;
 #pragma unroll
         for (int i = 0; i < NI; i++) dma16_cached(kr, st + i * 1024, kofs[i], 0);
 #pragma unroll
@@ -376,7 +384,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     }
 
 #pragma unroll
-    for (int j = 0; j < (WR == 1 || X3 ? NST : NST - 1); j++)
+    for (int j = 0; j < (SH == 1 || X3 ? NST : NST - 1); j++)
         if (j < steps) issue(j);
 
 #pragma unroll
@@ -418,8 +426,8 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     // by exclusive or (a row of pieces is 128 bytes or more), chunks 16.. of a row 256
     // bytes on; of d tile 0 of V^T, the others 32 d likewise.
     constexpr int NKA = RBC >= 256 ? 4 : 2, NVA = RBC >= 256 ? 8 : 4;
-    const int ka = n16 * RBC + ((kg ^ tree_kswz<CT, D>(n16)) * 16), vrow = kg * 4 + (n16 >> 2);
-    const int va = FM ? VOFF + kg * 4 * RBC + n16 * 16
+    const int hrow = half * 16, ka = (hrow + n16) * RBC + ((kg ^ tree_kswz<CT, D>(n16)) * 16), vrow = kg * 4 + (n16 >> 2);
+    const int va = FM ? VOFF + (hrow + kg * 4) * RBC + n16 * 16
                       : VOFF + vrow * RBC + ((((n16 & 3) >> 1) ^ tree_vswz<CT, D>(vrow)) * 16) + 8 * (n16 & 1);
     // Blocks from `clear0` up to `clear1` hold keys that every row of the workgroup sees.
     int clear0 = 0, last = 0;
@@ -480,7 +488,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
         }
     };
     constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
-    constexpr int KT = KB / 16;   // 16-key tiles of S^T
+    constexpr int KT = KB / 16 / KH;  // 16-key tiles of S^T of this wave
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
     bool mine = false;  // this wave's own tiles had infinities or NaN taken out
     // One tile, of block `blk` on, for the first NX of the wave's row tiles.  next: the
@@ -528,7 +536,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
                     }
                 }
                 if (__any(any != 0)) {
-                    if constexpr (WR > 1) unfinite = 1;
+                    if constexpr (SH > 1) unfinite = 1;
                     else mine = true;
                 }
             }
@@ -609,9 +617,9 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             for (int x = 0; x < NX; x++)
 #pragma unroll
                 for (int u = 0; u < BPC; u++) {
-                    const uint32_t s = see[x][u] >> (kg * 4);
+                    const uint32_t s = see[x][u] >> (hrow + kg * 4);
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                    for (int t = 0; t < 2 / KH; t++)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
                             if (!(s >> (t * 16 + i) & 1)) sacc[x][2 * u + t][i] = -INFINITY;
@@ -727,7 +735,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     // The pieces of the K and V that this wave fetched, from the f32 tile into pieces
     // (X3); the next tile is fetched as soon as they are read.
     auto convert = [&](int j) __attribute__((always_inline)) {
-        const uint32_t from = lds_addr(ring) + wr * NI * 1024 + lane * 16;
+        const uint32_t from = lds_addr(ring) + wi * NI * 1024 + lane * 16;
         const uint32_t to = lds_addr(ring) + NST * STAGE + (j & 1) * CONV;
         const bool masked = !whole((blk0 + (j * WK + wk) * BPT) * 32);
         u32x4 x[2][NI];
@@ -777,7 +785,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             wg_barrier();
             step(j, INT_MAX);
         }
-    } else if constexpr (WR == 1) {
+    } else if constexpr (SH == 1) {
         for (int j = 0; j < steps; j++) {
             if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
             else __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -797,8 +805,8 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
     }
 
     // ---- infinities and NaN in V, to the rows that see their keys ----
-    if constexpr (WR > 1 || WK > 1) __syncthreads();  // all tiles read, and the flag written
-    if (__builtin_expect(WR > 1 ? unfinite != 0 : mine, 0)) {
+    if constexpr (SH > 1 || WK > 1) __syncthreads();  // all tiles read, and the flag written
+    if (__builtin_expect(SH > 1 ? unfinite != 0 : mine, 0)) {
 #pragma unroll 1
         for (int k = 0; k < steps * BPT; k++) {
             const int t0 = blk0 + (k / BPT * WK + wk) * BPT + k % BPT / BPC * BPC, u = k % BPC;  // tile, block of it
@@ -812,7 +820,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
                 see[x] = u ? s[BPC - 1] : s[0];
             }
 #pragma unroll 1
-            for (int c = 0; c < 32 && key0 + c < end; c++) {
+            for (int c = hrow; c < hrow + 32 / KH && key0 + c < end; c++) {
                 int64_t at = b * kv.seq_b + (int64_t)(key0 + c) * kv.rb;
                 if (kv.tab) {
                     const int pi = (key0 + c) >> kv.shift;
@@ -867,7 +875,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
         else return oacc[x][c];
     };
     auto qcol = [&](int c) { return FM ? (c >> 2) * 64 + 16 * kg + 4 * (c & 3) : c * 16 + kg * 4; };
-    if constexpr (WK == 1) {
+    if constexpr (GR == 1) {
 #pragma unroll
         for (int x = 0; x < NR; x++) {
             const int r = (x * WR + wr) * 16 + n16;
@@ -879,28 +887,28 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
             if (parts > 1 && kg == 0) pl.ml[wrow0 + r] = float2{m_run[x], l_part[x]};
         }
     } else {
-        float *so = (float *)lds, *sml = (float *)(lds + WK * SMO);
+        float *so = (float *)lds, *sml = (float *)(lds + GR * SMO);
 #pragma unroll
         for (int x = 0; x < NR; x++) {
             const int r = (x * WR + wr) * 16 + n16;
 #pragma unroll
-            for (int c = 0; c < NDT; c++) *(f32x4 *)(so + ((int64_t)wk * ROWS + r) * (D + 4) + qcol(c)) = quad(x, c);
-            if (kg == 0) *(float2 *)(sml + (wk * ROWS + r) * 2) = float2{m_run[x], l_part[x]};
+            for (int c = 0; c < NDT; c++) *(f32x4 *)(so + ((int64_t)grp * ROWS + r) * (D + 4) + qcol(c)) = quad(x, c);
+            if (kg == 0) *(float2 *)(sml + (grp * ROWS + r) * 2) = float2{m_run[x], l_part[x]};
         }
         __syncthreads();
         for (int r = tid; r < ROWS; r += NT) {  // the groups' weights in a row's sum
-            float m = -INFINITY, l = 0.f, c[WK];
+            float m = -INFINITY, l = 0.f, c[GR];
 #pragma unroll
-            for (int w = 0; w < WK; w++) m = fmaxf(m, sml[(w * ROWS + r) * 2]);
+            for (int w = 0; w < GR; w++) m = fmaxf(m, sml[(w * ROWS + r) * 2]);
             const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int w = 0; w < WK; w++) {
+            for (int w = 0; w < GR; w++) {
                 c[w] = __builtin_amdgcn_exp2f(sml[(w * ROWS + r) * 2] - mu);
                 l += sml[(w * ROWS + r) * 2 + 1] * c[w];
             }
             const float inv = parts == 1 ? inverse(l) : 1.f;
 #pragma unroll
-            for (int w = 0; w < WK; w++) sml[(w * ROWS + r) * 2] = c[w] * inv;
+            for (int w = 0; w < GR; w++) sml[(w * ROWS + r) * 2] = c[w] * inv;
             if (parts > 1 && row0 + r < rows) pl.ml[wrow0 + r] = float2{m, l};
         }
         __syncthreads();
@@ -916,7 +924,7 @@ __global__ __launch_bounds__(64 * WR * WK, tree_waves(D *T::bytes, WR, WK)) void
                 at[u] = row_at(r);
                 o[u] = f32x4{};
 #pragma unroll
-                for (int w = 0; w < WK; w++)
+                for (int w = 0; w < GR; w++)
                     o[u] += *(const f32x4 *)(so + ((int64_t)w * ROWS + r) * (D + 4) + d) * sml[(w * ROWS + r) * 2];
             }
 #pragma unroll
@@ -1032,7 +1040,8 @@ inline TreeShape tree_narrower(int dtype, int D, const TreeShape &s) {
 template <class T, int D, int NR, int WR, int WK, int PB>
 static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
     const int64_t items = (int64_t)p.slots * p.n_kv * p.row_tiles;
-    launch_kernel(tree_kernel<T, D, NR, WR, WK, PB>, dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WR * WK), 0, st, a, kv, p);
+    launch_kernel(tree_kernel<T, D, NR, WR, WK, PB>, dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WR * WK * tree_halves(__is_same(T, F32), WR)), 0, st,
+                  a, kv, p);
     if (p.slots > p.batch) {
         constexpr int ODT = PB == 1 && !__is_same(T, F32) ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
         constexpr int RPB = 256 / (D / 4);  // rows of a workgroup with one group each
