@@ -19,14 +19,14 @@
 //    16-bit caches: 16x16x32, K by 16-byte LDS reads, V^T by the transposing
 //    LDS read.  f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads,
 //    the four elements of a read being four k-steps (K) or four d tiles (V); they
-//    run at a sixteenth of the 16-bit rate, which the stream of K and V hides up
-//    to 64 rows.  f32, more rows (X3): every value as the sum of three bf16 (8 bits
+//    run at a sixteenth of the 16-bit rate, which the stream of K and V about hides
+//    up to 64 rows.  f32, more rows (X3): every value as the sum of three bf16 (8 bits
 //    each, exact), six products of the 16-bit rate (those above 2^-24 of the
 //    whole), K and V tiles split once by the waves that fetched them.
 //  * K and V tiles come by LDS DMA into a ring, one 32-key block a page lookup.
 //  * A workgroup is WR x WK waves of 16*NR rows: the WR waves of a key group
-//    share its tiles, the WK key groups take tiles in turn and are added up
-//    through LDS at the end.
+//    share its tiles (f32 up to 32 rows: 2 WR waves, of 16 of a tile's keys each),
+//    the WK key groups take tiles in turn and are added up through LDS at the end.
 //  * The keys of a sequence are cut into parts, one workgroup each, so that the
 //    workgroups of all sequences are alike whatever their lengths; the lengths
 //    are on the device, so every workgroup works the cut out for itself
@@ -37,7 +37,7 @@
 // back to back; waves in two sets half a tile apart took 224); 24 sequences of 90-1500,
 // 7 nodes, 40/8 heads, bf16: 21.1 us, 84 MB at 4.0 TB/s, the chain of a workgroup's
 // start and end being 8 of them; f32, 2 sequences of 3K-8K, 48 nodes, 32/8 heads of 64:
-// 42.6 us, six products of 4.4 GFLOP at 620 TFLOP/s (with f32 products 75.6); one
+// 42.4 us, six products of 4.4 GFLOP at 620 TFLOP/s (with f32 products 75.6); one
 // sequence of 4K, 26 nodes, 12/2 heads of 128, f16: 11 us, of which the launch, the
 // first loads and the epilogue are 9.
 #include <algorithm>
@@ -199,7 +199,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 constexpr bool tree_pairs(int rb, int wr) { return rb <= 512 && wr < 8; }
 // Waves that share a tile's keys, 16 each: f32 products of few rows, whose rings leave
 // room for less than a wave a SIMD (8 sequences of 4K-8K, 14 rows x 256, 4 kv heads: 163
-// us with one wave a tile).
+// us with one wave a tile, 101 with two).
 constexpr int tree_halves(bool f32, int wr) { return f32 && wr <= 2 ? 2 : 1; }
 constexpr int tree_waves(int rb, int wr, int wk) {  // of a SIMD
     return std::max((tree_pairs(rb, wr) ? 2 : 1) * wr * wk / 4, 1);
