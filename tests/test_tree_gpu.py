@@ -182,6 +182,11 @@ CASES = [
     ("bf16", "f32", 64, 16, 128, [1500, 800], [64, 33], 64, 64, 0, "tree", 0),
     ("f16", "f32", 32, 16, 256, [700, 801], [60, 59], 60, 0, 300, "tree", 8),
     ("bf16", "bf16", 64, 16, 64, [1111, 2222], [50, 64], 64, 32, 0, "random", 0),
+    # and of 17 to 32 rows, whose waves share the keys of a tile over f32
+    ("f32", "f32", 64, 32, 64, [1100, 1000, 900], [16, 15, 9], 16, 32, 0, "tree", 0),
+    ("f32", "f32", 64, 32, 128, [1100, 950], [16, 10], 16, 0, 400, "tree", 0),
+    ("f32", "f32", 32, 16, 256, [1000, 333], [15, 16], 16, 64, 7, "tree", 4),
+    ("f16", "f16", 64, 32, 128, [1500, 1200], [16, 10], 16, 32, 0, "random", 0),
     # more sequences than are looked at by a wave at once, of one workgroup each and cut
     ("bf16", "bf16", 4, 2, 64, [(7 * i) % 201 for i in range(300)], [i % 4 for i in range(300)], 3, 32, 0, "tree", 0),
     ("f16", "f16", 4, 1, 64, [6000 if i % 29 == 3 else 37 * i % 90 for i in range(130)], [5 - i % 3 for i in range(130)], 5, 32, 0, "tree", 0),
@@ -251,31 +256,33 @@ def test_unseen_keys_reach_no_node(dev, dt, D, page):
             assert not torch.isfinite(out[b, 5]).all() and torch.isfinite(out[b, 5]).any()
 
 
-@pytest.mark.parametrize("dt,odt,D", [("f32", "f32", 64), ("f32", "f32", 128), ("f32", "f32", 256), ("bf16", "bf16", 128),
-                                      ("f16", "f32", 64), ("f16", "f16", 256), ("bf16", "f32", 256)])
-def test_unseen_keys_of_wide_trees(dev, dt, odt, D):
-    """The same with workgroups of 65 rows and more, whose waves share their tiles,
+@pytest.mark.parametrize("dt,odt,D,T,n", [
+    ("f32", "f32", 64, 60, 1000), ("f32", "f32", 128, 60, 1000), ("f32", "f32", 256, 60, 1000), ("bf16", "bf16", 128, 60, 1000),
+    ("f16", "f32", 64, 60, 1000), ("f16", "f16", 256, 60, 1000), ("bf16", "f32", 256, 60, 1000),
+    ("f32", "f32", 64, 45, 3200), ("f32", "f32", 64, 16, 3200), ("f32", "f32", 128, 16, 1600), ("f32", "f32", 256, 16, 1000)])
+def test_unseen_keys_of_wide_trees(dev, dt, odt, D, T, n):
+    """The same with workgroups of 17 rows and more, whose waves share their tiles,
     and with keys of a cut sequence: every node that does not see them is as if
     they were zeros, every other is not finite."""
-    t, rng, H, Hk, T, n = DT[dt], np.random.default_rng(D + 1), 64, 32, 60, 1000
+    t, rng, H, Hk, last = DT[dt], np.random.default_rng(D + 1), 64, 32, T - 3
     see, depth, _ = trees(rng, 1, T, "random")
-    see[0, :, 7] = see[0, :, 40] = False
-    see[0, 5, 7] = see[0, 33, 40] = True
+    see[0, :, 7] = see[0, :, last] = False
+    see[0, 5, 7] = see[0, 12, last] = True
     pos = n + depth
     caches, rows, _ = make(rng, dev, [n], [T], T, Hk, D, t, 0, 0, n + T)
     q = torch.randn(1, T, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(3)).to(t)
     args = (None, bits(see).to(dev), i32([n], dev), n + T, Hk, None, i32(pos, dev), 0)
-    for i in (7, 40):
+    for i in (7, last):
         for c in caches:
             c[0, n + i] = 0
     want = attend(q, caches, *args, out_dtype=DT[odt])
     caches[0][0, n + 7], caches[1][0, n + 7] = NAN, math.inf
-    caches[1][0, n + 40, 1::2] = NAN
-    caches[1][0, n + 40, ::2] = -math.inf
+    caches[1][0, n + last, 1::2] = NAN
+    caches[1][0, n + last, ::2] = -math.inf
     out = attend(q, caches, *args, out_dtype=DT[odt])
-    others = [i for i in range(T) if i not in (5, 33)]
+    others = [i for i in range(T) if i not in (5, 12)]
     assert torch.equal(out[0, others], want[0, others])
-    assert not torch.isfinite(out[0, [5, 33]]).any()
+    assert not torch.isfinite(out[0, [5, 12]]).any()
 
 
 @pytest.mark.parametrize("dt,H,Hk,D,T", [("f32", 32, 16, 128, 50), ("f32", 4, 2, 64, 5), ("f16", 8, 2, 128, 20), ("bf16", 4, 4, 256, 40)])
@@ -358,6 +365,30 @@ def test_strides_and_scale(dev):
     for b, m in enumerate((n, n - 50)):
         r = ref(q[b], k[:m + T], v[:m + T], see, m, T, np.arange(T) + m, 0, 0.3, D)
         check(out[b], *r, n, t, f"b={b}")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [0, 32])
+def test_keys_past_max_len_and_no_positions(dev, dt, page):
+    """A max_len inside the drafts cuts their keys, not their rows; without
+    positions a window goes by the slots (and is refused over a mask)."""
+    t, rng, H, Hk, D, T, lens = DT[dt], np.random.default_rng(4), 8, 2, 128, 11, [60, 90]
+    caches, rows, table = make(rng, dev, lens, [T, T], T, Hk, D, t, page, 0, 101)
+    q = torch.randn(2, T, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(6)).to(t)
+    see, _, mask = trees(rng, 2, T, "tree")
+    out = attend(q, caches, table, mask.to(dev), i32(lens, dev), 95, Hk, None, None, 0)
+    cut = see.copy()
+    cut[1, :, 5:] = False
+    for b in range(2):
+        r = ref(q[b], rows[0][b], rows[1][b], cut[b], lens[b], T, lens[b] + np.arange(T), 0, D ** -0.5, D)
+        check(out[b], *r, 101, t, f"b={b}")
+    out = attend(q, caches, table, None, i32(lens, dev), 101, Hk, None, None, 9)
+    for b in range(2):
+        r = ref(q[b], rows[0][b], rows[1][b], np.tril(np.ones((T, T), bool)), lens[b], T, lens[b] + np.arange(T), 9, D ** -0.5, D)
+        check(out[b], *r, 101, t, f"b={b}")
+    with pytest.raises(L.UllmHipError) as e:
+        attend(q, caches, table, mask.to(dev), i32(lens, dev), 101, Hk, None, None, 9)
+    assert e.value.code == L.E_INVALID
 
 
 def test_nothing_drafted(dev):
