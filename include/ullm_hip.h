@@ -489,7 +489,8 @@ int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype, int64_t kv
  * info:      int32[3]: pages copied, pages taken, pages missing
  * The pools hold n_layer layers, layer_stride elements apart (0: only the table
  * is made and nothing is copied).  page_size: a power of two; n_pages <= 2^20;
- * n_out <= 65535 (0: nothing is written); pools and strides 16-byte aligned.
+ * n_out <= 65535 (0: nothing is written), n_out * out_stride < 2^31; pools and
+ * strides 16-byte aligned.
  * workspace: DEVICE memory of ullm_hip_kv_pages_workspace_bytes, 256-byte
  * aligned, needs no initialisation, one call at a time. */
 int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,

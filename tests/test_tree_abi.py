@@ -122,7 +122,7 @@ UPDATE = dict(k=FAKE, v=FAKE, dtype=L.DT_F16, kvs=256, P=32, pages=99, NL=2, ls=
     (dict(dtype=3), L.E_UNSUPPORTED), (dict(P=33), L.E_INVALID), (dict(pages=0), L.E_UNSUPPORTED),
     (dict(pages=(1 << 20) + 1), L.E_UNSUPPORTED), (dict(NL=-1), L.E_INVALID), (dict(S=-1), L.E_INVALID),
     (dict(n=-1), L.E_INVALID), (dict(n=65536), L.E_INVALID), (dict(cols=0), L.E_INVALID), (dict(out_cols=0), L.E_INVALID),
-    (dict(out_cols=1 << 27), L.E_INVALID), (dict(cols=1 << 27), L.E_INVALID), (dict(kvs=0), L.E_INVALID),
+    (dict(out_cols=1 << 27), L.E_INVALID), (dict(n=65535, out_cols=(1 << 15) + 1), L.E_INVALID), (dict(n=3, out_cols=1 << 30, P=1), L.E_INVALID), (dict(cols=1 << 27), L.E_INVALID), (dict(kvs=0), L.E_INVALID),
     (dict(kvs=4), L.E_INVALID), (dict(ls=4), L.E_INVALID), (dict(ls=-8), L.E_INVALID), (dict(k=None), L.E_INVALID),
     (dict(tab=None), L.E_INVALID), (dict(lens=None), L.E_INVALID), (dict(parent=None), L.E_INVALID), (dict(cap=None), L.E_INVALID),
     (dict(to=None), L.E_INVALID), (dict(lo=None), L.E_INVALID), (dict(info=None), L.E_INVALID), (dict(k=ODD), L.E_INVALID),

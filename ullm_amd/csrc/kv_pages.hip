@@ -401,6 +401,8 @@ extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype,
         return set_error(ULLM_HIP_E_INVALID, "%s: bad sizes", fn);
     if ((int64_t)page_size * table_stride > INT_MAX || (int64_t)page_size * out_stride > INT_MAX)
         return set_error(ULLM_HIP_E_INVALID, "%s: a table of 2^31 positions or more", fn);
+    if ((int64_t)n_out * out_stride > INT_MAX)  // (the pages asked for are counted in 32 bits)
+        return set_error(ULLM_HIP_E_INVALID, "%s: a table of 2^31 entries or more", fn);
     if (n_out == 0) return ULLM_HIP_OK;
     if ((n_layer && (!k_pages || !v_pages)) || (n_seq && (!block_table || !seq_lens)) || !parent || !capacity ||
         !table_out || !lens_out || !info)
