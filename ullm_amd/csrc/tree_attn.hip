@@ -5,35 +5,80 @@
 
 namespace ullm {
 
-// The cut of a call: as many slots as make one workgroup a CU (two where they pair
-// up: 24 sequences of 1K and 35 rows, 8 kv heads, 21.2 us, by one a CU with all its
-// LDS 25.3), or one a sequence.  A workgroup holds as many rows as it can, so that K
-// and V are read as few times as can be, unless the keys are too few to give every
-// second CU a part of `least` blocks (three tiles a key group, below which the merge
-// grows by what the parts shrink): then fewer rows, and more workgroups (26 nodes x 6
-// heads at 4K, 2 kv heads, with the merge: 256 rows of a workgroup 18 us, 128 16.7, 64
-// 15.4, 32 14.8, in parts of two tiles 16.1 and of four 16.3; 4 sequences of 66 rows x
-// 256 with a window of 1K, 4 kv heads, without: 128 rows 16.0, 64 17.6, 32 16.8).
+// The cut of a call: the shape of a workgroup and the slots along the keys with the
+// least estimate, of all shapes that hold the rows and of the sequences whole, in 2, 3,
+// 4, 6, .. parts each, or in as many as the card holds workgroups (two a CU where they
+// pair up).  Wide workgroups read K and V the fewest times; narrow ones are more and
+// start sooner; parts cost the merge and the joined partials.  Measured, us: 4 sequences
+// of 64 nodes, 32/4 heads x 128, bf16, 300 tokens 12.0 (64 rows, whole; 256 rows in parts
+// 23.7), 1000 20.5 (29.4), 4000 38.0 (39.4); 26 nodes at 300 tokens, 12/2 heads, 9.4 (in
+// parts 11.6), at 4000 13.0 (16 rows, in parts; 256 rows 15.9); 2 sequences of 64 nodes,
+// 32/8 x 128, f32, 4000 tokens 57.7 (128 rows; 64 rows 82).
 struct TreeCut {
     TreeShape shape;
     TreePlan plan;
     int64_t rows;  // of the scratch
 };
+// Microseconds that a workgroup of 16, 32, 64, 128 or 256 rows takes for 32 keys, where
+// there are few of them and where they fill the card (8 kv heads, 8 and 64 sequences of
+// 416 and 1440 tokens, uncut).
+struct TreeCost {
+    float few, full;
+};
+static constexpr TreeCost kTreeCost[2][3][5] = {
+    {{{.31f, .60f}, {.45f, .55f}, {.34f, .60f}, {.63f, .92f}, {.66f, .73f}},      // 16 bits x 64
+     {{.41f, 1.58f}, {.67f, 1.59f}, {.57f, 1.67f}, {.83f, 1.90f}, {.88f, 1.04f}},  // x 128
+     {{1.05f, 3.01f}, {1.20f, 3.14f}, {1.07f, 3.21f}, {.99f, 1.85f}, {}}},         // x 256
+    {{{.60f, 1.55f}, {.70f, 1.78f}, {1.28f, 2.63f}, {2.11f, 3.51f}, {2.29f, 2.59f}},  // f32 x 64
+     {{1.50f, 3.01f}, {1.44f, 3.36f}, {2.35f, 4.90f}, {2.55f, 3.35f}, {}},
+     {{2.71f, 3.44f}, {2.80f, 3.72f}, {4.55f, 5.31f}, {7.68f, 7.58f}, {}}}};
 static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window, int n_head, int n_kv, int D) {
-    const int rows = nodes * (n_head / n_kv);
+    const int rows = nodes * (n_head / n_kv), rb = D * dtype_bytes(dtype);
     const int64_t keys = window > 0 ? std::min<int64_t>(max_len, (int64_t)window + nodes) : max_len;
+    const int64_t blocks = keys / 32 + 1;
+    TreeCut best{};
+    float least = INFINITY;
     for (TreeShape s = tree_shape(dtype, D, rows);; s = tree_narrower(dtype, D, s)) {
-        TreePlan p{};
-        p.batch = batch, p.n_kv = n_kv;
-        p.row_tiles = (rows + s.rows() - 1) / s.rows();
-        p.least = s.wr == 8 ? 4 : 3 * s.wk;
-        const int64_t units = (int64_t)n_kv * p.row_tiles;
-        const int64_t most = batch * ((keys / 32 + 2 + p.least - 1) / p.least);
-        const bool pairs = tree_pairs(D * dtype_bytes(dtype), s.wr);
-        if (s.wr > 1 && most * units < (pairs ? 512 : 128)) continue;
-        p.slots = batch;
-        if (batch <= 256) p.slots = std::max(batch, (int)std::min<int64_t>((pairs ? 512 : 256) / units, most));
-        return {s, p, p.slots > batch ? p.slots * units * s.rows() : 0};
+        const int row_tiles = (rows + s.rows() - 1) / s.rows();
+        const int64_t units = (int64_t)n_kv * row_tiles, room = tree_pairs(rb, s.wr) ? 512 : 256;
+        const TreeCost c = kTreeCost[dtype == ULLM_DT_F32][D / 128][__builtin_ctz(s.rows()) - 4];
+        const int part = s.wr == 8 ? 4 : 2 * s.wk;  // blocks that a part has at least
+        // Where they fill the card they wait for memory or for the matrix units: of what they
+        // read row tiles of one kv head share a part, but never less than the products take.
+        const int on = room / 256, widest = D == 256 ? 128 : 256;
+        const float read = room * 64 * rb / 5.3e6f;
+        const float products = dtype == ULLM_DT_F32
+                                   ? on * s.rows() * D * 4.5e-4f
+                                   : on * s.rows() * 1.35f * kTreeCost[0][D / 128][D == 256 ? 3 : 4].few / widest;
+        float full = c.full;
+        if (full > .9f * read && full < 1.25f * read)
+            full = std::min(full, std::max({c.few, products, full / std::sqrt((float)row_tiles)}));
+        const int64_t most = batch <= 256 ? std::min(room / units, batch * ((blocks + part) / part)) : 0;
+        for (int64_t slots = batch, k = 1;;) {
+            const float wgs = (float)slots * units / room;
+            const float block = c.few + (full - c.few) * std::min(std::max((wgs - .125f) / .875f, 0.f), 1.f);
+            float us = 4.5f + s.rows() * rb * 1e-4f;  // start and end of a workgroup
+            if (slots == batch) {
+                us = std::max(wgs, 1.f) * (us + blocks * block);
+            } else {
+                // (the sequences of a batch are taken to have 0.75 max_len on average)
+                const float len = std::ceil((batch > 1 ? .75f : 1.f) * blocks * batch / slots);
+                us += std::max(len, (float)part) * block;
+                us += 3 + (batch > 1 ? 1.5f : 0) + 1.2e-6f * slots * n_kv * rows * D;  // the merge, the cut, what is joined
+            }
+            if (us < least) {
+                least = us;
+                best.shape = s;
+                best.plan = TreePlan{};
+                best.plan.batch = batch, best.plan.n_kv = n_kv, best.plan.row_tiles = row_tiles;
+                best.plan.least = part, best.plan.slots = (int)slots;
+                best.rows = slots > batch ? slots * units * s.rows() : 0;
+            }
+            if (slots >= most) break;
+            k += k < 4 ? 1 : (k & (k - 1)) ? k / 3 : k / 2;  // 1, 2, 3, 4, 6, 8, 12, ..
+            slots = std::min(batch * k, most);
+        }
+        if (s.rows() == 16) return best;
     }
 }
 static size_t tree_bytes(int64_t rows, int batch, int D) {
