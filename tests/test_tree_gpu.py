@@ -215,6 +215,57 @@ def test_attn_tree(dev, case):
         assert not out[b, nodes[b]:].any()
 
 
+SHAPES = [
+    # (type, out, H, Hk, D, B, T, L): a small call for each shape of a workgroup, uncut and in parts
+    ("bf16", "f32", 12, 2, 128, 1, 1, 40), ("f16", "f32", 12, 2, 128, 1, 1, 700), ("bf16", "bf16", 12, 2, 128, 200, 3, 40),
+    ("f16", "f16", 16, 16, 128, 1, 20, 3000), ("bf16", "f32", 12, 2, 128, 200, 7, 40), ("f16", "f32", 16, 16, 128, 6, 33, 700),
+    ("bf16", "bf16", 64, 16, 128, 24, 20, 40), ("f16", "f16", 64, 16, 128, 1, 20, 12000),
+    ("bf16", "f32", 64, 16, 128, 16, 33, 300), ("f16", "f32", 64, 16, 128, 1, 33, 12000),
+    ("bf16", "bf16", 12, 2, 256, 1, 1, 40), ("f16", "f16", 12, 2, 256, 1, 1, 300), ("bf16", "f32", 12, 2, 256, 200, 3, 40),
+    ("f16", "f32", 16, 16, 256, 6, 20, 300), ("bf16", "bf16", 12, 2, 256, 200, 7, 40), ("f16", "f16", 16, 16, 256, 2, 33, 1500),
+    ("bf16", "f32", 32, 8, 256, 24, 20, 300), ("f16", "f32", 8, 4, 256, 2, 33, 12000), ("bf16", "bf16", 12, 2, 64, 1, 1, 40),
+    ("f16", "f16", 12, 2, 64, 1, 1, 700), ("bf16", "f32", 128, 16, 64, 16, 3, 40), ("f16", "f32", 12, 2, 64, 24, 3, 700),
+    ("bf16", "bf16", 32, 4, 64, 3, 64, 40), ("f16", "f16", 128, 16, 64, 1, 7, 700), ("bf16", "f32", 64, 16, 64, 24, 20, 40),
+    ("f16", "f32", 8, 4, 64, 4, 33, 12000), ("bf16", "bf16", 64, 16, 64, 16, 33, 300), ("f16", "f16", 12, 2, 64, 2, 33, 30000),
+    ("f32", "f32", 12, 2, 128, 1, 1, 40), ("f32", "f32", 12, 2, 128, 1, 1, 300), ("f32", "f32", 12, 2, 128, 200, 3, 40),
+    ("f32", "f32", 16, 16, 128, 6, 20, 300), ("f32", "f32", 12, 2, 128, 200, 7, 40), ("f32", "f32", 64, 8, 128, 1, 48, 700),
+    ("f32", "f32", 8, 4, 128, 64, 33, 40), ("f32", "f32", 12, 2, 128, 1, 20, 12000), ("f32", "f32", 12, 2, 256, 1, 1, 40),
+    ("f32", "f32", 12, 2, 256, 1, 1, 300), ("f32", "f32", 64, 8, 256, 24, 3, 40), ("f32", "f32", 32, 4, 256, 1, 33, 300),
+    ("f32", "f32", 64, 8, 256, 24, 7, 40), ("f32", "f32", 16, 16, 256, 1, 33, 1500), ("f32", "f32", 64, 16, 256, 8, 33, 40),
+    ("f32", "f32", 8, 4, 256, 16, 33, 700), ("f32", "f32", 12, 2, 64, 1, 1, 40), ("f32", "f32", 12, 2, 64, 1, 1, 300),
+    ("f32", "f32", 12, 2, 64, 200, 3, 40), ("f32", "f32", 16, 16, 64, 1, 20, 3000), ("f32", "f32", 12, 2, 64, 200, 7, 40),
+    ("f32", "f32", 64, 8, 64, 1, 48, 700), ("f32", "f32", 64, 16, 64, 24, 20, 40), ("f32", "f32", 128, 16, 64, 1, 48, 700),
+    ("f32", "f32", 128, 16, 64, 8, 64, 40), ("f32", "f32", 64, 8, 64, 1, 64, 1500),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_every_shape(dev, case):
+    dt, odt, H, Hk, D, B, T, L = SHAPES[case]
+    print(f"[tree] {SHAPES[case]}", flush=True)
+    t, rng = DT[dt], np.random.default_rng(case + 100)
+    lens = [L - (i * 11) % (L // 2) for i in range(B)]
+    nodes = [T - i % min(T, 3) for i in range(B)]
+    see, depth, _ = trees(rng, B, T, "random")
+    pos = np.array(lens)[:, None] + depth
+    page = (0, 32, 64)[case % 3]
+    caches, rows, table = make(rng, dev, lens, nodes, T, Hk, D, t, page, 0, L + T)
+    if T > 1:  # a key that no node of the first sequence sees
+        see[0, :, 1] = False
+        at = lens[0] + 1
+        at = (table[0, at // page], at % page) if page else (0, at)
+        for r, c, bad in ((rows[0], caches[0], NAN), (rows[1], caches[1], math.inf)):
+            r[0][lens[0] + 1] = bad
+            c[at] = bad
+    g = torch.Generator(device=dev).manual_seed(case)
+    q = (2 * torch.randn(B, T, H, D, device=dev, generator=g)).to(t)
+    out = attend(q, caches, table, bits(see).to(dev), i32(lens, dev), L + T, Hk, i32(nodes, dev), i32(pos, dev), 0, out_dtype=DT[odt])
+    for b in range(0, B, max(B // 6, 1)):
+        r = ref(q[b], rows[0][b], rows[1][b], see[b], lens[b], nodes[b], pos[b], 0, 1 / math.sqrt(D), D)
+        check(out[b], *r, lens[b] + nodes[b], t, f"case {case} b={b}")
+        assert not out[b, nodes[b]:].any()
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("page", [0, 32])
