@@ -38,8 +38,8 @@
 // 7 nodes, 40/8 heads, bf16: 21.1 us, 84 MB at 4.0 TB/s, the chain of a workgroup's
 // start and end being 8 of them; f32, 2 sequences of 3K-8K, 48 nodes, 32/8 heads of 64:
 // 42.4 us, six products of 4.4 GFLOP at 620 TFLOP/s (with f32 products 75.6); one
-// sequence of 4K, 26 nodes, 12/2 heads of 128, f16: 11 us, of which the launch, the
-// first loads and the epilogue are 9.
+// sequence of 4K, 26 nodes, 12/2 heads of 128, f16: 9.5 us, of which the launch, the
+// first loads and the epilogue are 8.
 #include <algorithm>
 #include <climits>
 #include <cmath>
