@@ -10,10 +10,10 @@ namespace ullm {
 // 4, 6, .. parts each, or in as many as the card holds workgroups (two a CU where they
 // pair up).  Wide workgroups read K and V the fewest times; narrow ones are more and
 // start sooner; parts cost the merge and the joined partials.  Measured, us: 4 sequences
-// of 64 nodes, 32/4 heads x 128, bf16, 300 tokens 12.0 (64 rows, whole; 256 rows in parts
-// 23.7), 1000 20.5 (29.4), 4000 38.0 (39.4); 26 nodes at 300 tokens, 12/2 heads, 9.4 (in
-// parts 11.6), at 4000 13.0 (16 rows, in parts; 256 rows 15.9); 2 sequences of 64 nodes,
-// 32/8 x 128, f32, 4000 tokens 57.7 (128 rows; 64 rows 82).
+// of 64 nodes, 32/4 heads x 128, bf16, 300 tokens 12.6 (16 rows; 256 rows 25.8), 1000 23.3
+// (16 rows 22.7, 256 rows 34.2), 4000 43.8 (64 rows 42.3, 256 rows 43.8, 16 rows 63.8); 26
+// nodes at 300 tokens, 12/2 heads, 9.9 (256 rows 16.8), at 4000 13.0 (16 rows, in parts; 256
+// rows 16.5); 2 sequences of 64 nodes, 32/8 x 128, f32, 4000 tokens 57.7 (128 rows; 64 rows 82).
 struct TreeCut {
     TreeShape shape;
     TreePlan plan;
@@ -26,9 +26,9 @@ struct TreeCost {
     float few, full;
 };
 static constexpr TreeCost kTreeCost[2][3][5] = {
-    {{{.31f, .60f}, {.45f, .55f}, {.34f, .60f}, {.63f, .92f}, {.66f, .73f}},      // 16 bits x 64
-     {{.41f, 1.58f}, {.67f, 1.59f}, {.57f, 1.67f}, {.83f, 1.90f}, {.88f, 1.04f}},  // x 128
-     {{1.05f, 3.01f}, {1.20f, 3.14f}, {1.07f, 3.21f}, {.99f, 1.85f}, {}}},         // x 256
+    {{{.32f, .60f}, {.50f, .57f}, {.40f, .62f}, {.73f, 1.11f}, {.88f, .95f}},       // 16 bits x 64
+     {{.46f, 1.56f}, {.75f, 1.58f}, {.62f, 1.67f}, {1.01f, 2.10f}, {1.17f, 1.34f}},  // x 128
+     {{1.18f, 2.88f}, {1.19f, 3.05f}, {1.06f, 3.17f}, {1.17f, 1.96f}, {}}},          // x 256
     {{{.60f, 1.55f}, {.70f, 1.78f}, {1.28f, 2.63f}, {2.11f, 3.51f}, {2.29f, 2.59f}},  // f32 x 64
      {{1.50f, 3.01f}, {1.44f, 3.36f}, {2.35f, 4.90f}, {2.55f, 3.35f}, {}},
      {{2.71f, 3.44f}, {2.80f, 3.72f}, {4.55f, 5.31f}, {7.68f, 7.58f}, {}}}};
@@ -41,7 +41,10 @@ static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window
     for (TreeShape s = tree_shape(dtype, D, rows);; s = tree_narrower(dtype, D, s)) {
         const int row_tiles = (rows + s.rows() - 1) / s.rows();
         const int64_t units = (int64_t)n_kv * row_tiles, room = tree_pairs(rb, s.wr) ? 512 : 256;
-        const TreeCost c = kTreeCost[dtype == ULLM_DT_F32][D / 128][__builtin_ctz(s.rows()) - 4];
+        TreeCost c = kTreeCost[dtype == ULLM_DT_F32][D / 128][__builtin_ctz(s.rows()) - 4];
+        // Up to 192 of 256 rows a SIMD's two waves hold three row tiles, not four (16 bits x
+        // 128, 192 rows: .94 and 1.15 a block; f32 x 64 1.93 and 2.04).
+        if (s.rows() == 256 && rows <= 192) c.few *= .8f, c.full *= .8f;
         const int part = s.wr == 8 ? 4 : 2 * s.wk;  // blocks that a part has at least
         // Where they fill the card they wait for memory or for the matrix units: of what they
         // read row tiles of one kv head share a part, but never less than the products take.

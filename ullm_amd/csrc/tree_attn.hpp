@@ -17,7 +17,10 @@
 //    row's maximum, sum and rescale live in the four lanes that own its output,
 //    and P^T is the S^T accumulator exponentiated: P never moves between lanes.
 //    16-bit caches: 16x16x32, K by 16-byte LDS reads, V^T by the transposing
-//    LDS read.  f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads,
+//    LDS read, P as two 16-bit values hi + lo whatever the output's type.  (P as one
+//    puts outputs 1.37 times as far from 64 bits over bf16, and 1.27 over f16, as their
+//    own rounding does; two take 260 us for 200 in the largest case below, where the
+//    products bind, 25.3 for 24.7 and 13.1 for 12.8 in the others.)  f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads,
 //    the four elements of a read being four k-steps (K) or four d tiles (V); they
 //    run at a sixteenth of the 16-bit rate, which the stream of K and V about hides
 //    up to 64 rows.  f32, more rows (X3): every value as the sum of three bf16 (8 bits
@@ -222,7 +225,7 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t (&w)[3]) {
     w[2] = __builtin_amdgcn_perm(__float_as_uint(r1 - m1), __float_as_uint(r0 - m0), pick);
 }
 
-template <class T, int D, int NR, int WR, int WK, int PB>
+template <class T, int D, int NR, int WR, int WK, int ODT>
 __global__ __launch_bounds__(64 * WR * WK * tree_halves(__is_same(T, F32), WR),
                              tree_waves(D *T::bytes, WR, WK *tree_halves(__is_same(T, F32), WR)))
 void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
@@ -236,7 +239,7 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && SH > 1 && FIT >= 4 ? 2 : 1;
     constexpr int TILE = KS * KB * RB, STAGE = 2 * TILE;  // a step's tiles as fetched, K and K and V
     using CT = typename std::conditional<X3, BF16, T>::type;  // operands
-    constexpr int NPL = X3 ? 3 : 1, NP = X3 ? 3 : PB;          // pieces of K, V and Q, and of P
+    constexpr int NPL = X3 ? 3 : 1, NP = F ? NPL : 2;         // pieces of K, V and Q, and of P
     constexpr int RBC = D * CT::bytes, CTILE = KB * RBC;       // a row and a tile of one piece
     constexpr int CONV = 2 * NPL * CTILE;                      // K pieces, V pieces
     constexpr int VOFF = X3 ? NPL * CTILE : TILE;              // of V behind K
@@ -283,7 +286,6 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
         const int t = node_of(r);
         return out0 + t * node_ld + (int64_t)(r - t * G) * D;
     };
-    constexpr int ODT = PB == 1 && !F ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
     auto store4 = [&](int64_t at, const f32x4 &o) {
         if constexpr (ODT == ULLM_DT_F32) *(f32x4 *)((float *)a.out + at) = o;
         else *(u32x2 *)((uint16_t *)a.out + at) = u32x2{pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
@@ -673,11 +675,9 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
                             split3(p0, p1, w);
 #pragma unroll
                             for (int k = 0; k < 3; k++) ph[x][u][k][i] = w[k];
-                        } else if constexpr (NP == 2) {
+                        } else {
                             const u32x2 hl = split2<CT>(p0, p1);
                             ph[x][u][0][i] = hl[0], ph[x][u][1][i] = hl[1];
-                        } else {
-                            ph[x][u][0][i] = pack2<CT>(p0, p1);
                         }
                     }
             }
@@ -1037,13 +1037,12 @@ inline TreeShape tree_narrower(int dtype, int D, const TreeShape &s) {
     return tree_shape(dtype, D, std::max(s.rows() / 2, 16));
 }
 
-template <class T, int D, int NR, int WR, int WK, int PB>
+template <class T, int D, int NR, int WR, int WK, int ODT>
 static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
     const int64_t items = (int64_t)p.slots * p.n_kv * p.row_tiles;
-    launch_kernel(tree_kernel<T, D, NR, WR, WK, PB>, dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WR * WK * tree_halves(__is_same(T, F32), WR)), 0, st,
+    launch_kernel(tree_kernel<T, D, NR, WR, WK, ODT>, dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WR * WK * tree_halves(__is_same(T, F32), WR)), 0, st,
                   a, kv, p);
     if (p.slots > p.batch) {
-        constexpr int ODT = PB == 1 && !__is_same(T, F32) ? (__is_same(T, F16) ? ULLM_DT_F16 : ULLM_DT_BF16) : ULLM_DT_F32;
         constexpr int RPB = 256 / (D / 4);  // rows of a workgroup with one group each
         const int64_t rows = (int64_t)a.nodes * a.n_head;
         int log_g = 0;  // groups for four of a sequence's parts each (8 sequences of 4 parts, 16384 rows x 128: 8.8
@@ -1054,22 +1053,22 @@ static void launch_tree(const TreeArgs &a, const TreeKv &kv, const TreePlan &p, 
                       __builtin_ctz(16 * NR * WR), log_g);
     }
 }
-template <class T, int D, int PB>
+template <class T, int D, int ODT>
 static void launch_shape(const TreeShape &s, const TreeArgs &a, const TreeKv &kv, const TreePlan &p, hipStream_t st) {
     constexpr bool F = __is_same(T, F32);
     constexpr int rb = D * T::bytes, wide = D == 256 || rb == 512 ? 1 : 2, most = F ? 1 : wide, wk = rb <= 256 ? 2 : 1;
-    if (s.wr == 8) launch_tree<T, D, wide, 8, 1, PB>(a, kv, p, st);
+    if (s.wr == 8) launch_tree<T, D, wide, 8, 1, ODT>(a, kv, p, st);
     else if (s.wr == 4) {
         if (F && wide == 2 && s.nr == 2) {
-            if constexpr (F && wide == 2) launch_tree<T, D, 2, 4, 1, PB>(a, kv, p, st);
+            if constexpr (F && wide == 2) launch_tree<T, D, 2, 4, 1, ODT>(a, kv, p, st);
         } else {
-            launch_tree<T, D, most, 4, 1, PB>(a, kv, p, st);
+            launch_tree<T, D, most, 4, 1, ODT>(a, kv, p, st);
         }
-    } else if (s.wr == 2) launch_tree<T, D, most, 2, wk, PB>(a, kv, p, st);
+    } else if (s.wr == 2) launch_tree<T, D, most, 2, wk, ODT>(a, kv, p, st);
     else if (s.nr == 2) {
-        if constexpr (most == 2) launch_tree<T, D, 2, 1, wk, PB>(a, kv, p, st);
+        if constexpr (most == 2) launch_tree<T, D, 2, 1, wk, ODT>(a, kv, p, st);
     } else {
-        launch_tree<T, D, 1, 1, wk, PB>(a, kv, p, st);
+        launch_tree<T, D, 1, 1, wk, ODT>(a, kv, p, st);
     }
 }
 
@@ -1083,11 +1082,11 @@ struct TreeCall {
     bool f32_out;
     hipStream_t st;
 };
-template <class T, int PB>
+template <class T, int ODT>
 static void launch_dims(const TreeCall &c) {
-    if (c.head_dim == 64) launch_shape<T, 64, PB>(c.shape, c.a, c.kv, c.plan, c.st);
-    else if (c.head_dim == 128) launch_shape<T, 128, PB>(c.shape, c.a, c.kv, c.plan, c.st);
-    else launch_shape<T, 256, PB>(c.shape, c.a, c.kv, c.plan, c.st);
+    if (c.head_dim == 64) launch_shape<T, 64, ODT>(c.shape, c.a, c.kv, c.plan, c.st);
+    else if (c.head_dim == 128) launch_shape<T, 128, ODT>(c.shape, c.a, c.kv, c.plan, c.st);
+    else launch_shape<T, 256, ODT>(c.shape, c.a, c.kv, c.plan, c.st);
 }
 void launch_tree_f32(const TreeCall &c);
 void launch_tree_f16(const TreeCall &c);

@@ -2,5 +2,5 @@
 #include "tree_attn.hpp"
 
 namespace ullm {
-void launch_tree_f32(const TreeCall &c) { launch_dims<F32, 1>(c); }
+void launch_tree_f32(const TreeCall &c) { launch_dims<F32, ULLM_DT_F32>(c); }
 }  // namespace ullm
