@@ -30,7 +30,11 @@ def bound(o, a, e, n_keys, t, out_t, most, v_max):
     ("f16", 8, 4, 64, [36], 1, 0, 0), ("bf16", 4, 4, 128, [9, 63], 17, 32, 0), ("f16", 12, 2, 128, [4095], 26, 0, 0),
     ("bf16", 40, 8, 128, [90, 700, 31, 1500], 7, 32, 0), ("f16", 8, 4, 256, [1500, 900], 33, 128, 1024),
     ("bf16", 8, 4, 256, [700], 5, 0, 0), ("bf16", 32, 4, 128, [9000, 5000], 64, 64, 0), ("f16", 64, 16, 64, [1111, 222], 50, 64, 0),
-    ("bf16", 12, 2, 64, [30] * 40, 7, 32, 0), ("f16", 64, 16, 256, [300] * 4, 33, 64, 0)])
+    ("bf16", 12, 2, 64, [30] * 40, 7, 32, 0), ("f16", 64, 16, 256, [300] * 4, 33, 64, 0),
+    # workgroups of the widths and cuts that the calls of test_tree_gpu.py do not reach
+    ("bf16", 64, 16, 128, [700] * 24, 20, 64, 0), ("f16", 8, 4, 256, [300] * 64, 64, 0, 0), ("bf16", 32, 8, 256, [12000], 20, 0, 0),
+    ("f16", 12, 2, 64, [40] * 200, 3, 32, 0), ("bf16", 12, 2, 64, [40] * 200, 7, 0, 0), ("f16", 64, 16, 64, [700] * 24, 20, 32, 0),
+    ("bf16", 64, 16, 64, [12000], 33, 64, 0)])
 def test_output_is_rounded_once(dev, dt, H, Hk, D, lens, T, page, window):
     """An output in the cache's type is the f32 output rounded, nothing less exact:
     both within the bound of two pieces of every weight."""
