@@ -410,7 +410,8 @@ int ullm_hip_qkv_append_tree_paged(const float *q_in, const float *k_in, const f
  * q, out: [batch][max_nodes][n_head][head_dim]; q in the cache's dtype (f32, f16
  *         or bf16), out in the cache's dtype or f32 (out_dtype): the same result,
  *         rounded once.  Over a 16-bit cache the softmax weights enter P.V as two
- *         values of its dtype; an f32 cache runs on f32 products, or with many
+ *         values of its dtype (over f16 to 2^-39 of the row's largest, if that is
+ *         more than its bits); an f32 cache runs on f32 products, or with many
  *         rows on exact bf16 pieces of its values whose products are as good
  * mask:   int64[batch][max_nodes][ceil(max_nodes/64)], bit c % 64 of word c / 64
  *         (its own bit too: a node sees itself only by it), or NULL: node i sees

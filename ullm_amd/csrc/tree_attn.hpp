@@ -489,7 +489,12 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
             see[u] = node < 0 ? 0 : s;
         }
     };
-    constexpr float kLazy = 8.f;  // the running maximum is raised by more than 2^8 at a time
+    // The running maximum is raised by more than 2^kLazy at a time, and a weight is held as
+    // 2^kUp of what it is to it, which the row's sum carries too.  f16 ends at 2^-24: with
+    // the largest weight at 2^14 or more those of 2^-28 of it keep f16's bits and its
+    // smallest step is 2^-38 of it (at 1 a long tail of weights below 2^-24 was lost).  The
+    // more frequent raises take 20.8 us for 19.8 (33 nodes, window 1024, 8/4 x 256).
+    constexpr float kLazy = __is_same(T, F16) ? 1.f : 8.f, kUp = __is_same(T, F16) ? 14.f : 0.f;
     constexpr int KT = KB / 16 / KH;  // 16-key tiles of S^T of this wave
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
     bool mine = false;  // this wave's own tiles had infinities or NaN taken out
@@ -655,12 +660,12 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
         u32x4 ph[NX][BPC][NP];
 #pragma unroll
         for (int x = 0; x < NX; x++) {
-            const float mu = m_run[x] == -INFINITY ? 0.f : m_run[x];
+            const float off = kUp - (m_run[x] == -INFINITY ? 0.f : m_run[x]);
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    sacc[x][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[x][t][i], a.qs, -mu));
+                    sacc[x][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[x][t][i], a.qs, off));
                     l_part[x] += sacc[x][t][i];
                 }
             if constexpr (!FM) {
