@@ -296,7 +296,8 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     }
     if (row0 >= rows) return;
 
-    // (waves that share tiles: the first barrier of the steps is behind it)
+    // (behind it: the first barrier of the steps, and behind that whoever sets it; X3 finds
+    // them ahead of that barrier, so its waves set it after the steps)
     if (SH > 1 && tid == 0) unfinite = 0;
     // ---- this part's tiles of KB keys, dealt to the key groups in turn ----
     constexpr int BPC = KB / 32, BPT = KS * BPC;  // blocks of a tile, of a step
@@ -497,7 +498,7 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr float kLazy = __is_same(T, F16) ? 1.f : 8.f, kUp = __is_same(T, F16) ? 14.f : 0.f;
     constexpr int KT = KB / 16 / KH;  // 16-key tiles of S^T of this wave
     auto whole = [&](int key0) { return key0 >= clear0 && key0 + KB <= clear1; };  // every row sees the tile's keys
-    bool mine = false;  // this wave's own tiles had infinities or NaN taken out
+    bool mine = false;  // this wave took infinities or NaN out of its own tiles (X3: out of what it fetched)
     // One tile, of block `blk` on, for the first NX of the wave's row tiles.  next: the
     // step whose fetch goes out under this tile's products, if there is one.
     auto tile_of = [&](auto nxc, uint32_t sb, int blk, int next) __attribute__((always_inline)) {
@@ -775,7 +776,7 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
 #pragma unroll
                 for (int k = 0; k < 3; k++) lds_write_b64(at + k * CTILE, u32x2{w0[k], w1[k]});
             }
-        if (masked && __any(any != 0)) unfinite = 1;
+        mine |= masked && __any(any != 0);
     };
 
     // ---- the pipeline: one key group's wave refills a stage as soon as it has
@@ -790,6 +791,7 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
             wg_barrier();
             step(j, INT_MAX);
         }
+        if (mine) unfinite = 1;  // (then there was a step, whose barrier is behind the 0)
     } else if constexpr (SH == 1) {
         for (int j = 0; j < steps; j++) {
             if (j + NST <= steps) __builtin_amdgcn_s_waitcnt(vm_wait(std::min((NST - 1) * 2 * NI, 63)));
