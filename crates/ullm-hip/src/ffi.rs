@@ -167,6 +167,12 @@ unsafe extern "C" {
         parent: *const i32, capacity: *const i32, held: *const u8, table_out: *mut i32,
         out_stride: c_int, lens_out: *mut i32, n_out: c_int, info: *mut i32,
         workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_kv_pages_update_rows(k_pages: *mut c_void, v_pages: *mut c_void, dtype: c_int,
+        kv_stride: i64, page_size: c_int, n_pages: c_int, kv_dim: c_int, n_layer: c_int,
+        layer_stride: i64, block_table: *const i32, table_stride: c_int, seq_lens: *const i32,
+        n_seq: c_int, parent: *const i32, capacity: *const i32, held: *const u8,
+        table_out: *mut i32, out_stride: c_int, lens_out: *mut i32, n_out: c_int, info: *mut i32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn ullm_hip_kv_pages_workspace_bytes(n_out: c_int, n_pages: c_int) -> usize;
 }
 

@@ -492,7 +492,8 @@ int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype, int64_t kv
  * n_out <= 65535 (0: nothing is written), n_out * out_stride < 2^31; pools and
  * strides 16-byte aligned.
  * workspace: DEVICE memory of ullm_hip_kv_pages_workspace_bytes, 256-byte
- * aligned, needs no initialisation, one call at a time. */
+ * aligned, needs no initialisation, one call at a time.
+ * Rows of kv_stride elements are copied whole: they are the pools' own. */
 int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
                              int page_size, int n_pages, int n_layer, int64_t layer_stride,
                              const int32_t *block_table, int table_stride, const int32_t *seq_lens,
@@ -500,6 +501,18 @@ int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv
                              const uint8_t *held, int32_t *table_out, int out_stride,
                              int32_t *lens_out, int n_out, int32_t *info, void *workspace,
                              size_t workspace_bytes, void *stream);
+/* The same over pools that are columns of wider rows (K and V side by side, the
+ * layers of a position together, another model's pool in the same buffer): the
+ * first kv_dim elements of each row are copied, what lies between them is left
+ * alone.  Layers must not share rows (layer_stride >= kv_dim). */
+int ullm_hip_kv_pages_update_rows(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
+                                  int page_size, int n_pages, int kv_dim, int n_layer,
+                                  int64_t layer_stride, const int32_t *block_table,
+                                  int table_stride, const int32_t *seq_lens, int n_seq,
+                                  const int32_t *parent, const int32_t *capacity,
+                                  const uint8_t *held, int32_t *table_out, int out_stride,
+                                  int32_t *lens_out, int n_out, int32_t *info, void *workspace,
+                                  size_t workspace_bytes, void *stream);
 size_t ullm_hip_kv_pages_workspace_bytes(int n_out, int n_pages);
 
 /* Measurement calibration (no counterpart in the reference): reads `bytes`

@@ -5,7 +5,9 @@ import numpy as np
 import pytest
 import torch
 
-from test_tree_gpu import NAN, attend, bits, i32, make
+from test_tree_gpu import DT, NAN, attend, bits, i32, make
+from ullm_amd import _lib as L
+from ullm_amd import attention as A
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +47,50 @@ def test_infinities_of_a_first_step_over_f32(dev, D, H, Hk, B, T, n, page):
             got = out[:, i, :, j % 2::2]
             assert got.isnan().all() if math.isnan(value) else (got == value).all(), (n, i)
             assert torch.isfinite(out[:, i, :, 1 - j % 2::2]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("form", ["side by side", "layers in a row", "narrow"])
+@pytest.mark.parametrize("P,kvd", [(32, 64), (64, 8), (2, 2056), (128, 328)])
+def test_page_copies_of_views_of_wider_rows(dev, dt, form, P, kvd):
+    """Pools that are columns of wider rows: a fork copies those columns of the filled
+    rows, and whatever else the rows hold stays as it was."""
+    t, NL, n_pages = DT[dt], 3, 9
+    g = torch.Generator(device=dev).manual_seed(P)
+    if form == "layers in a row":
+        both = [torch.randn(n_pages, P, NL + 1, kvd, device=dev, generator=g).to(t) for _ in "kv"]
+        views = [x.permute(2, 0, 1, 3)[:NL] for x in both]
+        of = lambda xs: [x.permute(2, 0, 1, 3)[:NL] for x in xs]  # noqa: E731
+    elif form == "side by side":
+        both = [torch.randn(NL, n_pages, P, 2 * kvd, device=dev, generator=g).to(t)]
+        of = lambda xs: [xs[0][..., :kvd], xs[0][..., kvd:]]  # noqa: E731
+    else:
+        both = [torch.randn(NL, n_pages, P, kvd + 24, device=dev, generator=g).to(t) for _ in "kv"]
+        of = lambda xs: [x[..., 8:8 + kvd] for x in xs]  # noqa: E731
+    views, want = of(both), [x.clone() for x in both]
+    part = P // 2 + 1 if P > 2 else 1
+    lens = [P + part, part]
+    table, new, info = A.kv_pages_update(*views, i32([[6, 3], [8, -1]], dev), i32(lens, dev), i32([0, 0, 1, 1, 0], dev),
+                                         i32([lens[0] + 1, 2 * P, P, P, lens[0]], dev))
+    assert table.tolist() == [[6, 3], [6, 0], [8, -1], [1, -1], [6, 2]] and info.tolist() == [3, 3, 0]
+    assert new.tolist() == [lens[0], lens[0], part, part, lens[0]]
+    for x, o in zip(of(want), of([x.clone() for x in both])):
+        for src, to in ((3, 0), (8, 1), (3, 2)):
+            x[:, to, :part] = o[:, src, :part]
+    for x, w in zip(both, want):
+        assert torch.equal(x, w)
+    if form != "narrow":  # one layer
+        before = [x.clone() for x in both]
+        A.kv_pages_update(*(x[1] for x in views), i32([[6, 3]], dev), i32([P + part], dev), i32([0, 0], dev), i32([2 * P] * 2, dev))
+        for x, o in zip(of(before), of([x.clone() for x in before])):
+            x[1, 0, :part] = o[1, 3, :part]
+        for x, w in zip(both, before):
+            assert torch.equal(x, w)
+
+
+def test_pools_whose_rows_overlap_are_refused(dev):
+    k = torch.zeros(1 << 14, device=dev, dtype=torch.float16)
+    for sizes, strides in (((4, 32, 64), (32 * 32, 32, 1)), ((2, 4, 32, 8), (0, 32 * 8, 8, 1)), ((2, 4, 32, 8), (4, 32 * 8, 8, 1))):
+        v = k.as_strided(sizes, strides)
+        with pytest.raises(L.UllmHipError):
+            A.kv_pages_update(v, v, i32([[0]], dev), i32([5], dev), i32([0, 0], dev), i32([6, 6], dev))

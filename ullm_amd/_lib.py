@@ -114,6 +114,11 @@ SIGNATURES = {
         [_vp, _vp, _i, _i64, _i, _i, _i, _i64, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp,
          _vp, _sz, _vp],
     ),
+    "ullm_hip_kv_pages_update_rows": (
+        _i,
+        [_vp, _vp, _i, _i64, _i, _i, _i, _i, _i64, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _i, _vp,
+         _vp, _sz, _vp],
+    ),
     "ullm_hip_kv_pages_workspace_bytes": (_sz, [_i, _i]),
 }
 

@@ -272,7 +272,8 @@ def kv_pages_update(k_pages, v_pages, block_table, seq_lens, parent, capacity, *
     rules).  Growing, forking, cutting back, ending and beginning are all this
     call.
 
-    Pools as for kv_accept_paged; block_table int32 [B, table_stride], seq_lens
+    Pools as for kv_accept_paged, also columns of wider rows, of which only those
+    columns are copied; block_table int32 [B, table_stride], seq_lens
     int32 [B]; parent, capacity: int32 [n]; held: bool [n_pages], pages to leave
     alone.  Returns (table [n, table_stride], lengths [n], info int32 [3]: pages
     copied, taken, missing)."""

@@ -727,13 +727,13 @@ PyObject *pages_update(const Args &a) {
     else if (const size_t need = ullm_hip_kv_pages_workspace_bytes(N, p.pages)) ws = st.scratch(tab, need);
     void *const ws_p = ws.defined() ? ws.data_ptr() : nullptr;
     const size_t ws_n = ws.defined() ? ws.nbytes() : 0;
-    const int kd = dt(k);
+    const int kd = dt(k), kvd = small(p.kvd, "kv_dim");
     call([&] {
-        return ullm_hip_kv_pages_update(k.data_ptr(), v.data_ptr(), kd, p.kvs, p.page, p.pages, p.layers,
-                                        p.layer_stride, (const int32_t *)tab.data_ptr(), (int)tab.size(1), len_p, S,
-                                        par_p, cap_p, held ? (const uint8_t *)held->data_ptr() : nullptr,
-                                        (int32_t *)to.data_ptr(), cols, (int32_t *)lo.data_ptr(), N,
-                                        (int32_t *)info.data_ptr(), ws_p, ws_n, st.s);
+        return ullm_hip_kv_pages_update_rows(
+            k.data_ptr(), v.data_ptr(), kd, p.kvs, p.page, p.pages, kvd, p.layers, p.layer_stride,
+            (const int32_t *)tab.data_ptr(), (int)tab.size(1), len_p, S, par_p, cap_p,
+            held ? (const uint8_t *)held->data_ptr() : nullptr, (int32_t *)to.data_ptr(), cols,
+            (int32_t *)lo.data_ptr(), N, (int32_t *)info.data_ptr(), ws_p, ws_n, st.s);
     });
     PyObject *r = PyTuple_New(3);
     if (!r) throw PyRaised{};

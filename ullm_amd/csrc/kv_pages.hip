@@ -161,7 +161,8 @@ static int kv_accept(const char *fn, AcceptArgs a, int dtype, int64_t kv_stride,
 // that nothing keeps, lowest number first.
 struct PagesArgs {
     char *k, *v;
-    int64_t rb, layer_b;
+    int64_t rb, layer_b;  // bytes of a row, from layer to layer
+    int cols;             // 16-byte columns of a row that are copied; 0: whole rows
     const int32_t *tab, *len, *parent, *cap;
     const uint8_t *held;
     int32_t *tab_out, *len_out, *info;
@@ -343,9 +344,17 @@ __global__ __launch_bounds__(256) void pages_apply_kernel(PagesArgs a) {
     char *base = ((z & 1) ? a.v : a.k) + (z >> 1) * a.layer_b;
     const char *src = base + ((int64_t)q.last << a.shift) * a.rb;
     char *dst = base + ((int64_t)a.free_list[q.first] << a.shift) * a.rb;
-    const int64_t n16 = q.part * a.rb / 16;
-    for (int64_t i = blockIdx.x * 256 + tid; i < n16; i += gridDim.x * 256)
-        *(u32x4 *)(dst + i * 16) = *(const u32x4 *)(src + i * 16);
+    if (!a.cols) {
+        const int64_t n16 = q.part * a.rb / 16;
+        for (int64_t i = blockIdx.x * 256 + tid; i < n16; i += gridDim.x * 256)
+            *(u32x4 *)(dst + i * 16) = *(const u32x4 *)(src + i * 16);
+        return;
+    }
+    // rows of a wider buffer, 2^log_c columns side by side
+    const int log_c = a.cols >= 256 ? 8 : 31 - __builtin_clz(2 * a.cols - 1);
+    for (int64_t r = blockIdx.x * (256 >> log_c) + (tid >> log_c); r < q.part; r += gridDim.x * (256 >> log_c))
+        for (int c = tid & ((1 << log_c) - 1); c < a.cols; c += 1 << log_c)
+            *(u32x4 *)(dst + r * a.rb + c * 16ll) = *(const u32x4 *)(src + r * a.rb + c * 16ll);
 }
 
 static size_t pages_ws(int n_out, int n_pages) {
@@ -384,13 +393,13 @@ extern "C" size_t ullm_hip_kv_pages_workspace_bytes(int n_out, int n_pages) {
     return n_out < 1 || n_pages < 1 ? 0 : pages_ws(n_out, n_pages);
 }
 
-extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride, int page_size,
-                                        int n_pages, int n_layer, int64_t layer_stride, const int32_t *block_table,
-                                        int table_stride, const int32_t *seq_lens, int n_seq, const int32_t *parent,
-                                        const int32_t *capacity, const uint8_t *held, int32_t *table_out,
-                                        int out_stride, int32_t *lens_out, int n_out, int32_t *info, void *workspace,
-                                        size_t workspace_bytes, void *stream) {
-    const char *fn = "kv_pages_update";
+// kv_dim 0: whole rows.
+static int pages_update(const char *fn, void *k_pages, void *v_pages, int dtype, int64_t kv_stride, int page_size,
+                        int n_pages, int kv_dim, int n_layer, int64_t layer_stride, const int32_t *block_table,
+                        int table_stride, const int32_t *seq_lens, int n_seq, const int32_t *parent,
+                        const int32_t *capacity, const uint8_t *held, int32_t *table_out, int out_stride,
+                        int32_t *lens_out, int n_out, int32_t *info, void *workspace, size_t workspace_bytes,
+                        void *stream) {
     if (!dtype_ok(dtype)) return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: dtype %d", fn, dtype);
     if (page_size < 1 || (page_size & (page_size - 1)))
         return set_error(ULLM_HIP_E_INVALID, "%s: page_size %d must be a power of two", fn, page_size);
@@ -403,13 +412,16 @@ extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype,
         return set_error(ULLM_HIP_E_INVALID, "%s: a table of 2^31 positions or more", fn);
     if ((int64_t)n_out * out_stride > INT_MAX)  // (the pages asked for are counted in 32 bits)
         return set_error(ULLM_HIP_E_INVALID, "%s: a table of 2^31 entries or more", fn);
+    if (kv_stride < kv_dim || (n_layer > 1 && layer_stride < kv_dim))
+        return set_error(ULLM_HIP_E_INVALID, "%s: rows or layers share memory", fn);
     if (n_out == 0) return ULLM_HIP_OK;
     if ((n_layer && (!k_pages || !v_pages)) || (n_seq && (!block_table || !seq_lens)) || !parent || !capacity ||
         !table_out || !lens_out || !info)
         return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
     const int eb = dtype_bytes(dtype);
-    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || kv_stride * eb % 16 || layer_stride * eb % 16)
-        return set_error(ULLM_HIP_E_INVALID, "%s: pools and strides must be 16-byte aligned", fn);
+    if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15 || kv_stride * eb % 16 || layer_stride * eb % 16 ||
+        (int64_t)kv_dim * eb % 16)
+        return set_error(ULLM_HIP_E_INVALID, "%s: pools, rows and strides must be 16-byte aligned", fn);
     const size_t nt = 4 * (size_t)n_out * out_stride, ot = 4 * (size_t)n_seq * table_stride;
     if (overlap(table_out, nt, block_table, ot) || overlap(lens_out, 4 * (size_t)n_out, block_table, ot))
         return set_error(ULLM_HIP_E_INVALID, "%s: the new table or lengths overlap the old table", fn);
@@ -417,8 +429,9 @@ extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype,
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255)
         return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, need);
     char *ws = (char *)workspace;
-    PagesArgs a{(char *)k_pages, (char *)v_pages, kv_stride * eb, layer_stride * eb, block_table, seq_lens, parent,
-                capacity, held, table_out, lens_out, info, table_stride, n_seq, out_stride, n_out, n_pages,
+    PagesArgs a{(char *)k_pages, (char *)v_pages, kv_stride * eb, layer_stride * eb,
+                kv_dim < kv_stride ? (int)((int64_t)kv_dim * eb / 16) : 0, block_table, seq_lens, parent, capacity,
+                held, table_out, lens_out, info, table_stride, n_seq, out_stride, n_out, n_pages,
                 __builtin_ctz(page_size), nullptr, nullptr, (int32_t *)ws, (PagesSeq *)(ws + 256)};
     a.owner = (int32_t *)(ws + 256 + (size_t)n_out * sizeof(PagesSeq));
     a.free_list = a.owner + n_pages;
@@ -427,4 +440,28 @@ extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype,
     if (int rc = check_hip(hipGetLastError(), "kv_pages_update launch")) return rc;
     launch_kernel(pages_apply_kernel, dim3(8, n_out, 1 + 2 * n_layer), dim3(256), 0, st, a);
     return check_hip(hipGetLastError(), "kv_pages_update launch");
+}
+
+extern "C" int ullm_hip_kv_pages_update(void *k_pages, void *v_pages, int dtype, int64_t kv_stride, int page_size,
+                                        int n_pages, int n_layer, int64_t layer_stride, const int32_t *block_table,
+                                        int table_stride, const int32_t *seq_lens, int n_seq, const int32_t *parent,
+                                        const int32_t *capacity, const uint8_t *held, int32_t *table_out,
+                                        int out_stride, int32_t *lens_out, int n_out, int32_t *info, void *workspace,
+                                        size_t workspace_bytes, void *stream) {
+    return pages_update("kv_pages_update", k_pages, v_pages, dtype, kv_stride, page_size, n_pages, 0, n_layer,
+                        layer_stride, block_table, table_stride, seq_lens, n_seq, parent, capacity, held, table_out,
+                        out_stride, lens_out, n_out, info, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ullm_hip_kv_pages_update_rows(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
+                                             int page_size, int n_pages, int kv_dim, int n_layer,
+                                             int64_t layer_stride, const int32_t *block_table, int table_stride,
+                                             const int32_t *seq_lens, int n_seq, const int32_t *parent,
+                                             const int32_t *capacity, const uint8_t *held, int32_t *table_out,
+                                             int out_stride, int32_t *lens_out, int n_out, int32_t *info,
+                                             void *workspace, size_t workspace_bytes, void *stream) {
+    if (kv_dim < 1) return set_error(ULLM_HIP_E_INVALID, "kv_pages_update_rows: kv_dim < 1");
+    return pages_update("kv_pages_update_rows", k_pages, v_pages, dtype, kv_stride, page_size, n_pages, kv_dim,
+                        n_layer, layer_stride, block_table, table_stride, seq_lens, n_seq, parent, capacity, held,
+                        table_out, out_stride, lens_out, n_out, info, workspace, workspace_bytes, stream);
 }
