@@ -372,7 +372,8 @@ int ullm_hip_attn_prefill_paged_ws(const void *q, const void *k_pages, const voi
  * n_nodes[b] on, and rows whose position is outside [0, rope_n_pos), give zeros
  * in q_out and nothing in the cache; a slot outside the cache (n_ctx rows per
  * sequence), the table or the pool drops the K/V row.
- * seq_stride: elements from sequence to sequence (ignored when batch == 1).
+ * seq_stride: elements from sequence to sequence (ignored when batch == 1); the
+ *             sequences must not share rows.
  * Every tensor and row stride 16-byte aligned (norms, rope_cs and the int32
  * arrays: by their elements). */
 int ullm_hip_qkv_append_tree(const float *q_in, const float *k_in, const float *v_in,
@@ -451,7 +452,7 @@ size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int ma
  * place.  path: int32[batch][path_stride], any order, a node also twice; entries
  * below 0 and rows outside the cache (n_ctx rows per sequence, the table, the
  * pool) are left as they are.  kv_dim elements of each row are moved; layers must
- * not share rows, nor sequences of a contiguous cache (strides >= kv_dim).
+ * not share rows (layer_stride >= kv_dim), nor sequences of a contiguous cache.
  * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; not seq_lens itself.
  * path_stride <= 1024; pools, rows and strides 16-byte aligned.  Sequences must
  * not share the pages of their drafts (ullm_hip_kv_pages_update sees to it). */

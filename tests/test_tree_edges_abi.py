@@ -1,8 +1,10 @@
 """Refusals of the drafted trees' and page tables' entry points at their edges, on
 the CPU: codes come before any device work."""
+import ctypes as C
+
 import pytest
 
-from test_tree_abi import FAKE, ODD, UPDATE, call
+from test_tree_abi import ACCEPT, APPEND, FAKE, ODD, UPDATE, call
 from ullm_amd import _lib as L
 
 ROWS = {**{n: x for n, x in UPDATE.items() if n in ("k", "v", "dtype", "kvs", "P", "pages")}, "kvd": 128,
@@ -19,3 +21,13 @@ def test_update_rows_refuses(change, code):
 
 def test_update_rows_of_nothing():
     assert call("kv_pages_update_rows", ROWS, n=0, k=None) == L.OK
+
+
+@pytest.mark.parametrize("kvs,ss", [(256, 0), (256, 8), (256, 248), (512, 256), (768, 256), (1024, 512)])
+def test_sequences_that_share_rows_are_refused(kvs, ss):
+    """Four sequences whose first rows overlap, or whose rows lie between another's."""
+    apart = {**APPEND, "qo": C.c_void_p(0x20000), "batch": 4, "kvs": kvs, "ss": ss}
+    assert call("qkv_append_tree", apart) == L.E_INVALID
+    assert b"share rows" in L.lib().ullm_hip_last_error()
+    assert call("kv_accept", {**ACCEPT, "batch": 4, "kvs": kvs, "ss": ss}) == L.E_INVALID
+    assert b"share rows" in L.lib().ullm_hip_last_error()

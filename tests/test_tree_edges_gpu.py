@@ -94,3 +94,42 @@ def test_pools_whose_rows_overlap_are_refused(dev):
         v = k.as_strided(sizes, strides)
         with pytest.raises(L.UllmHipError):
             A.kv_pages_update(v, v, i32([[0]], dev), i32([5], dev), i32([0, 0], dev), i32([6, 6], dev))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("pad", [0, 16])
+def test_strides_left_out_are_the_caches_own(dev, dt, pad):
+    """Caches [B, n_ctx, kv_dim], whole or columns of wider rows, without strides: every
+    sequence's rows go to its own, and are read from there."""
+    t, H, Hk, D, T, n_ctx, lens = DT[dt], 8, 2, 64, 5, 90, [60, 3, 85]
+    B = len(lens)
+    g = torch.Generator(device=dev).manual_seed(pad)
+    full = [torch.randn(B, n_ctx, Hk * D + pad, device=dev, generator=g).to(t) for _ in "kv"]
+    want = [x.clone() for x in full]
+    q, k, v = (torch.randn(B, T, n * D, device=dev, generator=g) for n in (H, Hk, Hk))
+    cs, ln = A.rope_table(n_ctx, D, 1e4), i32(lens, dev)
+    more = dict(n_head=H, n_kv_head=Hk, head_dim=D, q_dtype=t)
+    qs = [A.qkv_append_tree(q[b:b + 1], k[b:b + 1], v[b:b + 1], want[0][b], want[1][b], cs, ln[b:b + 1],
+                            kv_stride=Hk * D + pad, **more) for b in range(B)]
+    views = [x[..., :Hk * D] for x in full]
+    got = A.qkv_append_tree(q, k, v, *views, cs, ln, **more)
+    assert torch.equal(got, torch.cat(qs))
+    for x, w in zip(full, want):
+        assert torch.equal(x, w)
+    out = A.attn_tree(got.view(B, T, H, D), *views, None, ln, n_ctx, Hk)
+    assert torch.equal(out, attend(got.view(B, T, H, D), full, None, None, ln, n_ctx, Hk, None, None, 0))
+
+
+def test_one_cache_for_all_sequences_is_read_but_not_written(dev):
+    t, H, Hk, D, T, B = torch.float16, 4, 2, 64, 3, 2
+    k = torch.zeros(50, Hk * D, device=dev, dtype=t)
+    ln, cs = i32([20, 30], dev), A.rope_table(50, D, 1e4)
+    x = [torch.ones(B, T, n * D, device=dev) for n in (H, Hk, Hk)]
+    more = dict(n_head=H, n_kv_head=Hk, head_dim=D, q_dtype=t)
+    for cache, strides in ((k, {}), (k, dict(seq_stride=0)), (k.expand(B, 50, Hk * D), {}), (k[None], {})):
+        with pytest.raises(L.UllmHipError) as e:
+            A.qkv_append_tree(*x, cache, cache.clone(), cs, ln, **strides, **more)
+        assert e.value.code == L.E_INVALID
+        q = torch.ones(B, T, H, D, device=dev, dtype=t)
+        assert A.attn_tree(q, cache, cache, None, ln, 40, Hk, **strides).shape == q.shape
+    assert not k.any()

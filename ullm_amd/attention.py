@@ -188,15 +188,17 @@ def tree_masks(parents):
 
 
 def attn_tree(q, k_cache, v_cache, mask, seq_lens, max_len, n_kv_head, *, n_nodes=None,
-              positions=None, window=0, scale=None, kv_stride=None, seq_stride=0, out=None,
+              positions=None, window=0, scale=None, kv_stride=None, seq_stride=None, out=None,
               out_dtype=None, workspace=None, stream=None):
     """Attention of a tree of drafted tokens over the cache that holds its
     sequence and, from row seq_lens[b] on, the tokens themselves
     (ullm_hip_attn_tree has the rules).
 
     q: [B, nodes, n_head, D] in the cache's dtype.  k_cache/v_cache: layer base
-    with `kv_stride` elements per position (default n_kv_head*D) and
-    `seq_stride` between sequences.  mask: int64 [B, nodes, ceil(nodes/64)] (see
+    with `kv_stride` elements per position (default: the caches' own where their
+    rows are [.., n_kv_head*D], else n_kv_head*D) and `seq_stride` between
+    sequences (default: the caches' own where they are [B, n_ctx, kv_dim], else 0,
+    one cache for all).  mask: int64 [B, nodes, ceil(nodes/64)] (see
     tree_masks), or None: each node sees the nodes up to itself.  seq_lens:
     int32 [B], positions before the draft; n_nodes: int32 [B], nodes of each
     sequence (default: all); positions: int32 [B, nodes] (default: seq_lens + i).
@@ -221,12 +223,12 @@ def attn_tree_paged(q, k_pages, v_pages, block_table, mask, seq_lens, max_len, n
 def qkv_append_tree(q, k, v, k_cache, v_cache, rope_cs, seq_lens, positions=None, *, n_head,
                     n_kv_head, head_dim, n_nodes=None, rotary_dim=None, neox=True, q_norm=None,
                     k_norm=None, eps=1e-6, q_bias=None, k_bias=None, v_bias=None, q_out=None,
-                    q_dtype=None, kv_stride=None, seq_stride=0, n_ctx=None, stream=None):
+                    q_dtype=None, kv_stride=None, seq_stride=None, n_ctx=None, stream=None):
     """qkv_append of drafted tokens: q [B, nodes, n_head*D], k/v [B, nodes,
     n_kv_head*D] f32.  Node i of sequence b is rotated to positions[b, i]
     (default seq_lens[b] + i), its K/V rows land at position seq_lens[b] + i of
     a cache of n_ctx (default: the caches' second-last dimension) positions per
-    sequence.  Returns q_out [B, nodes, n_head*D] (q_dtype); rows past
+    sequence, with strides as for attn_tree; sequences must not share rows.  Returns q_out [B, nodes, n_head*D] (q_dtype); rows past
     n_nodes[b] are zeros and are not stored."""
     return _F.append_tree(q, k, v, k_cache, v_cache, None, seq_lens, n_nodes, positions, rope_cs,
                           n_head, n_kv_head, head_dim, rotary_dim, neox, q_norm, k_norm, eps, q_bias,

@@ -669,6 +669,8 @@ static int append_tree(const char *fn, const float *q_in, const float *k_in, con
     if (kv_stride < (int64_t)n_kv_head * head_dim) return set_error(ULLM_HIP_E_INVALID, "%s: kv_stride too small", fn);
     if (tm.rope_n_pos < 1) return set_error(ULLM_HIP_E_INVALID, "%s: rope_n_pos < 1", fn);
     if (batch == 0 || tm.nodes == 0) return ULLM_HIP_OK;
+    if (!tm.tab && !rows_apart(batch, tm.seq_stride, kv_stride, (int64_t)n_kv_head * head_dim))
+        return set_error(ULLM_HIP_E_INVALID, "%s: sequences share rows", fn);
     if (!q_in || !k_in || !v_in || !rope_cs || !q_out || !k_cache || !v_cache || !tm.len)
         return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
     if (q_out == (void *)q_in && q_dtype != ULLM_DT_F32)

@@ -120,6 +120,11 @@ inline int check_hip(hipError_t e, const char *what) {
 }
 inline int dtype_bytes(int dt) { return dt == ULLM_DT_F32 ? 4 : 2; }
 inline bool dtype_ok(int dt) { return dt == ULLM_DT_F32 || dt == ULLM_DT_F16 || dt == ULLM_DT_BF16; }
+// Whether `batch` sequences whose row t lies at b*seq_stride + t*kv_stride are apart:
+// sequence after sequence, or position after position.
+inline bool rows_apart(int64_t batch, int64_t seq_stride, int64_t kv_stride, int64_t kv_dim) {
+    return batch <= 1 || seq_stride >= kv_stride || (seq_stride >= kv_dim && (kv_stride - kv_dim) / (batch - 1) >= seq_stride);
+}
 
 // Merge of split-KV partials (decode_mfma.hip): acc [units][splits][gt][D]
 // and (m, l) [units][splits][gt][2] f32, units = batch * n_units.

@@ -516,6 +516,22 @@ int small(int64_t v, const char *msg) {
     if (v != (int)v) invalid(msg);
     return (int)v;
 }
+// Strides of contiguous caches, arguments i (from position to position) and j (from
+// sequence to sequence): where not given the caches' own, or rows of kvd elements
+// behind each other and one cache for all sequences.
+struct Strides {
+    int64_t kvs, ss;
+    Strides(const Args &a, int i, int j, const at::Tensor &k, const at::Tensor &v, int64_t B, int64_t kvd) {
+        auto rows = [&](const at::Tensor &t) {
+            return t.dim() >= 2 && t.size(-1) == kvd && t.stride(-1) == 1 && t.size(-2) > 1 ? t.stride(-2) : kvd;
+        };
+        auto seqs = [&](const at::Tensor &t) { return t.dim() == 3 && t.size(0) == B ? t.stride(0) : 0; };
+        if ((a.none(i) && rows(k) != rows(v)) || (a.none(j) && B > 1 && seqs(k) != seqs(v)))
+            invalid("k and v caches of different strides");
+        kvs = a.none(i) ? rows(k) : a.i64(i);
+        ss = a.none(j) ? seqs(k) : a.i64(j);
+    }
+};
 void out_check(const at::Tensor &t, at::IntArrayRef shape, const char *msg) {
     if (t.sizes() != shape || !t.is_contiguous()) invalid(msg);
 }
@@ -537,7 +553,7 @@ at::Tensor attn_tree(const Args &a) {
                  !mask->is_contiguous()))
         invalid("mask must be contiguous int64 [B, nodes, ceil(nodes/64)]");
     const float scale = a.none(11) ? (float)(1.0 / std::sqrt((double)D)) : (float)a.f(11);
-    int64_t kvs, ss = a.i64(13);
+    int64_t kvs, ss = 0;
     if (tab) {
         if (k.dim() != 3 || k.sizes() != v.sizes() || !k.is_contiguous() || !v.is_contiguous())
             invalid("k_pages/v_pages must be contiguous [n_pages, page_size, kv_stride]");
@@ -545,7 +561,8 @@ at::Tensor attn_tree(const Args &a) {
             invalid("block_table must be contiguous int32 [B, table_stride]");
         kvs = k.size(2);
     } else {
-        kvs = a.none(12) ? (int64_t)hk * D : a.i64(12);
+        const Strides s(a, 12, 13, k, v, B, (int64_t)hk * D);
+        kvs = s.kvs, ss = s.ss;
         const int64_t last = B && max_len > 0 ? (B - 1) * ss + (max_len - 1) * kvs + (int64_t)hk * D : 0;
         if (kvs < 0 || ss < 0 || last > elements_from(k) || last > elements_from(v))
             invalid("the caches end before max_len positions of every sequence");
@@ -599,7 +616,7 @@ at::Tensor append_tree(const Args &a) {
                   *nn_p = i32s(nn, {B}, "n_nodes must be contiguous int32 [B]"),
                   *pos_p = i32s(pos, {B, T}, "positions must be contiguous int32 [B, nodes]");
     if (kc.scalar_type() != vc.scalar_type()) invalid("k and v cache dtypes differ");
-    int64_t kvs, ss = a.i64(R + 3), n_ctx = 0;
+    int64_t kvs, ss = 0, n_ctx = 0;
     if (tab) {
         if (kc.dim() != 3 || kc.sizes() != vc.sizes() || !kc.is_contiguous() || !vc.is_contiguous())
             invalid("k_pages/v_pages must be contiguous [n_pages, page_size, kv_stride]");
@@ -607,7 +624,8 @@ at::Tensor append_tree(const Args &a) {
             invalid("block_table must be contiguous int32 [B, table_stride]");
         kvs = kc.size(2);
     } else {
-        kvs = a.none(R + 2) ? kvd : a.i64(R + 2);
+        const Strides s(a, R + 2, R + 3, kc, vc, B, kvd);
+        kvs = s.kvs, ss = s.ss;
         if (kc.dim() < 2 && a.none(R + 4)) invalid("caches must be [..., n_ctx, kv_dim], or n_ctx given");
         n_ctx = a.none(R + 4) ? kc.size(-2) : a.i64(R + 4);
         const int64_t last = B && n_ctx > 0 ? (B - 1) * ss + (n_ctx - 1) * kvs + kvd : 0;

@@ -129,7 +129,7 @@ static int kv_accept(const char *fn, AcceptArgs a, int dtype, int64_t kv_stride,
                          a.path_stride, kAcceptMax);
     if (n_layer < 1 || n_layer > 32767 || kv_dim < 1 || kv_stride < kv_dim || seq_stride < 0 || layer_stride < 0)
         return set_error(ULLM_HIP_E_INVALID, "%s: bad n_layer/kv_dim/strides", fn);
-    if ((n_layer > 1 && layer_stride < kv_dim) || (!a.tab && batch > 1 && seq_stride < kv_dim))
+    if ((n_layer > 1 && layer_stride < kv_dim) || (!a.tab && !rows_apart(batch, seq_stride, kv_stride, kv_dim)))
         return set_error(ULLM_HIP_E_INVALID, "%s: layers or sequences share rows", fn);
     if (batch == 0) return ULLM_HIP_OK;
     const int eb = dtype_bytes(dtype);
