@@ -171,10 +171,12 @@ def tree_masks(parents):
     the sequence's length for the nodes' positions.  Both on the host: a draft
     of fixed shape makes them once."""
     p = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+    if p.ndim == 0 or p.dtype.kind not in "iuf" or (p != np.floor(p)).any():
+        raise L.UllmHipError(L.E_INVALID, "parents must be whole numbers [..., nodes]")
     n = p.shape[-1]
-    flat = p.reshape(math.prod(p.shape[:-1]), n).astype(np.int64)
-    if (flat >= np.arange(n)).any():
+    if (p >= np.arange(n)).any():
         raise L.UllmHipError(L.E_INVALID, "a node must go on from an earlier one")
+    flat = np.maximum(p, -1).astype(np.int64).reshape(math.prod(p.shape[:-1]), n)
     mask = np.zeros((*flat.shape, -(-n // 64)), np.uint64)
     depth = np.zeros(flat.shape, np.int32)
     trees = np.arange(len(flat))
