@@ -133,3 +133,21 @@ def test_one_cache_for_all_sequences_is_read_but_not_written(dev):
         q = torch.ones(B, T, H, D, device=dev, dtype=t)
         assert A.attn_tree(q, cache, cache, None, ln, 40, Hk, **strides).shape == q.shape
     assert not k.any()
+
+
+@pytest.mark.parametrize("strides", [
+    dict(seq_stride=1 << 62), dict(seq_stride=(1 << 63) - 8), dict(kv_stride=1 << 62), dict(kv_stride=(1 << 63) - 8),
+    dict(kv_stride=1 << 61, seq_stride=1 << 62), dict(kv_stride=-128), dict(seq_stride=-8), dict(kv_stride=129 * 128)])
+def test_strides_past_the_caches_are_refused(dev, strides):
+    """Also those whose products pass 64 bits."""
+    t, H, Hk, D, T, B = torch.float16, 4, 2, 64, 3, 5
+    k = torch.zeros(B, 9, Hk * D, device=dev, dtype=t)
+    ln, cs = i32([2] * B, dev), A.rope_table(50, D, 1e4)
+    x = [torch.ones(B, T, n * D, device=dev) for n in (H, Hk, Hk)]
+    for n in (5, 9):
+        for call in (lambda: A.qkv_append_tree(*x, k, k.clone(), cs, ln, n_head=H, n_kv_head=Hk, head_dim=D, q_dtype=t, n_ctx=n, **strides),
+                     lambda: A.attn_tree(torch.ones(B, T, H, D, device=dev, dtype=t), k, k, None, ln, n, Hk, **strides)):
+            with pytest.raises(L.UllmHipError) as e:
+                call()
+            assert e.value.code == L.E_INVALID
+    assert not k.any()

@@ -531,6 +531,15 @@ struct Strides {
         kvs = a.none(i) ? rows(k) : a.i64(i);
         ss = a.none(j) ? seqs(k) : a.i64(j);
     }
+    // Whether `n` positions of B sequences, rows of kvd elements, end within both caches.
+    bool within(const at::Tensor &k, const at::Tensor &v, int64_t B, int64_t n, int64_t kvd) const {
+        if (kvs < 0 || ss < 0) return false;
+        if (B < 1 || n < 1) return true;
+        int64_t s, r, last;
+        return !__builtin_mul_overflow(B - 1, ss, &s) && !__builtin_mul_overflow(n - 1, kvs, &r) &&
+               !__builtin_add_overflow(s, r, &last) && !__builtin_add_overflow(last, kvd, &last) &&
+               last <= elements_from(k) && last <= elements_from(v);
+    }
 };
 void out_check(const at::Tensor &t, at::IntArrayRef shape, const char *msg) {
     if (t.sizes() != shape || !t.is_contiguous()) invalid(msg);
@@ -563,8 +572,7 @@ at::Tensor attn_tree(const Args &a) {
     } else {
         const Strides s(a, 12, 13, k, v, B, (int64_t)hk * D);
         kvs = s.kvs, ss = s.ss;
-        const int64_t last = B && max_len > 0 ? (B - 1) * ss + (max_len - 1) * kvs + (int64_t)hk * D : 0;
-        if (kvs < 0 || ss < 0 || last > elements_from(k) || last > elements_from(v))
+        if (!s.within(k, v, B, max_len, (int64_t)hk * D))
             invalid("the caches end before max_len positions of every sequence");
     }
     const Stream st(a, 17);
@@ -628,8 +636,7 @@ at::Tensor append_tree(const Args &a) {
         kvs = s.kvs, ss = s.ss;
         if (kc.dim() < 2 && a.none(R + 4)) invalid("caches must be [..., n_ctx, kv_dim], or n_ctx given");
         n_ctx = a.none(R + 4) ? kc.size(-2) : a.i64(R + 4);
-        const int64_t last = B && n_ctx > 0 ? (B - 1) * ss + (n_ctx - 1) * kvs + kvd : 0;
-        if (kvs < 0 || ss < 0 || last > elements_from(kc) || last > elements_from(vc))
+        if (!s.within(kc, vc, B, n_ctx, kvd))
             invalid("the caches end before n_ctx positions of every sequence");
     }
     const Stream st(a, R + 5);
