@@ -453,7 +453,7 @@ size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int ma
  * below 0 and rows outside the cache (n_ctx rows per sequence, the table, the
  * pool) are left as they are.  kv_dim elements of each row are moved; layers must
  * not share rows (layer_stride >= kv_dim), nor sequences of a contiguous cache.
- * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; not seq_lens itself.
+ * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; no memory of the inputs.
  * path_stride <= 1024; pools, rows and strides 16-byte aligned.  Sequences must
  * not share the pages of their drafts (ullm_hip_kv_pages_update sees to it). */
 int ullm_hip_kv_accept(void *k_cache, void *v_cache, int dtype, int64_t kv_stride,
@@ -482,7 +482,8 @@ int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype, int64_t kv
  *  - the others are taken, lowest number first, sequence by sequence, from the
  *    pages that no sequence keeps and that are not held;
  *  - entries past capacity[s], and where no page is left, are -1.
- * table_out: int32[n_out][out_stride]; not block_table itself
+ * table_out: int32[n_out][out_stride]; no output shares memory with block_table or
+ *            another output
  * lens_out:  int32[n_out], kept (less the positions that should have been copied
  *            where no page was left); may be seq_lens itself
  * held:      uint8[n_pages], pages to leave alone where not 0 (a stored prefix),

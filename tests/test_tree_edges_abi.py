@@ -49,3 +49,20 @@ def test_parents_of_a_tree():
     for parents in ([-1.0, 0.5], np.array([(1 << 64) - 1], np.uint64), [-1, 1 << 40], [True, False], [-1, float("nan")], 3):
         with pytest.raises(L.UllmHipError):
             A.tree_masks(parents)
+
+
+def test_outputs_in_what_is_still_read_are_refused():
+    """lens_out inside path or the block table, and page outputs inside the old table
+    or one another."""
+    far = {**ACCEPT, "path": C.c_void_p(0x60000), "lens": C.c_void_p(0x70000), "n": C.c_void_p(0x80000)}
+    for out in (0x60000, 0x60000 + 4 * 17, 0x60000 - 4):  # 2 x 9 entries
+        assert call("kv_accept", {**far, "out": C.c_void_p(out)}) == L.E_INVALID
+    paged = dict(k=FAKE, v=FAKE, dtype=L.DT_F16, kvs=256, P=32, pages=9, kvd=256, NL=3, ls=256 * 99 * 2, tab=C.c_void_p(0x90000),
+                 cols=3, path=far["path"], T=9, n=far["n"], lens=far["lens"], out=None, batch=2, st=None)
+    for out in (0x90000, 0x90000 + 4 * 5, 0x60000 + 4):
+        assert call("kv_accept_paged", {**paged, "out": C.c_void_p(out)}) == L.E_INVALID
+    far = {**ROWS, "tab": C.c_void_p(0x90000), "lens": C.c_void_p(0x70000), "parent": C.c_void_p(0x80000), "cap": C.c_void_p(0xa0000)}
+    for change in (dict(info=0x90000 + 4 * 11), dict(lo=0x90000 + 4 * 11), dict(info=0x20000 + 4 * 11), dict(lo=0x20000 + 4 * 11),
+                   dict(info=0x30000 + 8), dict(to=0x40000 - 4 * 11)):
+        assert call("kv_pages_update_rows", far, **{n: C.c_void_p(x) for n, x in change.items()}) == L.E_INVALID
+        assert b"overlap" in L.lib().ullm_hip_last_error()

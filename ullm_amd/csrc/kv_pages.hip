@@ -138,9 +138,11 @@ static int kv_accept(const char *fn, AcceptArgs a, int dtype, int64_t kv_stride,
     if (((uintptr_t)a.k | (uintptr_t)a.v) & 15 || (int64_t)kv_dim * eb % 16 || kv_stride * eb % 16 ||
         seq_stride * eb % 16 || layer_stride * eb % 16)
         return set_error(ULLM_HIP_E_INVALID, "%s: caches, rows and strides must be 16-byte aligned", fn);
-    if (overlap(a.len_out, 4 * (size_t)batch, a.len, 4 * (size_t)batch) ||
-        overlap(a.len_out, 4 * (size_t)batch, a.count, 4 * (size_t)batch))
-        return set_error(ULLM_HIP_E_INVALID, "%s: lens_out overlaps seq_lens or n_accept", fn);
+    // (one workgroup of a sequence writes its length while the others still read)
+    const size_t nl = 4 * (size_t)batch;
+    if (overlap(a.len_out, nl, a.len, nl) || overlap(a.len_out, nl, a.count, nl) ||
+        overlap(a.len_out, nl, a.path, nl * a.path_stride) || overlap(a.len_out, nl, a.tab, nl * a.tab_stride))
+        return set_error(ULLM_HIP_E_INVALID, "%s: lens_out overlaps seq_lens, n_accept, path or block_table", fn);
     a.rb = kv_stride * eb, a.seq_b = batch > 1 ? seq_stride * eb : 0, a.layer_b = layer_stride * eb;
     a.cols = (int)((int64_t)kv_dim * eb / 16);
     const int planes = a.tab || a.n_ctx ? 2 * n_layer : 0;  // (no rows: only the lengths)
@@ -423,8 +425,12 @@ static int pages_update(const char *fn, void *k_pages, void *v_pages, int dtype,
         (int64_t)kv_dim * eb % 16)
         return set_error(ULLM_HIP_E_INVALID, "%s: pools, rows and strides must be 16-byte aligned", fn);
     const size_t nt = 4 * (size_t)n_out * out_stride, ot = 4 * (size_t)n_seq * table_stride;
-    if (overlap(table_out, nt, block_table, ot) || overlap(lens_out, 4 * (size_t)n_out, block_table, ot))
-        return set_error(ULLM_HIP_E_INVALID, "%s: the new table or lengths overlap the old table", fn);
+    if (overlap(table_out, nt, block_table, ot) || overlap(lens_out, 4 * (size_t)n_out, block_table, ot) ||
+        overlap(info, 12, block_table, ot))
+        return set_error(ULLM_HIP_E_INVALID, "%s: an output overlaps the old table", fn);
+    if (overlap(table_out, nt, lens_out, 4 * (size_t)n_out) || overlap(table_out, nt, info, 12) ||
+        overlap(lens_out, 4 * (size_t)n_out, info, 12))
+        return set_error(ULLM_HIP_E_INVALID, "%s: the outputs overlap", fn);
     const size_t need = pages_ws(n_out, n_pages);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace & 255)
         return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, need);
