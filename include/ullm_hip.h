@@ -451,7 +451,8 @@ size_t ullm_hip_tree_workspace_bytes(int dtype, int batch, int max_nodes, int ma
  * 0..path_stride), in each of n_layer layers layer_stride elements apart, in
  * place.  path: int32[batch][path_stride], any order, a node also twice; entries
  * below 0 and rows outside the cache (n_ctx rows per sequence, the table, the
- * pool) are left as they are.  kv_dim elements of each row are moved; layers must
+ * pool) are left as they are.  kv_dim elements of each row are moved (once, where V
+ * is K's memory; else the two must not overlap); layers must
  * not share rows (layer_stride >= kv_dim), nor sequences of a contiguous cache.
  * lens_out: int32[batch], seq_lens[b] + n_accept[b], or NULL; no memory of the inputs.
  * path_stride <= 1024; pools, rows and strides 16-byte aligned.  Sequences must

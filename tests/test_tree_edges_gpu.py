@@ -151,3 +151,20 @@ def test_strides_past_the_caches_are_refused(dev, strides):
                 call()
             assert e.value.code == L.E_INVALID
     assert not k.any()
+
+
+@pytest.mark.parametrize("page", [0, 32])
+@pytest.mark.parametrize("NL", [1, 5])
+def test_accept_of_a_cache_that_is_both_k_and_v(dev, page, NL):
+    """One tensor given as K and V moves once: twice would undo a path that turns round."""
+    T, n, kvd = 40, 30, 512
+    x = torch.randn(NL, 96, kvd, device=dev, generator=torch.Generator(device=dev).manual_seed(NL)).bfloat16()
+    want, path = x.clone(), np.random.default_rng(NL).permutation(T)
+    want[:, n:n + T] = x[:, torch.from_numpy(n + path).to(dev)]
+    count, ln, p = i32([T], dev), i32([n], dev), i32(path[None], dev)
+    if page:
+        k = x.view(NL, 3, page, kvd)
+        new = A.kv_accept_paged(k, k, i32([[0, 1, 2]], dev), p, count, ln)
+    else:
+        new = A.kv_accept(x, x, p, count, ln)
+    assert new.tolist() == [n + T] and torch.equal(x, want)

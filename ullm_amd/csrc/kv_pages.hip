@@ -9,7 +9,7 @@ namespace ullm {
 
 // ---- the accepted rows of a drafted tree ----
 // Row len + j of sequence b takes what row len + path[b][j] held, j < count[b],
-// for K and V of every layer (2 n_layer planes).  A workgroup takes a sequence
+// for K and V of every layer (2 n_layer planes, n_layer where V is K).  A workgroup takes a sequence
 // and some planes: it finds its rows' places once, then for 2^log_c columns of
 // 16 bytes at a time reads all source rows into registers and stores after a
 // barrier, the next columns' loads in flight.  So any path is right, also one
@@ -24,6 +24,7 @@ struct AcceptArgs {
     int tab_stride, shift, n_pages, n_ctx;
     const int32_t *path, *count, *len;
     int path_stride, cols;  // 16-byte columns of a row that are moved
+    int one;                // K and V are the same memory, which moves once
     int32_t *len_out;
 };
 constexpr int kAcceptT = 256, kAcceptU = 8;
@@ -55,8 +56,8 @@ __device__ __forceinline__ void accept_planes(const AcceptArgs &a, const int64_t
     const int gx = gridDim.x, passes = (((a.cols - 1) >> log_c) - (int)blockIdx.x + gx) / gx;
     auto col = [&](int i) { return (((int)blockIdx.x + i % passes * gx) << log_c) + c; };
     auto base = [&](int i) {  // of pass i over this workgroup's planes and columns
-        const int p = p0 + i / passes;
-        return ((p & 1) ? a.v : a.k) + (p >> 1) * a.layer_b;
+        const int p = p0 + i / passes, layer = a.one ? p : p >> 1;
+        return (!a.one && (p & 1) ? a.v : a.k) + layer * a.layer_b;
     };
     auto load = [&](int i, u32x4 (&x)[U]) {
         const char *at = base(i) + (int64_t)min(col(i), a.cols - 1) * 16;
@@ -145,7 +146,8 @@ static int kv_accept(const char *fn, AcceptArgs a, int dtype, int64_t kv_stride,
         return set_error(ULLM_HIP_E_INVALID, "%s: lens_out overlaps seq_lens, n_accept, path or block_table", fn);
     a.rb = kv_stride * eb, a.seq_b = batch > 1 ? seq_stride * eb : 0, a.layer_b = layer_stride * eb;
     a.cols = (int)((int64_t)kv_dim * eb / 16);
-    const int planes = a.tab || a.n_ctx ? 2 * n_layer : 0;  // (no rows: only the lengths)
+    a.one = a.k == a.v;
+    const int planes = a.tab || a.n_ctx ? (a.one ? 1 : 2) * n_layer : 0;  // (no rows: only the lengths)
     const int gx = std::max(1, std::min((a.cols + 255) / 256, kAcceptWgs / batch));  // passes of 256 columns side by side
     const int64_t wgs = (int64_t)batch * gx * planes;
     const int per = (int)std::max<int64_t>(1, std::min<int64_t>(planes, wgs / kAcceptWgs));
@@ -373,7 +375,7 @@ extern "C" int ullm_hip_kv_accept(void *k_cache, void *v_cache, int dtype, int64
                                   int32_t *lens_out, int batch, void *stream) {
     if (n_ctx < 0) return set_error(ULLM_HIP_E_INVALID, "kv_accept: n_ctx < 0");
     const AcceptArgs a{(char *)k_cache, (char *)v_cache, 0, 0, 0, nullptr, 0, 0, 0, n_ctx,
-                       path, n_accept, seq_lens, path_stride, 0, lens_out};
+                       path, n_accept, seq_lens, path_stride, 0, 0, lens_out};
     return kv_accept("kv_accept", a, dtype, kv_stride, seq_stride, kv_dim, n_layer, layer_stride, batch, stream);
 }
 
@@ -387,7 +389,7 @@ extern "C" int ullm_hip_kv_accept_paged(void *k_pages, void *v_pages, int dtype,
     if (n_pages < 1 || table_stride < 1 || (batch > 0 && !block_table))
         return set_error(ULLM_HIP_E_INVALID, "kv_accept_paged: bad n_pages/block_table");
     const AcceptArgs a{(char *)k_pages, (char *)v_pages, 0, 0, 0, block_table, table_stride, __builtin_ctz(page_size),
-                       n_pages, 0, path, n_accept, seq_lens, path_stride, 0, lens_out};
+                       n_pages, 0, path, n_accept, seq_lens, path_stride, 0, 0, lens_out};
     return kv_accept("kv_accept_paged", a, dtype, kv_stride, 0, kv_dim, n_layer, layer_stride, batch, stream);
 }
 
