@@ -374,6 +374,7 @@ int ullm_hip_attn_prefill_paged_ws(const void *q, const void *k_pages, const voi
  * sequence), the table or the pool drops the K/V row.
  * seq_stride: elements from sequence to sequence (ignored when batch == 1); the
  *             sequences must not share rows.
+ * batch * max_nodes < 2^24.
  * Every tensor and row stride 16-byte aligned (norms, rope_cs and the int32
  * arrays: by their elements). */
 int ullm_hip_qkv_append_tree(const float *q_in, const float *k_in, const float *v_in,

@@ -66,3 +66,9 @@ def test_outputs_in_what_is_still_read_are_refused():
                    dict(info=0x30000 + 8), dict(to=0x40000 - 4 * 11)):
         assert call("kv_pages_update_rows", far, **{n: C.c_void_p(x) for n, x in change.items()}) == L.E_INVALID
         assert b"overlap" in L.lib().ullm_hip_last_error()
+
+
+def test_append_of_more_rows_than_a_launch_has():
+    apart = {**APPEND, "qo": C.c_void_p(0x20000), "kvs": 256, "ss": 256 * 99}
+    for batch, nodes in ((1 << 24, 1), (1, 1 << 24), (1 << 14, 1 << 10), ((1 << 29) - 1, 1)):
+        assert call("qkv_append_tree", {**apart, "batch": batch, "nodes": nodes}) == L.E_INVALID
