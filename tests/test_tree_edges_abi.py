@@ -70,5 +70,5 @@ def test_outputs_in_what_is_still_read_are_refused():
 
 def test_append_of_more_rows_than_a_launch_has():
     apart = {**APPEND, "qo": C.c_void_p(0x20000), "kvs": 256, "ss": 256 * 99}
-    for batch, nodes in ((1 << 24, 1), (1, 1 << 24), (1 << 14, 1 << 10), ((1 << 29) - 1, 1)):
+    for batch, nodes in ((1 << 24, 1), (1, 1 << 24), (1 << 14, 1 << 10), ((1 << 29) - 1, 1), ((1 << 31) - 1, (1 << 31) - 1), (1 << 30, 1 << 26)):
         assert call("qkv_append_tree", {**apart, "batch": batch, "nodes": nodes}) == L.E_INVALID

@@ -661,7 +661,7 @@ static int append_tree(const char *fn, const float *q_in, const float *k_in, con
     if (head_dim != 64 && head_dim != 128 && head_dim != 256)
         return set_error(ULLM_HIP_E_UNSUPPORTED, "%s: head_dim %d not in {64,128,256}", fn, head_dim);
     // (a workgroup a row, and a grid has less than 2^32 threads)
-    if (batch < 0 || tm.nodes < 0 || (int64_t)batch * tm.nodes * kAppendWaves * 64 >= 1ll << 32)
+    if (batch < 0 || tm.nodes < 0 || (int64_t)batch * tm.nodes >= (1ll << 32) / (kAppendWaves * 64))
         return set_error(ULLM_HIP_E_INVALID, "%s: bad batch/max_nodes", fn);
     if (n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || (int64_t)n_head * head_dim > 0x7fffffff)
         return set_error(ULLM_HIP_E_INVALID, "%s: bad heads", fn);
