@@ -418,7 +418,7 @@ int ullm_hip_qkv_append_tree_paged(const float *q_in, const float *k_in, const f
  * mask:   int64[batch][max_nodes][ceil(max_nodes/64)], bit c % 64 of word c / 64
  *         (its own bit too: a node sees itself only by it), or NULL: node i sees
  *         the nodes up to i.  positions must be given where window > 0 and mask
- *         is
+ *         is; for a window those below seq_lens[b] count as seq_lens[b]
  * max_len: host-side upper bound of seq_lens[b] + n_nodes[b]; keys from it on are
  *         not attended.  Keys 0..max_len-1 of a contiguous cache must be
  *         readable

@@ -14,6 +14,8 @@ namespace ullm {
 // (16 rows 22.7, 256 rows 34.2), 4000 43.8 (64 rows 42.3, 256 rows 43.8, 16 rows 63.8); 26
 // nodes at 300 tokens, 12/2 heads, 9.9 (256 rows 16.8), at 4000 13.0 (16 rows, in parts; 256
 // rows 16.5); 2 sequences of 64 nodes, 32/8 x 128, f32, 4000 tokens 57.7 (128 rows; 64 rows 82).
+// Over 66 calls of 16 bits, 300 to 32000 tokens, the choice takes at most 1.14 times the
+// best shape's time, but for two (1.17 and 1.23).
 struct TreeCut {
     TreeShape shape;
     TreePlan plan;
@@ -48,6 +50,11 @@ static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window
         const int part = s.wr == 8 ? 4 : 2 * s.wk;  // blocks that a part has at least
         // Where they fill the card they wait for memory or for the matrix units: of what they
         // read row tiles of one kv head share a part, but never less than the products take.
+        // (It is memory that they wait for where `full` is within .9 and 1.25 of the reads of
+        // K and V at 5.3 TB/s.  The part that tiles share goes by the square root of their
+        // number: the number itself chose too narrow shapes.  The products of a row are put at
+        // a third over the widest 16-bit shape's time of one, which they bind, and over f32 at
+        // 4.5e-4 us a row and column, half the rate of a large f32 product.)
         const int on = room / 256, widest = D == 256 ? 128 : 256;
         const float read = room * 64 * rb / 5.3e6f;
         const float products = dtype == ULLM_DT_F32
@@ -60,14 +67,17 @@ static TreeCut tree_cut(int dtype, int batch, int nodes, int max_len, int window
         for (int64_t slots = batch, k = 1;;) {
             const float wgs = (float)slots * units / room;
             const float block = c.few + (full - c.few) * std::min(std::max((wgs - .125f) / .875f, 0.f), 1.f);
-            float us = 4.5f + s.rows() * rb * 1e-4f;  // start and end of a workgroup
+            // start and end of a workgroup: what is left at no keys of the times that kTreeCost
+            // is the slope of (16 bits x 128, 16 to 256 rows: 4.4, 5.6, 7.3, 7.3, 10.9)
+            float us = 4.5f + s.rows() * rb * 1e-4f;
             if (slots == batch) {
                 us = std::max(wgs, 1.f) * (us + blocks * block);
             } else {
                 // (the sequences of a batch are taken to have 0.75 max_len on average)
                 const float len = std::ceil((batch > 1 ? .75f : 1.f) * blocks * batch / slots);
                 us += std::max(len, (float)part) * block;
-                us += 3 + (batch > 1 ? 1.5f : 0) + 1.2e-6f * slots * n_kv * rows * D;  // the merge, the cut, what is joined
+                // the merge, the cut, and the joined partials: 8 bytes an element at 6.6 TB/s
+                us += 3 + (batch > 1 ? 1.5f : 0) + 1.2e-6f * slots * n_kv * rows * D;
             }
             if (us < least) {
                 least = us;

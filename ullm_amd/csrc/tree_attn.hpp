@@ -34,15 +34,16 @@
 //    workgroups of all sequences are alike whatever their lengths; the lengths
 //    are on the device, so every workgroup works the cut out for itself
 //    (find_part).  tree_merge_kernel adds the parts up.
-// Measured (trace, this kernel without the merge): 8 sequences of 4K-32K, 64 nodes,
-// 32/4 heads of 128, bf16: 206 us, 143 GFLOP at 695 TFLOP/s (matrix instructions 31%
-// of the cycles, other vector instructions as many; the clock falls under it, 226 us
-// back to back; waves in two sets half a tile apart took 224); 24 sequences of 90-1500,
-// 7 nodes, 40/8 heads, bf16: 21.1 us, 84 MB at 4.0 TB/s, the chain of a workgroup's
+// Measured (trace of 400 calls back to back, this kernel without the merge): 8 sequences
+// of 4K-32K, 64 nodes, 32/4 heads of 128, bf16: 261 us, 215 GFLOP of products (P.V twice)
+// at 822 TFLOP/s, matrix units busy in 48% of the cycles of a busy CU, and CUs busy in 71%
+// of the kernel's (the second row tile of a sequence of 40 to 56 nodes is part-filled); with
+// P in one piece 206, and 224 with waves in two sets half a tile apart; 24 sequences of
+// 90-1500, 7 nodes, 40/8 heads, bf16: 20.9 us, 84 MB at 4.0 TB/s, the chain of a workgroup's
 // start and end being 8 of them; f32, 2 sequences of 3K-8K, 48 nodes, 32/8 heads of 64:
-// 42.4 us, six products of 4.4 GFLOP at 620 TFLOP/s (with f32 products 75.6); one
-// sequence of 4K, 26 nodes, 12/2 heads of 128, f16: 9.5 us, of which the launch, the
-// first loads and the epilogue are 8.
+// 39.6 us, six products of 4.4 GFLOP at 667 TFLOP/s (with f32 products 75.6); one sequence
+// of 4K, 26 nodes, 12/2 heads of 128, f16: 9.9 us, of which the launch, the first loads and
+// the epilogue are 8.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -232,10 +233,10 @@ void tree_kernel(TreeArgs a, TreeKv kv, TreePlan pl) {
     constexpr bool F = __is_same(T, F32);
     constexpr int KH = tree_halves(F, WR), SH = WR * KH, GR = WK * KH;  // waves of a ring, groups of waves to add up
     constexpr int EB = T::bytes, RB = D * EB, SLOTS = RB / 16, RPI = 1024 / RB;
-    constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile (256 rows x 128 of bf16: 240 us, with 32 keys 305)
+    constexpr int KB = WR == 8 && RB <= 256 ? 64 : 32;  // keys of a tile (256 rows x 128 of bf16, P in one piece: 240 us, with 32 keys 305)
     constexpr bool X3 = F && NR * WR > 4 && D <= 128, FM = F && !X3;
     // Where four tiles fit the ring, waves that share them take two a step: half the
-    // barriers (256 rows x 128 of bf16: 225 us, 252 with one).
+    // barriers (256 rows x 128 of bf16, P in one piece: 225 us, 252 with one).
     constexpr int FIT = tree_stages<RB, WR, WK, 2 * KB * RB>(), KS = !X3 && SH > 1 && FIT >= 4 ? 2 : 1;
     constexpr int TILE = KS * KB * RB, STAGE = 2 * TILE;  // a step's tiles as fetched, K and K and V
     using CT = typename std::conditional<X3, BF16, T>::type;  // operands
