@@ -168,3 +168,13 @@ def test_accept_of_a_cache_that_is_both_k_and_v(dev, page, NL):
     else:
         new = A.kv_accept(x, x, p, count, ln)
     assert new.tolist() == [n + T] and torch.equal(x, want)
+
+
+def test_a_cache_of_heads_with_as_many_positions_as_sequences(dev):
+    """[n_ctx, n_kv_head, head_dim] is one cache, also where n_ctx is the batch."""
+    t, H, Hk, D, T, B = torch.float16, 4, 2, 64, 2, 40
+    g = torch.Generator(device=dev).manual_seed(1)
+    k, v = (torch.randn(B, Hk, D, device=dev, generator=g).to(t) for _ in "kv")
+    q, ln = torch.randn(B, T, H, D, device=dev, generator=g).to(t), i32([i % 38 for i in range(B)], dev)
+    out = A.attn_tree(q, k, v, None, ln, B, Hk)
+    assert torch.equal(out, A.attn_tree(q, k.view(B, -1), v.view(B, -1), None, ln, B, Hk, kv_stride=Hk * D, seq_stride=0))

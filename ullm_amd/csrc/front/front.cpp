@@ -525,7 +525,7 @@ struct Strides {
         auto rows = [&](const at::Tensor &t) {
             return t.dim() >= 2 && t.size(-1) == kvd && t.stride(-1) == 1 && t.size(-2) > 1 ? t.stride(-2) : kvd;
         };
-        auto seqs = [&](const at::Tensor &t) { return t.dim() == 3 && t.size(0) == B ? t.stride(0) : 0; };
+        auto seqs = [&](const at::Tensor &t) { return t.dim() == 3 && t.size(0) == B && t.size(2) == kvd ? t.stride(0) : 0; };
         if ((a.none(i) && rows(k) != rows(v)) || (a.none(j) && B > 1 && seqs(k) != seqs(v)))
             invalid("k and v caches of different strides");
         kvs = a.none(i) ? rows(k) : a.i64(i);
