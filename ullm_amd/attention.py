@@ -230,8 +230,9 @@ def qkv_append_tree(q, k, v, k_cache, v_cache, rope_cs, seq_lens, positions=None
     n_kv_head*D] f32.  Node i of sequence b is rotated to positions[b, i]
     (default seq_lens[b] + i), its K/V rows land at position seq_lens[b] + i of
     a cache of n_ctx (default: the caches' second-last dimension) positions per
-    sequence, with strides as for attn_tree; sequences must not share rows.  Returns q_out [B, nodes, n_head*D] (q_dtype); rows past
-    n_nodes[b] are zeros and are not stored."""
+    sequence, with strides as for attn_tree; sequences must not share rows.
+    Returns q_out [B, nodes, n_head*D] (q_dtype); rows past n_nodes[b] are zeros
+    and are not stored."""
     return _F.append_tree(q, k, v, k_cache, v_cache, None, seq_lens, n_nodes, positions, rope_cs,
                           n_head, n_kv_head, head_dim, rotary_dim, neox, q_norm, k_norm, eps, q_bias,
                           k_bias, v_bias, q_out, q_dtype, kv_stride, seq_stride, n_ctx, stream)

@@ -14,7 +14,7 @@ namespace ullm {
 // (16 rows 22.7, 256 rows 34.2), 4000 43.8 (64 rows 42.3, 256 rows 43.8, 16 rows 63.8); 26
 // nodes at 300 tokens, 12/2 heads, 9.9 (256 rows 16.8), at 4000 13.0 (16 rows, in parts; 256
 // rows 16.5); 2 sequences of 64 nodes, 32/8 x 128, f32, 4000 tokens 57.7 (128 rows; 64 rows 82).
-// Over 66 calls of 16 bits, 300 to 32000 tokens, the choice takes at most 1.14 times the
+// Over 69 calls, 65 of them of 16 bits, 300 to 32000 tokens, the choice takes at most 1.14 times the
 // best shape's time, but for two (1.17 and 1.23).
 struct TreeCut {
     TreeShape shape;

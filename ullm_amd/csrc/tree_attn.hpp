@@ -20,12 +20,13 @@
 //    LDS read, P as two 16-bit values hi + lo whatever the output's type.  (P as one
 //    puts outputs 1.37 times as far from 64 bits over bf16, and 1.27 over f16, as their
 //    own rounding does; two take 260 us for 200 in the largest case below, where the
-//    products bind, 25.3 for 24.7 and 13.1 for 12.8 in the others.)  f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads,
-//    the four elements of a read being four k-steps (K) or four d tiles (V); they
-//    run at a sixteenth of the 16-bit rate, which the stream of K and V about hides
-//    up to 64 rows.  f32, more rows (X3): every value as the sum of three bf16 (8 bits
-//    each, exact), six products of the 16-bit rate (those above 2^-24 of the
-//    whole), K and V tiles split once by the waves that fetched them.
+//    products bind, 25.3 for 24.7 and 13.1 for 12.8 in the others.)
+//    f32, few rows: 16x16x4 products of f32, K and V by 16-byte reads, the four elements
+//    of a read being four k-steps (K) or four d tiles (V); they run at a sixteenth of the
+//    16-bit rate, which the stream of K and V about hides up to 64 rows.  f32, more rows
+//    (X3): every value as the sum of three bf16 (8 bits each, exact), six products of the
+//    16-bit rate (those above 2^-24 of the whole), K and V tiles split once by the waves
+//    that fetched them.
 //  * K and V tiles come by LDS DMA into a ring, one 32-key block a page lookup.
 //  * A workgroup is WR x WK waves of 16*NR rows: the WR waves of a key group
 //    share its tiles (f32 up to 32 rows: 2 WR waves, of 16 of a tile's keys each),
