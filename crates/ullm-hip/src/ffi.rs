@@ -174,6 +174,41 @@ unsafe extern "C" {
         table_out: *mut i32, out_stride: c_int, lens_out: *mut i32, n_out: c_int, info: *mut i32,
         workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn ullm_hip_kv_pages_workspace_bytes(n_out: c_int, n_pages: c_int) -> usize;
+    pub fn ullm_hip_tree_verify(target: *const c_void, target_seq: i64, target_row: i64,
+        draft: *const c_void, draft_seq: i64, draft_row: i64, dtype: c_int, vocab: c_int,
+        tokens: *const i32, parents: *const i32, n_nodes: *const i32, uniform: *const f32,
+        max_nodes: c_int, distinct: c_int, batch: c_int, path: *mut i32, n_accept: *mut i32,
+        next: *mut i32, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_tree_verify_workspace_bytes(vocab: c_int, batch: c_int) -> usize;
+    pub fn ullm_hip_key_weights(q: *const c_void, q_dtype: c_int, k_cache: *const c_void,
+        kv_dtype: c_int, kv_stride: i64, seq_stride: i64, seq_lens: *const i32,
+        n_rows: *const i32, max_rows: c_int, max_len: c_int, window: c_int, batch: c_int,
+        n_head: c_int, n_kv_head: c_int, head_dim: c_int, scale: f32, decay: f32,
+        weights: *mut f32, weights_stride: i64, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_key_weights_paged(q: *const c_void, q_dtype: c_int, k_pages: *const c_void,
+        kv_dtype: c_int, kv_stride: i64, page_size: c_int, n_pages: c_int,
+        block_table: *const i32, table_stride: c_int, seq_lens: *const i32, n_rows: *const i32,
+        max_rows: c_int, max_len: c_int, window: c_int, batch: c_int, n_head: c_int,
+        n_kv_head: c_int, head_dim: c_int, scale: f32, decay: f32, weights: *mut f32,
+        weights_stride: i64, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_key_weights_workspace_bytes(kv_dtype: c_int, batch: c_int, max_rows: c_int,
+        max_len: c_int, window: c_int, n_head: c_int, n_kv_head: c_int,
+        head_dim: c_int) -> usize;
+    pub fn ullm_hip_kv_evict(k_cache: *mut c_void, v_cache: *mut c_void, dtype: c_int,
+        kv_stride: i64, seq_stride: i64, n_ctx: c_int, kv_dim: c_int, n_layer: c_int,
+        layer_stride: i64, scores: *const f32, scores_out: *mut f32, score_stride: i64,
+        groups: c_int, seq_lens: *const i32, budget: *const i32, max_budget: c_int, sink: c_int,
+        recent: c_int, kept: *mut i32, lens_out: *mut i32, batch: c_int,
+        stream: *mut c_void) -> c_int;
+    pub fn ullm_hip_kv_evict_paged(k_pages: *mut c_void, v_pages: *mut c_void, dtype: c_int,
+        kv_stride: i64, page_size: c_int, n_pages: c_int, kv_dim: c_int, n_layer: c_int,
+        layer_stride: i64, block_table: *const i32, table_stride: c_int, scores: *const f32,
+        scores_out: *mut f32, score_stride: i64, groups: c_int, seq_lens: *const i32,
+        budget: *const i32, max_budget: c_int, sink: c_int, recent: c_int, kept: *mut i32,
+        lens_out: *mut i32, batch: c_int, stream: *mut c_void) -> c_int;
 }
 
 /// Status -> ullm_core::Error, as forward.rs:369-380 reports unsupported dtypes.

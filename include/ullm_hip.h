@@ -519,6 +519,128 @@ int ullm_hip_kv_pages_update_rows(void *k_pages, void *v_pages, int dtype, int64
                                   size_t workspace_bytes, void *stream);
 size_t ullm_hip_kv_pages_workspace_bytes(int n_out, int n_pages);
 
+/* ---- which drafted tokens are kept, and which positions of a long sequence ----
+ * No counterpart in the reference, which samples one token at a time
+ * (crates/ullm-model/src/sample.rs) and keeps every position. */
+
+/* Verification of drafted tokens against the target's probabilities, so that what
+ * is kept, and the token that follows, are distributed as the target's alone.
+ * Row 0 of target[b] is the target's distribution behind the sequence, row 1 + i
+ * that behind node i; row r of draft[b] is what the children of node r - 1 (r = 0:
+ * of the sequence) were drawn from.  The nodes are taken in order, each only if its
+ * parent is the last one kept (at first: the sequence).  With p and q the rows behind
+ * that one, c = 0 and S = Z = 1 when it was reached, and R = max(p - c q, 0), a child
+ * of token x is kept if R(x) > 0 and
+ *     uniform[b][i] * q(x) / Z * S < R(x);
+ * if it is not, c grows by S / Z, Z shrinks by q(x) (where `distinct` is not 0: the
+ * children were drawn without return; to 2^-24 at least) and S becomes sum(R).  The next
+ * token is the first whose cumulative sum of R exceeds uniform[b][max_nodes] * sum(R);
+ * of p where R is zero everywhere; -1 where p is too.
+ * draft NULL: the drafts have no probabilities (found by lookup, or the likeliest
+ * ones).  Then R is p without the tokens rejected so far, and a child is kept if
+ *     uniform[b][i] * S < R(x),  S = 1 - the p of those tokens.
+ * Sums and products are held in 64 bits.  What is no probability (below 0, infinite,
+ * NaN) counts as 0, and a number outside [0, 1) as the nearest inside.
+ * target: [batch][max_nodes + 1][vocab] in dtype, *_seq elements from sequence to
+ *         sequence and *_row from row to row; draft: [batch][max_nodes][vocab], the
+ *         same dtype; need only be aligned to their elements
+ * tokens: int32[batch][max_nodes]; a node whose token is outside [0, vocab) is passed
+ *         over, as if it were not there
+ * parents: int32[batch][max_nodes], an earlier node or below 0 (the sequence); a node
+ *         that names itself or a later one is never reached.  NULL: a chain
+ * n_nodes: int32[batch] (clamped to 0..max_nodes), or NULL: max_nodes each
+ * uniform: f32[batch][max_nodes + 1]
+ * path:   int32[batch][max_nodes], the nodes kept, in order, then -1; n_accept:
+ *         int32[batch], how many (both as ullm_hip_kv_accept takes them); next:
+ *         int32[batch].  No output shares memory with an input or another output
+ * max_nodes <= 1024 (0: a token is drawn from row 0), vocab <= 2^30
+ * workspace: DEVICE memory of ullm_hip_tree_verify_workspace_bytes (enough for every
+ *         smaller vocab and batch), 256-byte aligned, needs no initialisation, one
+ *         call at a time. */
+int ullm_hip_tree_verify(const void *target, int64_t target_seq, int64_t target_row,
+                         const void *draft, int64_t draft_seq, int64_t draft_row, int dtype,
+                         int vocab, const int32_t *tokens, const int32_t *parents,
+                         const int32_t *n_nodes, const float *uniform, int max_nodes, int distinct,
+                         int batch, int32_t *path, int32_t *n_accept, int32_t *next,
+                         void *workspace, size_t workspace_bytes, void *stream);
+size_t ullm_hip_tree_verify_workspace_bytes(int vocab, int batch);
+
+/* The attention weight that each position of a cache gets, collected for
+ * ullm_hip_kv_evict:
+ *   weights[b][j][t] = decay * weights[b][j][t] + sum over the rows i < n_rows[b] and
+ *       the query heads h of kv head j of softmax_t(scale * q[b,i,h,:].K[t,j,:])
+ * for the positions t < seq_lens[b]; the others are left as they are.  Row i stands at
+ * position seq_lens[b] - n_rows[b] + i (the rows are the sequence's last ones, whose
+ * keys the cache holds) and sees the positions up to its own, with a window > 0 the
+ * last `window` of them; a row before position 0 sees nothing.  Keys that a row does
+ * not see do not reach it, whatever they hold.  With decay 0 the old weights are not
+ * read.
+ * q:        [batch][max_rows][n_head][head_dim] in the cache's dtype or f32 (q_dtype)
+ * k_cache:  as for ullm_hip_attn_decode; keys 0..max_len-1 must be readable
+ * seq_lens: int32[batch] (clamped to 0..max_len); n_rows: int32[batch] (clamped to
+ *           0..max_rows) or NULL: max_rows each
+ * weights:  f32[batch][n_kv_head][weights_stride], weights_stride >= max_len
+ * workspace: DEVICE memory of ullm_hip_key_weights_workspace_bytes, 256-byte aligned,
+ *           needs no initialisation, one call at a time; one for max_len, batch and
+ *           max_rows serves every call with smaller ones
+ * max_rows * n_head <= 2^23; head_dim 64, 128 or 256; n_head % n_kv_head == 0; q, k_cache
+ * and row strides 16-byte aligned. */
+int ullm_hip_key_weights(const void *q, int q_dtype, const void *k_cache, int kv_dtype,
+                         int64_t kv_stride, int64_t seq_stride, const int32_t *seq_lens,
+                         const int32_t *n_rows, int max_rows, int max_len, int window, int batch,
+                         int n_head, int n_kv_head, int head_dim, float scale, float decay,
+                         float *weights, int64_t weights_stride, void *workspace,
+                         size_t workspace_bytes, void *stream);
+/* Over pages (see ullm_hip_attn_decode_paged): page_size a power of two >= 32, pages
+ * outside [0, n_pages) read as zeros, table_stride * page_size >= max_len. */
+int ullm_hip_key_weights_paged(const void *q, int q_dtype, const void *k_pages, int kv_dtype,
+                               int64_t kv_stride, int page_size, int n_pages,
+                               const int32_t *block_table, int table_stride,
+                               const int32_t *seq_lens, const int32_t *n_rows, int max_rows,
+                               int max_len, int window, int batch, int n_head, int n_kv_head,
+                               int head_dim, float scale, float decay, float *weights,
+                               int64_t weights_stride, void *workspace, size_t workspace_bytes,
+                               void *stream);
+size_t ullm_hip_key_weights_workspace_bytes(int kv_dtype, int batch, int max_rows, int max_len,
+                                            int window, int n_head, int n_kv_head, int head_dim);
+
+/* A cache cut down to a budget.  Of the positions of sequence b,
+ *   n = min(seq_lens[b], budget[b])
+ * stay in each layer and group of columns: the first min(sink, n), the last recent (or
+ * as many as n has room for) and of those between the ones of the largest score, the
+ * lowest position of equals (NaN is below every number).  They keep their order: row j
+ * of the group takes position kept[j], and what lies behind row n - 1 is left as it is.
+ * The columns of a row are cut into `groups` of kv_dim / groups: n_kv_head groups give
+ * each kv head positions of its own (keys are stored rotated, so attention without a
+ * window does not see where a row lies), 1 keeps whole rows.  Later tokens are stored
+ * from row n on and stand at positions of their own: ullm_hip_qkv_append_tree takes the
+ * two apart.
+ * scores:   f32[n_layer][batch][groups][score_stride] (ullm_hip_key_weights)
+ * scores_out: the scores that stay, moved as the rows, and 0 for rows n to
+ *           seq_lens[b] - 1; scores itself, or other memory of its size, or NULL
+ * seq_lens: int32[batch], clamped to the positions that the cache (n_ctx rows, or the
+ *           table) and score_stride have; budget: int32[batch], clamped to 0..max_budget
+ * kept:     int32[n_layer][batch][groups][max_budget], then -1
+ * lens_out: int32[batch], n, or NULL
+ * No output shares memory with an input or another output (scores_out apart).  The
+ * strides and layers are those of ullm_hip_kv_accept; layers and sequences must not
+ * share rows (in pages: no page that is written), nor may K and V overlap unless they are
+ * one.  batch * groups <= 65535; pools, groups of columns and strides 16-byte aligned. */
+int ullm_hip_kv_evict(void *k_cache, void *v_cache, int dtype, int64_t kv_stride,
+                      int64_t seq_stride, int n_ctx, int kv_dim, int n_layer, int64_t layer_stride,
+                      const float *scores, float *scores_out, int64_t score_stride, int groups,
+                      const int32_t *seq_lens, const int32_t *budget, int max_budget, int sink,
+                      int recent, int32_t *kept, int32_t *lens_out, int batch, void *stream);
+/* page_size: a power of two; rows in pages outside [0, n_pages) are neither read nor
+ * written. */
+int ullm_hip_kv_evict_paged(void *k_pages, void *v_pages, int dtype, int64_t kv_stride,
+                            int page_size, int n_pages, int kv_dim, int n_layer,
+                            int64_t layer_stride, const int32_t *block_table, int table_stride,
+                            const float *scores, float *scores_out, int64_t score_stride,
+                            int groups, const int32_t *seq_lens, const int32_t *budget,
+                            int max_budget, int sink, int recent, int32_t *kept, int32_t *lens_out,
+                            int batch, void *stream);
+
 /* Measurement calibration (no counterpart in the reference): reads `bytes`
  * bytes of DEVICE memory at `src` (16-byte aligned) once, with 16-byte loads
  * split over `workgroups` 256-thread workgroups, and writes at most one word

@@ -13,14 +13,19 @@ from .attention import (  # noqa: F401
     attn_tree,
     attn_tree_paged,
     decode_workspace_bytes,
+    key_weights,
+    key_weights_paged,
     kv_accept,
     kv_accept_paged,
+    kv_evict,
+    kv_evict_paged,
     kv_pages_update,
     qkv_append,
     qkv_append_tree,
     qkv_append_tree_paged,
     rope_table,
     tree_masks,
+    tree_verify,
 )
 
 __version__ = "0.1.0"

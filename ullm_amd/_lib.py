@@ -120,6 +120,33 @@ SIGNATURES = {
          _vp, _sz, _vp],
     ),
     "ullm_hip_kv_pages_workspace_bytes": (_sz, [_i, _i]),
+    "ullm_hip_tree_verify": (
+        _i,
+        [_vp, _i64, _i64, _vp, _i64, _i64, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz,
+         _vp],
+    ),
+    "ullm_hip_tree_verify_workspace_bytes": (_sz, [_i, _i]),
+    "ullm_hip_key_weights": (
+        _i,
+        [_vp, _i, _vp, _i, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _i64, _vp, _sz,
+         _vp],
+    ),
+    "ullm_hip_key_weights_paged": (
+        _i,
+        [_vp, _i, _vp, _i, _i64, _i, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _f, _vp, _i64,
+         _vp, _sz, _vp],
+    ),
+    "ullm_hip_key_weights_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "ullm_hip_kv_evict": (
+        _i,
+        [_vp, _vp, _i, _i64, _i64, _i, _i, _i, _i64, _vp, _vp, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _i,
+         _vp],
+    ),
+    "ullm_hip_kv_evict_paged": (
+        _i,
+        [_vp, _vp, _i, _i64, _i, _i, _i, _i, _i64, _vp, _i, _vp, _vp, _i64, _i, _vp, _vp, _i, _i, _i, _vp,
+         _vp, _i, _vp],
+    ),
 }
 
 

@@ -286,6 +286,77 @@ def kv_pages_update(k_pages, v_pages, block_table, seq_lens, parent, capacity, *
                            table_stride, table_out, lens_out, info, workspace, stream)
 
 
+def tree_verify(target, draft, tokens, uniform, *, parents=None, n_nodes=None, distinct=False, path=None,
+                n_accept=None, next_token=None, workspace=None, stream=None):
+    """Which nodes of drafted trees are kept, by the target's probabilities, the
+    draft's and given random numbers, so that what is kept and the token that
+    follows are distributed as the target's alone (ullm_hip_tree_verify has the
+    rules).
+
+    target: [B, nodes + 1, vocab] f32, f16 or bf16, row 0 behind the sequence,
+    row 1 + i behind node i; draft: [B, nodes, vocab] in the same dtype, row r
+    what the children of node r - 1 were drawn from (`distinct`: without
+    return), or None for drafts without probabilities; rows at any stride.
+    tokens: int32 [B, nodes]; uniform: f32 [B, nodes + 1], numbers of [0, 1), one
+    a node and the last for the token that follows; parents: int32 [B, nodes]
+    (below 0: the sequence), or None: a chain; n_nodes: int32 [B] (default: all).
+    Returns (path int32 [B, nodes], n_accept int32 [B], as kv_accept takes them,
+    next token int32 [B])."""
+    return _F.tree_verify(target, draft, tokens, uniform, parents, n_nodes, distinct, path, n_accept,
+                          next_token, workspace, stream)
+
+
+def key_weights(q, k_cache, weights, seq_lens, max_len, n_kv_head, *, n_rows=None, window=0, scale=None,
+                decay=1.0, kv_stride=None, seq_stride=None, workspace=None, stream=None):
+    """Add to `weights` (f32 [B, n_kv_head, >= max_len], in place; times `decay`
+    first) the attention weight that each position of the cache gets from rows of
+    queries, summed over them and over the query heads of a kv head
+    (ullm_hip_key_weights has the rules).
+
+    q: [B, rows, n_head, D] or, for one row, [B, n_head, D], in the cache's dtype
+    or f32: the last n_rows (int32 [B], default: all) positions of each sequence
+    of seq_lens (int32 [B]), whose keys the cache holds.  k_cache and its strides
+    as for attn_tree.  Returns weights."""
+    return _F.key_weights(q, k_cache, None, weights, seq_lens, max_len, n_kv_head, n_rows, window, scale,
+                          decay, kv_stride, seq_stride, workspace, stream)
+
+
+def key_weights_paged(q, k_pages, block_table, weights, seq_lens, max_len, n_kv_head, *, n_rows=None,
+                      window=0, scale=None, decay=1.0, workspace=None, stream=None):
+    """key_weights over a paged cache: k_pages [n_pages, page_size, kv_stride],
+    block_table int32 [B, table_stride] (see attn_decode_paged)."""
+    return _F.key_weights(q, k_pages, block_table, weights, seq_lens, max_len, n_kv_head, n_rows, window,
+                          scale, decay, None, 0, workspace, stream)
+
+
+def kv_evict(k_cache, v_cache, scores, seq_lens, budget, *, max_budget, sink=0, recent=0,
+             scores_out=None, kept=None, lens_out=None, stream=None):
+    """Cut a cache down to `budget` positions of each sequence, in place: the first
+    `sink`, the last `recent`, and of those between the ones of the largest score,
+    in order (ullm_hip_kv_evict has the rules).
+
+    Caches as for kv_accept.  scores: contiguous f32 [n_layer, B, groups, n]
+    (without the first where the caches have no layers; for one sequence also
+    without B), what key_weights collected: groups = n_kv_head gives each kv head
+    positions of its own, 1 keeps whole rows.  They move as the rows do, into
+    scores_out (default: in place), with 0 where positions were dropped.
+    seq_lens, budget: int32 [B], max_budget: host-side upper bound of budget.
+    Returns (kept int32 [n_layer, B, groups, max_budget], the position that each
+    row now holds, then -1; new lengths int32 [B])."""
+    return _F.evict(k_cache, v_cache, None, scores, seq_lens, budget, max_budget, sink, recent, scores_out,
+                    kept, lens_out, stream)
+
+
+def kv_evict_paged(k_pages, v_pages, block_table, scores, seq_lens, budget, *, max_budget, sink=0,
+                   recent=0, scores_out=None, kept=None, lens_out=None, stream=None):
+    """kv_evict over a paged cache: pools as for kv_accept_paged, block_table int32
+    [B, table_stride].  Sequences must not share pages that are written; those
+    behind the new lengths stay in the table until kv_pages_update gives them
+    back."""
+    return _F.evict(k_pages, v_pages, block_table, scores, seq_lens, budget, max_budget, sink, recent,
+                    scores_out, kept, lens_out, stream)
+
+
 _proj_ws = {}
 
 

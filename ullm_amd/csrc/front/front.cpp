@@ -678,6 +678,26 @@ struct Pools {
     }
 };
 
+// Contiguous caches of one or all layers: [n_ctx, kv_dim], [B, n_ctx, kv_dim] (one
+// sequence: [n_layer, n_ctx, kv_dim]), [n_layer, B, n_ctx, kv_dim].
+struct Caches {
+    int layers, n_ctx, kvd;
+    int64_t ls, ss;
+    Caches(const at::Tensor &k, const at::Tensor &v, int B) {
+        const int64_t d = k.dim();
+        const bool fits = d == 2 ? B == 1 : d == 3 ? B == 1 || k.size(0) == B : d == 4 && k.size(1) == B;
+        if (!fits || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type() ||
+            k.stride(-1) != 1)
+            invalid("caches must be [n_ctx, kv_dim], [B, n_ctx, kv_dim], [n_layer, n_ctx, kv_dim] of one sequence or "
+                    "[n_layer, B, n_ctx, kv_dim], alike");
+        const bool layered = d == 4 || (d == 3 && B == 1);
+        layers = layered ? small(k.size(0), "n_layer") : 1;
+        ls = layered ? k.stride(0) : 0, ss = d == 4 ? k.stride(1) : d == 3 && !layered ? k.stride(0) : 0;
+        if ((layers > 1 && !ls) || (B > 1 && !ss)) invalid("layers and sequences must not share memory");
+        n_ctx = small(k.size(-2), "n_ctx"), kvd = small(k.size(-1), "kv_dim");
+    }
+};
+
 at::Tensor accept(const Args &a) {
     // k v table path n_accept lens lens_out stream
     const at::Tensor &k = a.t(0), &v = a.t(1), &path = a.t(3), &count = a.t(4), &lens = a.t(5);
@@ -704,24 +724,21 @@ at::Tensor accept(const Args &a) {
         });
         return out;
     }
-    // [n_ctx, kv_dim], [B, n_ctx, kv_dim] (one sequence: [n_layer, n_ctx, kv_dim]),
-    // [n_layer, B, n_ctx, kv_dim]
-    const int64_t d = k.dim();
-    const bool fits = d == 2 ? B == 1 : d == 3 ? B == 1 || k.size(0) == B : d == 4 && k.size(1) == B;
-    if (!fits || k.sizes() != v.sizes() || k.strides() != v.strides() || k.scalar_type() != v.scalar_type() ||
-        k.stride(-1) != 1)
-        invalid("caches must be [n_ctx, kv_dim], [B, n_ctx, kv_dim], [n_layer, n_ctx, kv_dim] of one sequence or "
-                "[n_layer, B, n_ctx, kv_dim], alike");
-    const bool layered = d == 4 || (d == 3 && B == 1);
-    const int layers = layered ? small(k.size(0), "n_layer") : 1;
-    const int64_t ls = layered ? k.stride(0) : 0, ss = d == 4 ? k.stride(1) : d == 3 && !layered ? k.stride(0) : 0;
-    if ((layers > 1 && !ls) || (B > 1 && !ss)) invalid("layers and sequences must not share memory");
-    const int n_ctx = small(k.size(-2), "n_ctx"), kvd = small(k.size(-1), "kv_dim");
+    const Caches c(k, v, B);
     call([&] {
-        return ullm_hip_kv_accept(k.data_ptr(), v.data_ptr(), kd, k.stride(-2), ss, n_ctx, kvd, layers, ls, path_p, A,
-                                  count_p, len_p, (int32_t *)out.data_ptr(), B, st.s);
+        return ullm_hip_kv_accept(k.data_ptr(), v.data_ptr(), kd, k.stride(-2), c.ss, c.n_ctx, c.kvd, c.layers, c.ls,
+                                  path_p, A, count_p, len_p, (int32_t *)out.data_ptr(), B, st.s);
     });
     return out;
+}
+
+// A tuple of tensors.
+PyObject *tuple(std::initializer_list<at::Tensor> ts) {
+    PyObject *r = PyTuple_New(ts.size());
+    if (!r) throw PyRaised{};
+    Py_ssize_t i = 0;
+    for (const at::Tensor &t : ts) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t));
+    return r;
 }
 
 PyObject *pages_update(const Args &a) {
@@ -760,12 +777,140 @@ PyObject *pages_update(const Args &a) {
             held ? (const uint8_t *)held->data_ptr() : nullptr, (int32_t *)to.data_ptr(), cols,
             (int32_t *)lo.data_ptr(), N, (int32_t *)info.data_ptr(), ws_p, ws_n, st.s);
     });
-    PyObject *r = PyTuple_New(3);
-    if (!r) throw PyRaised{};
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(to));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lo));
-    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(info));
-    return r;
+    return tuple({to, lo, info});
+}
+
+at::Tensor key_weights(const Args &a) {
+    // q k table weights lens max_len n_kv n_rows window scale decay kv_stride seq_stride ws stream
+    const at::Tensor &q = a.t(0), &k = a.t(1), &w = a.t(3), &lens = a.t(4);
+    const at::Tensor *tab = a.ot(2), *nr = a.ot(7), *gws = a.ot(13);
+    if (q.dim() != 3 && q.dim() != 4) raise(PyExc_ValueError, "q must be [B, rows, n_head, head_dim] or [B, n_head, head_dim]");
+    const c10::DeviceGuard on(one_gpu({&q, &k, &w, &lens, tab, nr, gws}));
+    const int B = small(q.size(0), "q: batch"), R = q.dim() == 4 ? small(q.size(1), "q: rows") : 1,
+              H = small(q.size(-2), "q: n_head"), D = small(q.size(-1), "q: head_dim"), max_len = a.i32(5), hk = a.i32(6),
+              win = a.window(8);
+    if (!q.is_contiguous()) invalid("q must be contiguous");
+    const int32_t *len_p = i32s(&lens, {B}, "seq_lens must be contiguous int32 [B]"),
+                  *nr_p = i32s(nr, {B}, "n_rows must be contiguous int32 [B]");
+    // [B, n_kv_head, n], rows at any stride that is the same from head to head and on to the next sequence
+    if (w.scalar_type() != at::kFloat || w.dim() != 3 || w.size(0) != B || w.size(1) != hk || w.size(2) < max_len ||
+        (w.size(2) > 1 && w.stride(2) != 1))
+        invalid("weights must be f32 [B, n_kv_head, n], n >= max_len");
+    const int64_t ws_row = hk > 1 ? w.stride(1) : B > 1 ? w.stride(0) : std::max<int64_t>(w.size(2), 1);
+    if ((B > 1 && w.stride(0) != hk * ws_row) || ws_row < w.size(2))
+        invalid("weights must have their rows at one stride");
+    const float scale = a.none(9) ? (float)(1.0 / std::sqrt((double)D)) : (float)a.f(9), decay = (float)a.f(10);
+    int64_t kvs, ss = 0;
+    if (tab) {
+        if (k.dim() != 3 || !k.is_contiguous()) invalid("k_pages must be contiguous [n_pages, page_size, kv_stride]");
+        if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(0) != B || !tab->is_contiguous())
+            invalid("block_table must be contiguous int32 [B, table_stride]");
+        kvs = k.size(2);
+    } else {
+        const Strides s(a, 11, 12, k, k, B, (int64_t)hk * D);
+        kvs = s.kvs, ss = s.ss;
+        const bool rows = a.none(11) && k.dim() >= 2 && k.size(-1) == (int64_t)hk * D;
+        if ((rows && k.size(-2) < max_len) || !s.within(k, k, B, max_len, (int64_t)hk * D))
+            invalid("the cache ends before max_len positions of every sequence");
+    }
+    const Stream st(a, 14);
+    const int qd = dt(q), kd = dt(k);
+    at::Tensor ws;
+    if (gws) ws = *gws;
+    else if (const size_t need = ullm_hip_key_weights_workspace_bytes(kd, B, R, max_len, win, H, hk, D))
+        ws = st.scratch(q, need);
+    void *const ws_p = ws.defined() ? ws.data_ptr() : nullptr;
+    const size_t ws_n = ws.defined() ? ws.nbytes() : 0;
+    call([&] {
+        return tab ? ullm_hip_key_weights_paged(q.data_ptr(), qd, k.data_ptr(), kd, kvs, (int)k.size(1), (int)k.size(0),
+                                                (const int32_t *)tab->data_ptr(), (int)tab->size(1), len_p, nr_p, R,
+                                                max_len, win, B, H, hk, D, scale, decay, (float *)w.data_ptr(), ws_row,
+                                                ws_p, ws_n, st.s)
+                   : ullm_hip_key_weights(q.data_ptr(), qd, k.data_ptr(), kd, kvs, ss, len_p, nr_p, R, max_len, win, B,
+                                          H, hk, D, scale, decay, (float *)w.data_ptr(), ws_row, ws_p, ws_n, st.s);
+    });
+    return w;
+}
+
+PyObject *evict(const Args &a) {
+    // k v table scores lens budget max_budget sink recent scores_out kept lens_out stream
+    const at::Tensor &k = a.t(0), &v = a.t(1), &sc = a.t(3), &lens = a.t(4), &bud = a.t(5);
+    const at::Tensor *tab = a.ot(2), *so = a.ot(9), *gk = a.ot(10), *gl = a.ot(11);
+    const c10::DeviceGuard on(one_gpu({&k, &v, tab, &sc, &lens, &bud, so, gk, gl}));
+    const int B = small(lens.numel(), "seq_lens"), top = a.i32(6), sink = a.i32(7), recent = a.i32(8);
+    const int32_t *len_p = i32s(&lens, {B}, "seq_lens must be contiguous int32 [B]"),
+                  *bud_p = i32s(&bud, {B}, "budget must be contiguous int32 [B]");
+    const int kd = dt(k);
+    int layers, kvd, n_ctx = 0;
+    int64_t ls, kvs, ss = 0;
+    if (tab) {
+        const Pools p(k, v);
+        if (tab->scalar_type() != at::kInt || tab->dim() != 2 || tab->size(0) != B || !tab->is_contiguous())
+            invalid("block_table must be contiguous int32 [B, table_stride]");
+        layers = p.layers, ls = p.layer_stride, kvs = p.kvs, kvd = small(p.kvd, "kv_dim");
+    } else {
+        const Caches c(k, v, B);
+        layers = c.layers, ls = c.ls, ss = c.ss, n_ctx = c.n_ctx, kvd = c.kvd, kvs = k.stride(-2);
+    }
+    if (sc.scalar_type() != at::kFloat || sc.dim() < 2 || !sc.is_contiguous())
+        invalid("scores must be contiguous f32 [n_layer, B, groups, n]");
+    const int64_t n = sc.size(-1), G = sc.size(-2);
+    if (G < 1 || (n && sc.numel() / n != layers * (int64_t)B * G) || (!n && sc.numel()))
+        invalid("scores must be [n_layer, B, groups, n] of the caches' layers and sequences");
+    if (so && (so->scalar_type() != at::kFloat || so->sizes() != sc.sizes() || !so->is_contiguous()))
+        invalid("scores_out must be as scores");
+    if (top < 0) invalid("max_budget < 0");
+    if (gk) i32s(gk, {layers, B, G, top}, "kept must be contiguous int32 [n_layer, B, groups, max_budget]");
+    if (gl) i32s(gl, {B}, "lens_out must be contiguous int32 [B]");
+    const Stream st(a, 12);
+    const at::Tensor kept = out_or(gk, {layers, B, G, top}, lens, at::kInt), out = out_or(gl, {B}, lens, at::kInt);
+    const int groups = small(G, "groups");
+    float *const so_p = (float *)(so ? so->data_ptr() : sc.data_ptr());
+    call([&] {
+        return tab ? ullm_hip_kv_evict_paged(k.data_ptr(), v.data_ptr(), kd, kvs, (int)k.size(-2), (int)k.size(-3), kvd,
+                                             layers, ls, (const int32_t *)tab->data_ptr(), (int)tab->size(1), fptr(&sc),
+                                             so_p, n, groups, len_p, bud_p, top, sink, recent,
+                                             (int32_t *)kept.data_ptr(), (int32_t *)out.data_ptr(), B, st.s)
+                   : ullm_hip_kv_evict(k.data_ptr(), v.data_ptr(), kd, kvs, ss, n_ctx, kvd, layers, ls, fptr(&sc), so_p,
+                                       n, groups, len_p, bud_p, top, sink, recent, (int32_t *)kept.data_ptr(),
+                                       (int32_t *)out.data_ptr(), B, st.s);
+    });
+    return tuple({kept, out});
+}
+
+PyObject *tree_verify(const Args &a) {
+    // target draft tokens uniform parents n_nodes distinct path n_accept next ws stream
+    const at::Tensor &p = a.t(0), &tok = a.t(2), &u = a.t(3);
+    const at::Tensor *q = a.ot(1), *par = a.ot(4), *nn = a.ot(5), *gp = a.ot(7), *gc = a.ot(8), *gt = a.ot(9), *gws = a.ot(10);
+    const c10::DeviceGuard on(one_gpu({&p, q, &tok, &u, par, nn, gp, gc, gt, gws}));
+    if (p.dim() != 3) raise(PyExc_ValueError, "target must be [B, nodes + 1, vocab]");
+    const int B = small(p.size(0), "target: batch"), T = small(p.size(1) - 1, "target: nodes"), V = small(p.size(2), "target: vocab");
+    if (T < 0 || p.stride(2) != 1) invalid("target must be [B, nodes + 1, vocab], its rows without gaps");
+    if (q && (q->sizes() != at::IntArrayRef({B, T, V}) || (T && q->stride(2) != 1) || q->scalar_type() != p.scalar_type()))
+        invalid("draft must be [B, nodes, vocab] in target's dtype, its rows without gaps");
+    const int32_t *tok_p = i32s(&tok, {B, T}, "tokens must be contiguous int32 [B, nodes]"),
+                  *par_p = i32s(par, {B, T}, "parents must be contiguous int32 [B, nodes]"),
+                  *nn_p = i32s(nn, {B}, "n_nodes must be contiguous int32 [B]");
+    if (!f32_rows(u) || u.sizes() != at::IntArrayRef({B, T + 1})) invalid("uniform must be contiguous f32 [B, nodes + 1]");
+    if (gp) i32s(gp, {B, T}, "path must be contiguous int32 [B, nodes]");
+    if (gc) i32s(gc, {B}, "n_accept must be contiguous int32 [B]");
+    if (gt) i32s(gt, {B}, "next_token must be contiguous int32 [B]");
+    const int distinct = a.truth(6), pd = dt(p);
+    const Stream st(a, 11);
+    const at::Tensor path = out_or(gp, {B, T}, tok, at::kInt), count = out_or(gc, {B}, tok, at::kInt),
+                     next = out_or(gt, {B}, tok, at::kInt);
+    at::Tensor ws;
+    if (gws) ws = *gws;
+    else if (const size_t need = ullm_hip_tree_verify_workspace_bytes(V, B)) ws = st.scratch(p, need);
+    void *const ws_p = ws.defined() ? ws.data_ptr() : nullptr;
+    const size_t ws_n = ws.defined() ? ws.nbytes() : 0;
+    call([&] {
+        return ullm_hip_tree_verify(p.data_ptr(), p.stride(0), p.stride(1), ptr(q), q ? q->stride(0) : 0,
+                                    q ? q->stride(1) : 0, pd, V, tok_p, par_p, nn_p, fptr(&u), T, distinct, B,
+                                    (int32_t *)path.data_ptr(), (int32_t *)count.data_ptr(), (int32_t *)next.data_ptr(),
+                                    ws_p, ws_n, st.s);
+    });
+    return tuple({path, count, next});
 }
 
 // ---- Python entry ----
@@ -795,9 +940,10 @@ PyObject *proj_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 8 + Prep::N + 5) return PyErr_Format(PyExc_TypeError, "%zd arguments given", n), nullptr;
     return guard([&] { return proj(Args{args}); });
 }
-PyObject *pages_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments expected, %zd given", n), nullptr;
-    return guard([&] { return pages_update(Args{args}); });
+template <PyObject *(*F)(const Args &), int N>
+PyObject *several(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != N) return PyErr_Format(PyExc_TypeError, "%d arguments expected, %zd given", N, n), nullptr;
+    return guard([&] { return F(Args{args}); });
 }
 PyObject *set_error(PyObject *, PyObject *cls) {
     Py_INCREF(cls);
@@ -819,7 +965,10 @@ PyMethodDef methods[] = {
     {"attn_tree", FAST((entry<attn_tree, 18>)), METH_FASTCALL, nullptr},
     {"append_tree", FAST((entry<append_tree, 9 + Prep::N + 6>)), METH_FASTCALL, nullptr},
     {"accept", FAST((entry<accept, 8>)), METH_FASTCALL, nullptr},
-    {"pages_update", FAST(pages_entry), METH_FASTCALL, nullptr},
+    {"pages_update", FAST((several<pages_update, 13>)), METH_FASTCALL, nullptr},
+    {"key_weights", FAST((entry<key_weights, 15>)), METH_FASTCALL, nullptr},
+    {"evict", FAST((several<evict, 13>)), METH_FASTCALL, nullptr},
+    {"tree_verify", FAST((several<tree_verify, 12>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
