@@ -11,13 +11,18 @@
 //    in registers, the keys streamed;
 //  - more: weight_keys_kernel, the keys in registers, the queries streamed, and
 //    weight_join_kernel adds up its parts.
-// Scores come from 16x16 matrix instructions; both operands are read straight from
-// memory in their layout (lane l: row l % 16, 16 bytes at 64 c + 16 (l / 16)), no LDS.
+// Scores come from 16x16 matrix instructions.  What is streamed comes by LDS DMA, whole
+// rows to consecutive lanes, into a ring of the wave's own (no barriers), and is read
+// from there in the operands' layout (lane l: row l % 16, 16 bytes at 64 c + 16 (l / 16)),
+// the 16-byte columns of a row exchanged by its number so that no two lanes meet in a
+// bank.  Read straight from memory in that layout, a lane's neighbours all lie in other
+// rows, and a decode step over 8 sequences of 4K-32K took 50 us in place of KW_US.
 // f32 queries over a 16-bit cache enter as exact pieces of its type: three of bf16, or
 // two of f16 (22 bits, the row scaled by a power of two into f16's range).  An f32 cache
 // takes f32 products.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include "common.hpp"
 #include "mfma_util.hpp"
 #include "wave.hpp"
@@ -32,6 +37,8 @@ struct WeightArgs {
     int tab_stride, shift, n_pages;
     const int32_t *len, *n_rows;
     int max_rows, max_len, window, batch, n_head, n_kv, gq;
+    uint32_t gq_mul;  // r / gq of a whole number r >= 0: r * gq_mul >> (32 + gq_shift), or r >> gq_shift where it is 0
+    int gq_shift;
     float qs, decay;  // scale * log2(e)
     float *w;
     int64_t w_stride;
@@ -40,6 +47,7 @@ struct WeightArgs {
     int rows_pad;    // rows of a unit in the arrays below, a multiple of the blocks'
     int blocks;      // row blocks of a unit
     int chunk, splits;  // keys of a part of a row block, the most parts
+    int64_t tiles;  // of the scores of a unit
     int row_chunk, parts;  // rows of a part of a key block, the most parts (weight_keys_kernel)
     float2 *ml;      // [units][rows_pad][splits]: largest score and sum of exp2 of a part
     float *row_qs;   // [units][rows_pad]: qs over the row's power of two
@@ -48,21 +56,46 @@ struct WeightArgs {
     float *part;     // [parts][units][max_len]: sums over some rows
 };
 
+__device__ __forceinline__ int query_row(const WeightArgs &a, int r) {
+    return (a.gq_mul ? __umulhi(r, a.gq_mul) : r) >> a.gq_shift;
+}
+
 // What a workgroup knows of its sequence.
 struct WeightSeq {
     int len, n, rows, first;  // positions, query rows, rows of a unit, position of query row 0
-    __device__ WeightSeq(const WeightArgs &a, int b) {
+    __device__ __forceinline__ WeightSeq(const WeightArgs &a, int b) {
         len = min(max(a.len[b], 0), a.max_len);
         n = a.n_rows ? min(max(a.n_rows[b], 0), a.max_rows) : a.max_rows;
         rows = n * a.gq, first = len - n;
     }
     // Positions of rows r0 .. r1 - 1, and the keys from lo to hi that any of them sees.
-    __device__ void keys(const WeightArgs &a, int r0, int r1, int &lo, int &hi) const {
-        const int p0 = first + r0 / a.gq, p1 = first + (r1 - 1) / a.gq;
+    __device__ __forceinline__ void keys(const WeightArgs &a, int r0, int r1, int &lo, int &hi) const {
+        const int p0 = first + query_row(a, r0), p1 = first + query_row(a, r1 - 1);
         hi = p1 + 1;
         lo = a.window ? max(0, p0 + 1 - a.window) : 0;
     }
 };
+
+// 16 rows of RB bytes in LDS: chunk (16 bytes) c of row r lies at r RB + 16 (c ^ swz(r)).
+template <int RB>
+struct Tile {
+    static constexpr int C = RB / 16, N = RB / 64, bytes = 16 * RB;  // chunks of a row, DMA instructions of a tile
+    __device__ __forceinline__ static int swz(int row) { return C == 8 ? (row >> 1) & 7 : row & 15; }
+    // What lane l fetches in instruction d: its row, and its bytes in it.
+    __device__ __forceinline__ static int row(int d) { return (d * 64 + (int)(threadIdx.x & 63)) / C; }
+    __device__ __forceinline__ static int col(int d) { return (((int)(threadIdx.x & 63) % C) ^ swz(row(d))) * 16; }
+    // Where lane l reads chunk c of row l % 16.
+    __device__ __forceinline__ static uint32_t at(int c) {
+        const int r = threadIdx.x & 15;
+        return r * RB + ((c ^ swz(r)) * 16);
+    }
+};
+// Waits until at most N vector-memory operations of this wave are outstanding.
+template <int N>
+__device__ __forceinline__ void vm_wait_n() {
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
 
 // An operand of a row of D values of K: KC pieces of 16 bytes a lane; of a row of q NP
 // times as many.
@@ -72,45 +105,56 @@ struct Dot {
     static constexpr int KC = D * TK::bytes / 64;
     static constexpr int NP = f32 || __is_same(TQ, TK) ? 1 : __is_same(TK, F16) ? 2 : 3;
     static constexpr int q_regs = 4 * KC * NP;
-    static constexpr int max_rt = q_regs <= 16 ? 8 : q_regs <= 32 ? 4 : q_regs <= 64 ? 2 : 1;  // row tiles of a wave
-    static constexpr int kt = KC <= 4 ? 8 : KC <= 8 ? 4 : 2;  // key tiles of a wave (weight_keys_kernel)
+    // most row tiles of a wave where the rows stay in registers
+    static constexpr int rt = q_regs <= 16 ? 4 : q_regs <= 48 ? 2 : 1;
+    // weight_keys_kernel: key tiles of a wave
+    static constexpr int kt = (KC <= 4 ? 8 : KC <= 8 ? 4 : 2) / (NP > 1 && KC > 2 ? 2 : 1);
+    using KTile = Tile<D * TK::bytes>;
+    using QTile = Tile<D * TQ::bytes>;
+    static constexpr int H = KC <= 4 ? 2 : 1;  // key tiles of a step where the keys are streamed
+    static constexpr int step_bytes = H * KTile::bytes;
+    static constexpr int waves = step_bytes > 8192 ? 1 : 2, keys_waves = QTile::bytes > 8192 ? 1 : 2;  // of a SIMD, by the rings
     struct K { u32x4 x[KC]; };
     struct Q { u32x4 x[NP][KC]; };
-
-    __device__ static void load_k(K &k, const char *row) {  // row: this lane's, its 16 bytes of each 64
-#pragma unroll
-        for (int c = 0; c < KC; c++) k.x[c] = *(const u32x4 *)(row + 64 * c);
-    }
-    // Row `row` of q (null: zeros); returns the power of two that it was divided by.
-    __device__ static float load_q(Q &q, const char *row) {
+    struct Raw { u32x4 x[QTile::N]; };  // chunks of a row of q: of K's type 4 c + l / 16, f32 8 (c / 2) + 2 (l / 16) + c % 2
+    __device__ __forceinline__ static int raw_chunk(int c) {
         const int part = (threadIdx.x & 63) >> 4;
+        return NP == 1 ? 4 * c + part : 8 * (c >> 1) + 2 * part + (c & 1);
+    }
+    __device__ __forceinline__ static void load_raw(Raw &r, const char *row) {
+#pragma unroll
+        for (int c = 0; c < QTile::N; c++) r.x[c] = *(const u32x4 *)(row + raw_chunk(c) * 16);
+    }
+    // The operand of a row of q, of other sign if `neg`; returns the power of two that it was
+    // divided by.
+    __device__ __forceinline__ static float make_q(Q &q, const Raw &raw, bool neg) {
         if constexpr (NP == 1) {
 #pragma unroll
-            for (int c = 0; c < KC; c++) q.x[0][c] = row ? *(const u32x4 *)(row + 64 * c + 16 * part) : u32x4{};
+            for (int c = 0; c < KC; c++) q.x[0][c] = raw.x[c];
+            if (neg)
+#pragma unroll
+                for (int c = 0; c < KC; c++) q.x[0][c] ^= f32 ? 0x80000000u : 0x80008000u;
             return 1.f;
         } else {
             float f = 1.f, back = 1.f;
-            u32x4 raw[KC][2];
-#pragma unroll
-            for (int c = 0; c < KC; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) raw[c][h] = row ? *(const u32x4 *)(row + 128 * c + 32 * part + 16 * h) : u32x4{};
             if constexpr (NP == 2) {
                 float m = 0.f;
 #pragma unroll
-                for (int c = 0; c < KC; c++)
+                for (int c = 0; c < 2 * KC; c++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(__uint_as_float(raw[c][i >> 2][i & 3])));
+                    for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(__uint_as_float(raw.x[c][i])));
                 m = rows_max(m);  // the lanes of one row
                 // 2^14 <= m f < 2^15 (exponents kept where f and 1 / f are normal numbers)
                 const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 14, -126), 113);
                 f = __uint_as_float((uint32_t)(127 - e) << 23), back = __uint_as_float((uint32_t)(127 + e) << 23);
             }
+            if (neg) f = -f;
 #pragma unroll
             for (int c = 0; c < KC; c++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float x0 = __uint_as_float(raw[c][i >> 1][2 * i & 3]) * f, x1 = __uint_as_float(raw[c][i >> 1][(2 * i & 3) + 1]) * f;
+                    const u32x4 &r = raw.x[2 * c + (i >> 1)];
+                    float x0 = __uint_as_float(r[2 * i & 3]) * f, x1 = __uint_as_float(r[(2 * i & 3) + 1]) * f;
 #pragma unroll
                     for (int p = 0; p < NP; p++) {
                         q.x[p][c][i] = pack2<TK>(x0, x1);
@@ -123,10 +167,15 @@ struct Dot {
             return back;
         }
     }
+    __device__ __forceinline__ static float load_q(Q &q, const char *row, bool neg) {
+        Raw raw;
+        load_raw(raw, row);
+        return make_q(q, raw, neg);
+    }
     // The 16x16 products of 16 keys and 16 rows: element i of lane l is key 4 (l / 16) + i of
     // row l % 16, or with ROWS row 4 (l / 16) + i of key l % 16.
     template <bool ROWS>
-    __device__ static f32x4 dot(const K &k, const Q &q) {
+    __device__ __forceinline__ static f32x4 dot(const K &k, const Q &q) {
         f32x4 s{};
 #pragma unroll
         for (int p = NP - 1; p >= 0; p--)
@@ -145,175 +194,237 @@ struct Dot {
             }
         return s;
     }
-    // Row r of unit (b, g), null past the last.
-    __device__ static const char *q_row(const WeightArgs &a, const WeightSeq &s, int b, int g, int r) {
-        if (r >= s.rows) return nullptr;
-        const int i = r / a.gq, h = r - i * a.gq;
+    // Row r of unit (b, g); past the last: the last again.
+    __device__ __forceinline__ static const char *q_row(const WeightArgs &a, const WeightSeq &s, int b, int g, int r) {
+        r = min(r, s.rows - 1);
+        const int i = query_row(a, r), h = r - i * a.gq;
         return (const char *)a.q + (((int64_t)b * a.max_rows + i) * a.n_head + g * a.gq + h) * D * TQ::bytes;
     }
 };
 
-// Keys of a unit, tile by tile: a wave has the pages of 2048 keys in its lanes (a page
-// has 32 or more).
+// Keys of a unit: a wave has the pages of 2048 keys in its lanes (a page has 32 or more).
 constexpr int kWeightKeys = 2048;
 template <class P>
 struct KeySource {
-    const char *base;  // of the lane: its row of tile 0 of the sequence, or of the pool
+    const char *base;  // of the kv head's part of row 0 of the sequence, or of the pool
     int64_t rb;
     int len, shift, n_pages, page0, pages;
     bool paged;
-    __device__ KeySource(const WeightArgs &a, const WeightSeq &s, int b, int g, int k0) {
+    __device__ __forceinline__ KeySource(const WeightArgs &a, const WeightSeq &s, int b, int g, int k0) {
         const int lane = threadIdx.x & 63;
         paged = a.tab, rb = a.rb, len = s.len, shift = a.shift, n_pages = a.n_pages;
-        base = a.k + (int64_t)g * P::KC * 64 + (lane >> 4) * 16 + (paged ? 0 : b * a.seq_b);
+        base = a.k + (int64_t)g * P::KC * 64 + (paged ? 0 : b * a.seq_b);
         page0 = k0 >> shift, pages = -1;
         if (paged && page0 + lane < a.tab_stride) pages = a.tab[(int64_t)b * a.tab_stride + page0 + lane];
     }
-    // Keys t0 .. t0 + 15 (past the last: the last again).
-    __device__ void load(typename P::K &k, int t0) const {
-        const int t = min(t0 + (int)(threadIdx.x & 15), len - 1);
-        if (!paged) {
-            P::load_k(k, base + t * rb);
-            return;
+    // Keys t0 .. t0 + n - 1 (in one page); those past the last, and those of pages outside the
+    // pool, read as zeros.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(int t0, int n) const {
+        int64_t row = t0;
+        int bytes = t0 < len ? (min(n, len - t0) - 1) * (int)rb + P::KC * 64 : 0;
+        if (paged) {
+            const int page = __builtin_amdgcn_readlane(pages, (t0 >> shift) - page0);
+            const bool there = (unsigned)page < (unsigned)n_pages;
+            row = ((int64_t)(there ? page : 0) << shift) + (t0 & ((1 << shift) - 1));
+            bytes = there ? bytes : 0;
         }
-        const int page = __builtin_amdgcn_readlane(pages, (t0 >> shift) - page0);
-        if (page < 0 || page >= n_pages) {
-            k = typename P::K{};
-            return;
-        }
-        P::load_k(k, base + (((int64_t)page << shift) + (t & ((1 << shift) - 1))) * rb);
+        return __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(base + row * rb), 0, bytes, kRsrcWord3);
     }
 };
 
 constexpr int kWeightT = 256, kWeightW = 4;
 
-// f(tile, its first key) over the tiles of keys k0 .. k1 - 1 that are this wave's, NB of
-// them in flight.
-template <class P, int NB, class F>
-__device__ __forceinline__ void each_tile(const WeightArgs &a, const WeightSeq &s, int b, int g, int k0, int k1, int wave, F &&f) {
-    typename P::K k[NB];
+// f(P::H tiles, their first key) over the steps of H tiles of keys k0 .. k1 - 1 (k0 a multiple
+// of 32) that are this wave's, one of W, NB steps in flight in its ring.  start() is called
+// once the first are.
+template <class P, int NB, int W, bool ONCE, class S, class F>
+__device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &s, int b, int g, int k0, int k1, int wave,
+                                          char *ring, S &&start, F &&f) {
+    using T = typename P::KTile;
+    constexpr int H = P::H, N = 16 * H, step = N * W;
+    int off[T::N];
+    uint32_t at[P::KC];
+#pragma unroll
+    for (int d = 0; d < T::N; d++) off[d] = T::row(d) * (int)a.rb + T::col(d);
+#pragma unroll
+    for (int c = 0; c < P::KC; c++) at[c] = lds_addr(ring) + T::at(4 * c + ((threadIdx.x & 63) >> 4));
     for (int e0 = k0; e0 < k1; e0 = (e0 & -kWeightKeys) + kWeightKeys) {
-        const int e1 = min(k1, (e0 & -kWeightKeys) + kWeightKeys), first = e0 + 16 * wave, last = (e1 - 1) & ~15;
+        const int e1 = min(k1, (e0 & -kWeightKeys) + kWeightKeys), first = e0 + N * wave, last = (e1 - 1) & -N;
         const KeySource<P> src(a, s, b, g, e0);
+        auto fetch = [&](int j, int t) __attribute__((always_inline)) {
+            const __amdgpu_buffer_rsrc_t r = src.rows(t, N);
 #pragma unroll
-        for (int j = 0; j < NB; j++) src.load(k[j], min(first + 16 * kWeightW * j, last));
-        for (int t0 = first; t0 < e1; t0 += 16 * kWeightW * NB)
+            for (int h = 0; h < H; h++)
 #pragma unroll
-            for (int j = 0; j < NB; j++) {
-                const int t = t0 + 16 * kWeightW * j;
-                if (t >= e1) break;
-                f(k[j], t);
-                src.load(k[j], min(t + 16 * kWeightW * NB, last));
-            }
+                for (int d = 0; d < T::N; d++) {
+                    char *dst = ring + j * P::step_bytes + h * T::bytes + d * 1024;
+                    if (ONCE) dma16(r, dst, off[d] + h * 16 * (int)a.rb, 0);
+                    else dma16_cached(r, dst, off[d] + h * 16 * (int)a.rb, 0);
+                }
+        };
+#pragma unroll
+        for (int j = 0; j < NB; j++) fetch(j, min(first + step * j, last));
+        if (e0 == k0) start();
+        for (int t0 = first; t0 < e1; t0 += step * NB)
+            static_for<0, NB>([&](auto J) __attribute__((always_inline)) {
+                constexpr int j = decltype(J)::value;
+                const int t = t0 + step * j;
+                if (t >= e1) return;
+                typename P::K k[H];
+                vm_wait_n<(NB - 1) * H * T::N>();
+                static_for<0, H>([&](auto HH) __attribute__((always_inline)) {
+                    constexpr int h = decltype(HH)::value;
+#pragma unroll
+                    for (int c = 0; c < P::KC; c++) k[h].x[c] = lds_read_b128_at<j * P::step_bytes + h * T::bytes>(at[c]);
+                });
+#pragma unroll
+                for (int h = 0; h < H; h++) lds_wait(k[h].x);
+                fetch(j, min(t + step * NB, last));
+                f(k, t);
+            });
+        vm_wait_n<0>();  // (the ring is refilled, or given up)
     }
 }
 
-// exp2 of a difference of scores; equal ones (also both -inf) give 1.
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float exp2_diff(float x, float m) { return x == m ? 1.f : exp2_of(x - m); }
+
+// The workgroup's unit and what comes after it in the grid: units of one part of the keys
+// next to each other, in turn from part to part, so that the parts of long sequences are
+// dealt to all XCDs, and those that share keys to one.
+__device__ __forceinline__ int weight_unit(const WeightArgs &a, int &rest, int parts) {
+    rest = blockIdx.x / a.units;
+    return (blockIdx.x % a.units + rest % parts) % a.units;
+}
+
+constexpr float kNoScore = -3e38f;  // a running maximum before any score
 
 // Largest score and sum of RT * 16 rows over a part of their keys; the four waves
-// take its tiles in turn.  STORE: and the scores.  A lane's maximum is only raised where
-// a score passes it by 8 (sums stay below 2^8 times their terms' count: nothing is lost).
+// take its tiles in turn.  STORE: and the scores.
 template <class TQ, class TK, int D, int RT, bool STORE>
-__global__ __launch_bounds__(kWeightT, 2) void weight_rows_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows_kernel(WeightArgs a) {
     using P = Dot<TQ, TK, D>;
-    constexpr int NB = RT * P::q_regs >= 128 ? (P::KC <= 4 ? 2 : 1) : P::KC <= 4 ? 4 : P::KC <= 8 ? 2 : 1;
+    constexpr int H = P::H, NB = P::KC <= 2 ? 4 : 2;
+    __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * P::step_bytes];
     __shared__ float2 join[kWeightW][RT * 16];
+    __shared__ int pos[RT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units, split = rest % a.splits;
+    int rest;
+    const int unit = weight_unit(a, rest, a.splits), split = rest % a.splits;
     const int r0 = (a.blocks - 1 - rest / a.splits) * RT * 16, b = unit / a.n_kv, g = unit % a.n_kv;
     const WeightSeq s(a, b);
     const int r1 = min(r0 + RT * 16, s.rows);
     if (r0 >= r1) return;
     int lo, hi;
     s.keys(a, r0, r1, lo, hi);
-    const int k0 = max(lo & ~15, (lo / a.chunk + split) * a.chunk), k1 = min(hi, (lo / a.chunk + split + 1) * a.chunk);
+    const int k0 = max(lo & ~31, (lo / a.chunk + split) * a.chunk), k1 = min(hi, (lo / a.chunk + split + 1) * a.chunk);
     if (k0 >= k1) return;
+    const int window = a.window, score_tile = a.rows_pad * 16;
+    const float aqs = fabsf(a.qs);
+    float *const score = STORE ? a.score + (unit * a.tiles * a.rows_pad + (lane & 15)) * 16 + 4 * (lane >> 4) : nullptr;
     typename P::Q q[RT];
-    float qs[RT], m[RT], l[RT];
-    int pos[RT];
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        const int r = r0 + i * 16 + (lane & 15);
-        qs[i] = a.qs * P::load_q(q[i], P::q_row(a, s, b, g, r));
-        pos[i] = r < s.rows ? s.first + r / a.gq : -1;
-        m[i] = -INFINITY, l[i] = 0.f;
-    }
-    // tiles that every row sees whole
-    const int all_lo = a.window ? s.first + (r1 - 1) / a.gq + 1 - a.window : 0;
-    const int all_hi = r1 - r0 < RT * 16 ? 0 : s.first + r0 / a.gq + 1;
-    const int64_t tiles = (a.max_len + 15) >> 4;
-    auto tile = [&](const typename P::K &k, int t0) {
-        const bool all = t0 >= all_lo && t0 + 16 <= all_hi;
+    float row_qs[P::NP == 2 ? RT : 1], m[RT], l[RT];
+    auto qs = [&](int i) __attribute__((always_inline)) { return P::NP == 2 ? row_qs[P::NP == 2 ? i : 0] : aqs; };
+    auto start = [&]() __attribute__((always_inline)) {
+        if (tid < RT * 16) pos[tid] = r0 + tid < s.rows ? s.first + query_row(a, r0 + tid) : -1;
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            f32x4 x = P::template dot<false>(k, q[i]);
+            const float back = P::load_q(q[i], P::q_row(a, s, b, g, r0 + i * 16 + (lane & 15)), a.qs < 0.f);
+            if (P::NP == 2) row_qs[P::NP == 2 ? i : 0] = aqs * back;
+            m[i] = kNoScore, l[i] = 0.f;
+        }
+        __syncthreads();
+    };
+    // tiles that every row sees whole
+    const int all_lo = a.window ? s.first + query_row(a, r1 - 1) + 1 - a.window : 0, all_hi = s.first + query_row(a, r0) + 1;
+    auto tiles = [&](const typename P::K *k, int t0, auto mask) __attribute__((always_inline)) {
+        f32x4 x[RT][H];
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] *= qs[i];
-            if (!all) {
-                const int t = t0 + 4 * (lane >> 4);
+        for (int i = 0; i < RT; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (t + j > pos[i] || (a.window && t + j <= pos[i] - a.window)) x[j] = -INFINITY;
+            for (int h = 0; h < H; h++) x[i][h] = P::template dot<false>(k[h], q[i]);
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            if constexpr (mask.value) {
+                const int d = pos[i * 16 + (lane & 15)] - t0 - 4 * (lane >> 4);  // keys up to d are seen
+#pragma unroll
+                for (int j = 0; j < 4 * H; j++) {
+                    const int t = (j & 3) + (j >> 2) * 16;
+                    if (t > d || (window && t <= d - window)) x[i][j >> 2][j & 3] = -INFINITY;
+                }
             }
             if constexpr (STORE) {
                 if ((lane & 15) < s.rows)
-                    *(f32x4 *)(a.score + ((unit * tiles + (t0 >> 4)) * a.rows_pad + (lane & 15)) * 16 + 4 * (lane >> 4)) = x;
+#pragma unroll
+                    for (int h = 0; h < H; h++)
+                        *(f32x4 *)(score + ((t0 >> 4) + h) * (int64_t)score_tile) =
+                            x[i][h] * qs(i);
             }
-            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            if (__any(top > m[i] + 8.f)) {
-                const float up = fmaxf(m[i], top);
-                l[i] *= exp2_diff(m[i], up);
-                m[i] = up;
-            }
-            const float base = m[i] == -INFINITY ? 0.f : m[i];
-            l[i] += (exp2_of(x[0] - base) + exp2_of(x[1] - base)) + (exp2_of(x[2] - base) + exp2_of(x[3] - base));
+            float top = -INFINITY, e[4 * H], add[H];
+#pragma unroll
+            for (int j = 0; j < 4 * H; j++) top = fmaxf(top, x[i][j >> 2][j & 3]);
+            const float up = fmaxf(m[i], top * qs(i)), back = exp2_of(m[i] - up);
+            m[i] = up;
+#pragma unroll
+            for (int j = 0; j < 4 * H; j++) e[j] = exp2_of(fmaf(x[i][j >> 2][j & 3], qs(i), -up));
+#pragma unroll
+            for (int h = 0; h < H; h++) add[h] = (e[4 * h] + e[4 * h + 1]) + (e[4 * h + 2] + e[4 * h + 3]);
+            l[i] = fmaf(l[i], back, add[0] + (H > 1 ? add[H - 1] : 0.f));
         }
     };
-    each_tile<P, NB>(a, s, b, g, k0, k1, wave, tile);
+    each_step<P, NB, kWeightW, STORE>(a, s, b, g, k0, k1, wave, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
+        if (t0 >= all_lo && t0 + 16 * H <= all_hi) tiles(k, t0, Int<0>{});
+        else tiles(k, t0, Int<1>{});
+    });
 #pragma unroll
     for (int i = 0; i < RT; i++) {
         const float top = rows_max(m[i]);
-        const float sum = rows_sum(l[i] * exp2_diff(m[i], top));
+        const float sum = rows_sum(l[i] * exp2_of(m[i] - top));
         if (lane < 16) join[wave][i * 16 + lane] = float2{top, sum};
     }
     __syncthreads();
     if (tid < r1 - r0) {
         float top = join[0][tid].x, sum = 0.f;
         for (int w = 1; w < kWeightW; w++) top = fmaxf(top, join[w][tid].x);
-        for (int w = 0; w < kWeightW; w++) sum += join[w][tid].y * exp2_diff(join[w][tid].x, top);
+        for (int w = 0; w < kWeightW; w++) sum += join[w][tid].y * exp2_of(join[w][tid].x - top);
         a.ml[((int64_t)unit * a.rows_pad + r0 + tid) * a.splits + split] = float2{top, sum};
     }
     if (P::NP == 2 && !STORE && split == 0 && wave == 0 && lane < 16)
 #pragma unroll
-        for (int i = 0; i < RT; i++) a.row_qs[(int64_t)unit * a.rows_pad + r0 + i * 16 + lane] = qs[i];
+        for (int i = 0; i < RT; i++) a.row_qs[(int64_t)unit * a.rows_pad + r0 + i * 16 + lane] = qs(i);
 }
 
-// log2 of a row's denominator from its parts, +inf where it sees nothing (its weights
-// are then 2^-inf); ROWS: rows of a block.
+// log2 of a row's denominator from its parts, by 16 lanes; +inf where it sees nothing
+// (its weights are then 2^-inf).
 __device__ __forceinline__ float row_lse(const WeightArgs &a, const WeightSeq &s, int unit, int r, int block_rows) {
-    if (r >= s.rows) return INFINITY;
-    const int r0 = r / block_rows * block_rows;
-    int lo, hi;
-    s.keys(a, r0, min(r0 + block_rows, s.rows), lo, hi);
-    if (hi <= lo) return INFINITY;
-    const int n = (hi - 1) / a.chunk - lo / a.chunk + 1;
+    int lo = 0, hi = 0;
+    if (r < s.rows) {
+        const int r0 = r / block_rows * block_rows;
+        s.keys(a, r0, min(r0 + block_rows, s.rows), lo, hi);
+    }
+    const int n = hi <= lo ? 0 : (hi - 1) / a.chunk - lo / a.chunk + 1;
     const float2 *p = a.ml + ((int64_t)unit * a.rows_pad + r) * a.splits;
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < n; i++) m = fmaxf(m, p[i].x);
-    for (int i = 0; i < n; i++) l += p[i].y * exp2_diff(p[i].x, m);
-    return m == -INFINITY || l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    float m = kNoScore, l = 0.f;
+    for (int i = threadIdx.x & 15; i < n; i += 16) {
+        const float2 x = p[i];
+        const float up = fmaxf(m, x.x);
+        l = l * exp2_of(m - up) + x.y * exp2_of(x.x - up);
+        m = up;
+    }
+    float top = m;
+    top = fmaxf(top, dpp<kDppXor1>(top)), top = fmaxf(top, dpp<kDppXor2>(top));
+    top = fmaxf(top, dpp<kDppHalfMirror>(top)), top = fmaxf(top, dpp<kDppMirror>(top));
+    l = group_sum<16>(l * exp2_of(m - top));
+    return l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
-// The denominators of all rows, a thread a row.
+// The denominators of all rows, 16 lanes a row.
 __global__ __launch_bounds__(256) void weight_merge_kernel(WeightArgs a, int block_rows, int scaled) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (at >= (int64_t)a.units * a.rows_pad) return;
     const int unit = (int)(at / a.rows_pad), r = (int)(at % a.rows_pad);
     const WeightSeq s(a, unit / a.n_kv);
     const float lse = row_lse(a, s, unit, r, block_rows);
-    a.lse[at] = float2{lse, scaled && lse != INFINITY ? a.row_qs[at] : a.qs};
+    if ((threadIdx.x & 15) == 0) a.lse[at] = float2{lse, scaled && lse != INFINITY ? a.row_qs[at] : fabsf(a.qs)};
 }
 
 __device__ __forceinline__ void put_weight(const WeightArgs &a, int unit, int t, float sum) {
@@ -327,18 +438,21 @@ __global__ __launch_bounds__(kWeightT) void weight_sums_kernel(WeightArgs a) {
     const int tid = threadIdx.x, unit = blockIdx.x % a.units, t0 = (blockIdx.x / a.units * kWeightT + tid) * 4;
     const WeightSeq s(a, unit / a.n_kv);
     if ((int)(blockIdx.x / a.units) * kWeightT * 4 >= s.len) return;
-    if (tid < a.rows_pad) lse[tid] = row_lse(a, s, unit, tid, 16);
+    {
+        const float x = tid >> 4 < a.rows_pad ? row_lse(a, s, unit, tid >> 4, 16) : INFINITY;
+        if ((tid & 15) == 0) lse[tid >> 4] = x;
+    }
     __syncthreads();
     if (t0 >= s.len) return;
     int lo = 0, hi = 0;
     if (s.rows) s.keys(a, 0, s.rows, lo, hi);
     f32x4 sum{};
-    if (t0 < hi && t0 + 3 >= (lo & ~15)) {  // (tiles that were stored)
-        const float *x = a.score + (unit * (int64_t)((a.max_len + 15) >> 4) + (t0 >> 4)) * a.rows_pad * 16 + (t0 & 15);
+    if (t0 < hi && t0 + 3 >= (lo & ~31)) {  // (tiles that were stored)
+        const float *x = a.score + (unit * a.tiles + (t0 >> 4)) * a.rows_pad * 16 + (t0 & 15);
         for (int r = 0; r < s.rows; r++) {
             const f32x4 v = *(const f32x4 *)(x + r * 16);
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum[j] += v[j] == -INFINITY ? 0.f : exp2_of(v[j] - lse[r]);
+            for (int j = 0; j < 4; j++) sum[j] += exp2_of(v[j] - lse[r]);
         }
     }
 #pragma unroll
@@ -346,15 +460,23 @@ __global__ __launch_bounds__(kWeightT) void weight_sums_kernel(WeightArgs a) {
         if (t0 + j < s.len) put_weight(a, unit, t0 + j, sum[j]);
 }
 
-// Weights of up to RT * 16 rows, which stay in registers, over streamed keys.
-template <class TQ, class TK, int D, int RT>
-__global__ __launch_bounds__(kWeightT, 2) void weight_stream_kernel(WeightArgs a) {
+// Weights of up to RS * RT * 16 rows, which stay in registers, over streamed keys: RS waves
+// share a step's keys, each with its own rows; their sums meet in LDS at the end.
+template <class TQ, class TK, int D, int RT, int RS>
+__global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stream_kernel(WeightArgs a) {
     using P = Dot<TQ, TK, D>;
-    constexpr int NB = RT * P::q_regs >= 128 ? 1 : P::KC <= 4 ? 4 : P::KC <= 8 ? 2 : 1;
+    constexpr int W = kWeightW / RS, rows = RS * RT * 16;
+    constexpr int NB = P::KC <= 2 ? 4 : 2;
+    __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * P::step_bytes];
+    __shared__ float sums[RS][kWeightKeys / RS];
+    constexpr int H = P::H;
+    __shared__ int pos[rows];
+    __shared__ float lse[rows], row_qs[rows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int unit = blockIdx.x % a.units, b = unit / a.n_kv, g = unit % a.n_kv;
+    int rest;
+    const int unit = weight_unit(a, rest, INT_MAX), b = unit / a.n_kv, g = unit % a.n_kv;
     const WeightSeq s(a, b);
-    const int k0 = blockIdx.x / a.units * a.chunk, k1 = min(s.len, k0 + a.chunk);
+    const int chunk = min(a.chunk, kWeightKeys / RS), k0 = rest * chunk, k1 = min(s.len, k0 + chunk), i0 = wave % RS * RT;
     if (k0 >= k1) return;
     int lo = 0, hi = 0;
     if (s.rows) s.keys(a, 0, s.rows, lo, hi);
@@ -362,107 +484,186 @@ __global__ __launch_bounds__(kWeightT, 2) void weight_stream_kernel(WeightArgs a
         for (int t = k0 + tid; t < k1; t += kWeightT) put_weight(a, unit, t, 0.f);
         return;
     }
+    const int window = a.window;
+    const float aqs = fabsf(a.qs);
     typename P::Q q[RT];
-    f32x4 lse[RT], qs[RT];
-    int pos[RT];  // of the rows, four to a lane: those of the first, the others in turn
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
-        P::load_q(q[i], P::q_row(a, s, b, g, i * 16 + (lane & 15)));
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 x = a.lse[(int64_t)unit * a.rows_pad + i * 16 + 4 * (lane >> 4) + j];
-            lse[i][j] = x.x, qs[i][j] = P::NP == 2 ? x.y : a.qs;
+    auto start = [&]() __attribute__((always_inline)) {
+        if (tid < rows) {
+            const float2 x = a.lse[(int64_t)unit * a.rows_pad + tid];
+            lse[tid] = x.x, row_qs[tid] = x.y;
+            pos[tid] = x.x == INFINITY ? -1 : s.first + query_row(a, tid);  // (also where there is no row)
         }
-        pos[i] = 0;
-    }
-    (void)pos;
-    const int all_lo = a.window ? s.first + (s.rows - 1) / a.gq + 1 - a.window : 0;
-    const int all_hi = s.rows < RT * 16 ? 0 : s.first + 1;
-    auto tile = [&](const typename P::K &k, int t0) {
-        const bool all = t0 >= all_lo && t0 + 16 <= all_hi;
-        const int t = t0 + (lane & 15);
-        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < RT; i++) P::load_q(q[i], P::q_row(a, s, b, g, (i0 + i) * 16 + (lane & 15)), a.qs < 0.f);
+        __syncthreads();
+    };
+    const int all_lo = a.window ? s.first + query_row(a, s.rows - 1) + 1 - a.window : 0, all_hi = s.first + 1;
+    auto tiles = [&](const typename P::K *k, int t0, auto mask) __attribute__((always_inline)) {
+        f32x4 x[RT][H];
+        float sum[H];
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int h = 0; h < H; h++) x[i][h] = P::template dot<true>(k[h], q[i]);
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const f32x4 x = P::template dot<true>(k, q[i]);
-            float e[4];
+            const int r = (i0 + i) * 16 + 4 * (lane >> 4);  // the lane's four rows
+            const f32x4 ls = *(const f32x4 *)(lse + r);
+            f32x4 qs;
+            if (P::NP == 2) qs = *(const f32x4 *)(row_qs + r);
+            int ps[4];
+            if (mask.value) {
+                const int4 p = *(const int4 *)(pos + r);
+                ps[0] = p.x, ps[1] = p.y, ps[2] = p.z, ps[3] = p.w;
+            }
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[j] = exp2_of(fmaf(x[j], qs[i][j], -lse[i][j]));
-            if (!all) {
+            for (int h = 0; h < H; h++) {
+                float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const int r = i * 16 + 4 * (lane >> 4) + j, p = s.first + r / a.gq;
-                    if (r >= s.rows || t > p || (a.window && t <= p - a.window) || lse[i][j] == INFINITY) e[j] = 0.f;
+                    e[j] = exp2_of(fmaf(x[i][h][j], P::NP == 2 ? qs[j] : aqs, -ls[j]));
+                    const int t = t0 + 16 * h + (lane & 15);
+                    if (mask.value && (t > ps[j] || (window && t <= ps[j] - window))) e[j] = 0.f;
                 }
+                const float add = (e[0] + e[1]) + (e[2] + e[3]);
+                sum[h] = i ? sum[h] + add : add;
             }
-            sum += (e[0] + e[1]) + (e[2] + e[3]);
         }
-        sum = rows_sum(sum);
-        if (lane < 16 && t < k1) put_weight(a, unit, t, sum);
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            sum[h] = rows_sum(sum[h]);
+            if (lane < 16) sums[wave % RS][t0 - k0 + 16 * h + lane] = sum[h];
+        }
     };
-    each_tile<P, NB>(a, s, b, g, k0, k1, wave, tile);
+    each_step<P, NB, W, false>(a, s, b, g, k0, k1, wave / RS, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
+        if (t0 >= all_lo && t0 + 16 * H <= all_hi) tiles(k, t0, Int<0>{});
+        else tiles(k, t0, Int<1>{});
+    });
+    __syncthreads();
+    for (int t = k0 + tid; t < k1; t += kWeightT) {
+        float all = sums[0][t - k0];
+#pragma unroll
+        for (int i = 1; i < RS; i++) all += sums[i][t - k0];
+        put_weight(a, unit, t, all);
+    }
 }
 
 // Sums of the weights of KT * 16 keys, which stay in registers, over row_chunk streamed
-// rows; the four waves take row tiles in turn.
+// rows; the four waves take row tiles in turn, the next one in flight.
 template <class TQ, class TK, int D>
-__global__ __launch_bounds__(kWeightT, 2) void weight_keys_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight_keys_kernel(WeightArgs a) {
     using P = Dot<TQ, TK, D>;
-    constexpr int KT = P::kt;
+    using T = typename P::QTile;
+    constexpr int KT = P::kt, NB = 2, R = 16 * kWeightW, stage = T::bytes + 1024;  // the rows, their (lse, qs)
+    __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * stage];
     __shared__ float join[kWeightW][KT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units, part = rest % a.parts, b = unit / a.n_kv, g = unit % a.n_kv;
+    int rest;
+    const int unit = weight_unit(a, rest, a.parts), part = rest % a.parts, b = unit / a.n_kv, g = unit % a.n_kv;
     const int k0 = rest / a.parts * KT * 16;
     const WeightSeq s(a, b);
     const int k1 = min(k0 + KT * 16, s.len);
     if (k0 >= k1) return;
     // rows that see any of the keys
-    int lo = max(part * a.row_chunk, max(0, k0 - s.first) * a.gq) & ~15, hi = min(s.rows, (part + 1) * a.row_chunk);
+    const int lo = max(part * a.row_chunk, max(0, k0 - s.first) * a.gq) & ~15;
+    int hi = min(s.rows, (part + 1) * a.row_chunk);
     if (a.window) hi = (int)min((int64_t)hi, (int64_t)max(0, k1 - 1 + a.window - s.first) * a.gq);
     float *out = a.part + ((int64_t)part * a.units + unit) * a.max_len;
     if (lo >= hi) {
         for (int t = k0 + tid; t < k1; t += kWeightT) out[t] = 0.f;
         return;
     }
+    const int window = a.window;
+    const float aqs = fabsf(a.qs);
     typename P::K k[KT];
-    const KeySource<P> src(a, s, b, g, k0);
+    {
+        const KeySource<P> src(a, s, b, g, k0);
 #pragma unroll
-    for (int i = 0; i < KT; i++) src.load(k[i], min(k0 + 16 * i, (k1 - 1) & ~15));
+        for (int i = 0; i < KT; i += 2) {
+            const __amdgpu_buffer_rsrc_t r = src.rows(min(k0 + 16 * i, (k1 - 1) & ~31), 32);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < P::KC; c++)
+                    k[i + h].x[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                        r, ((lane & 15) + 16 * h) * (int)a.rb + (lane >> 4) * 16 + 64 * c, 0, 0));
+        }
+    }
+    uint32_t at[T::N];
+#pragma unroll
+    for (int c = 0; c < T::N; c++) at[c] = lds_addr(ring[wave]) + T::at(P::raw_chunk(c));
+    const uint32_t at_ls = lds_addr(ring[wave]) + T::bytes + (lane >> 4) * 32;
+    auto fetch = [&](int j, int r0) __attribute__((always_inline)) {
+        const int i0 = query_row(a, r0);
+        const char *base = (const char *)a.q + (((int64_t)b * a.max_rows + i0) * a.n_head + g * a.gq) * D * TQ::bytes;
+        const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(base), 0, 0x7fffffff, kRsrcWord3);
+        char *dst = ring[wave] + j * stage;
+#pragma unroll
+        for (int d = 0; d < T::N; d++) {
+            const int r = min(r0 + T::row(d), s.rows - 1), i = query_row(a, r);
+            dma16_cached(rows, dst + d * 1024, ((i - i0) * a.n_head + r - i * a.gq) * D * TQ::bytes + T::col(d), 0);
+        }
+        // (lse, qs) of 16 rows in the first 8 lanes; past them nothing is read
+        const __amdgpu_buffer_rsrc_t ls =
+            __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(a.lse + (int64_t)unit * a.rows_pad + r0), 0, 128, kRsrcWord3);
+        dma16_cached(ls, dst + T::bytes, lane * 16, 0);
+    };
     float sum[KT];
 #pragma unroll
     for (int i = 0; i < KT; i++) sum[i] = 0.f;
-    for (int r0 = lo + 16 * wave; r0 < hi; r0 += 16 * kWeightW) {
-        typename P::Q q;
-        P::load_q(q, P::q_row(a, s, b, g, r0 + (lane & 15)));
-        float lse[4], qs[4];
+    auto tile = [&](const typename P::Q &q, const f32x4 (&w)[2], int r0, auto mask) __attribute__((always_inline)) {
+        const float lse[4] = {w[0][0], w[0][2], w[1][0], w[1][2]}, qs[4] = {w[0][1], w[0][3], w[1][1], w[1][3]};
         int pos[4];
-        const float4 *ls = (const float4 *)(a.lse + (int64_t)unit * a.rows_pad + r0 + 4 * (lane >> 4));
-        const float4 l0 = ls[0], l1 = ls[1];
-        lse[0] = l0.x, lse[1] = l0.z, lse[2] = l1.x, lse[3] = l1.z;
-        qs[0] = l0.y, qs[1] = l0.w, qs[2] = l1.y, qs[3] = l1.w;
-        const int p0 = s.first + r0 / a.gq, p1 = s.first + (min(r0 + 16, s.rows) - 1) / a.gq;
-        const bool all = r0 + 16 <= s.rows && k0 + KT * 16 - 1 <= p0 && (!a.window || k0 > p1 - a.window);
-        if (!all)
+        if constexpr (mask.value)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int r = r0 + 4 * (lane >> 4) + j;
-                pos[j] = r < s.rows && lse[j] != INFINITY ? s.first + r / a.gq : -1;
+                pos[j] = r < s.rows && lse[j] != INFINITY ? s.first + query_row(a, r) : -1;
             }
 #pragma unroll
         for (int i = 0; i < KT; i++) {
             const f32x4 x = P::template dot<true>(k[i], q);
             float e[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[j] = exp2_of(fmaf(x[j], qs[j], -lse[j]));
-            if (!all) {
+            for (int j = 0; j < 4; j++) e[j] = exp2_of(fmaf(x[j], P::NP == 2 ? qs[j] : aqs, -lse[j]));
+            if constexpr (mask.value) {
                 const int t = k0 + 16 * i + (lane & 15);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (t > pos[j] || (a.window && t <= pos[j] - a.window)) e[j] = 0.f;
+                    if (t > pos[j] || (window && t <= pos[j] - window)) e[j] = 0.f;
             }
             sum[i] += (e[0] + e[1]) + (e[2] + e[3]);
         }
-    }
+    };
+    const int last = (hi - 1) & ~15;
+#pragma unroll
+    for (int i = 0; i < KT; i++)
+#pragma unroll
+        for (int c = 0; c < P::KC; c++) tie(k[i].x[c]);  // (the keys have come before the rows are counted)
+#pragma unroll
+    for (int j = 0; j < NB; j++) fetch(j, min(lo + 16 * wave + j * R, last));
+    for (int r0 = lo + 16 * wave; r0 < hi; r0 += NB * R)
+        static_for<0, NB>([&](auto J) __attribute__((always_inline)) {
+            constexpr int j = decltype(J)::value;
+            const int r = r0 + j * R;
+            if (r >= hi) return;
+            typename P::Raw raw;
+            u32x4 ls[2];
+            vm_wait_n<(NB - 1) * (T::N + 1)>();
+#pragma unroll
+            for (int c = 0; c < T::N; c++) raw.x[c] = lds_read_b128_at<j * stage>(at[c]);
+            ls[0] = lds_read_b128_at<j * stage>(at_ls), ls[1] = lds_read_b128_at<j * stage + 16>(at_ls);
+            lds_wait(raw.x);
+            tie(ls[0]), tie(ls[1]);
+            fetch(j, min(r + NB * R, last));
+            typename P::Q q;
+            P::make_q(q, raw, a.qs < 0.f);
+            const f32x4 w[2] = {__builtin_bit_cast(f32x4, ls[0]), __builtin_bit_cast(f32x4, ls[1])};
+            const int p0 = s.first + query_row(a, r), p1 = s.first + query_row(a, min(r + 16, s.rows) - 1);
+            if (k0 + KT * 16 - 1 <= p0 && (!window || k0 > p1 - window)) tile(q, w, r, Int<0>{});
+            else tile(q, w, r, Int<1>{});
+        });
+    vm_wait_n<0>();
 #pragma unroll
     for (int i = 0; i < KT; i++) {
         sum[i] = rows_sum(sum[i]);
@@ -487,26 +688,27 @@ struct WeightCut {
     int rows_pad, blocks, chunk, splits, row_chunk, parts;
     size_t ml, qs, lse, score, part, bytes;  // offsets
 };
-static int weight_max_rt(int q_dtype, int dtype, int D) {
-    const int kc = D * dtype_bytes(dtype) / 64, np = q_dtype == dtype ? 1 : dtype == ULLM_DT_F16 ? 2 : 3, regs = 4 * kc * np;
-    return regs <= 16 ? 8 : regs <= 32 ? 4 : regs <= 64 ? 2 : 1;
+// Registers of a row tile, and the most of them in a wave (Dot::q_regs, Dot::rt).
+static int weight_q_regs(int q_dtype, int dtype, int D) {
+    return D * dtype_bytes(dtype) / 16 * (q_dtype == dtype ? 1 : dtype == ULLM_DT_F16 ? 2 : 3);
 }
+static int weight_rt(int regs) { return regs <= 16 ? 4 : regs <= 48 ? 2 : 1; }
 constexpr int64_t kWeightWgs = 1024;  // workgroups aimed at: two to four rounds of the card
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows, int max_len, int window, int n_head,
                             int64_t n_kv, int D) {
     WeightCut c{};
     const int64_t rows = (int64_t)max_rows * (n_head / n_kv), units = batch * n_kv;
-    const int top = weight_max_rt(q_dtype, dtype, D);
+    const int regs = weight_q_regs(q_dtype, dtype, D), top = weight_rt(regs);
     c.rt = 1;
     while (c.rt < top && c.rt * 16 < rows) c.rt *= 2;
     c.blocks = (int)((rows + c.rt * 16 - 1) / (c.rt * 16));
-    c.mode = rows <= 16 ? 0 : c.blocks == 1 ? 1 : 2;
-    c.rows_pad = c.mode == 0 ? (int)rows : c.blocks * c.rt * 16;
+    c.mode = rows <= 16 ? 0 : rows <= kWeightW * top * 16 ? 1 : 2;
+    c.rows_pad = c.mode == 0 ? (int)rows : (int)((rows + 255) / 256 * 256);
     // parts of a row block's keys, whole tiles for every wave
     const int64_t keys = window > 0 && window < max_len ? std::min<int64_t>(max_len, (int64_t)window + max_rows) : max_len;
     const int64_t want = (keys * units * c.blocks + kWeightWgs - 1) / kWeightWgs;
-    c.chunk = (int)std::max<int64_t>(std::min<int64_t>((want + 63) / 64, (max_len + 63) / 64) * 64, 128);
+    c.chunk = (int)std::max<int64_t>(std::min<int64_t>((want + 127) / 128, (max_len + 127) / 128) * 128, 128);
     c.splits = (int)((keys + c.chunk - 1) / c.chunk + (window > 0 ? 1 : 0));
     c.parts = (int)std::min<int64_t>(16, (rows + 255) / 256);
     c.row_chunk = (int)(((rows + c.parts - 1) / std::max(c.parts, 1) + 63) / 64 * 64);
@@ -515,41 +717,49 @@ static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows,
     c.ml = at, at += up256(entries * c.splits * sizeof(float2));
     c.qs = at, at += up256(entries * sizeof(float));
     c.lse = at, at += c.mode ? up256(entries * sizeof(float2)) : 0;
-    c.score = at, at += c.mode == 0 ? up256((size_t)units * ((max_len + 15) / 16) * c.rows_pad * 16 * sizeof(float)) : 0;
+    c.score = at, at += c.mode == 0 ? up256((size_t)units * ((max_len + 31) / 32) * c.rows_pad * 32 * sizeof(float)) : 0;
     c.part = at, at += c.mode == 2 ? up256((size_t)c.parts * units * max_len * sizeof(float)) : 0;
     c.bytes = at;
     return c;
 }
 
+template <class TQ, class TK, int D, int RT, int RS>
+static void launch_stream(const WeightArgs &a, hipStream_t st) {
+    const int chunk = std::min(a.chunk, kWeightKeys / RS);
+    if constexpr (RT <= Dot<TQ, TK, D>::rt)
+        launch_kernel(weight_stream_kernel<TQ, TK, D, RT, RS>, dim3(a.units * ((a.max_len + chunk - 1) / chunk)), dim3(kWeightT), 0, st, a);
+}
 template <class TQ, class TK, int D, int RT>
-static void launch_rows(const WeightArgs &a, const WeightCut &c, hipStream_t st) {
+static void launch_rows(const WeightArgs &a, hipStream_t st) {
+    if constexpr (RT <= Dot<TQ, TK, D>::rt)
+        launch_kernel(weight_rows_kernel<TQ, TK, D, RT, false>, dim3((unsigned)a.units * a.splits * a.blocks), dim3(kWeightT), 0, st, a);
+}
+template <class TQ, class TK, int D>
+static void launch_weights(const WeightArgs &a, const WeightCut &c, hipStream_t st) {
     using P = Dot<TQ, TK, D>;
     const dim3 wg(kWeightT);
     const unsigned units = a.units;
     if (c.mode == 0) {
-        if constexpr (RT == 1) {
-            launch_kernel(weight_rows_kernel<TQ, TK, D, 1, true>, dim3(units * c.splits), wg, 0, st, a);
-            launch_kernel(weight_sums_kernel, dim3(units * ((a.max_len + 4 * kWeightT - 1) / (4 * kWeightT))), wg, 0, st, a);
-        }
+        launch_kernel(weight_rows_kernel<TQ, TK, D, 1, true>, dim3(units * c.splits), wg, 0, st, a);
+        launch_kernel(weight_sums_kernel, dim3(units * ((a.max_len + 4 * kWeightT - 1) / (4 * kWeightT))), wg, 0, st, a);
         return;
     }
-    launch_kernel(weight_rows_kernel<TQ, TK, D, RT, false>, dim3(units * c.splits * c.blocks), wg, 0, st, a);
-    launch_kernel(weight_merge_kernel, dim3(((size_t)units * c.rows_pad + 255) / 256), dim3(256), 0, st, a, RT * 16, (int)(P::NP == 2));
+    if (c.rt == 1) launch_rows<TQ, TK, D, 1>(a, st);
+    else if (c.rt == 2) launch_rows<TQ, TK, D, 2>(a, st);
+    else launch_rows<TQ, TK, D, 4>(a, st);
+    launch_kernel(weight_merge_kernel, dim3(((size_t)units * c.rows_pad + 15) / 16), dim3(256), 0, st, a, c.rt * 16, (int)(P::NP == 2));
     if (c.mode == 1) {
-        launch_kernel(weight_stream_kernel<TQ, TK, D, RT>, dim3(units * ((a.max_len + a.chunk - 1) / a.chunk)), wg, 0, st, a);
+        // as few waves to a key as hold the rows
+        const int tiles = (a.max_rows * a.gq + 15) / 16;
+        if (tiles <= 2 && P::rt >= 2) launch_stream<TQ, TK, D, 2, 1>(a, st);
+        else if (tiles <= 4 && P::rt >= 4) launch_stream<TQ, TK, D, 4, 1>(a, st);
+        else if (tiles <= 2 * P::rt) launch_stream<TQ, TK, D, P::rt, 2>(a, st);
+        else launch_stream<TQ, TK, D, P::rt, 4>(a, st);
         return;
     }
     constexpr int keys = P::kt * 16;
     launch_kernel(weight_keys_kernel<TQ, TK, D>, dim3(units * a.parts * ((a.max_len + keys - 1) / keys)), wg, 0, st, a);
     launch_kernel(weight_join_kernel, dim3(units * ((a.max_len + kWeightT - 1) / kWeightT)), wg, 0, st, a);
-}
-template <class TQ, class TK, int D>
-static void launch_weights(const WeightArgs &a, const WeightCut &c, hipStream_t st) {
-    constexpr int top = Dot<TQ, TK, D>::max_rt;
-    if (c.rt == 1) launch_rows<TQ, TK, D, 1>(a, c, st);
-    if constexpr (top >= 2) if (c.rt == 2) launch_rows<TQ, TK, D, 2>(a, c, st);
-    if constexpr (top >= 4) if (c.rt == 4) launch_rows<TQ, TK, D, 4>(a, c, st);
-    if constexpr (top >= 8) if (c.rt == 8) launch_rows<TQ, TK, D, 8>(a, c, st);
 }
 template <class TQ, class TK>
 static void launch_weights(const WeightArgs &a, const WeightCut &c, int D, hipStream_t st) {
@@ -571,8 +781,8 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     if (a.max_len > 1 << 30) return set_error(ULLM_HIP_E_INVALID, "%s: max_len %d > 2^30", fn, a.max_len);
     if (a.window >= a.max_len) a.window = 0;  // (what every row sees)
     if ((int64_t)a.max_rows * a.n_head > 1 << 23) return set_error(ULLM_HIP_E_INVALID, "%s: too many rows", fn);
-    if (kv_stride < (int64_t)a.n_kv * head_dim || a.w_stride < a.max_len)
-        return set_error(ULLM_HIP_E_INVALID, "%s: kv_stride or weights_stride too small", fn);
+    if (kv_stride < (int64_t)a.n_kv * head_dim || kv_stride > INT_MAX / 256 || a.w_stride < a.max_len)
+        return set_error(ULLM_HIP_E_INVALID, "%s: bad kv_stride, or weights_stride too small", fn);
     if (a.batch == 0 || a.max_len == 0) return ULLM_HIP_OK;
     if ((!a.q && a.max_rows) || !a.k || !a.len || !a.w) return set_error(ULLM_HIP_E_INVALID, "%s: null tensor pointer", fn);
     const int eb = dtype_bytes(dtype);
@@ -587,10 +797,13 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     if (!ws || ws_bytes < c.bytes || (uintptr_t)ws & 255)
         return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, c.bytes);
     a.gq = a.n_head / a.n_kv;
-    a.qs = scale * kLog2e;
+    a.gq_shift = 31 - __builtin_clz(a.gq);
+    a.gq_mul = a.gq & (a.gq - 1) ? (uint32_t)((1ull << (32 + a.gq_shift)) / a.gq + 1) : 0;
+    // (a scale of 0 as the least normal number: 0 times a masked score of -inf is none)
+    a.qs = std::copysign(std::max(std::fabs(scale * kLog2e), 1.17549435e-38f), scale);
     a.rb = kv_stride * eb;
     a.units = (int)units, a.rows_pad = c.rows_pad, a.blocks = c.blocks, a.chunk = c.chunk, a.splits = c.splits;
-    a.row_chunk = c.row_chunk, a.parts = c.parts;
+    a.row_chunk = c.row_chunk, a.parts = c.parts, a.tiles = (a.max_len + 31) / 32 * 2;
     char *const at = (char *)ws;
     a.ml = (float2 *)(at + c.ml), a.row_qs = (float *)(at + c.qs), a.lse = (float2 *)(at + c.lse);
     a.score = (float *)(at + c.score), a.part = (float *)(at + c.part);
@@ -612,7 +825,7 @@ extern "C" int ullm_hip_key_weights(const void *q, int q_dtype, const void *k_ca
                                     size_t workspace_bytes, void *stream) {
     if (seq_stride < 0) return set_error(ULLM_HIP_E_INVALID, "key_weights: seq_stride < 0");
     const WeightArgs a{q, (const char *)k_cache, 0, batch > 1 && dtype_ok(kv_dtype) ? seq_stride * dtype_bytes(kv_dtype) : 0,
-                       nullptr, 0, 0, 0, seq_lens, n_rows, max_rows, max_len, window, batch, n_head, n_kv_head, 0, 0.f,
+                       nullptr, 0, 0, 0, seq_lens, n_rows, max_rows, max_len, window, batch, n_head, n_kv_head, 0, 0, 0, 0.f,
                        decay, weights, weights_stride};
     return key_weights("key_weights", a, q_dtype, kv_dtype, kv_stride, head_dim, scale, workspace, workspace_bytes, stream);
 }
@@ -632,7 +845,7 @@ extern "C" int ullm_hip_key_weights_paged(const void *q, int q_dtype, const void
     if (batch > 0 && max_len > 0 && !block_table)
         return set_error(ULLM_HIP_E_INVALID, "key_weights_paged: null tensor pointer");
     const WeightArgs a{q, (const char *)k_pages, 0, 0, block_table, table_stride, __builtin_ctz(page_size), n_pages,
-                       seq_lens, n_rows, max_rows, max_len, window, batch, n_head, n_kv_head, 0, 0.f, decay, weights,
+                       seq_lens, n_rows, max_rows, max_len, window, batch, n_head, n_kv_head, 0, 0, 0, 0.f, decay, weights,
                        weights_stride};
     return key_weights("key_weights_paged", a, q_dtype, kv_dtype, kv_stride, head_dim, scale, workspace,
                        workspace_bytes, stream);
@@ -650,10 +863,11 @@ extern "C" size_t ullm_hip_key_weights_workspace_bytes(int kv_dtype, int batch, 
     const int64_t rows = (int64_t)max_rows * gq, units = (int64_t)batch * n_kv_head;
     size_t most = 0;
     for (int q_dtype : {(int)ULLM_DT_F32, kv_dtype}) {
-        const int block = 16 * weight_max_rt(q_dtype, kv_dtype, head_dim);
-        const int64_t blocks = (rows + block - 1) / block;
-        size_t n = up256((kWeightWgs + 3 * units * blocks) * block * sizeof(float2)) + 2 * up256(units * blocks * block * sizeof(float2));
-        n += std::max((size_t)(gq <= 16 ? up256((size_t)units * ((max_len + 15) / 16) * std::min<int64_t>(rows, 16) * 16 * sizeof(float)) : 0),
+        const int block = 16 * weight_rt(weight_q_regs(q_dtype, kv_dtype, head_dim));
+        const int64_t blocks = (rows + block - 1) / block, pad = (rows + 255) / 256 * 256;
+        // (parts of a row are counted for the rows of a block, of which the last may be padded to 256)
+        size_t n = up256((kWeightWgs + 3 * units * blocks) * 256 * sizeof(float2)) + 2 * up256(units * pad * sizeof(float2));
+        n += std::max((size_t)(gq <= 16 ? up256((size_t)units * ((max_len + 31) / 32) * std::min<int64_t>(rows, 16) * 32 * sizeof(float)) : 0),
                       up256((size_t)std::min<int64_t>(16, (rows + 255) / 256) * units * max_len * sizeof(float)));
         most = std::max(most, n);
     }
