@@ -47,9 +47,10 @@ struct WeightArgs {
     int rows_pad;    // rows of a unit in the arrays below, a multiple of the blocks'
     int blocks;      // row blocks of a unit
     int chunk, splits;  // keys of a part of a row block, the most parts
+    int spread;         // or: parts that all sequences have together, cut by their lengths (see weight_spread)
     int64_t tiles;  // of the scores of a unit
     int row_chunk, parts;  // rows of a part of a key block, the most parts (weight_keys_kernel)
-    float2 *ml;      // [units][rows_pad][splits]: largest score and sum of exp2 of a part
+    float2 *ml;      // [parts][rows of a block]: largest score and sum of exp2 of a part (see weight_part)
     float *row_qs;   // [units][rows_pad]: qs over the row's power of two
     float2 *lse;     // [units][rows_pad]: log2 of the denominator, row_qs
     float *score;    // [units][tiles][rows][16]: scores (log2 domain)
@@ -104,7 +105,7 @@ struct Dot {
     static constexpr bool f32 = __is_same(TK, F32);
     static constexpr int KC = D * TK::bytes / 64;
     static constexpr int NP = f32 || __is_same(TQ, TK) ? 1 : __is_same(TK, F16) ? 2 : 3;
-    static constexpr int q_regs = 4 * KC * NP;
+    static constexpr int q_regs = 4 * KC * NP, q_bytes = D * TQ::bytes;
     // most row tiles of a wave where the rows stay in registers
     static constexpr int rt = q_regs <= 16 ? 4 : q_regs <= 48 ? 2 : 1;
     // weight_keys_kernel: key tiles of a wave
@@ -120,10 +121,6 @@ struct Dot {
     __device__ __forceinline__ static int raw_chunk(int c) {
         const int part = (threadIdx.x & 63) >> 4;
         return NP == 1 ? 4 * c + part : 8 * (c >> 1) + 2 * part + (c & 1);
-    }
-    __device__ __forceinline__ static void load_raw(Raw &r, const char *row) {
-#pragma unroll
-        for (int c = 0; c < QTile::N; c++) r.x[c] = *(const u32x4 *)(row + raw_chunk(c) * 16);
     }
     // The operand of a row of q, of other sign if `neg`; returns the power of two that it was
     // divided by.
@@ -167,38 +164,34 @@ struct Dot {
             return back;
         }
     }
-    __device__ __forceinline__ static float load_q(Q &q, const char *row, bool neg) {
-        Raw raw;
-        load_raw(raw, row);
-        return make_q(q, raw, neg);
-    }
-    // The 16x16 products of 16 keys and 16 rows: element i of lane l is key 4 (l / 16) + i of
-    // row l % 16, or with ROWS row 4 (l / 16) + i of key l % 16.
-    template <bool ROWS>
-    __device__ __forceinline__ static f32x4 dot(const K &k, const Q &q) {
-        f32x4 s{};
+    // The 16x16 products of NK key tiles and NQ row tiles, x[i][h] of rows i and keys h: element
+    // j of lane l is key 4 (l / 16) + j of row l % 16, or with ROWS row 4 (l / 16) + j of key
+    // l % 16.  Tiles in turn (a tile's next product waits for its last one).
+    template <bool ROWS, int NQ, int NK>
+    __device__ __forceinline__ static void dots(f32x4 (&x)[NQ][NK], const K *k, const Q *q) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int h = 0; h < NK; h++) x[i][h] = f32x4{};
 #pragma unroll
         for (int p = NP - 1; p >= 0; p--)
 #pragma unroll
-            for (int c = 0; c < KC; c++) {
-                if constexpr (f32) {
+            for (int c = 0; c < KC; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = __uint_as_float(k.x[c][i]), y = __uint_as_float(q.x[0][c][i]);
-                        s = ROWS ? __builtin_amdgcn_mfma_f32_16x16x4f32(y, x, s, 0, 0, 0)
-                                 : __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, s, 0, 0, 0);
-                    }
-                } else {
-                    s = ROWS ? mfma16<TK>(q.x[p][c], k.x[c], s) : mfma16<TK>(k.x[c], q.x[p][c], s);
-                }
-            }
-        return s;
-    }
-    // Row r of unit (b, g); past the last: the last again.
-    __device__ __forceinline__ static const char *q_row(const WeightArgs &a, const WeightSeq &s, int b, int g, int r) {
-        r = min(r, s.rows - 1);
-        const int i = query_row(a, r), h = r - i * a.gq;
-        return (const char *)a.q + (((int64_t)b * a.max_rows + i) * a.n_head + g * a.gq + h) * D * TQ::bytes;
+                for (int e = 0; e < (f32 ? 4 : 1); e++)
+#pragma unroll
+                    for (int i = 0; i < NQ; i++)
+#pragma unroll
+                        for (int h = 0; h < NK; h++) {
+                            f32x4 &s = x[i][h];
+                            if constexpr (f32) {
+                                const float a = __uint_as_float(k[h].x[c][e]), b = __uint_as_float(q[i].x[0][c][e]);
+                                s = ROWS ? __builtin_amdgcn_mfma_f32_16x16x4f32(b, a, s, 0, 0, 0)
+                                         : __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, s, 0, 0, 0);
+                            } else {
+                                s = ROWS ? mfma16<TK>(q[i].x[p][c], k[h].x[c], s) : mfma16<TK>(k[h].x[c], q[i].x[p][c], s);
+                            }
+                        }
     }
 };
 
@@ -232,12 +225,37 @@ struct KeySource {
     }
 };
 
+// Fetches rows r0 .. r0 + 15 of a unit's queries into a tile in LDS (past the last row: the
+// last again).
+template <class P>
+__device__ __forceinline__ void fetch_q(const WeightArgs &a, const WeightSeq &s, int b, int g, int r0, char *dst) {
+    using T = typename P::QTile;
+    r0 = min(r0, s.rows - 1);
+    const int i0 = query_row(a, r0);
+    const char *base = (const char *)a.q + (((int64_t)b * a.max_rows + i0) * a.n_head + g * a.gq) * P::q_bytes;
+    const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(base), 0, 0x7fffffff, kRsrcWord3);
+#pragma unroll
+    for (int d = 0; d < T::N; d++) {
+        const int r = min(r0 + T::row(d), s.rows - 1), i = query_row(a, r);
+        dma16_cached(rows, dst + d * 1024, ((i - i0) * a.n_head + r - i * a.gq) * P::q_bytes + T::col(d), 0);
+    }
+}
+// A tile of queries from LDS, as an operand (see Dot::make_q).
+template <class P>
+__device__ __forceinline__ float read_q(typename P::Q &q, const char *tile, bool neg) {
+    typename P::Raw raw;
+#pragma unroll
+    for (int c = 0; c < P::QTile::N; c++) raw.x[c] = lds_read_b128(lds_addr(tile) + P::QTile::at(P::raw_chunk(c)));
+    lds_wait(raw.x);
+    return P::make_q(q, raw, neg);
+}
+
 constexpr int kWeightT = 256, kWeightW = 4;
 
 // f(P::H tiles, their first key) over the steps of H tiles of keys k0 .. k1 - 1 (k0 a multiple
-// of 32) that are this wave's, one of W, NB steps in flight in its ring.  start() is called
-// once the first are.
-template <class P, int NB, int W, bool ONCE, class S, class F>
+// of 32) that are this wave's, one of W, NB steps in flight in its ring.  f makes STORES stores (0: or none), which are counted with the
+// loads and may be in flight as long as these.  start() is called behind the first loads.
+template <class P, int NB, int W, int STORES, class S, class F>
 __device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &s, int b, int g, int k0, int k1, int wave,
                                           char *ring, S &&start, F &&f) {
     using T = typename P::KTile;
@@ -258,7 +276,7 @@ __device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &
 #pragma unroll
                 for (int d = 0; d < T::N; d++) {
                     char *dst = ring + j * P::step_bytes + h * T::bytes + d * 1024;
-                    if (ONCE) dma16(r, dst, off[d] + h * 16 * (int)a.rb, 0);
+                    if (STORES) dma16(r, dst, off[d] + h * 16 * (int)a.rb, 0);
                     else dma16_cached(r, dst, off[d] + h * 16 * (int)a.rb, 0);
                 }
         };
@@ -271,7 +289,11 @@ __device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &
                 const int t = t0 + step * j;
                 if (t >= e1) return;
                 typename P::K k[H];
-                vm_wait_n<(NB - 1) * H * T::N>();
+                // newer than this step's loads: NB - 1 steps' loads, and from the second round on NB
+                // steps' stores
+                constexpr int loads = (NB - 1) * H * T::N;
+                if (STORES == 0 || t0 == first) vm_wait_n<loads>();
+                else vm_wait_n<loads + NB * STORES>();
                 static_for<0, H>([&](auto HH) __attribute__((always_inline)) {
                     constexpr int h = decltype(HH)::value;
 #pragma unroll
@@ -288,12 +310,43 @@ __device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The workgroup's unit and what comes after it in the grid: units of one part of the keys
-// next to each other, in turn from part to part, so that the parts of long sequences are
-// dealt to all XCDs, and those that share keys to one.
-__device__ __forceinline__ int weight_unit(const WeightArgs &a, int &rest, int parts) {
-    rest = blockIdx.x / a.units;
-    return (blockIdx.x % a.units + rest % parts) % a.units;
+// The lengths of a batch are on the device.  Where a call has few row blocks, all its
+// sequences together are cut into about `spread` parts of one length, so that one round of
+// workgroups is busy to its end: returns that length, and in lane b the parts of
+// sequences 0 .. b (up to 64 of them).
+__device__ __forceinline__ int weight_spread(const WeightArgs &a, int &upto) {
+    const int lane = threadIdx.x & 63;
+    int keys = 0;
+    if (lane < a.batch) {
+        const WeightSeq s(a, lane);
+        int lo = 0, hi = 0;
+        if (s.rows) s.keys(a, 0, s.rows, lo, hi);
+        keys = max(0, hi - (lo & ~31));
+    }
+    const int total = __builtin_amdgcn_readlane(wave_scan(keys), 63);
+    const int chunk = max(128, ((total + a.spread - 1) / a.spread + 127) & ~127);
+    upto = wave_scan((keys + chunk - 1) / chunk);
+    return chunk;
+}
+// The parts of a row block: part j has the keys from org + j chunk on; it is part
+// first + j * step of the call.
+struct WeightParts {
+    int chunk, org, first, step;
+};
+__device__ __forceinline__ WeightParts weight_parts(const WeightArgs &a, const WeightSeq &s, int b, int g, int block, int lo, int chunk,
+                                                    int upto) {
+    WeightParts p{chunk, 0, 0, 1};
+    if (!a.spread) {
+        p.org = lo / chunk * chunk;
+        p.first = ((b * a.n_kv + g) * a.blocks + block) * a.splits;
+        return p;
+    }
+    int all_lo, all_hi;
+    s.keys(a, 0, s.rows, all_lo, all_hi);
+    p.org = all_lo & ~31;
+    p.first = ((b ? __shfl(upto, b - 1) : 0) * a.blocks + block) * a.n_kv + g;
+    p.step = a.blocks * a.n_kv;
+    return p;
 }
 
 constexpr float kNoScore = -3e38f;  // a running maximum before any score
@@ -304,19 +357,40 @@ template <class TQ, class TK, int D, int RT, bool STORE>
 __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows_kernel(WeightArgs a) {
     using P = Dot<TQ, TK, D>;
     constexpr int H = P::H, NB = P::KC <= 2 ? 4 : 2;
+    // the queries come through the ring, or where there is room beside it while it fills
+    constexpr bool APART = RT == 1 && P::QTile::bytes <= 8192;
+    static_assert(RT * P::QTile::bytes <= kWeightW * NB * P::step_bytes, "queries in the ring");
     __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * P::step_bytes];
+    __shared__ __attribute__((aligned(1024))) char apart[APART ? P::QTile::bytes : 16];
     __shared__ float2 join[kWeightW][RT * 16];
     __shared__ int pos[RT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int rest;
-    const int unit = weight_unit(a, rest, a.splits), split = rest % a.splits;
-    const int r0 = (a.blocks - 1 - rest / a.splits) * RT * 16, b = unit / a.n_kv, g = unit % a.n_kv;
+    int b, g, block, split, chunk = a.chunk;
+    if (a.spread) {
+        int upto;
+        chunk = weight_spread(a, upto);
+        const int slot = blockIdx.x / (a.n_kv * a.blocks);
+        b = __popcll(__ballot(upto <= slot));
+        if (b >= a.batch) return;
+        split = slot - (b ? __builtin_amdgcn_readlane(upto, b - 1) : 0);
+        g = blockIdx.x % a.n_kv, block = blockIdx.x / a.n_kv % a.blocks;
+    } else {
+        const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units;  // (what shares keys on one XCD)
+        split = rest % a.splits, block = a.blocks - 1 - rest / a.splits, b = unit / a.n_kv, g = unit % a.n_kv;
+    }
+    const int unit = b * a.n_kv + g, r0 = block * RT * 16;
     const WeightSeq s(a, b);
     const int r1 = min(r0 + RT * 16, s.rows);
     if (r0 >= r1) return;
     int lo, hi;
     s.keys(a, r0, r1, lo, hi);
-    const int k0 = max(lo & ~31, (lo / a.chunk + split) * a.chunk), k1 = min(hi, (lo / a.chunk + split + 1) * a.chunk);
+    int org = lo / chunk * chunk;
+    if (a.spread) {
+        int all_lo, all_hi;
+        s.keys(a, 0, s.rows, all_lo, all_hi);
+        org = all_lo & ~31;
+    }
+    const int k0 = max(lo & ~31, org + split * chunk), k1 = min(hi, org + (split + 1) * chunk);
     if (k0 >= k1) return;
     const int window = a.window, score_tile = a.rows_pad * 16;
     const float aqs = fabsf(a.qs);
@@ -324,24 +398,31 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
     typename P::Q q[RT];
     float row_qs[P::NP == 2 ? RT : 1], m[RT], l[RT];
     auto qs = [&](int i) __attribute__((always_inline)) { return P::NP == 2 ? row_qs[P::NP == 2 ? i : 0] : aqs; };
-    auto start = [&]() __attribute__((always_inline)) {
-        if (tid < RT * 16) pos[tid] = r0 + tid < s.rows ? s.first + query_row(a, r0 + tid) : -1;
+    char *const staged = APART ? apart : ring[0];
+    auto load_q = [&](auto behind) __attribute__((always_inline)) {  // behind: newer loads than the queries'
+        vm_wait_n<decltype(behind)::value>();
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const float back = P::load_q(q[i], P::q_row(a, s, b, g, r0 + i * 16 + (lane & 15)), a.qs < 0.f);
+            const float back = read_q<P>(q[i], staged + i * P::QTile::bytes, a.qs < 0.f);
             if (P::NP == 2) row_qs[P::NP == 2 ? i : 0] = aqs * back;
             m[i] = kNoScore, l[i] = 0.f;
         }
+    };
+    if (tid < RT * 16) pos[tid] = r0 + tid < s.rows ? s.first + query_row(a, r0 + tid) : -1;
+    if (wave < RT) fetch_q<P>(a, s, b, g, r0 + wave * 16, staged + wave * P::QTile::bytes);
+    if (!APART) {
+        load_q(Int<0>{});
         __syncthreads();
+    }
+    auto start = [&]() __attribute__((always_inline)) {
+        if (APART) load_q(Int<NB * H * P::KTile::N>{});
     };
     // tiles that every row sees whole
     const int all_lo = a.window ? s.first + query_row(a, r1 - 1) + 1 - a.window : 0, all_hi = s.first + query_row(a, r0) + 1;
     auto tiles = [&](const typename P::K *k, int t0, auto mask) __attribute__((always_inline)) {
         f32x4 x[RT][H];
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int h = 0; h < H; h++) x[i][h] = P::template dot<false>(k[h], q[i]);
+        P::template dots<false>(x, k, q);
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             if constexpr (mask.value) {
@@ -371,7 +452,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
             l[i] = fmaf(l[i], back, add[0] + (H > 1 ? add[H - 1] : 0.f));
         }
     };
-    each_step<P, NB, kWeightW, STORE>(a, s, b, g, k0, k1, wave, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
+    each_step<P, NB, kWeightW, STORE ? H : 0>(a, s, b, g, k0, k1, wave, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
         if (t0 >= all_lo && t0 + 16 * H <= all_hi) tiles(k, t0, Int<0>{});
         else tiles(k, t0, Int<1>{});
     });
@@ -386,29 +467,31 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
         float top = join[0][tid].x, sum = 0.f;
         for (int w = 1; w < kWeightW; w++) top = fmaxf(top, join[w][tid].x);
         for (int w = 0; w < kWeightW; w++) sum += join[w][tid].y * exp2_of(join[w][tid].x - top);
-        a.ml[((int64_t)unit * a.rows_pad + r0 + tid) * a.splits + split] = float2{top, sum};
+        const int part = a.spread ? (int)blockIdx.x : (unit * a.blocks + block) * a.splits + split;
+        a.ml[(int64_t)part * RT * 16 + tid] = float2{top, sum};
     }
-    if (P::NP == 2 && !STORE && split == 0 && wave == 0 && lane < 16)
+    if (P::NP == 2 && !STORE && k0 == max(lo & ~31, org) && wave == 0 && lane < 16)
 #pragma unroll
         for (int i = 0; i < RT; i++) a.row_qs[(int64_t)unit * a.rows_pad + r0 + i * 16 + lane] = qs(i);
 }
 
 // log2 of a row's denominator from its parts, by 16 lanes; +inf where it sees nothing
-// (its weights are then 2^-inf).
-__device__ __forceinline__ float row_lse(const WeightArgs &a, const WeightSeq &s, int unit, int r, int block_rows) {
+// (its weights are then 2^-inf).  upto: of weight_spread, in every lane of the wave.
+__device__ __forceinline__ float row_lse(const WeightArgs &a, const WeightSeq &s, int b, int g, int r, int block_rows, int chunk,
+                                         int upto) {
+    const int block = r / block_rows, r0 = block * block_rows;
     int lo = 0, hi = 0;
-    if (r < s.rows) {
-        const int r0 = r / block_rows * block_rows;
-        s.keys(a, r0, min(r0 + block_rows, s.rows), lo, hi);
-    }
-    const int n = hi <= lo ? 0 : (hi - 1) / a.chunk - lo / a.chunk + 1;
-    const float2 *p = a.ml + ((int64_t)unit * a.rows_pad + r) * a.splits;
+    if (r < s.rows) s.keys(a, r0, min(r0 + block_rows, s.rows), lo, hi);
+    const WeightParts p = weight_parts(a, s, b, g, block, lo, chunk, upto);
     float m = kNoScore, l = 0.f;
-    for (int i = threadIdx.x & 15; i < n; i += 16) {
-        const float2 x = p[i];
-        const float up = fmaxf(m, x.x);
-        l = l * exp2_of(m - up) + x.y * exp2_of(x.x - up);
-        m = up;
+    if (hi > lo) {
+        const int last = (hi - 1 - p.org) / chunk;
+        for (int j = (lo - p.org) / chunk + (threadIdx.x & 15); j <= last; j += 16) {
+            const float2 x = a.ml[(int64_t)(p.first + j * p.step) * block_rows + r - r0];
+            const float up = fmaxf(m, x.x);
+            l = l * exp2_of(m - up) + x.y * exp2_of(x.x - up);
+            m = up;
+        }
     }
     float top = m;
     top = fmaxf(top, dpp<kDppXor1>(top)), top = fmaxf(top, dpp<kDppXor2>(top));
@@ -419,12 +502,14 @@ __device__ __forceinline__ float row_lse(const WeightArgs &a, const WeightSeq &s
 
 // The denominators of all rows, 16 lanes a row.
 __global__ __launch_bounds__(256) void weight_merge_kernel(WeightArgs a, int block_rows, int scaled) {
-    const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (at >= (int64_t)a.units * a.rows_pad) return;
-    const int unit = (int)(at / a.rows_pad), r = (int)(at % a.rows_pad);
+    const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), all = (int64_t)a.units * a.rows_pad;
+    int upto = 0, chunk = a.chunk;
+    if (a.spread) chunk = weight_spread(a, upto);
+    const int unit = (int)(min(at, all - 1) / a.rows_pad), r = (int)(min(at, all - 1) % a.rows_pad);
     const WeightSeq s(a, unit / a.n_kv);
-    const float lse = row_lse(a, s, unit, r, block_rows);
-    if ((threadIdx.x & 15) == 0) a.lse[at] = float2{lse, scaled && lse != INFINITY ? a.row_qs[at] : fabsf(a.qs)};
+    const float lse = row_lse(a, s, unit / a.n_kv, unit % a.n_kv, r, block_rows, chunk, upto);
+    if (at < all && (threadIdx.x & 15) == 0)
+        a.lse[at] = float2{lse, scaled && lse != INFINITY ? a.row_qs[at] : fabsf(a.qs)};
 }
 
 __device__ __forceinline__ void put_weight(const WeightArgs &a, int unit, int t, float sum) {
@@ -432,32 +517,39 @@ __device__ __forceinline__ void put_weight(const WeightArgs &a, int unit, int t,
     *w = a.decay == 0.f ? sum : fmaf(a.decay, *w, sum);
 }
 
-// Stored scores of up to 16 rows: a thread four keys.
+// Stored scores of up to 16 rows: a thread four keys, whose scores and old weights are
+// on their way while the denominators are found.
 __global__ __launch_bounds__(kWeightT) void weight_sums_kernel(WeightArgs a) {
     __shared__ float lse[16];
     const int tid = threadIdx.x, unit = blockIdx.x % a.units, t0 = (blockIdx.x / a.units * kWeightT + tid) * 4;
-    const WeightSeq s(a, unit / a.n_kv);
+    const int b = unit / a.n_kv;
+    const WeightSeq s(a, b);
     if ((int)(blockIdx.x / a.units) * kWeightT * 4 >= s.len) return;
-    {
-        const float x = tid >> 4 < a.rows_pad ? row_lse(a, s, unit, tid >> 4, 16) : INFINITY;
-        if ((tid & 15) == 0) lse[tid >> 4] = x;
-    }
-    __syncthreads();
-    if (t0 >= s.len) return;
     int lo = 0, hi = 0;
     if (s.rows) s.keys(a, 0, s.rows, lo, hi);
-    f32x4 sum{};
-    if (t0 < hi && t0 + 3 >= (lo & ~31)) {  // (tiles that were stored)
-        const float *x = a.score + (unit * a.tiles + (t0 >> 4)) * a.rows_pad * 16 + (t0 & 15);
-        for (int r = 0; r < s.rows; r++) {
-            const f32x4 v = *(const f32x4 *)(x + r * 16);
+    const bool stored = t0 < hi && t0 + 3 >= (lo & ~31);  // (whole tiles were)
+    const float *x = a.score + (unit * a.tiles + (stored ? t0 >> 4 : 0)) * a.rows_pad * 16 + (t0 & 15);
+    float *w = a.w + (int64_t)unit * a.w_stride + t0;
+    f32x4 v[16], sum{};
+    float old[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum[j] += exp2_of(v[j] - lse[r]);
-        }
-    }
+    for (int r = 0; r < 16; r++)
+        if (r < s.rows && stored) v[r] = *(const f32x4 *)(x + r * 16);
+#pragma unroll
+    for (int j = 0; j < 4; j++) old[j] = a.decay != 0.f && t0 + j < s.len ? w[j] : 0.f;
+    int upto = 0, chunk = a.chunk;
+    if (a.spread) chunk = weight_spread(a, upto);
+    const float mine = row_lse(a, s, b, unit % a.n_kv, min(tid >> 4, a.rows_pad - 1), 16, chunk, upto);
+    if ((tid & 15) == 0) lse[tid >> 4] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        if (r < s.rows && stored)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum[j] += exp2_of(v[r][j] - lse[r]);
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (t0 + j < s.len) put_weight(a, unit, t0 + j, sum[j]);
+        if (t0 + j < s.len) w[j] = a.decay == 0.f ? sum[j] : fmaf(a.decay, old[j], sum[j]);
 }
 
 // Weights of up to RS * RT * 16 rows, which stay in registers, over streamed keys: RS waves
@@ -468,13 +560,13 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stre
     constexpr int W = kWeightW / RS, rows = RS * RT * 16;
     constexpr int NB = P::KC <= 2 ? 4 : 2;
     __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * P::step_bytes];
+    static_assert(RS * RT * P::QTile::bytes <= kWeightW * NB * P::step_bytes, "queries in the ring");
     __shared__ float sums[RS][kWeightKeys / RS];
     constexpr int H = P::H;
     __shared__ int pos[rows];
     __shared__ float lse[rows], row_qs[rows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int rest;
-    const int unit = weight_unit(a, rest, INT_MAX), b = unit / a.n_kv, g = unit % a.n_kv;
+    const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units, b = unit / a.n_kv, g = unit % a.n_kv;
     const WeightSeq s(a, b);
     const int chunk = min(a.chunk, kWeightKeys / RS), k0 = rest * chunk, k1 = min(s.len, k0 + chunk), i0 = wave % RS * RT;
     if (k0 >= k1) return;
@@ -487,24 +579,23 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stre
     const int window = a.window;
     const float aqs = fabsf(a.qs);
     typename P::Q q[RT];
-    auto start = [&]() __attribute__((always_inline)) {
-        if (tid < rows) {
-            const float2 x = a.lse[(int64_t)unit * a.rows_pad + tid];
-            lse[tid] = x.x, row_qs[tid] = x.y;
-            pos[tid] = x.x == INFINITY ? -1 : s.first + query_row(a, tid);  // (also where there is no row)
-        }
+    if (tid < rows) {
+        const float2 x = a.lse[(int64_t)unit * a.rows_pad + tid];
+        lse[tid] = x.x, row_qs[tid] = x.y;
+        pos[tid] = x.x == INFINITY ? -1 : s.first + query_row(a, tid);  // (also where there is no row)
+    }
+    for (int i = wave; i < RS * RT; i += kWeightW) fetch_q<P>(a, s, b, g, i * 16, ring[0] + i * P::QTile::bytes);
+    vm_wait_n<0>();
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; i++) P::load_q(q[i], P::q_row(a, s, b, g, (i0 + i) * 16 + (lane & 15)), a.qs < 0.f);
-        __syncthreads();
-    };
+    for (int i = 0; i < RT; i++) read_q<P>(q[i], ring[0] + (i0 + i) * P::QTile::bytes, a.qs < 0.f);
+    __syncthreads();
+    auto start = [] {};
     const int all_lo = a.window ? s.first + query_row(a, s.rows - 1) + 1 - a.window : 0, all_hi = s.first + 1;
     auto tiles = [&](const typename P::K *k, int t0, auto mask) __attribute__((always_inline)) {
         f32x4 x[RT][H];
         float sum[H];
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int h = 0; h < H; h++) x[i][h] = P::template dot<true>(k[h], q[i]);
+        P::template dots<true>(x, k, q);
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const int r = (i0 + i) * 16 + 4 * (lane >> 4);  // the lane's four rows
@@ -535,7 +626,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stre
             if (lane < 16) sums[wave % RS][t0 - k0 + 16 * h + lane] = sum[h];
         }
     };
-    each_step<P, NB, W, false>(a, s, b, g, k0, k1, wave / RS, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
+    each_step<P, NB, W, 0>(a, s, b, g, k0, k1, wave / RS, ring[wave], start, [&](const typename P::K *k, int t0) __attribute__((always_inline)) {
         if (t0 >= all_lo && t0 + 16 * H <= all_hi) tiles(k, t0, Int<0>{});
         else tiles(k, t0, Int<1>{});
     });
@@ -555,11 +646,11 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight
     using P = Dot<TQ, TK, D>;
     using T = typename P::QTile;
     constexpr int KT = P::kt, NB = 2, R = 16 * kWeightW, stage = T::bytes + 1024;  // the rows, their (lse, qs)
+    static_assert(KT * P::KTile::bytes <= kWeightW * NB * stage, "keys in the ring");
     __shared__ __attribute__((aligned(1024))) char ring[kWeightW][NB * stage];
     __shared__ float join[kWeightW][KT * 16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int rest;
-    const int unit = weight_unit(a, rest, a.parts), part = rest % a.parts, b = unit / a.n_kv, g = unit % a.n_kv;
+    const int unit = blockIdx.x % a.units, rest = blockIdx.x / a.units, part = rest % a.parts, b = unit / a.n_kv, g = unit % a.n_kv;
     const int k0 = rest / a.parts * KT * 16;
     const WeightSeq s(a, b);
     const int k1 = min(k0 + KT * 16, s.len);
@@ -575,39 +666,19 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight
     }
     const int window = a.window;
     const float aqs = fabsf(a.qs);
-    typename P::K k[KT];
-    {
-        const KeySource<P> src(a, s, b, g, k0);
-#pragma unroll
-        for (int i = 0; i < KT; i += 2) {
-            const __amdgpu_buffer_rsrc_t r = src.rows(min(k0 + 16 * i, (k1 - 1) & ~31), 32);
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int c = 0; c < P::KC; c++)
-                    k[i + h].x[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                        r, ((lane & 15) + 16 * h) * (int)a.rb + (lane >> 4) * 16 + 64 * c, 0, 0));
-        }
-    }
     uint32_t at[T::N];
 #pragma unroll
     for (int c = 0; c < T::N; c++) at[c] = lds_addr(ring[wave]) + T::at(P::raw_chunk(c));
     const uint32_t at_ls = lds_addr(ring[wave]) + T::bytes + (lane >> 4) * 32;
     auto fetch = [&](int j, int r0) __attribute__((always_inline)) {
-        const int i0 = query_row(a, r0);
-        const char *base = (const char *)a.q + (((int64_t)b * a.max_rows + i0) * a.n_head + g * a.gq) * D * TQ::bytes;
-        const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(base), 0, 0x7fffffff, kRsrcWord3);
         char *dst = ring[wave] + j * stage;
-#pragma unroll
-        for (int d = 0; d < T::N; d++) {
-            const int r = min(r0 + T::row(d), s.rows - 1), i = query_row(a, r);
-            dma16_cached(rows, dst + d * 1024, ((i - i0) * a.n_head + r - i * a.gq) * D * TQ::bytes + T::col(d), 0);
-        }
+        fetch_q<P>(a, s, b, g, r0, dst);
         // (lse, qs) of 16 rows in the first 8 lanes; past them nothing is read
         const __amdgpu_buffer_rsrc_t ls =
             __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(a.lse + (int64_t)unit * a.rows_pad + r0), 0, 128, kRsrcWord3);
         dma16_cached(ls, dst + T::bytes, lane * 16, 0);
     };
+    typename P::K k[KT];
     float sum[KT];
 #pragma unroll
     for (int i = 0; i < KT; i++) sum[i] = 0.f;
@@ -620,26 +691,47 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight
                 const int r = r0 + 4 * (lane >> 4) + j;
                 pos[j] = r < s.rows && lse[j] != INFINITY ? s.first + query_row(a, r) : -1;
             }
+        constexpr int G = KT < 4 ? KT : 4;
 #pragma unroll
-        for (int i = 0; i < KT; i++) {
-            const f32x4 x = P::template dot<true>(k[i], q);
-            float e[4];
+        for (int i0 = 0; i0 < KT; i0 += G) {
+            f32x4 x[1][G];
+            P::template dots<true>(x, k + i0, &q);
 #pragma unroll
-            for (int j = 0; j < 4; j++) e[j] = exp2_of(fmaf(x[j], P::NP == 2 ? qs[j] : aqs, -lse[j]));
-            if constexpr (mask.value) {
-                const int t = k0 + 16 * i + (lane & 15);
+            for (int i = 0; i < G; i++) {
+                float e[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (t > pos[j] || (window && t <= pos[j] - window)) e[j] = 0.f;
+                for (int j = 0; j < 4; j++) e[j] = exp2_of(fmaf(x[0][i][j], P::NP == 2 ? qs[j] : aqs, -lse[j]));
+                if constexpr (mask.value) {
+                    const int t = k0 + 16 * (i0 + i) + (lane & 15);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (t > pos[j] || (window && t <= pos[j] - window)) e[j] = 0.f;
+                }
+                sum[i0 + i] += (e[0] + e[1]) + (e[2] + e[3]);
             }
-            sum[i] += (e[0] + e[1]) + (e[2] + e[3]);
         }
     };
     const int last = (hi - 1) & ~15;
+    {  // the keys, through the ring
+        using KT_ = typename P::KTile;
+        const KeySource<P> src(a, s, b, g, k0);
+        for (int i = wave; i < KT; i += kWeightW) {
+            const __amdgpu_buffer_rsrc_t rsrc = src.rows(min(k0 + 16 * i, (k1 - 1) & ~15), 16);
 #pragma unroll
-    for (int i = 0; i < KT; i++)
+            for (int d = 0; d < KT_::N; d++)
+                dma16_cached(rsrc, ring[0] + i * KT_::bytes + d * 1024, KT_::row(d) * (int)a.rb + KT_::col(d), 0);
+        }
+        vm_wait_n<0>();
+        __syncthreads();
 #pragma unroll
-        for (int c = 0; c < P::KC; c++) tie(k[i].x[c]);  // (the keys have come before the rows are counted)
+        for (int i = 0; i < KT; i++) {
+#pragma unroll
+            for (int c = 0; c < P::KC; c++)
+                k[i].x[c] = lds_read_b128(lds_addr(ring[0]) + i * KT_::bytes + KT_::at(4 * c + (lane >> 4)));
+            lds_wait(k[i].x);
+        }
+        __syncthreads();
+    }
 #pragma unroll
     for (int j = 0; j < NB; j++) fetch(j, min(lo + 16 * wave + j * R, last));
     for (int r0 = lo + 16 * wave; r0 < hi; r0 += NB * R)
@@ -685,7 +777,8 @@ __global__ __launch_bounds__(kWeightT) void weight_join_kernel(WeightArgs a) {
 // ---- how a call is cut ----
 struct WeightCut {
     int rt, mode;  // row tiles of a wave; 0: scores stored, 1: rows in registers, 2: keys in registers
-    int rows_pad, blocks, chunk, splits, row_chunk, parts;
+    int rows_pad, blocks, chunk, splits, spread, row_chunk, parts;
+    int64_t wgs;  // of weight_rows_kernel, its parts
     size_t ml, qs, lse, score, part, bytes;  // offsets
 };
 // Registers of a row tile, and the most of them in a wave (Dot::q_regs, Dot::rt).
@@ -710,11 +803,18 @@ static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows,
     const int64_t want = (keys * units * c.blocks + kWeightWgs - 1) / kWeightWgs;
     c.chunk = (int)std::max<int64_t>(std::min<int64_t>((want + 127) / 128, (max_len + 127) / 128) * 128, 128);
     c.splits = (int)((keys + c.chunk - 1) / c.chunk + (window > 0 ? 1 : 0));
-    c.parts = (int)std::min<int64_t>(16, (rows + 255) / 256);
+    c.wgs = units * c.blocks * c.splits;
+    // one sequence's keys or those of up to 64 together: one round of the card
+    if (c.mode <= 1 && batch <= 64 && batch * max_len <= INT_MAX) {
+        const int64_t each = n_kv * c.blocks, round = D * dtype_bytes(dtype) > 512 ? 256 : 512;
+        c.spread = (int)std::max<int64_t>(round / each - batch, std::max<int64_t>(batch, 1));
+        c.wgs = (c.spread + batch) * each;
+    }
+    c.parts = (int)std::min<int64_t>(8, (rows + 511) / 512);
     c.row_chunk = (int)(((rows + c.parts - 1) / std::max(c.parts, 1) + 63) / 64 * 64);
     size_t at = 0;
     const size_t entries = (size_t)units * c.rows_pad;
-    c.ml = at, at += up256(entries * c.splits * sizeof(float2));
+    c.ml = at, at += up256((size_t)c.wgs * c.rt * 16 * sizeof(float2));
     c.qs = at, at += up256(entries * sizeof(float));
     c.lse = at, at += c.mode ? up256(entries * sizeof(float2)) : 0;
     c.score = at, at += c.mode == 0 ? up256((size_t)units * ((max_len + 31) / 32) * c.rows_pad * 32 * sizeof(float)) : 0;
@@ -730,9 +830,9 @@ static void launch_stream(const WeightArgs &a, hipStream_t st) {
         launch_kernel(weight_stream_kernel<TQ, TK, D, RT, RS>, dim3(a.units * ((a.max_len + chunk - 1) / chunk)), dim3(kWeightT), 0, st, a);
 }
 template <class TQ, class TK, int D, int RT>
-static void launch_rows(const WeightArgs &a, hipStream_t st) {
+static void launch_rows(const WeightArgs &a, unsigned wgs, hipStream_t st) {
     if constexpr (RT <= Dot<TQ, TK, D>::rt)
-        launch_kernel(weight_rows_kernel<TQ, TK, D, RT, false>, dim3((unsigned)a.units * a.splits * a.blocks), dim3(kWeightT), 0, st, a);
+        launch_kernel(weight_rows_kernel<TQ, TK, D, RT, false>, dim3(wgs), dim3(kWeightT), 0, st, a);
 }
 template <class TQ, class TK, int D>
 static void launch_weights(const WeightArgs &a, const WeightCut &c, hipStream_t st) {
@@ -740,13 +840,13 @@ static void launch_weights(const WeightArgs &a, const WeightCut &c, hipStream_t 
     const dim3 wg(kWeightT);
     const unsigned units = a.units;
     if (c.mode == 0) {
-        launch_kernel(weight_rows_kernel<TQ, TK, D, 1, true>, dim3(units * c.splits), wg, 0, st, a);
+        launch_kernel(weight_rows_kernel<TQ, TK, D, 1, true>, dim3((unsigned)c.wgs), wg, 0, st, a);
         launch_kernel(weight_sums_kernel, dim3(units * ((a.max_len + 4 * kWeightT - 1) / (4 * kWeightT))), wg, 0, st, a);
         return;
     }
-    if (c.rt == 1) launch_rows<TQ, TK, D, 1>(a, st);
-    else if (c.rt == 2) launch_rows<TQ, TK, D, 2>(a, st);
-    else launch_rows<TQ, TK, D, 4>(a, st);
+    if (c.rt == 1) launch_rows<TQ, TK, D, 1>(a, c.wgs, st);
+    else if (c.rt == 2) launch_rows<TQ, TK, D, 2>(a, c.wgs, st);
+    else launch_rows<TQ, TK, D, 4>(a, c.wgs, st);
     launch_kernel(weight_merge_kernel, dim3(((size_t)units * c.rows_pad + 15) / 16), dim3(256), 0, st, a, c.rt * 16, (int)(P::NP == 2));
     if (c.mode == 1) {
         // as few waves to a key as hold the rows
@@ -792,7 +892,7 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     const WeightCut c = weight_cut(q_dtype, dtype, a.batch, rows, a.max_len, a.window, a.n_head, a.n_kv, head_dim);
     const int64_t units = (int64_t)a.batch * a.n_kv;
     // (a grid has less than 2^32 threads)
-    if (units * c.splits * c.blocks >= 1 << 24 || units * c.rows_pad > INT_MAX || units * ((a.max_len + 31) / 32) * c.parts >= 1 << 24)
+    if (c.wgs >= 1 << 24 || units * c.blocks * c.splits >= 1 << 30 || units * c.rows_pad > INT_MAX || units * ((a.max_len + 31) / 32) * c.parts >= 1 << 24)
         return set_error(ULLM_HIP_E_INVALID, "%s: too many rows or keys", fn);
     if (!ws || ws_bytes < c.bytes || (uintptr_t)ws & 255)
         return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, c.bytes);
@@ -802,7 +902,7 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     // (a scale of 0 as the least normal number: 0 times a masked score of -inf is none)
     a.qs = std::copysign(std::max(std::fabs(scale * kLog2e), 1.17549435e-38f), scale);
     a.rb = kv_stride * eb;
-    a.units = (int)units, a.rows_pad = c.rows_pad, a.blocks = c.blocks, a.chunk = c.chunk, a.splits = c.splits;
+    a.units = (int)units, a.rows_pad = c.rows_pad, a.blocks = c.blocks, a.chunk = c.chunk, a.splits = c.splits, a.spread = c.spread;
     a.row_chunk = c.row_chunk, a.parts = c.parts, a.tiles = (a.max_len + 31) / 32 * 2;
     char *const at = (char *)ws;
     a.ml = (float2 *)(at + c.ml), a.row_qs = (float *)(at + c.qs), a.lse = (float2 *)(at + c.lse);
@@ -865,10 +965,9 @@ extern "C" size_t ullm_hip_key_weights_workspace_bytes(int kv_dtype, int batch, 
     for (int q_dtype : {(int)ULLM_DT_F32, kv_dtype}) {
         const int block = 16 * weight_rt(weight_q_regs(q_dtype, kv_dtype, head_dim));
         const int64_t blocks = (rows + block - 1) / block, pad = (rows + 255) / 256 * 256;
-        // (parts of a row are counted for the rows of a block, of which the last may be padded to 256)
-        size_t n = up256((kWeightWgs + 3 * units * blocks) * 256 * sizeof(float2)) + 2 * up256(units * pad * sizeof(float2));
+        size_t n = up256((kWeightWgs + 3 * units * blocks) * block * sizeof(float2)) + 2 * up256(units * pad * sizeof(float2));
         n += std::max((size_t)(gq <= 16 ? up256((size_t)units * ((max_len + 31) / 32) * std::min<int64_t>(rows, 16) * 32 * sizeof(float)) : 0),
-                      up256((size_t)std::min<int64_t>(16, (rows + 255) / 256) * units * max_len * sizeof(float)));
+                      up256((size_t)std::min<int64_t>(8, (rows + 511) / 512) * units * max_len * sizeof(float)));
         most = std::max(most, n);
     }
     return most;
