@@ -66,11 +66,16 @@ __device__ __forceinline__ int pick_scan(int v, int *tmp, int &total) {
 // at first: 2048 bins over floats as whole numbers are about a hundred to an
 // octave, so that few lanes meet in a bin), until a bin holds one value or
 // exactly as many keys as are wanted.  Then one pass in order writes what stays.
+// Up to TILES * 4096 scores stay in registers, four neighbours a thread (0: any number, read
+// anew in each pass): bound by the barriers of three to four passes.  8192 scores in each of 256
+// workgroups took 24.3 us from memory, 14.8 so.
+template <int TILES>
 __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
     __shared__ int hist[kPickBins];
     __shared__ int tmp[kPickT / 64];
     __shared__ uint32_t range[2];
     __shared__ int found[2];
+    constexpr int tile = 4 * kPickT;
     const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y;
     const int64_t row = ((int64_t)blockIdx.z * a.batch + b) * a.groups + g;
     const float *x = a.score + row * a.score_stride;
@@ -80,18 +85,49 @@ __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
     if (a.len_out && g == 0 && blockIdx.z == 0 && tid == 0) a.len_out[b] = s.n;
     for (int j = s.n + tid; j < a.max_budget; j += kPickT) kept[j] = -1;
     const int from = s.first, to = s.len - s.last;
+    float v[TILES ? TILES : 1][4];
+    auto read = [&](float (&w)[4], int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = t0 + 4 * tid + i < s.len ? x[t0 + 4 * tid + i] : 0.f;
+    };
+#pragma unroll
+    for (int k = 0; k < TILES; k++) read(v[k], k * tile);
+    // f(the thread's four scores of a tile, their first position), tile by tile
+    auto each = [&](auto &&f) __attribute__((always_inline)) {
+        if constexpr (TILES > 0) {
+#pragma unroll
+            for (int k = 0; k < TILES; k++)
+                if (k * tile < s.len) f(v[k], k * tile + 4 * tid);
+        } else {
+            for (int t0 = 0; t0 < s.len; t0 += tile) {
+                read(v[0], t0);
+                f(v[0], t0 + 4 * tid);
+            }
+        }
+    };
     uint32_t limit = 0xffffffffu;  // keys above it stay, and the first `ties` that equal it
     int ties = 0;
     if (s.n < s.len && s.best) {
         if (tid == 0) range[0] = 0xffffffffu, range[1] = 0;
         __syncthreads();
         uint32_t lo = 0xffffffffu, hi = 0;
-        for (int t = from + tid; t < to; t += kPickT) {
-            const uint32_t key = score_key(x[t]);
-            lo = min(lo, key), hi = max(hi, key);
+        each([&](const float (&w)[4], int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (t + i >= from && t + i < to) {
+                    const uint32_t key = score_key(w[i]);
+                    lo = min(lo, key), hi = max(hi, key);
+                }
+        });
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            lo = min(lo, (uint32_t)__shfl_xor((int)lo, o));
+            hi = max(hi, (uint32_t)__shfl_xor((int)hi, o));
         }
-        atomicMin(&range[0], lo);
-        atomicMax(&range[1], hi);
+        if ((tid & 63) == 0) {
+            atomicMin(&range[0], lo);
+            atomicMax(&range[1], hi);
+        }
         __syncthreads();
         lo = range[0], hi = range[1];
         int need = s.best, bits = hi > lo ? 32 - __builtin_clz(hi - lo) : 0;
@@ -100,10 +136,13 @@ __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
             const int shift = max(bits - 11, 0);
             for (int i = tid; i < kPickBins; i += kPickT) hist[i] = 0;
             __syncthreads();
-            for (int t = from + tid; t < to; t += kPickT) {
-                const uint32_t d = score_key(x[t]) - lo;  // (below lo: past the range too)
-                if (d >> (bits - 1) < 2) atomicAdd(&hist[d >> shift], 1);
-            }
+            each([&](const float (&w)[4], int t) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t d = score_key(w[i]) - lo;  // (below lo: past the range too)
+                    if (t + i >= from && t + i < to && d >> (bits - 1) < 2) atomicAdd(&hist[d >> shift], 1);
+                }
+            });
             __syncthreads();
             // two bins a thread, the largest first
             const int top = kPickBins - 1 - 2 * tid, n0 = hist[top], n1 = hist[top - 1];
@@ -126,18 +165,14 @@ __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
             __syncthreads();
         }
     }
-    // in order, four positions a thread
     int kept_n = 0, tie_n = 0;  // kept for certain so far, ties so far
-    for (int t0 = 0; t0 < s.len; t0 += 4 * kPickT) {
-        float v[4];
+    each([&](const float (&w)[4], int t) __attribute__((always_inline)) {
         int sure = 0, tie = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int t = t0 + 4 * tid + i;
-            v[i] = t < s.len && (out || (t >= from && t < to)) ? x[t] : 0.f;
-            const uint32_t key = score_key(v[i]);
-            const bool mid = t >= from && t < to;
-            if (t < s.len && (s.n == s.len || !mid || key > limit)) sure |= 1 << i;
+            const uint32_t key = score_key(w[i]);
+            const bool mid = t + i >= from && t + i < to;
+            if (t + i < s.len && (s.n == s.len || !mid || key > limit)) sure |= 1 << i;
             else if (mid && key == limit) tie |= 1 << i;
         }
         const int mine = __popc(sure) | __popc(tie) << 16;
@@ -146,63 +181,79 @@ __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
         int c = kept_n + (before & 0xffff), e = tie_n + (before >> 16);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int t = t0 + 4 * tid + i;
             const bool yes = (sure >> i & 1) || ((tie >> i & 1) && e < ties);
             const int j = c + min(e, ties);
             c += sure >> i & 1, e += tie >> i & 1;
             if (yes && j < s.n) {
-                kept[j] = t;
-                if (out) out[j] = v[i];
+                kept[j] = t + i;
+                if (out) out[j] = w[i];
             }
         }
         kept_n += total & 0xffff, tie_n += total >> 16;
-    }
+    });
     if (!out) return;
     __syncthreads();
     for (int t = s.n + tid; t < s.len; t += kPickT) out[t] = 0.f;
 }
 
-// Byte offset of position t of sequence b, < 0 where the cache has none.
-__device__ __forceinline__ int64_t evict_row(const EvictArgs &a, int b, int t) {
-    if (!a.tab) return b * a.seq_b + t * a.rb;
-    const int pg = t >> a.shift;
-    const int phys = a.tab[(int64_t)b * a.tab_stride + pg];
-    if (phys < 0 || phys >= a.n_pages) return -1;
-    return (((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1))) * a.rb;
-}
-
 constexpr int kMoveT = 256, kMoveU = 8;
+constexpr int kMoveWgs = 1024;
+constexpr int kMovePages = 2048;  // entries of a sequence's table that fit LDS
 
 // Rows of one group of one plane (K or V of a layer), some of its columns.  Row j
 // takes position kept[j] >= j, so that rows go down in order: a pass reads its
 // rows into registers and stores them when every wave has read; what later
-// passes read lies behind what this one writes, so the next pass's loads are
-// in flight meanwhile.
+// passes read lies behind what this one writes.  The places of the next pass's rows are
+// looked up under this one's loads.  Bound by HBM where there are workgroups enough to
+// have their passes (32 KB) cover its latency; columns are cut to 64 bytes for that:
+// 8 sequences x 2048 rows x 1 KB in 8 layers took 210 us (2.6 TB/s) with a workgroup a
+// group, 129 so.
 __global__ __launch_bounds__(kMoveT) void evict_move_kernel(EvictArgs a, int log_c) {
+    __shared__ int pages[kMovePages];
     const int tid = threadIdx.x, gb = blockIdx.y, g = gb % a.groups, b = gb / a.groups;
     const int layer = a.one ? blockIdx.z : blockIdx.z >> 1;
     const EvictSeq s(a, b);
     if (s.n >= s.len) return;
     const int32_t *kept = a.kept + (((int64_t)layer * a.batch + b) * a.groups + g) * a.max_budget;
+    const int32_t *tab = a.tab ? a.tab + (int64_t)b * a.tab_stride : nullptr;
+    const int used = a.tab ? ((s.len - 1) >> a.shift) + 1 : 0;
+    const bool in_lds = used <= kMovePages;
+    if (in_lds)
+        for (int i = tid; i < used; i += kMoveT) pages[i] = tab[i];
+    __syncthreads();
     const int c = ((int)blockIdx.x << log_c) + (tid & ((1 << log_c) - 1)), r0 = tid >> log_c, step = kMoveT >> log_c;
     char *base = (!a.one && (blockIdx.z & 1) ? a.v : a.k) + layer * a.layer_b +
                  ((int64_t)g * a.cols + min(c, a.cols - 1)) * 16;
+    // byte offset of position t, < 0 where the cache has none
+    auto place = [&](int t) __attribute__((always_inline)) -> int64_t {
+        if (!a.tab) return b * a.seq_b + t * a.rb;
+        const int pg = t >> a.shift, phys = in_lds ? pages[pg] : tab[pg];
+        if (phys < 0 || phys >= a.n_pages) return -1;
+        return (((int64_t)phys << a.shift) + (t & ((1 << a.shift) - 1))) * a.rb;
+    };
     const int rows = step * kMoveU, passes = (s.n + rows - 1) / rows;
-    auto load = [&](int p, u32x4 (&x)[kMoveU], int64_t (&to)[kMoveU]) {
+    int next[kMoveU];
+    auto look = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kMoveU; u++) {
             const int j = p * rows + u * step + r0;
-            const int t = j < s.n ? kept[j] : j;
-            to[u] = -1;
-            if (t != j && c < a.cols) {
-                const int64_t src = evict_row(a, b, t);
-                to[u] = evict_row(a, b, j);
-                if (src < 0) to[u] = -1;
-                else x[u] = *(const u32x4 *)(base + src);
-            }
+            next[u] = j < s.n ? kept[j] : -1;
         }
     };
-    auto store = [&](u32x4 (&x)[kMoveU], int64_t (&to)[kMoveU]) {
+    look(0);
+    for (int p = 0; p < passes; p++) {  // the same for every wave
+        u32x4 x[kMoveU];
+        int64_t to[kMoveU];
+#pragma unroll
+        for (int u = 0; u < kMoveU; u++) {
+            const int j = p * rows + u * step + r0, t = next[u];
+            to[u] = -1;
+            if (t > j && c < a.cols) {
+                const int64_t from = place(t);
+                if (from >= 0) x[u] = *(const u32x4 *)(base + from), to[u] = place(j);
+            }
+        }
+        look(p + 1);
         // this wave's loads have come, then every wave's
 #pragma unroll
         for (int u = 0; u < kMoveU; u++) asm volatile("" : "+v"(x[u])::"memory");
@@ -210,16 +261,6 @@ __global__ __launch_bounds__(kMoveT) void evict_move_kernel(EvictArgs a, int log
 #pragma unroll
         for (int u = 0; u < kMoveU; u++)
             if (to[u] >= 0) *(u32x4 *)(base + to[u]) = x[u];
-    };
-    u32x4 x[kMoveU] = {}, y[kMoveU] = {};
-    int64_t tx[kMoveU], ty[kMoveU];
-    load(0, x, tx);
-    for (int p = 0; p < passes; p += 2) {  // the same for every wave
-        load(p + 1, y, ty);
-        store(x, tx);
-        if (p + 1 >= passes) break;
-        load(p + 2, x, tx);
-        store(y, ty);
     }
 }
 
@@ -266,10 +307,20 @@ static int kv_evict(const char *fn, EvictArgs a, int dtype, int64_t kv_stride, i
     a.cols = (int)((int64_t)kv_dim / a.groups * eb / 16);
     a.one = a.k == a.v;
     hipStream_t st = (hipStream_t)stream;
-    launch_kernel(evict_pick_kernel, dim3(a.groups, a.batch, n_layer), dim3(kPickT), 0, st, a);
+    const dim3 rows_grid(a.groups, a.batch, n_layer), pick(kPickT);
+    const int tiles = (a.n_ctx + 4 * kPickT - 1) / (4 * kPickT);
+    if (tiles <= 1) launch_kernel(evict_pick_kernel<1>, rows_grid, pick, 0, st, a);
+    else if (tiles <= 2) launch_kernel(evict_pick_kernel<2>, rows_grid, pick, 0, st, a);
+    else if (tiles <= 4) launch_kernel(evict_pick_kernel<4>, rows_grid, pick, 0, st, a);
+    else if (tiles <= 8) launch_kernel(evict_pick_kernel<8>, rows_grid, pick, 0, st, a);
+    else launch_kernel(evict_pick_kernel<0>, rows_grid, pick, 0, st, a);
     if (int rc = check_hip(hipGetLastError(), "kv_evict launch")) return rc;
     if (a.n_ctx == 0 || a.max_budget == 0) return ULLM_HIP_OK;
-    const int log_c = std::min(8, 32 - __builtin_clz(2 * a.cols - 1) - 1);
+    // columns of a workgroup: those of the group, cut down to 64 bytes until there are
+    // workgroups for a round of the card
+    int log_c = std::min(8, 32 - __builtin_clz(2 * a.cols - 1) - 1);
+    const int64_t planes = (int64_t)(a.one ? 1 : 2) * n_layer * a.batch * a.groups;
+    while (log_c > 2 && planes * ((a.cols + (1 << log_c) - 1) >> log_c) < kMoveWgs) log_c--;
     launch_kernel(evict_move_kernel, dim3((a.cols + (1 << log_c) - 1) >> log_c, a.batch * a.groups, (a.one ? 1 : 2) * n_layer),
                   dim3(kMoveT), 0, st, a, log_c);
     return check_hip(hipGetLastError(), "kv_evict launch");
