@@ -47,6 +47,7 @@ struct WeightArgs {
     int rows_pad;    // rows of a unit in the arrays below, a multiple of the blocks'
     int blocks;      // row blocks of a unit
     int chunk, splits;  // keys of a part of a row block, the most parts
+    int direct;         // one part a row block: its denominators are the rows'
     int spread;         // or: parts that all sequences have together, cut by their lengths (see weight_spread)
     int64_t tiles;  // of the scores of a unit
     int row_chunk, parts;  // rows of a part of a key block, the most parts (weight_keys_kernel)
@@ -392,7 +393,9 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
     }
     const int k0 = max(lo & ~31, org + split * chunk), k1 = min(hi, org + (split + 1) * chunk);
     if (k0 >= k1) return;
-    const int window = a.window, score_tile = a.rows_pad * 16;
+    // a row at position p sees the keys t with 0 <= p - t < span
+    const unsigned span = a.window ? a.window : INT_MAX;
+    const int score_tile = a.rows_pad * 16;
     const float aqs = fabsf(a.qs);
     float *const score = STORE ? a.score + (unit * a.tiles * a.rows_pad + (lane & 15)) * 16 + 4 * (lane >> 4) : nullptr;
     typename P::Q q[RT];
@@ -430,7 +433,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
 #pragma unroll
                 for (int j = 0; j < 4 * H; j++) {
                     const int t = (j & 3) + (j >> 2) * 16;
-                    if (t > d || (window && t <= d - window)) x[i][j >> 2][j & 3] = -INFINITY;
+                    if ((unsigned)(d - t) >= span) x[i][j >> 2][j & 3] = -INFINITY;
                 }
             }
             if constexpr (STORE) {
@@ -463,10 +466,15 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
         if (lane < 16) join[wave][i * 16 + lane] = float2{top, sum};
     }
     __syncthreads();
-    if (tid < r1 - r0) {
+    if (tid < (a.direct ? RT * 16 : r1 - r0)) {
         float top = join[0][tid].x, sum = 0.f;
         for (int w = 1; w < kWeightW; w++) top = fmaxf(top, join[w][tid].x);
         for (int w = 0; w < kWeightW; w++) sum += join[w][tid].y * exp2_of(join[w][tid].x - top);
+        if (a.direct) {  // (past the last row: weights of 0)
+            const float lse = tid < r1 - r0 && sum != 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+            a.lse[(int64_t)unit * a.rows_pad + r0 + tid] = float2{lse, aqs};
+            return;
+        }
         const int part = a.spread ? (int)blockIdx.x : (unit * a.blocks + block) * a.splits + split;
         a.ml[(int64_t)part * RT * 16 + tid] = float2{top, sum};
     }
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stre
         for (int t = k0 + tid; t < k1; t += kWeightT) put_weight(a, unit, t, 0.f);
         return;
     }
-    const int window = a.window;
+    const unsigned span = a.window ? a.window : INT_MAX;
     const float aqs = fabsf(a.qs);
     typename P::Q q[RT];
     if (tid < rows) {
@@ -614,7 +622,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_stre
                 for (int j = 0; j < 4; j++) {
                     e[j] = exp2_of(fmaf(x[i][h][j], P::NP == 2 ? qs[j] : aqs, -ls[j]));
                     const int t = t0 + 16 * h + (lane & 15);
-                    if (mask.value && (t > ps[j] || (window && t <= ps[j] - window))) e[j] = 0.f;
+                    if (mask.value && (unsigned)(ps[j] - t) >= span) e[j] = 0.f;
                 }
                 const float add = (e[0] + e[1]) + (e[2] + e[3]);
                 sum[h] = i ? sum[h] + add : add;
@@ -665,6 +673,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight
         return;
     }
     const int window = a.window;
+    const unsigned span = window ? window : INT_MAX;
     const float aqs = fabsf(a.qs);
     uint32_t at[T::N];
 #pragma unroll
@@ -705,7 +714,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::keys_waves)) void weight
                     const int t = k0 + 16 * (i0 + i) + (lane & 15);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        if (t > pos[j] || (window && t <= pos[j] - window)) e[j] = 0.f;
+                        if ((unsigned)(pos[j] - t) >= span) e[j] = 0.f;
                 }
                 sum[i0 + i] += (e[0] + e[1]) + (e[2] + e[3]);
             }
@@ -847,7 +856,7 @@ static void launch_weights(const WeightArgs &a, const WeightCut &c, hipStream_t 
     if (c.rt == 1) launch_rows<TQ, TK, D, 1>(a, c.wgs, st);
     else if (c.rt == 2) launch_rows<TQ, TK, D, 2>(a, c.wgs, st);
     else launch_rows<TQ, TK, D, 4>(a, c.wgs, st);
-    launch_kernel(weight_merge_kernel, dim3(((size_t)units * c.rows_pad + 15) / 16), dim3(256), 0, st, a, c.rt * 16, (int)(P::NP == 2));
+    if (!a.direct) launch_kernel(weight_merge_kernel, dim3(((size_t)units * c.rows_pad + 15) / 16), dim3(256), 0, st, a, c.rt * 16, (int)(P::NP == 2));
     if (c.mode == 1) {
         // as few waves to a key as hold the rows
         const int tiles = (a.max_rows * a.gq + 15) / 16;
@@ -903,6 +912,7 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     a.qs = std::copysign(std::max(std::fabs(scale * kLog2e), 1.17549435e-38f), scale);
     a.rb = kv_stride * eb;
     a.units = (int)units, a.rows_pad = c.rows_pad, a.blocks = c.blocks, a.chunk = c.chunk, a.splits = c.splits, a.spread = c.spread;
+    a.direct = c.mode == 2 && c.splits == 1 && (q_dtype == dtype || dtype != ULLM_DT_F16);
     a.row_chunk = c.row_chunk, a.parts = c.parts, a.tiles = (a.max_len + 31) / 32 * 2;
     char *const at = (char *)ws;
     a.ml = (float2 *)(at + c.ml), a.row_qs = (float *)(at + c.qs), a.lse = (float2 *)(at + c.lse);
