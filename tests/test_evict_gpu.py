@@ -122,6 +122,11 @@ def test_long_rows(dev, n):
     case(dev, "f16", 1, 1, 2, 8, [n], [n - 1], 4, 100, kind="ties", seed=n, out=False)
 
 
+def test_short_and_long_sequences_of_a_long_cache(dev):
+    """Scores that fit a workgroup's registers beside some that do not."""
+    case(dev, "f16", 1, 4, 2, 8, [5000, 39000, 32768, 32769], [4000, 30000, 100, 32768], 4, 100, n_ctx=40000)
+
+
 def test_columns_of_wider_rows(dev):
     for page in (0, 32):
         case(dev, "bf16", 2, 2, 2, 32, [100, 200], [50, 60], 2, 8, page, wide=True)

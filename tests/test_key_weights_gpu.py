@@ -142,6 +142,30 @@ def test_counts_and_lengths_outside_their_range(dev):
     assert torch.equal(w, ref) and (w[0].sum(-1) - 4).abs().max() < 1e-4 and (w[1] == 0).all()
 
 
+@pytest.mark.parametrize("B", [63, 64, 65, 130])
+def test_many_sequences(dev, B):
+    """Up to 64 sequences are cut together on the device, more of them each alone."""
+    lens = [1 + (b * 37) % 300 for b in range(B)]
+    for rows, page in ((1, 32), (1, 0), (9, 64)):
+        case(dev, "bf16", "kv", B, rows, 8, 2, 64, lens, [min(rows, n) for n in lens], page=page, seed=B)
+    case(dev, "f16", "f32", B, 6, 6, 2, 64, [max(1, n // 20) for n in lens[:-1]] + [2000], [1] * (B - 1) + [6], window=700, seed=B)
+
+
+@pytest.mark.parametrize("kv,qt", [("f32", "f32"), ("f16", "f32"), ("bf16", "f32"), ("f16", "kv")])
+def test_queries_of_zeros(dev, kv, qt):
+    """Every key that is seen gets the same weight, with any scale."""
+    for rows in (1, 40, 300):
+        for scale in (0.125, 0.0, 1e-30):
+            q = torch.zeros(1, rows, 4, 64, device=dev).to(DT[kv if qt == "kv" else "f32"])
+            k = torch.randn(1, 400, 128, device=dev).to(DT[kv])
+            w = torch.zeros(1, 2, 400, device=dev)
+            A.key_weights(q, k, w, i32([400], dev), 400, 2, scale=scale, window=100)
+            pos, key = torch.arange(400 - rows, 400)[:, None], torch.arange(400)
+            see = ((key <= pos) & (key > pos - 100)).double()
+            want = 2 * (see / see.sum(1, keepdim=True)).sum(0)
+            assert (w[0].double().cpu() - want).abs().max() <= want.max() * (400 + rows + 20) * U
+
+
 def test_all_rows_before_the_sequence(dev):
     """n_rows past the length: only the rows that stand at a position count."""
     q = torch.randn(1, 30, 4, 64, device=dev).half()

@@ -142,8 +142,8 @@ struct Dot {
 #pragma unroll
                     for (int i = 0; i < 4; i++) m = fmaxf(m, fabsf(__uint_as_float(raw.x[c][i])));
                 m = rows_max(m);  // the lanes of one row
-                // 2^14 <= m f < 2^15 (exponents kept where f and 1 / f are normal numbers)
-                const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 14, -126), 113);
+                // 2^14 <= m f < 2^15, or less where m is below 2^-46
+                const int e = min(max((int)(__float_as_uint(m) >> 23) - 127 - 14, -60), 113);
                 f = __uint_as_float((uint32_t)(127 - e) << 23), back = __uint_as_float((uint32_t)(127 + e) << 23);
             }
             if (neg) f = -f;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(kWeightT, (Dot<TQ, TK, D>::waves)) void weight_rows
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const float back = read_q<P>(q[i], staged + i * P::QTile::bytes, a.qs < 0.f);
-            if (P::NP == 2) row_qs[P::NP == 2 ? i : 0] = aqs * back;
+            if (P::NP == 2) row_qs[P::NP == 2 ? i : 0] = fmaxf(aqs * back, 1.17549435e-38f);  // (not 0: see a.qs)
             m[i] = kNoScore, l[i] = 0.f;
         }
     };

@@ -66,7 +66,7 @@ __device__ __forceinline__ int pick_scan(int v, int *tmp, int &total) {
 // at first: 2048 bins over floats as whole numbers are about a hundred to an
 // octave, so that few lanes meet in a bin), until a bin holds one value or
 // exactly as many keys as are wanted.  Then one pass in order writes what stays.
-// Up to TILES * 4096 scores stay in registers, four neighbours a thread (0: any number, read
+// Up to TILES * 4096 scores stay in registers, four neighbours a thread (more are read
 // anew in each pass): bound by the barriers of three to four passes.  8192 scores in each of 256
 // workgroups took 24.3 us from memory, 14.8 so.
 template <int TILES>
@@ -85,24 +85,27 @@ __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
     if (a.len_out && g == 0 && blockIdx.z == 0 && tid == 0) a.len_out[b] = s.n;
     for (int j = s.n + tid; j < a.max_budget; j += kPickT) kept[j] = -1;
     const int from = s.first, to = s.len - s.last;
-    float v[TILES ? TILES : 1][4];
+    const bool held = s.len <= TILES * tile;
+    float v[TILES][4];
     auto read = [&](float (&w)[4], int t0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) w[i] = t0 + 4 * tid + i < s.len ? x[t0 + 4 * tid + i] : 0.f;
     };
 #pragma unroll
-    for (int k = 0; k < TILES; k++) read(v[k], k * tile);
+    for (int k = 0; k < TILES; k++)
+        if (held && k * tile < s.len) read(v[k], k * tile);
     // f(the thread's four scores of a tile, their first position), tile by tile
     auto each = [&](auto &&f) __attribute__((always_inline)) {
-        if constexpr (TILES > 0) {
+        if (held) {
 #pragma unroll
             for (int k = 0; k < TILES; k++)
                 if (k * tile < s.len) f(v[k], k * tile + 4 * tid);
-        } else {
-            for (int t0 = 0; t0 < s.len; t0 += tile) {
-                read(v[0], t0);
-                f(v[0], t0 + 4 * tid);
-            }
+            return;
+        }
+        for (int t0 = 0; t0 < s.len; t0 += tile) {
+            float w[4];
+            read(w, t0);
+            f(w, t0 + 4 * tid);
         }
     };
     uint32_t limit = 0xffffffffu;  // keys above it stay, and the first `ties` that equal it
@@ -312,8 +315,7 @@ static int kv_evict(const char *fn, EvictArgs a, int dtype, int64_t kv_stride, i
     if (tiles <= 1) launch_kernel(evict_pick_kernel<1>, rows_grid, pick, 0, st, a);
     else if (tiles <= 2) launch_kernel(evict_pick_kernel<2>, rows_grid, pick, 0, st, a);
     else if (tiles <= 4) launch_kernel(evict_pick_kernel<4>, rows_grid, pick, 0, st, a);
-    else if (tiles <= 8) launch_kernel(evict_pick_kernel<8>, rows_grid, pick, 0, st, a);
-    else launch_kernel(evict_pick_kernel<0>, rows_grid, pick, 0, st, a);
+    else launch_kernel(evict_pick_kernel<8>, rows_grid, pick, 0, st, a);
     if (int rc = check_hip(hipGetLastError(), "kv_evict launch")) return rc;
     if (a.n_ctx == 0 || a.max_budget == 0) return ULLM_HIP_OK;
     // columns of a workgroup: those of the group, cut down to 64 bytes until there are
