@@ -16,10 +16,18 @@
 // from there in the operands' layout (lane l: row l % 16, 16 bytes at 64 c + 16 (l / 16)),
 // the 16-byte columns of a row exchanged by its number so that no two lanes meet in a
 // bank.  Read straight from memory in that layout, a lane's neighbours all lie in other
-// rows, and a decode step over 8 sequences of 4K-32K took 50 us in place of KW_US.
+// rows, 64 lines a load: the last 32 rows of a 32K prompt took 77 us so, 50 with the keys
+// and 38 with the queries through LDS.
 // f32 queries over a 16-bit cache enter as exact pieces of its type: three of bf16, or
 // two of f16 (22 bits, the row scaled by a power of two into f16's range).  An f32 cache
 // takes f32 products.
+//
+// Measured (us, 32/8 or 32/4 heads x 128, bf16): one row over 8 sequences of 4K-32K (154 MB of
+// keys) 50-53: 41 in the rows (their loads alone take 31, 27 is what reads of as many bytes
+// take; 19 MB of scores written beside them do the rest) and 9 in the sums; the last
+// 32 rows of 32K 37.7: 19.8 and 17.1 over 64 MB of keys each, 4.8 in the merge; all 2048
+// rows of a prompt 69.7: 30.8 and 43.7, vector instructions (an exponential counts four) for
+// about 40 of it, a workgroup's start, 3 to 4 us, for most of the rest.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -312,7 +320,7 @@ __device__ __forceinline__ void each_step(const WeightArgs &a, const WeightSeq &
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The lengths of a batch are on the device.  Where a call has few row blocks, all its
-// sequences together are cut into about `spread` parts of one length, so that one round of
+// sequences together are cut into up to spread + batch parts of one length, so that one round of
 // workgroups is busy to its end: returns that length, and in lane b the parts of
 // sequences 0 .. b (up to 64 of them).
 __device__ __forceinline__ int weight_spread(const WeightArgs &a, int &upto) {
@@ -324,10 +332,14 @@ __device__ __forceinline__ int weight_spread(const WeightArgs &a, int &upto) {
         if (s.rows) s.keys(a, 0, s.rows, lo, hi);
         keys = max(0, hi - (lo & ~31));
     }
-    const int total = __builtin_amdgcn_readlane(wave_scan(keys), 63);
-    const int chunk = max(128, ((total + a.spread - 1) / a.spread + 127) & ~127);
-    upto = wave_scan((keys + chunk - 1) / chunk);
-    return chunk;
+    // the shortest length, in steps of a sixteenth, that makes no more than spread + batch parts
+    // (total / spread always does)
+    const int total = __builtin_amdgcn_readlane(wave_scan(keys), 63), most = a.spread + a.batch;
+    int chunk = max(128, (total / most + 127) & ~127);
+    for (;; chunk += max(128, chunk / 16 & ~127)) {
+        upto = wave_scan((keys + chunk - 1) / chunk);
+        if (__builtin_amdgcn_readlane(upto, 63) <= most) return chunk;
+    }
 }
 // The parts of a row block: part j has the keys from org + j chunk on; it is part
 // first + j * step of the call.
@@ -784,6 +796,10 @@ __global__ __launch_bounds__(kWeightT) void weight_join_kernel(WeightArgs a) {
 }
 
 // ---- how a call is cut ----
+// Which way (us, scores stored / computed again, bf16 x 128): 8 sequences of 16K, 8 rows of a
+// kv head 77 / 103, 16 rows 85 / 103; of 4K-32K, 8 rows 53 / 81; one of 32K 20.6 / 28.6.
+// Sequences cut together / each alone: 4K-32K 53 / 56, one of 32K 19.5 / 23.8, equal lengths
+// the same.
 struct WeightCut {
     int rt, mode;  // row tiles of a wave; 0: scores stored, 1: rows in registers, 2: keys in registers
     int rows_pad, blocks, chunk, splits, spread, row_chunk, parts;
@@ -795,7 +811,9 @@ static int weight_q_regs(int q_dtype, int dtype, int D) {
     return D * dtype_bytes(dtype) / 16 * (q_dtype == dtype ? 1 : dtype == ULLM_DT_F16 ? 2 : 3);
 }
 static int weight_rt(int regs) { return regs <= 16 ? 4 : regs <= 48 ? 2 : 1; }
-constexpr int64_t kWeightWgs = 1024;  // workgroups aimed at: two to four rounds of the card
+// Workgroups aimed at where row blocks are many: a 2048-token prompt takes 32.5 us in its rows
+// with 512 or 1024, 43.5 with 2048, 60 with 4096 (a start each).
+constexpr int64_t kWeightWgs = 1024;
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows, int max_len, int window, int n_head,
                             int64_t n_kv, int D) {
@@ -819,6 +837,7 @@ static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows,
         c.spread = (int)std::max<int64_t>(round / each - batch, std::max<int64_t>(batch, 1));
         c.wgs = (c.spread + batch) * each;
     }
+    // (8192 rows of a kv head over 2048 keys: 44 us in 8 parts, 52 in 4, 49 in 16)
     c.parts = (int)std::min<int64_t>(8, (rows + 511) / 512);
     c.row_chunk = (int)(((rows + c.parts - 1) / std::max(c.parts, 1) + 63) / 64 * 64);
     size_t at = 0;

@@ -68,7 +68,7 @@ __device__ __forceinline__ int pick_scan(int v, int *tmp, int &total) {
 // exactly as many keys as are wanted.  Then one pass in order writes what stays.
 // Up to TILES * 4096 scores stay in registers, four neighbours a thread (more are read
 // anew in each pass): bound by the barriers of three to four passes.  8192 scores in each of 256
-// workgroups took 24.3 us from memory, 14.8 so.
+// workgroups took 24.3 us from memory, 15 so.
 template <int TILES>
 __global__ __launch_bounds__(kPickT) void evict_pick_kernel(EvictArgs a) {
     __shared__ int hist[kPickBins];
@@ -210,7 +210,7 @@ constexpr int kMovePages = 2048;  // entries of a sequence's table that fit LDS
 // looked up under this one's loads.  Bound by HBM where there are workgroups enough to
 // have their passes (32 KB) cover its latency; columns are cut to 64 bytes for that:
 // 8 sequences x 2048 rows x 1 KB in 8 layers took 210 us (2.6 TB/s) with a workgroup a
-// group, 129 so.
+// group, 115 (4.7 TB/s read and written) with 128 bytes of it.
 __global__ __launch_bounds__(kMoveT) void evict_move_kernel(EvictArgs a, int log_c) {
     __shared__ int pages[kMovePages];
     const int tid = threadIdx.x, gb = blockIdx.y, g = gb % a.groups, b = gb / a.groups;
