@@ -583,8 +583,8 @@ size_t ullm_hip_tree_verify_workspace_bytes(int vocab, int batch);
  * workspace: DEVICE memory of ullm_hip_key_weights_workspace_bytes, 256-byte aligned,
  *           needs no initialisation, one call at a time; one for max_len, batch and
  *           max_rows serves every call with smaller ones
- * max_rows * n_head <= 2^23, max_len <= 2^30; batch * n_kv_head * max_len < 2^26 is always
- * taken; head_dim 64, 128 or 256; n_head % n_kv_head == 0; q, k_cache and row strides
+ * max_rows * n_head <= 2^23, max_len <= 2^30; what has batch * n_kv_head <= 2^18 and both
+ * batch * n_head * max_rows and batch * n_kv_head * max_len < 2^26 is always taken; head_dim 64, 128 or 256; n_head % n_kv_head == 0; q, k_cache and row strides
  * 16-byte aligned. */
 int ullm_hip_key_weights(const void *q, int q_dtype, const void *k_cache, int kv_dtype,
                          int64_t kv_stride, int64_t seq_stride, const int32_t *seq_lens,
@@ -626,7 +626,8 @@ size_t ullm_hip_key_weights_workspace_bytes(int kv_dtype, int batch, int max_row
  * No output shares memory with an input or another output (scores_out apart).  The
  * strides and layers are those of ullm_hip_kv_accept; layers and sequences must not
  * share rows (in pages: no page that is written), nor may K and V overlap unless they are
- * one.  batch * groups <= 65535; pools, groups of columns and strides 16-byte aligned. */
+ * one.  batch * groups <= 65535, n_layer * batch * groups < 2^22, n_layer * batch * kv_dim <
+ * 2^28, score_stride <= 2^30; pools, groups of columns and strides 16-byte aligned. */
 int ullm_hip_kv_evict(void *k_cache, void *v_cache, int dtype, int64_t kv_stride,
                       int64_t seq_stride, int n_ctx, int kv_dim, int n_layer, int64_t layer_stride,
                       const float *scores, float *scores_out, int64_t score_stride, int groups,

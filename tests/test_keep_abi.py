@@ -82,7 +82,8 @@ BAD_EVICT = [
     (dict(budget=None), L.E_INVALID), (dict(s=None), L.E_INVALID), (dict(kept=None), L.E_INVALID), (dict(k=ODD), L.E_INVALID),
     (dict(out=at(4)), L.E_INVALID), (dict(out=at(5)), L.E_INVALID), (dict(kept=at(3)), L.E_INVALID), (dict(kept=at(4)), L.E_INVALID),
     (dict(kept=at(7)), L.E_INVALID), (dict(so=C.c_void_p((3 << 32) + 4)), L.E_INVALID), (dict(so=at(4)), L.E_INVALID),
-    (dict(so=at(6), s=at(8)), L.E_INVALID)]
+    (dict(so=at(6), s=at(8)), L.E_INVALID), (dict(ss_row=(1 << 30) + 1), L.E_INVALID),
+    (dict(NL=32767, batch=100, G=2), L.E_INVALID), (dict(NL=32767, kvd=16384, kvs=16384, ss=16384 * 99, ls=16384 * 99 * 2), L.E_INVALID)]
 
 
 @pytest.mark.parametrize("change,code", BAD_EVICT + [
@@ -101,7 +102,7 @@ def test_evict_paged_refuses(change, code):
         a.update(dict(P=32, pages=9) if n == "ss" else {} if n == "n_ctx" else {n: x})
         if n == "ls":
             a.update(tab=at(9), cols=4)
-    assert call("kv_evict_paged", a, **change) == code
+    assert call("kv_evict_paged", a, **{n: x for n, x in change.items() if n != "ss"}) == code
 
 
 def test_nothing_to_do():

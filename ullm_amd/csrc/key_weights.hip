@@ -118,7 +118,7 @@ struct Dot {
     // most row tiles of a wave where the rows stay in registers
     static constexpr int rt = q_regs <= 16 ? 4 : q_regs <= 48 ? 2 : 1;
     // weight_keys_kernel: key tiles of a wave
-    static constexpr int kt = (KC <= 4 ? 8 : KC <= 8 ? 4 : 2) / (NP > 1 && KC > 2 ? 2 : 1);
+    static constexpr int kt = KC <= 2 ? 8 : KC <= 4 ? 4 : NP > 1 || KC > 8 ? 2 : 4;
     using KTile = Tile<D * TK::bytes>;
     using QTile = Tile<D * TQ::bytes>;
     static constexpr int H = KC <= 4 ? 2 : 1;  // key tiles of a step where the keys are streamed
@@ -920,7 +920,7 @@ static int key_weights(const char *fn, WeightArgs a, int q_dtype, int dtype, int
     const WeightCut c = weight_cut(q_dtype, dtype, a.batch, rows, a.max_len, a.window, a.n_head, a.n_kv, head_dim);
     const int64_t units = (int64_t)a.batch * a.n_kv;
     // (a grid has less than 2^32 threads)
-    if (c.wgs >= 1 << 24 || units * c.blocks * c.splits >= 1 << 30 || units * c.rows_pad > INT_MAX || units * ((a.max_len + 31) / 32) * c.parts >= 1 << 24)
+    if (c.wgs >= 1 << 24 || units * c.blocks * c.splits >= 1 << 30 || units * c.rows_pad >= 1 << 28 || units * ((a.max_len + 31) / 32) * c.parts >= 1 << 24)
         return set_error(ULLM_HIP_E_INVALID, "%s: too many rows or keys", fn);
     if (!ws || ws_bytes < c.bytes || (uintptr_t)ws & 255)
         return set_error(ULLM_HIP_E_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed", fn, c.bytes);

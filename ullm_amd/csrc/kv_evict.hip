@@ -279,8 +279,11 @@ static int kv_evict(const char *fn, EvictArgs a, int dtype, int64_t kv_stride, i
         return set_error(ULLM_HIP_E_INVALID, "%s: bad n_layer, or batch * groups not in 0..65535", fn);
     if (kv_dim < 1 || kv_dim % a.groups || kv_stride < kv_dim || seq_stride < 0 || layer_stride < 0)
         return set_error(ULLM_HIP_E_INVALID, "%s: bad kv_dim/strides, or kv_dim no multiple of groups", fn);
-    if (a.max_budget < 0 || a.sink < 0 || a.recent < 0 || a.score_stride < 0)
-        return set_error(ULLM_HIP_E_INVALID, "%s: max_budget, sink, recent or score_stride < 0", fn);
+    if (a.max_budget < 0 || a.sink < 0 || a.recent < 0 || a.score_stride < 0 || a.score_stride > 1 << 30)
+        return set_error(ULLM_HIP_E_INVALID, "%s: max_budget, sink or recent < 0, or score_stride not in 0..2^30", fn);
+    // (a grid has less than 2^32 threads)
+    if ((int64_t)n_layer * a.batch * a.groups >= 1 << 22 || (int64_t)n_layer * a.batch * kv_dim >= 1ll << 28)
+        return set_error(ULLM_HIP_E_INVALID, "%s: too many layers, sequences and groups", fn);
     if ((n_layer > 1 && layer_stride < kv_dim) || (!a.tab && !rows_apart(a.batch, seq_stride, kv_stride, kv_dim)))
         return set_error(ULLM_HIP_E_INVALID, "%s: layers or sequences share rows", fn);
     if (a.batch == 0) return ULLM_HIP_OK;
