@@ -26,7 +26,7 @@
 // keys) 50-53: 41 in the rows (their loads alone take 31, 27 is what reads of as many bytes
 // take; 19 MB of scores written beside them do the rest) and 9 in the sums; the last
 // 32 rows of 32K 37.7: 19.8 and 17.1 over 64 MB of keys each, 4.8 in the merge; all 2048
-// rows of a prompt 69.7: 30.8 and 43.7, vector instructions (an exponential counts four) for
+// rows of a prompt 66 to 69: 31 and 41, vector instructions (an exponential counts four) for
 // about 40 of it, a workgroup's start, 3 to 4 us, for most of the rest.
 #include <algorithm>
 #include <climits>
@@ -837,7 +837,7 @@ static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows,
         c.spread = (int)std::max<int64_t>(round / each - batch, std::max<int64_t>(batch, 1));
         c.wgs = (c.spread + batch) * each;
     }
-    // (8192 rows of a kv head over 2048 keys: 44 us in 8 parts, 52 in 4, 49 in 16)
+    // (8192 rows of a kv head over 2048 keys, the whole call: 69 us in 8 parts, 70 in 6, 81 in 4, 83 in 2)
     c.parts = (int)std::min<int64_t>(8, (rows + 511) / 512);
     c.row_chunk = (int)(((rows + c.parts - 1) / std::max(c.parts, 1) + 63) / 64 * 64);
     size_t at = 0;
