@@ -229,3 +229,25 @@ def test_captured_and_replayed(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((*got, k, v), (*want, ke, ve)))
         assert torch.equal(so[:, 0], se[:, 0])
+
+
+@pytest.mark.parametrize("page", [0, 32])
+def test_offsets_past_32_bits(dev, page):
+    """Rows 128 KB apart, 5.2 GB of them, against the same rows close together."""
+    n, G, hd, keep = 40000, 2, 64, 36000
+    g = torch.Generator(device=dev).manual_seed(4)
+    k = torch.randn(1, 1, n, G * hd, device=dev, generator=g).half()
+    wide = torch.full((1, 1, n, 65536), 3.0, device=dev, dtype=torch.float16)
+    far = wide[..., 65536 - G * hd:]
+    far.copy_(k)
+    sc = torch.rand(1, 1, G, n, device=dev, generator=g)
+    lens, budget = i32([n - 3], dev), i32([keep], dev)
+    more = dict(max_budget=keep, sink=4, recent=100)
+    want, _ = A.kv_evict(k, k, sc.clone(), lens, budget, **more)
+    if page:
+        pool = far.view(1, n // page, page, G * hd)
+        got, _ = A.kv_evict_paged(pool, pool, i32([list(range(n // page))], dev), sc, lens, budget, **more)
+    else:
+        got, _ = A.kv_evict(far, far, sc, lens, budget, **more)
+    assert torch.equal(got, want) and torch.equal(far, k)
+    assert (wide[0, 0, ::1000, :65536 - G * hd] == 3).all()

@@ -299,3 +299,22 @@ def test_captured_and_replayed(dev, rows):
         A.key_weights(q, k, want, n, 3000, 2, decay=0.0)
         torch.cuda.synchronize()
         assert torch.equal(w, want)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 100])
+def test_offsets_past_32_bits(dev, rows):
+    """A cache whose rows lie 128 KB apart, 5.2 GB of them, against the same rows close
+    together; as one sequence and as pages."""
+    H, Hk, D, n = 8, 2, 64, 40000
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn(1, rows, H, D, device=dev, generator=g).half()
+    k = torch.randn(1, n, Hk * D, device=dev, generator=g).half()
+    wide = torch.empty(1, n, 65536, device=dev, dtype=torch.float16)
+    far = wide[..., :Hk * D]
+    far.copy_(k)
+    ref, out, paged = (torch.zeros(1, Hk, n, device=dev) for _ in range(3))
+    lens = i32([n - 3], dev)
+    A.key_weights(q, k, ref, lens, n, Hk)
+    A.key_weights(q, far, out, lens, n, Hk)
+    A.key_weights_paged(q, wide.view(n // 32, 32, 65536), i32([list(range(n // 32))], dev), paged, lens, n, Hk)
+    assert torch.equal(out, ref) and torch.equal(paged, ref) and ref[..., -100:-3].sum() > 0
