@@ -578,7 +578,8 @@ size_t ullm_hip_tree_verify_workspace_bytes(int vocab, int batch);
  * q:        [batch][max_rows][n_head][head_dim] in the cache's dtype or f32 (q_dtype)
  * k_cache:  as for ullm_hip_attn_decode; keys 0..max_len-1 must be readable
  * seq_lens: int32[batch] (clamped to 0..max_len); n_rows: int32[batch] (clamped to
- *           0..max_rows) or NULL: max_rows each
+ *           0..max_rows) or NULL: max_rows each; with max_rows 0 the weights only fade
+ *           and q may be NULL
  * weights:  f32[batch][n_kv_head][weights_stride], weights_stride >= max_len
  * workspace: DEVICE memory of ullm_hip_key_weights_workspace_bytes, 256-byte aligned,
  *           needs no initialisation, one call at a time; one for max_len, batch and

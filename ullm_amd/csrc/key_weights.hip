@@ -982,10 +982,11 @@ extern "C" int ullm_hip_key_weights_paged(const void *q, int q_dtype, const void
 
 extern "C" size_t ullm_hip_key_weights_workspace_bytes(int kv_dtype, int batch, int max_rows, int max_len, int window,
                                                        int n_head, int n_kv_head, int head_dim) {
-    if (!dtype_ok(kv_dtype) || (head_dim != 64 && head_dim != 128 && head_dim != 256) || batch < 1 || max_rows < 1 ||
+    if (!dtype_ok(kv_dtype) || (head_dim != 64 && head_dim != 128 && head_dim != 256) || batch < 1 || max_rows < 0 ||
         max_len < 1 || max_len > 1 << 30 || window < 0 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || n_head > 65535 ||
         (int64_t)max_rows * n_head > 1 << 23)
         return 0;
+    max_rows = std::max(max_rows, 1);  // (a call without rows is planned as one of one row)
     // For every call with fewer sequences, rows and positions too: parts of row blocks are at most
     // kWeightWgs and three more a block; the scores are those of up to 16 rows.
     const int gq = n_head / n_kv_head;
