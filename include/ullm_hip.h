@@ -585,8 +585,9 @@ size_t ullm_hip_tree_verify_workspace_bytes(int vocab, int batch);
  *           needs no initialisation, one call at a time; one for max_len, batch and
  *           max_rows serves every call with smaller ones
  * max_rows * n_head <= 2^23, max_len <= 2^30; what has batch * n_kv_head <= 2^18 and both
- * batch * n_head * max_rows and batch * n_kv_head * max_len < 2^26 is always taken; head_dim 64, 128 or 256; n_head % n_kv_head == 0; q, k_cache and row strides
- * 16-byte aligned. */
+ * batch * n_head * max_rows and batch * n_kv_head * max_len < 2^26 is always taken, larger
+ * calls may be refused (a launch has less than 2^32 threads); head_dim 64, 128 or 256;
+ * n_head % n_kv_head == 0; q, k_cache and row strides 16-byte aligned. */
 int ullm_hip_key_weights(const void *q, int q_dtype, const void *k_cache, int kv_dtype,
                          int64_t kv_stride, int64_t seq_stride, const int32_t *seq_lens,
                          const int32_t *n_rows, int max_rows, int max_len, int window, int batch,

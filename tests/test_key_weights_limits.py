@@ -33,3 +33,21 @@ def test_workspace_of_a_call_without_rows(dt, H, Hk, D, window):
             assert rc == L.E_WORKSPACE and 0 < need <= f(dt, 2, 0, max_len, window, H, Hk, D)
             assert f(dt, 2, 0, max_len, window, H, Hk, D) <= f(dt, 2, 1, max_len, window, H, Hk, D)
     assert f(dt, 2, -1, 99, window, H, Hk, D) == 0
+
+
+@pytest.mark.parametrize("D,dt", [(64, L.DT_BF16), (256, L.DT_F32)])
+@pytest.mark.parametrize("batch,H,Hk,rows,max_len", [
+    (1, 1, 1, 4096, (1 << 26) - 1), (1, 1, 1, 1 << 23, (1 << 26) - 1), (2250, 8, 8, 3700, 3713), (2304, 8, 8, 3600, 3640),
+    (32768, 8, 8, 255, 255), (32768, 8, 8, 255, 1), (1 << 12, 64, 64, 255, 255), (8, 8, 8, 1 << 20, (1 << 20) - 1),
+    (65535, 4, 4, 255, 255), (1, 64, 64, 1 << 17, (1 << 20) - 1), (1, 64, 1, 1 << 17, (1 << 26) - 1), (1023, 256, 256, 255, 255)])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_what_is_always_taken(batch, H, Hk, rows, max_len, D, dt, window):
+    """batch * n_kv_head <= 2^18, batch * n_head * max_rows and batch * n_kv_head * max_len
+    < 2^26, max_rows * n_head <= 2^23: taken, as far as its workspace, which the size covers."""
+    rows = min(rows, ((1 << 26) - 1) // (batch * H))
+    assert batch * Hk <= 1 << 18 and batch * Hk * max_len < 1 << 26 and rows * H <= 1 << 23
+    size = L.lib().ullm_hip_key_weights_workspace_bytes(dt, batch, rows, max_len, window, H, Hk, D)
+    for page in (0, 1 << 16):
+        for qdt in {dt, L.DT_F32}:
+            rc, need = needs(dt, qdt, rows, max_len, window, batch, H, Hk, D, page)
+            assert rc == L.E_WORKSPACE and need <= size

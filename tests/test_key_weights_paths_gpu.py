@@ -4,9 +4,11 @@ import numpy as np
 import pytest
 import torch
 
+from test_key_weights_gpu import rule
 from ullm_amd import attention as A
 
 pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
 
 
 def i32(x, dev):
@@ -29,3 +31,35 @@ def test_no_rows(dev, kv, H, Hk, D):
             for w in (A.key_weights(q, k, old.clone(), lens, 96, Hk, window=window, decay=decay),
                       A.key_weights_paged(q, k.view(9, 32, Hk * D), table, old.clone(), lens, 96, Hk, window=window, decay=decay)):
                 assert torch.equal(w, want)
+
+
+def against_64_bits(w, old, q, k, lens, n_rows, decay=1.0, window=0):
+    """w [B, Hk, n] after a call over k [B, n, Hk * D] (old before it), by the bounds of
+    test_key_weights_gpu.py."""
+    B, rows, H, D = q.shape
+    Hk = w.shape[1]
+    G = H // Hk
+    for b in range(B):
+        n, r = min(max(lens[b], 0), k.shape[1]), min(max(n_rows[b], 0), rows)
+        assert torch.equal(w[b, :, n:], old[b, :, n:]), "positions past the length"
+        for j in range(Hk):
+            want, rel, low = rule(q[b, :, j * G:(j + 1) * G].double(), k[b, :n, j * D:(j + 1) * D].double(), n, r, window, D ** -0.5)
+            was = decay * old[b, j, :n].double() if decay else torch.zeros(n, dtype=torch.float64, device=w.device)
+            over = (w[b, j, :n].double() - want - was).abs() - (want * rel + low + 4 * U * (want + was))
+            assert n == 0 or over.max().item() <= 0, (b, j, over.max().item())
+
+
+@pytest.mark.parametrize("kv,D", [(torch.float16, 64), (torch.float32, 256)])
+def test_longest_that_is_always_taken(dev, kv, D):
+    """2^26 - 1 positions of one kv head and 4096 rows, as far as launches and workspace go: the
+    sequence itself is 5000 positions of one large page."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    rows, n, page, max_len = 4096, 5000, 1 << 16, (1 << 26) - 1
+    q = torch.randn(1, rows, 1, D, device=dev, generator=g).to(kv)
+    pool = torch.randn(1, page, D, device=dev, generator=g).to(kv)
+    table = torch.full((1, 1024), -1, dtype=torch.int32, device=dev)
+    table[0, 0] = 0
+    w = torch.full((1, 1, max_len), 0.5, device=dev)
+    A.key_weights_paged(q, pool, table, w, i32([n], dev), max_len, 1)
+    assert (w[0, 0, n:] == 0.5).all()
+    against_64_bits(w[..., :n], torch.full((1, 1, n), 0.5, device=dev), q, pool[:, :n], [n], [rows])

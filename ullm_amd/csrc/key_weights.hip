@@ -839,6 +839,9 @@ static WeightCut weight_cut(int q_dtype, int dtype, int64_t batch, int max_rows,
     }
     // (8192 rows of a kv head over 2048 keys, the whole call: 69 us in 8 parts, 70 in 6, 81 in 4, 83 in 2)
     c.parts = (int)std::min<int64_t>(8, (rows + 511) / 512);
+    // (fewer where the key blocks, of 32 keys or more, alone come near the 2^24 workgroups of a grid)
+    const int64_t key_blocks = units * ((max_len + 31) / 32);
+    while (c.parts > 1 && key_blocks * c.parts >= 1 << 24) c.parts--;
     c.row_chunk = (int)(((rows + c.parts - 1) / std::max(c.parts, 1) + 63) / 64 * 64);
     size_t at = 0;
     const size_t entries = (size_t)units * c.rows_pad;
