@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from test_key_weights_gpu import rule
+from ullm_amd import _lib as L
 from ullm_amd import attention as A
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +64,46 @@ def test_longest_that_is_always_taken(dev, kv, D):
     A.key_weights_paged(q, pool, table, w, i32([n], dev), max_len, 1)
     assert (w[0, 0, n:] == 0.5).all()
     against_64_bits(w[..., :n], torch.full((1, 1, n), 0.5, device=dev), q, pool[:, :n], [n], [rows])
+
+
+# cache, f32 queries, rows, heads, kv heads, head_dim, max_len: scores stored; query rows in
+# registers, shared by one, two and four waves; keys in registers, the denominators of one
+# part a row block (128 keys; 32 kv heads' rows, which fill the card) and of several
+F16, F32, BF16 = torch.float16, torch.float32, torch.bfloat16
+WAYS = [(BF16, False, 4, 8, 2, 128, 700), (F16, True, 1, 14, 2, 64, 333), (F32, True, 3, 4, 1, 256, 260),
+        (BF16, False, 12, 8, 2, 128, 700), (F16, True, 30, 8, 2, 64, 900), (BF16, True, 50, 2, 1, 128, 500),
+        (F16, False, 250, 1, 1, 64, 1300), (F32, True, 60, 1, 1, 128, 300),
+        (BF16, False, 300, 2, 1, 64, 128), (BF16, True, 600, 32, 8, 64, 700), (F16, True, 300, 6, 2, 128, 900),
+        (F16, False, 300, 6, 2, 64, 900), (F32, True, 90, 8, 2, 256, 400)]
+
+
+@pytest.mark.parametrize("fill", [255, 127, 0])
+@pytest.mark.parametrize("kv,f32,rows,H,Hk,D,max_len", WAYS)
+def test_odd_counts_over_a_full_workspace(dev, kv, f32, rows, H, Hk, D, max_len, fill):
+    """Lengths past max_len and below 0, rows past max_rows and more than positions, over a
+    workspace that holds NaN, 3.4e38 or 0, on a stream of its own; windows and pages."""
+    g = torch.Generator(device=dev).manual_seed(rows + D)
+    B, page = 4, 32
+    lens, n_rows = [1 << 20, -5, max_len * 3 // 4, 41], [rows, rows, 1 << 20, rows]
+    q = torch.randn(B, rows, H, D, device=dev, generator=g).to(F32 if f32 else kv)
+    cols = -(-max_len // page)
+    pool = torch.randn(B * cols, page, Hk * D, device=dev, generator=g).to(kv)
+    k = pool.view(B, cols * page, Hk * D)[:, :max_len]
+    table = torch.arange(B * cols, dtype=torch.int32, device=dev).view(B, cols).contiguous()
+    old = torch.rand(B, Hk, max_len + 3, device=dev, generator=g)
+    code = {F32: L.DT_F32, F16: L.DT_F16, BF16: L.DT_BF16}[kv]
+    count, length, stream = i32(n_rows, dev), i32(lens, dev), torch.cuda.Stream()
+    for window in (0, 50):
+        size = L.lib().ullm_hip_key_weights_workspace_bytes(code, B, rows, max_len, window, H, Hk, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        for paged in (False, True):
+            ws.fill_(fill)
+            w = old.clone()
+            more = dict(n_rows=count, window=window, decay=0.5, workspace=ws, stream=stream)
+            torch.cuda.synchronize()
+            if paged:
+                A.key_weights_paged(q, pool, table, w, length, max_len, Hk, **more)
+            else:
+                A.key_weights(q, k, w, length, max_len, Hk, **more)
+            stream.synchronize()
+            against_64_bits(w, old, q, k, lens, n_rows, 0.5, window)
