@@ -18,6 +18,7 @@
 #include <climits>
 #include <cmath>
 #include <optional>
+#include <vector>
 
 #include "../../../include/ullm_hip.h"
 
@@ -855,7 +856,14 @@ PyObject *evict(const Args &a) {
     if (sc.scalar_type() != at::kFloat || sc.dim() < 2 || !sc.is_contiguous())
         invalid("scores must be contiguous f32 [n_layer, B, groups, n]");
     const int64_t n = sc.size(-1), G = sc.size(-2);
-    if (G < 1 || (n && sc.numel() / n != layers * (int64_t)B * G) || (!n && sc.numel()))
+    // (a dimension of one layer or one sequence may be left out)
+    auto not_one = [](at::IntArrayRef sizes) {
+        std::vector<int64_t> r;
+        for (int64_t x : sizes)
+            if (x != 1) r.push_back(x);
+        return r;
+    };
+    if (G < 1 || sc.dim() > 4 || not_one(sc.sizes().slice(0, sc.dim() - 2)) != not_one({layers, B}))
         invalid("scores must be [n_layer, B, groups, n] of the caches' layers and sequences");
     if (so && (so->scalar_type() != at::kFloat || so->sizes() != sc.sizes() || !so->is_contiguous()))
         invalid("scores_out must be as scores");
