@@ -18,16 +18,22 @@
 // bank.  Read straight from memory in that layout, a lane's neighbours all lie in other
 // rows, 64 lines a load: the last 32 rows of a 32K prompt took 77 us so, 50 with the keys
 // and 38 with the queries through LDS.
-// f32 queries over a 16-bit cache enter as exact pieces of its type: three of bf16, or
-// two of f16 (22 bits, the row scaled by a power of two into f16's range).  An f32 cache
-// takes f32 products.
+// f32 queries over a 16-bit cache enter in pieces of its type: three of bf16, which hold
+// all 24 bits, or two of f16, the row scaled by a power of two into f16's range.  These hold 22
+// bits, off by at most 2^-23 of a value or 2^-39 of the row's largest, well inside the
+// bound of a score's sum of head_dim products in 32 bits; a third piece would be half as
+// many products again.  An f32 cache takes f32 products.
 //
 // Measured (us, 32/8 or 32/4 heads x 128, bf16): one row over 8 sequences of 4K-32K (154 MB of
-// keys) 50-53: 41 in the rows (their loads alone take 31, 27 is what reads of as many bytes
-// take; 19 MB of scores written beside them do the rest) and 9 in the sums; the last
+// keys) 50-53: 41 to 44 in the rows (33 with their loads alone, where reads of as many bytes
+// take 27; 34 with the arithmetic and no scores stored; the rest are the 19 MB of scores, written
+// beside the loads and counted with them) and 9 in the sums; the last
 // 32 rows of 32K 37.7: 19.8 and 17.1 over 64 MB of keys each, 4.8 in the merge; all 2048
 // rows of a prompt 66 to 69: 31 and 41, vector instructions (an exponential counts four) for
-// about 40 of it, a workgroup's start, 3 to 4 us, for most of the rest.
+// about 40 of it, a workgroup's start, 3 to 4 us, for most of the rest.  In weight_keys_kernel
+// a step of 16 rows and 64 keys has 47 of the formula, 16 of them exponentials, and 36 that
+// find the places of the next query rows, 8 of them whole products at an exponential's
+// rate: two fifths of the step.
 #include <algorithm>
 #include <climits>
 #include <cmath>
